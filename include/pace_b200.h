@@ -452,6 +452,105 @@ int pace_append_paged_kv_cache_by_indptr(const void* key, const void* value, int
                                          const int32_t* kv_last_page_len, int64_t batch_size,
                                          int32_t* bad_tokens, int dtype, cudaStream_t stream);
 
+/* ---- quantised paged KV cache --------------------------------------------
+ * Two tensors per layer, paged like the 16-bit cache:
+ *   codes     [num_pages, 2, page_size, kv_heads, head_dim]  e4m3
+ *   exponents [num_pages, 2, page_size, kv_heads]            uint8
+ * A row x (one token's K or V of one head) is held as code = e4m3(x * 2^-e),
+ * exponent = e + 127, with e the smallest integer >= -126 that has
+ * max|x| <= 448 * 2^e (0 for a row of zeros), so value = code * 2^e and each
+ * element is rounded once, to nearest even.  Infinities saturate at the
+ * largest code and stay out of the maximum; a row with a NaN has exponent 255
+ * and reads as NaN.  head_dim: a multiple of 8 up to 256.
+ *
+ * Quantise and append nnz new tokens; arguments as
+ * pace_append_paged_kv_cache_by_indptr (key and value float32, float16 or
+ * bfloat16 rows).  New: the reference's cache has the model's dtype
+ * (flashinfer_attention_wrapper.py:53-73). */
+int pace_append_quantised_paged_kv_cache(const void* key, const void* value, int64_t nnz,
+                                         int num_kv_heads, int head_dim, int64_t key_row_stride,
+                                         int64_t value_row_stride, const int32_t* append_indptr,
+                                         void* codes, void* exponents, int64_t num_pages,
+                                         int page_size, const int32_t* kv_indices,
+                                         int64_t num_kv_indices, const int32_t* kv_indptr,
+                                         const int32_t* kv_last_page_len, int64_t batch_size,
+                                         int32_t* bad_tokens, int dtype, cudaStream_t stream);
+
+/* Read the rows of every request back in sequence order: output row
+ * out_indptr[b] + i is token i of request b, for i < out_indptr[b+1] -
+ * out_indptr[b] (at most the request's length), as [kv_heads * head_dim] values
+ * of `dtype`, row strides in elements.  Rows that no request has, or whose page
+ * is out of range, are left alone and counted into *bad_tokens. */
+int pace_read_quantised_paged_kv_cache(void* key, void* value, int64_t rows, int num_kv_heads,
+                                       int head_dim, int64_t key_row_stride,
+                                       int64_t value_row_stride, const int32_t* out_indptr,
+                                       const void* codes, const void* exponents,
+                                       int64_t num_pages, int page_size,
+                                       const int32_t* kv_indices, int64_t num_kv_indices,
+                                       const int32_t* kv_indptr, const int32_t* kv_last_page_len,
+                                       int64_t batch_size, int32_t* bad_tokens, int dtype,
+                                       cudaStream_t stream);
+
+/* ---- paged attention ------------------------------------------------------
+ * Attention of each request's newest tokens over its paged sequence.  For query
+ * token i of a request (position p = kv_len - q_len + i), head h and key j
+ *   s = cap * tanh(sm_scale * q.k / cap)   (cap 0: sm_scale * q.k)
+ *       - slope[h] * |p - j|               (with alibi_slopes)
+ *   out = sum_j softmax_j(s) v_j over the visible keys; 0 where there is none.
+ * Visible are the keys j <= p and, with a prefix, j < prefix_lens[request], of
+ * which those before p - window_left (window_left >= 0) and before
+ * doc_starts[token] are hidden.  With a tree, the request's q_len tokens are
+ * drafted nodes: visible are all earlier keys and the nodes k whose bit k of
+ * tree_mask[token] ([total_q, tree_words] 64-bit words) is set; a tree takes no
+ * other mask and no slopes.
+ *
+ * A step is planned once on the host, then run for each layer.  The plan is a
+ * struct and an array of int32 words: write it with pace_paged_attention_plan
+ * into host memory of pace_paged_attention_plan_words() words, then copy its
+ * first plan.num_words words to the device.  All array arguments of the plan
+ * are host arrays; prefix_lens [batch], doc_starts [total_q] may be NULL.
+ * Replaces the begin_forward / run pair of FlashInfer's paged wrappers
+ * (flashinfer_attention_wrapper.py:165-188,257-275) and adds the capped scores,
+ * the bias and the masks. */
+typedef struct {
+  int64_t total_q, batch_size;
+  int64_t num_words;                                /* of the plan array */
+  int64_t few_offset, many_offset, indices_offset;  /* in words */
+  size_t workspace_bytes;
+  int num_heads, num_kv_heads, head_dim, page_size, tree_words;
+  int num_few, num_many;      /* pieces of the few-row and of the tile kernel */
+  int few_slots, many_slots;  /* their partial results */
+  int few_tiles, many_tiles;  /* their cut groups of rows */
+  int max_page;
+} pace_attention_plan;
+
+/* Words that a plan may need (0 for a bad argument). */
+int64_t pace_paged_attention_plan_words(int64_t batch_size, int64_t total_q,
+                                        int64_t num_kv_indices, int num_sms);
+int pace_paged_attention_plan(pace_attention_plan* plan, int32_t* words, int64_t num_words,
+                              const int32_t* qo_indptr, const int32_t* kv_indptr,
+                              const int32_t* kv_indices, int64_t num_kv_indices,
+                              const int32_t* kv_last_page_len, int64_t batch_size, int num_heads,
+                              int num_kv_heads, int head_dim, int page_size, int window_left,
+                              const int32_t* prefix_lens, const int32_t* doc_starts,
+                              int tree_words, int num_sms);
+
+/* Runs a plan.  query and out: [total_q, heads, head_dim] of `dtype`, heads
+ * contiguous, token strides in elements.  cache: the paged cache of `dtype`, or
+ * with `exponents` the codes of a quantised one.  lse ([total_q, heads], may be
+ * NULL) receives the natural log of each row's sum of e^s (-inf where nothing is
+ * visible).  workspace: plan.workspace_bytes bytes, zeroed once by the caller
+ * before its first use (each call leaves its counters zero again); calls that
+ * may overlap need one each.  A kernel wait that runs out sets bit 30 of
+ * *fault_flags (device int32, may be NULL). */
+int pace_paged_attention(const pace_attention_plan* plan, const int32_t* plan_words, void* out,
+                         const void* query, int64_t query_token_stride, int64_t out_token_stride,
+                         const void* cache, const void* exponents, int64_t num_pages,
+                         float sm_scale, float logits_soft_cap, const float* alibi_slopes,
+                         const uint64_t* tree_mask, float* lse, void* workspace,
+                         size_t workspace_bytes, int32_t* fault_flags, int dtype,
+                         cudaStream_t stream);
+
 /* ---- peer access and CUDA IPC (KV promotion across processes) ----------- */
 #define PACE_IPC_HANDLE_BYTES 64
 /* Make `peer`'s memory addressable from `device` (idempotent).  New: the

@@ -35,8 +35,10 @@ pos_encoding_ops = _C.pos_encoding_ops
 activation_ops = _C.activation_ops
 moe_ops = _C.moe_ops
 kv_transfer_ops = _C.kv_transfer_ops
+attention_ops = _C.attention_ops
 
-for _name in ("layernorm_ops", "pos_encoding_ops", "activation_ops", "moe_ops", "kv_transfer_ops"):
+for _name in ("layernorm_ops", "pos_encoding_ops", "activation_ops", "moe_ops", "kv_transfer_ops",
+              "attention_ops"):
     sys.modules[f"{__name__}.{_name}"] = getattr(_C, _name)
 
 LIBRARY_PATH = os.path.join(_HERE, "libpace_b200.so")
@@ -89,6 +91,7 @@ __all__ = [
     "activation_ops",
     "moe_ops",
     "kv_transfer_ops",
+    "attention_ops",
     "install_as_paceserve",
     "fold_rmsnorm_weight",
     "set_pdl",

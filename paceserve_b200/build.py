@@ -4,7 +4,7 @@ Outputs, next to this file:
   * ``libpace_b200.so`` -- the C-ABI library (every kernel, ``include/pace_b200.h``),
     compiled with nvcc for ``sm_100a`` and linked against the static CUDA runtime;
   * ``_C.so`` -- the torch extension (pybind modules layernorm_ops, pos_encoding_ops,
-    activation_ops, moe_ops, kv_transfer_ops) that validates tensors and calls
+    activation_ops, moe_ops, kv_transfer_ops, attention_ops) that validates tensors and calls
     the C ABI; it links ``libpace_b200.so`` through ``$ORIGIN``.
 
 Objects go to ``<repo>/_build``.  Steps whose outputs are newer than every
@@ -48,6 +48,8 @@ CUDA_SOURCES = [
     "moe_kernels.cu",
     "kv_transfer_kernels.cu",
     "kv_append_kernels.cu",
+    "kv_quant_kernels.cu",
+    "attention_kernels.cu",
     "gemm_rope_kernels.cu",
     "moe_gemm_kernels.cu",
 ]

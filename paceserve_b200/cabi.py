@@ -33,6 +33,18 @@ class KvCopyOpts(ctypes.Structure):
                 ("test_overarm_bytes", c_int)]
 
 
+class AttentionPlan(ctypes.Structure):
+    """``pace_attention_plan``."""
+
+    _fields_ = [("total_q", c_int64), ("batch_size", c_int64), ("num_words", c_int64),
+                ("few_offset", c_int64), ("many_offset", c_int64), ("indices_offset", c_int64),
+                ("workspace_bytes", c_size_t)] + [
+                    (name, c_int) for name in (
+                        "num_heads", "num_kv_heads", "head_dim", "page_size", "tree_words",
+                        "num_few", "num_many", "few_slots", "many_slots", "few_tiles",
+                        "many_tiles", "max_page")]
+
+
 _P = c_void_p  # device pointer / stream
 _ACT = [_P, _P, c_int64, c_int64, c_int64, c_int64, c_int, _P]
 
@@ -131,6 +143,27 @@ SIGNATURES: dict[str, tuple] = {
         c_int,
         [_P, _P, c_int64, c_int, c_int, c_int64, c_int64, _P, _P, c_int64, c_int, _P, c_int64, _P,
          _P, c_int64, _P, c_int, _P],
+    ),
+    "pace_append_quantised_paged_kv_cache": (
+        c_int,
+        [_P, _P, c_int64, c_int, c_int, c_int64, c_int64, _P, _P, _P, c_int64, c_int, _P, c_int64,
+         _P, _P, c_int64, _P, c_int, _P],
+    ),
+    "pace_read_quantised_paged_kv_cache": (
+        c_int,
+        [_P, _P, c_int64, c_int, c_int, c_int64, c_int64, _P, _P, _P, c_int64, c_int, _P, c_int64,
+         _P, _P, c_int64, _P, c_int, _P],
+    ),
+    "pace_paged_attention_plan_words": (c_int64, [c_int64, c_int64, c_int64, c_int]),
+    "pace_paged_attention_plan": (
+        c_int,
+        [POINTER(AttentionPlan), _P, c_int64, _P, _P, _P, c_int64, _P, c_int64, c_int, c_int,
+         c_int, c_int, c_int, _P, _P, c_int, c_int],
+    ),
+    "pace_paged_attention": (
+        c_int,
+        [POINTER(AttentionPlan), _P, _P, _P, c_int64, c_int64, _P, _P, c_int64, c_float, c_float,
+         _P, _P, _P, _P, c_size_t, _P, c_int, _P],
     ),
     "pace_enable_peer_access": (c_int, [c_int, c_int]),
     "pace_can_access_peer": (c_int, [c_int, c_int, POINTER(c_int)]),

@@ -18,63 +18,19 @@
 // short index chain (request -> page table -> page), then the stores.  K/V
 // rows may be strided views of a fused qkv tensor.  A token whose request,
 // position or page is out of range is skipped and counted.
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace pace {
 namespace {
 
 constexpr int kAppendThreads = 256;
-// Requests whose per-request metadata (append_indptr, kv_indptr,
-// kv_last_page_len) each CTA stages in shared memory: 3 x 2049 x 4 B.
-constexpr int64_t kMaxStagedBatch = 2048;
-
-struct AppendJob {
+struct AppendJob : PageTable {
   int64_t nnz;
   int heads;
   int head_dim;
   int64_t key_stride;
   int64_t value_stride;
-  int64_t num_pages;
-  int page_size;
-  int64_t batch;
-  int64_t num_indices;  // entries of kv_indices
 };
-
-// Page and slot of a token of request b at sequence position pos, or false
-// if any index is out of range.  ip / last: kv_indptr and kv_last_page_len
-// (global or staged copies).  A last-page length outside [1, page_size] makes
-// the request's length inconsistent with its page count, so its tokens are
-// rejected rather than placed on a page past the request's range.
-__device__ __forceinline__ bool locate_token(const AppendJob& j, int b, int64_t pos,
-                                             const int32_t* kv_indices, const int32_t* ip,
-                                             const int32_t* last, int64_t* page, int* slot) {
-  if (b < 0 || b >= j.batch || pos < 0) return false;
-  const int64_t p0 = ip[b];
-  const int64_t np = (int64_t)ip[b + 1] - p0;
-  if (np <= 0 || p0 < 0 || p0 + np > j.num_indices) return false;
-  const int64_t lp = last[b];
-  if (lp < 1 || lp > j.page_size) return false;
-  const int64_t seq_len = (np - 1) * j.page_size + lp;
-  if (pos >= seq_len) return false;  // so pos / page_size < np
-  const int64_t pg = kv_indices[p0 + pos / j.page_size];
-  if (pg < 0 || pg >= j.num_pages) return false;
-  *page = pg;
-  *slot = (int)(pos % j.page_size);
-  return true;
-}
-
-// Request of token i from append_indptr (ascending, batch + 1 entries).
-__device__ __forceinline__ int find_request(const int32_t* indptr, int64_t batch, int64_t i) {
-  int lo = 0, hi = (int)batch - 1;  // largest b with indptr[b] <= i
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (indptr[mid] <= i)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
-}
 
 // BY_INDPTR: derive (request, position) from append_indptr; otherwise read
 // batch_indices / positions.  VEC: 16-byte vectors; otherwise elements.
@@ -183,8 +139,8 @@ int run_append(const void* key, const void* value, int64_t nnz, int heads, int h
       (BY_INDPTR ? !append_indptr : (!batch_indices || !positions)))
     return fail(PACE_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   StreamDeviceGuard guard(stream);
-  AppendJob job{nnz, heads, head_dim, key_stride, value_stride, num_pages, page_size, batch,
-                num_indices};
+  AppendJob job{{num_pages, page_size, batch, num_indices}, nnz, heads, head_dim, key_stride,
+                value_stride};
   const bool staged = batch <= kMaxStagedBatch;
   const size_t smem = staged ? (size_t)(3 * batch + 2) * 4 : 0;
   return PACE_DISPATCH_FLOAT(dtype, what, [&] {

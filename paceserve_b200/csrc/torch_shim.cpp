@@ -4,8 +4,9 @@
 // csrc/activation.cpp:3-28, csrc/moe.cpp:3-28) as submodules
 // layernorm_ops / pos_encoding_ops / activation_ops / moe_ops of
 // paceserve_b200._C, adds the new ops (fused_add_rms_norm, gelu_and_mul,
-// gelu_tanh_and_mul) in the same style, and a kv_transfer_ops submodule for
-// the paged-KV block copy.  Tensors are validated here; every launch goes
+// gelu_tanh_and_mul) in the same style, a kv_transfer_ops submodule for the
+// paged-KV block copy, append and quantised cache, and an attention_ops
+// submodule for paged attention.  Tensors are validated here; every launch goes
 // through the C ABI on the current stream of the tensors' device, and a
 // non-zero status becomes a RuntimeError carrying pace_last_error().
 #include <ATen/cuda/CUDAContext.h>
@@ -923,6 +924,206 @@ void append_paged_kv_cache_by_indptr(const Tensor& append_key, const Tensor& app
                op);
 }
 
+// -------------------------------------------------- quantised paged KV cache --
+struct QuantisedCache {
+  PagedCache pc;
+  void* codes;
+  void* exponents;
+};
+
+QuantisedCache quantised_cache_of(const Tensor& codes, const Tensor& exponents, const char* op) {
+  const PagedCache pc = paged_cache_of(codes, "NHD", op);
+  TORCH_CHECK(codes.scalar_type() == at::kFloat8_e4m3fn, op, ": codes must be float8_e4m3fn");
+  TORCH_CHECK(exponents.device() == codes.device() && exponents.scalar_type() == at::kByte &&
+                  exponents.dim() == 4 && exponents.is_contiguous() &&
+                  exponents.sizes() == codes.sizes().slice(0, 4),
+              op, ": exponents must be a contiguous uint8 tensor [pages, 2, page_size, kv_heads] "
+              "on the codes' device");
+  return {pc, codes.data_ptr(), exponents.data_ptr()};
+}
+
+template <typename Fn>
+void quantised_cache_op(Fn fn, const char* op, const Tensor& key, const Tensor& value,
+                        const Tensor& indptr, const Tensor& codes, const Tensor& exponents,
+                        const Tensor& kv_indices, const Tensor& kv_indptr,
+                        const Tensor& kv_last_page_len, const c10::optional<Tensor>& bad_tokens) {
+  const QuantisedCache q = quantised_cache_of(codes, exponents, op);
+  check_same_device(key, codes, op);
+  check_same_device(value, codes, op);
+  TORCH_CHECK(is_float_type(key) && key.scalar_type() == value.scalar_type(), op,
+              ": key and value must share one of float32, float16 and bfloat16");
+  const int64_t ks = kv_row_stride(key, q.pc.heads, q.pc.hd, op, "key");
+  const int64_t vs = kv_row_stride(value, q.pc.heads, q.pc.hd, op, "value");
+  const int64_t rows = key.size(0);
+  TORCH_CHECK(value.size(0) == rows, op, ": key and value token counts differ");
+  Tensor ai = int32_on(indptr, codes, op, "indptr");
+  Tensor ki = int32_on(kv_indices, codes, op, "kv_indices");
+  Tensor kp = int32_on(kv_indptr, codes, op, "kv_indptr");
+  Tensor kl = int32_on(kv_last_page_len, codes, op, "kv_last_page_len");
+  TORCH_CHECK(ai.numel() == kp.numel() && kl.numel() >= kp.numel() - 1 && kp.numel() >= 1, op,
+              ": the token indptr and kv_indptr need batch + 1 entries, kv_last_page_len batch");
+  int32_t* bad = counter_ptr(bad_tokens, codes.device(), op, "bad_tokens");
+  const at::cuda::CUDAGuard guard(codes.device());
+  check_status(fn(key.data_ptr(), value.data_ptr(), rows, (int)q.pc.heads, (int)q.pc.hd, ks, vs,
+                  ai.data_ptr<int32_t>(), q.codes, q.exponents, q.pc.pages, (int)q.pc.page_size,
+                  ki.data_ptr<int32_t>(), ki.numel(), kp.data_ptr<int32_t>(),
+                  kl.data_ptr<int32_t>(), kp.numel() - 1, bad, pace_dtype(key), stream_of(codes)),
+               op);
+}
+
+void append_quantised_paged_kv_cache(const Tensor& append_key, const Tensor& append_value,
+                                     const Tensor& append_indptr, Tensor& codes, Tensor& exponents,
+                                     const Tensor& kv_indices, const Tensor& kv_indptr,
+                                     const Tensor& kv_last_page_len,
+                                     const c10::optional<Tensor>& bad_tokens) {
+  quantised_cache_op(pace_append_quantised_paged_kv_cache, "append_quantised_paged_kv_cache",
+                     append_key, append_value, append_indptr, codes, exponents, kv_indices,
+                     kv_indptr, kv_last_page_len, bad_tokens);
+}
+
+void read_quantised_paged_kv_cache(Tensor& key, Tensor& value, const Tensor& out_indptr,
+                                   const Tensor& codes, const Tensor& exponents,
+                                   const Tensor& kv_indices, const Tensor& kv_indptr,
+                                   const Tensor& kv_last_page_len,
+                                   const c10::optional<Tensor>& bad_tokens) {
+  quantised_cache_op(pace_read_quantised_paged_kv_cache, "read_quantised_paged_kv_cache", key,
+                     value, out_indptr, codes, exponents, kv_indices, kv_indptr, kv_last_page_len,
+                     bad_tokens);
+}
+
+// ------------------------------------------------------------ paged attention --
+// A planned step: the C struct and its words in host memory (page-locked where
+// a GPU is present, so that the copy to the device need not be waited for).
+struct AttentionPlan {
+  pace_attention_plan plan{};
+  Tensor words;
+};
+
+const int32_t* host_ints(const c10::optional<Tensor>& t, int64_t n, const char* name, Tensor* keep) {
+  const char* op = "plan_paged_attention";
+  if (!t.has_value()) return nullptr;
+  TORCH_CHECK(t->is_cpu() && t->scalar_type() == at::kInt && t->dim() == 1 && t->numel() >= n, op,
+              ": ", name, " must be a 1-D int32 CPU tensor of at least ", n, " entries");
+  *keep = t->contiguous();
+  return keep->data_ptr<int32_t>();
+}
+
+AttentionPlan plan_paged_attention(const Tensor& qo_indptr, const Tensor& kv_indptr,
+                                   const Tensor& kv_indices, const Tensor& kv_last_page_len,
+                                   int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                                   int64_t page_size, int64_t window_left,
+                                   const c10::optional<Tensor>& prefix_lens,
+                                   const c10::optional<Tensor>& doc_starts, int64_t tree_words,
+                                   int64_t num_sms) {
+  const char* op = "plan_paged_attention";
+  TORCH_CHECK(qo_indptr.dim() == 1 && qo_indptr.numel() >= 1 &&
+                  qo_indptr.numel() == kv_indptr.numel(),
+              op, ": qo_indptr and kv_indptr need batch + 1 entries");
+  const int64_t batch = qo_indptr.numel() - 1;
+  for (int64_t v : {num_heads, num_kv_heads, head_dim, page_size, window_left, tree_words, num_sms})
+    TORCH_CHECK(v >= INT32_MIN && v <= INT32_MAX, op, ": argument out of range");
+  Tensor keep[6];
+  const int32_t* qo = host_ints(qo_indptr, batch + 1, "qo_indptr", &keep[0]);
+  const int32_t* kp = host_ints(kv_indptr, batch + 1, "kv_indptr", &keep[1]);
+  const int32_t* ki = host_ints(kv_indices, 0, "kv_indices", &keep[2]);
+  const int32_t* kl = host_ints(kv_last_page_len, batch, "kv_last_page_len", &keep[3]);
+  const int64_t total_q = qo[batch];
+  TORCH_CHECK(total_q >= 0, op, ": qo_indptr must be ascending");
+  const int32_t* pl = host_ints(prefix_lens, batch, "prefix_lens", &keep[4]);
+  const int32_t* ds = host_ints(doc_starts, total_q, "doc_starts", &keep[5]);
+  const int64_t words =
+      pace_paged_attention_plan_words(batch, total_q, kv_indices.numel(), (int)num_sms);
+  AttentionPlan p;
+  p.words = torch::empty({words}, torch::TensorOptions().dtype(torch::kInt32).pinned_memory(
+                                      at::cuda::is_available()));
+  check_status(pace_paged_attention_plan(&p.plan, p.words.data_ptr<int32_t>(), words, qo, kp, ki,
+                                         kv_indices.numel(), kl, batch, (int)num_heads,
+                                         (int)num_kv_heads, (int)head_dim, (int)page_size,
+                                         (int)window_left, pl, ds, (int)tree_words, (int)num_sms),
+               op);
+  p.words = p.words.narrow(0, 0, p.plan.num_words);
+  return p;
+}
+
+int64_t heads_stride(const Tensor& t, int64_t heads, int64_t hd, const char* op, const char* name) {
+  TORCH_CHECK(t.dim() == 3 && t.size(1) == heads && t.size(2) == hd, op, ": ", name, " must be [",
+              "tokens, ", heads, ", ", hd, "]");
+  TORCH_CHECK((hd <= 1 || t.stride(2) == 1) && (heads <= 1 || t.stride(1) == hd), op, ": ", name,
+              " heads must be contiguous");
+  return t.size(0) <= 1 ? heads * hd : t.stride(0);
+}
+
+void paged_attention(Tensor& out, const Tensor& query, const Tensor& paged_kv_cache,
+                     const AttentionPlan& plan, const Tensor& plan_words, const Tensor& workspace,
+                     double sm_scale, double logits_soft_cap,
+                     const c10::optional<Tensor>& exponents,
+                     const c10::optional<Tensor>& alibi_slopes,
+                     const c10::optional<Tensor>& tree_mask, const c10::optional<Tensor>& lse,
+                     const c10::optional<Tensor>& fault_flags) {
+  const char* op = "paged_attention";
+  const pace_attention_plan& pl = plan.plan;
+  check_cuda(query, op, "query");
+  check_same_device(out, query, op);
+  check_same_device(paged_kv_cache, query, op);
+  TORCH_CHECK(is_float_type(query) && out.scalar_type() == query.scalar_type(), op,
+              ": query and out must share one of float32, float16 and bfloat16");
+  const PagedCache pc = paged_cache_of(paged_kv_cache, "NHD", op);
+  TORCH_CHECK(pc.heads == pl.num_kv_heads && pc.hd == pl.head_dim && pc.page_size == pl.page_size,
+              op, ": the cache's pages [", pc.page_size, ", ", pc.heads, ", ", pc.hd,
+              "] are not the plan's");
+  if (exponents.has_value())
+    quantised_cache_of(paged_kv_cache, *exponents, op);
+  else
+    TORCH_CHECK(paged_kv_cache.scalar_type() == query.scalar_type(), op,
+                ": the cache must have the query's dtype, or be float8_e4m3fn codes with exponents");
+  TORCH_CHECK(query.size(0) == pl.total_q && out.size(0) == pl.total_q, op, ": the plan is for ",
+              pl.total_q, " tokens");
+  const int64_t qs = heads_stride(query, pl.num_heads, pl.head_dim, op, "query");
+  const int64_t os = heads_stride(out, pl.num_heads, pl.head_dim, op, "out");
+  TORCH_CHECK(plan_words.device() == query.device() && plan_words.scalar_type() == at::kInt &&
+                  plan_words.is_contiguous() && plan_words.numel() >= pl.num_words,
+              op, ": plan_words must hold the plan's words on the query's device");
+  TORCH_CHECK(workspace.device() == query.device() && workspace.scalar_type() == at::kByte &&
+                  workspace.is_contiguous(),
+              op, ": workspace must be a contiguous uint8 tensor on the query's device");
+  const float* slopes = nullptr;
+  if (alibi_slopes.has_value()) {
+    TORCH_CHECK(alibi_slopes->device() == query.device() &&
+                    alibi_slopes->scalar_type() == at::kFloat && alibi_slopes->is_contiguous() &&
+                    alibi_slopes->numel() == pl.num_heads,
+                op, ": alibi_slopes must be a float32 tensor [", pl.num_heads, "] on the query's "
+                "device");
+    slopes = alibi_slopes->data_ptr<float>();
+  }
+  const uint64_t* bits = nullptr;
+  if (tree_mask.has_value()) {
+    TORCH_CHECK(tree_mask->device() == query.device() && tree_mask->scalar_type() == at::kLong &&
+                    tree_mask->is_contiguous() && tree_mask->dim() == 2 &&
+                    tree_mask->size(0) == pl.total_q && tree_mask->size(1) == pl.tree_words,
+                op, ": tree_mask must be a contiguous int64 tensor [", pl.total_q, ", ",
+                pl.tree_words, "] on the query's device");
+    bits = reinterpret_cast<const uint64_t*>(tree_mask->data_ptr<int64_t>());
+  }
+  float* lse_ptr = nullptr;
+  if (lse.has_value()) {
+    TORCH_CHECK(lse->device() == query.device() && lse->scalar_type() == at::kFloat &&
+                    lse->is_contiguous() && lse->dim() == 2 && lse->size(0) == pl.total_q &&
+                    lse->size(1) == pl.num_heads,
+                op, ": lse must be a contiguous float32 tensor [", pl.total_q, ", ", pl.num_heads,
+                "] on the query's device");
+    lse_ptr = lse->data_ptr<float>();
+  }
+  int32_t* fault = counter_ptr(fault_flags, query.device(), op, "fault_flags");
+  const at::cuda::CUDAGuard guard(query.device());
+  check_status(pace_paged_attention(&pl, plan_words.data_ptr<int32_t>(), out.data_ptr(),
+                                    query.data_ptr(), qs, os, paged_kv_cache.data_ptr(),
+                                    exponents.has_value() ? exponents->data_ptr() : nullptr,
+                                    pc.pages, (float)sm_scale, (float)logits_soft_cap, slopes, bits,
+                                    lse_ptr, workspace.data_ptr(), (size_t)workspace.numel(), fault,
+                                    pace_dtype(query), stream_of(query)),
+               op);
+}
+
 py::tuple ipc_get_handle(const Tensor& t) {
   TORCH_CHECK(t.is_cuda(), "ipc_get_handle: tensor must be on a CUDA device");
   const at::cuda::CUDAGuard guard(t.device());
@@ -1050,6 +1251,32 @@ PYBIND11_MODULE(_C, m) {
           py::arg("topk_weights") = py::none(), py::arg("mode") = 0,
           py::arg("fault_flags") = py::none());
 
+  auto at_ = m.def_submodule("attention_ops");
+  py::class_<AttentionPlan>(at_, "AttentionPlan")
+      .def_property_readonly("words", [](const AttentionPlan& p) { return p.words; })
+      .def_property_readonly("total_q", [](const AttentionPlan& p) { return p.plan.total_q; })
+      .def_property_readonly("workspace_bytes",
+                             [](const AttentionPlan& p) { return p.plan.workspace_bytes; })
+      .def_property_readonly("num_few", [](const AttentionPlan& p) { return p.plan.num_few; })
+      .def_property_readonly("num_many", [](const AttentionPlan& p) { return p.plan.num_many; })
+      .def_property_readonly("few_slots", [](const AttentionPlan& p) { return p.plan.few_slots; })
+      .def_property_readonly("many_slots",
+                             [](const AttentionPlan& p) { return p.plan.many_slots; });
+  at_.def("plan_paged_attention", &plan_paged_attention,
+          "Plan one step's attention from its host metadata (int32 CPU tensors).",
+          py::arg("qo_indptr"), py::arg("kv_indptr"), py::arg("kv_indices"),
+          py::arg("kv_last_page_len"), py::arg("num_heads"), py::arg("num_kv_heads"),
+          py::arg("head_dim"), py::arg("page_size"), py::arg("window_left") = -1,
+          py::arg("prefix_lens") = py::none(), py::arg("doc_starts") = py::none(),
+          py::arg("tree_words") = 0, py::arg("num_sms") = 148);
+  at_.def("paged_attention", &paged_attention,
+          "Attention of a planned step over a paged KV cache (16-bit, float32 or quantised).",
+          py::arg("out"), py::arg("query"), py::arg("paged_kv_cache"), py::arg("plan"),
+          py::arg("plan_words"), py::arg("workspace"), py::arg("sm_scale"),
+          py::arg("logits_soft_cap") = 0.0, py::arg("exponents") = py::none(),
+          py::arg("alibi_slopes") = py::none(), py::arg("tree_mask") = py::none(),
+          py::arg("lse") = py::none(), py::arg("fault_flags") = py::none());
+
   auto kv = m.def_submodule("kv_transfer_ops");
   kv.def("copy_blocks_p2p", &copy_blocks_p2p,
          "Copy KV blocks src_block_ids of src_caches onto dst_block_ids of dst_caches "
@@ -1082,6 +1309,17 @@ PYBIND11_MODULE(_C, m) {
          py::arg("append_key"), py::arg("append_value"), py::arg("append_indptr"),
          py::arg("paged_kv_cache"), py::arg("kv_indices"), py::arg("kv_indptr"),
          py::arg("kv_last_page_len"), py::arg("bad_tokens") = py::none());
+  kv.def("append_quantised_paged_kv_cache", &append_quantised_paged_kv_cache,
+         "Quantise K/V rows of new tokens (e4m3 codes, one power-of-two exponent per row and head) "
+         "and append them to a paged cache of codes and exponents.",
+         py::arg("append_key"), py::arg("append_value"), py::arg("append_indptr"),
+         py::arg("codes"), py::arg("exponents"), py::arg("kv_indices"), py::arg("kv_indptr"),
+         py::arg("kv_last_page_len"), py::arg("bad_tokens") = py::none());
+  kv.def("read_quantised_paged_kv_cache", &read_quantised_paged_kv_cache,
+         "Read requests' rows of a quantised paged cache back in sequence order.", py::arg("key"),
+         py::arg("value"), py::arg("out_indptr"), py::arg("codes"), py::arg("exponents"),
+         py::arg("kv_indices"), py::arg("kv_indptr"), py::arg("kv_last_page_len"),
+         py::arg("bad_tokens") = py::none());
   kv.def("ipc_get_handle", &ipc_get_handle, py::arg("tensor"));
   kv.def("ipc_open_handle", &ipc_open_handle, py::arg("handle"), py::arg("device"));
   kv.def("ipc_close_handle", &ipc_close_handle, py::arg("base"));
