@@ -50,6 +50,7 @@ CUDA_SOURCES = [
     "kv_append_kernels.cu",
     "kv_quant_kernels.cu",
     "attention_kernels.cu",
+    "attention_few_kernels.cu",
     "gemm_rope_kernels.cu",
     "moe_gemm_kernels.cu",
 ]

@@ -1,0 +1,431 @@
+// Paged attention of few query rows: a request's new tokens times the query
+// heads of one kv head, at most 16 rows (single tokens of grouped heads, short
+// drafts).  Every key and value is read once for so few products that memory
+// bounds it: the 16 x 8 x 16 matrix instructions of a warp are enough, and
+// what counts is the bytes in flight.
+//
+// A CTA takes one piece of the plan (keys [kv_begin, kv_end) of one request)
+// for one kv head.  Its four warps walk the keys in turns of KEYS each, every
+// warp on its own: it copies its keys' K and V rows page by page into its own
+// ring of STAGES slots (cp.async, no barrier between warps), multiplies them
+// with the queries that sit in registers, and keeps the running maximum m, sum
+// l and unnormalised output of its keys in registers, all fp32.  The warps'
+// results are joined at the end:
+//   M = max m_w,  o = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w.
+// Pieces of the same rows leave (m, l, o) in the workspace; the last to arrive
+// joins them in the same way, in piece order, so results do not depend on the
+// order of arrival.
+//
+// A quantised cache is copied as it is and unpacked between shared memory and
+// the matrix instruction: an e4m3 code moved to the top of the target type's
+// bits is the code's value times a power of two (2^-120 in bf16, 2^-8 in fp16),
+// subnormals included, so one multiplication restores it exactly.
+#include "attention.cuh"
+#include "attention_mma.cuh"
+
+namespace pace {
+namespace attn {
+
+constexpr int kFewWarps = 4;
+
+template <int D, bool Q8>
+struct FewTile {
+  static constexpr int kKeys = D == 128 && !Q8 ? 16 : 32;  // of a warp's turn
+  static constexpr int kRowBytes = Q8 ? D : 2 * D;
+  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kKvBytes = kKeys * kRowBytes;
+  static constexpr int kStages = 3;
+  static constexpr int kRingBytes = kStages * 2 * kKvBytes;
+  static constexpr int kJoinBytes = 16 * D * 4;  // a warp's output, over its ring
+  static constexpr int kWarpBytes = kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes;
+  static constexpr int kFactorBytes = Q8 ? kStages * 2 * kKeys * 4 : 0;
+  static constexpr int kSmemBytes = kFewWarps * (kWarpBytes + kFactorBytes) + kFewWarps * 32 * 4;
+  // 16-byte chunk c of row r, placed so that eight rows' same chunk, and one
+  // row's eight chunks, lie in different banks
+  __device__ static __forceinline__ int at(int r, int c) {
+    const int x = kChunks >= 8 ? (r & 7) : ((r >> 1) & 3);
+    return r * kRowBytes + ((c ^ x) << 4);
+  }
+};
+
+template <typename T, int D, bool Q8>
+__global__ void __launch_bounds__(kFewWarps * 32, 2)
+    attention_few_kernel(const Problem p, const Item* __restrict__ items, float* partial,
+                         float2* partial_ml, int32_t* counters, bool q_even) {
+  using Tile = FewTile<D, Q8>;
+  using M = Mma<T>;
+  constexpr int KEYS = Tile::kKeys, NT = KEYS / 8, KB = D / 16, STAGES = Tile::kStages;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  const int kvh = blockIdx.x % p.kv_heads;
+  const Item w = items[blockIdx.x / p.kv_heads];
+  const int group = p.heads / p.kv_heads;
+  const int rows = w.ntok * group;
+  uint8_t* ring = smem + warp * Tile::kWarpBytes;
+  float* factors = reinterpret_cast<float*>(smem + kFewWarps * Tile::kWarpBytes +
+                                            warp * Tile::kFactorBytes);
+  float* join_ml = reinterpret_cast<float*>(
+      smem + kFewWarps * (Tile::kWarpBytes + Tile::kFactorBytes));  // [warp][16][m, l]
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- rows g and g + 8 of this thread: visible keys, slope, queries --------
+  int lo[2], hi[2], pos[2];
+  float slope[2];
+  const uint64_t* bits[2] = {nullptr, nullptr};
+  int all_lo = 0, all_hi = INT32_MAX;  // keys that every row sees
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = g + 8 * i;
+    lo[i] = 0;
+    hi[i] = INT32_MAX;
+    pos[i] = 0;
+    slope[i] = 0.f;
+    if (r < rows) {
+      const int tok = w.tok0 + r / group;
+      const TokenInfo t = p.tokens[tok];
+      lo[i] = t.lo;
+      hi[i] = t.hi;
+      pos[i] = t.pos;
+      if (p.slopes) slope[i] = p.slopes[kvh * group + r % group] * kLog2e;
+      if (p.tree_mask) bits[i] = p.tree_mask + (int64_t)tok * p.tree_words;
+      all_lo = max(all_lo, lo[i]);
+      all_hi = min(all_hi, hi[i]);
+    }
+  }
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) {
+    all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, o));
+    all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, o));
+  }
+  uint32_t qf[KB][4];
+  {
+    const T* q[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = g + 8 * i;
+      q[i] = r < rows ? static_cast<const T*>(p.query) + (int64_t)(w.tok0 + r / group) * p.q_stride +
+                            (int64_t)(kvh * group + r % group) * D
+                      : nullptr;
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const T* row = q[i & 1];
+        // the two dimensions of this register: those that the keys' register of the same
+        // index holds (a quantised key's registers hold bytes 0, 2 and 1, 3 of four)
+        const int d0 = Q8 ? kb * 16 + 4 * c + (i >> 1) : kb * 16 + 2 * c + 8 * (i >> 1);
+        const int d1 = d0 + (Q8 ? 2 : 1);
+        if (!row)
+          qf[kb][i] = 0;
+        else if (!Q8 && q_even)
+          qf[kb][i] = *reinterpret_cast<const uint32_t*>(row + d0);
+        else
+          qf[kb][i] = M::pair(row[d0], row[d1]);
+      }
+  }
+
+  // ---- the ring ---------------------------------------------------------------
+  const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
+  const int64_t v_rows = (int64_t)p.page_size * p.kv_heads;
+  const int begin = w.kv_begin + warp * KEYS;
+  const int steps = begin < w.kv_end ? (w.kv_end - begin + kFewWarps * KEYS - 1) / (kFewWarps * KEYS) : 0;
+  const int my_key = lane % KEYS;
+  auto page_of = [&](int step) -> int {
+    const int j = begin + step * kFewWarps * KEYS + my_key;
+    return step < steps && j < w.kv_end ? p.kv_indices[w.page_base + j / p.page_size] : -1;
+  };
+  // row number (of the whole cache, K part) of this lane's key of a step
+  auto row_of = [&](int step, int page) -> uint32_t {
+    const int j = begin + step * kFewWarps * KEYS + my_key;
+    return (uint32_t)(((int64_t)page * 2 * p.page_size + j % p.page_size) * p.kv_heads + kvh);
+  };
+  uint32_t ex = 0;  // exponents (K | V << 8) of this lane's key of the step issued last
+  auto issue = [&](int step, int page) {
+    const uint32_t row = page >= 0 ? row_of(step, page) : 0;
+    uint8_t* slot = ring + (step % STAGES) * 2 * Tile::kKvBytes;
+#pragma unroll
+    for (int i = 0; i < KEYS * Tile::kChunks / 32; ++i) {
+      const int r = (i * 32 + lane) / Tile::kChunks, ch = (i * 32 + lane) % Tile::kChunks;
+      const uint32_t src_row = __shfl_sync(0xffffffffu, row, r);
+      const bool there = __shfl_sync(0xffffffffu, page, r) >= 0;
+      const uint8_t* k = cache + (int64_t)src_row * Tile::kRowBytes + ch * 16;
+      const int at = Tile::at(r, ch);
+      cp_async16(slot + at, k, there);
+      cp_async16(slot + Tile::kKvBytes + at, k + (there ? v_rows * Tile::kRowBytes : 0), there);
+    }
+    if constexpr (Q8) {
+      ex = 0;
+      if (page >= 0)
+        ex = (uint32_t)p.exponents[row] | (uint32_t)p.exponents[row + v_rows] << 8;
+    }
+  };
+  auto put_factors = [&](int step) {
+    if constexpr (Q8) {
+      float* f = factors + (step % STAGES) * 2 * KEYS;
+      f[lane] = exponent_factor(ex & 0xff);
+      f[KEYS + lane] = exponent_factor(ex >> 8);
+    }
+  };
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const float scale2 = p.scale * kLog2e;
+  const float cap2 = p.cap * kLog2e, cap_in = p.cap > 0.f ? 2.f * scale2 / p.cap : 0.f;
+
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    issue(s, page_of(s));
+    put_factors(s);
+    cp_async_commit();
+  }
+  int page = page_of(STAGES - 1);
+  for (int step = 0; step < steps; ++step) {
+    if (step > 0) put_factors(step + STAGES - 2);  // their loads had a step's time
+    issue(step + STAGES - 1, page);
+    cp_async_commit();
+    page = page_of(step + STAGES);
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const uint8_t* ks = ring + (step % STAGES) * 2 * Tile::kKvBytes;
+    const uint8_t* vs = ks + Tile::kKvBytes;
+    const float* kf = factors + (step % STAGES) * 2 * KEYS;
+    const float* vf = kf + KEYS;
+    // ---- S = Q K^T ------------------------------------------------------------
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      if constexpr (Q8) {
+        uint32_t r[4];
+        ldmatrix4(r, ks + Tile::at(lane, kb));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint32_t b0, b1;
+          M::unpack_codes(r[n], b0, b1);
+          M::mma(s[n], qf[kb], M::code_scale(b0), M::code_scale(b1));
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          uint32_t r[4];
+          ldmatrix4(r, ks + Tile::at(n * 8 + (lane >> 4) * 8 + (lane & 7), 2 * kb + ((lane >> 3) & 1)));
+          M::mma(s[n], qf[kb], r[0], r[1]);
+          M::mma(s[n + 1], qf[kb], r[2], r[3]);
+        }
+      }
+    }
+    // ---- scores in powers of two, masks ---------------------------------------
+    const int j0 = begin + step * kFewWarps * KEYS;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = s[n][e];
+        if constexpr (Q8) x *= kf[n * 8 + 2 * c + (e & 1)];
+        if (p.cap > 0.f)
+          x = cap2 - 2.f * cap2 * rcp_approx(1.f + exp2_approx(x * cap_in));  // cap tanh
+        else
+          x *= scale2;
+        if (p.slopes) x -= slope[e >> 1] * fabsf((float)(pos[e >> 1] - (j0 + n * 8 + 2 * c + (e & 1))));
+        s[n][e] = x;
+      }
+    if (j0 < all_lo || j0 + KEYS > min(all_hi, w.kv_end)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + n * 8 + 2 * c + (e & 1), i = e >> 1;
+          bool see = j >= lo[i] && j < hi[i] && j < w.kv_end;
+          if (bits[i] && j >= hi[i]) see = j < min(pos[i], w.kv_end) && tree_bit(bits[i], j - hi[i]);
+          if (!see) s[n][e] = -INFINITY;
+        }
+    }
+    // ---- running maximum and sum ----------------------------------------------
+    float base[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float t = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) t = fmaxf(t, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      const float m2 = fmaxf(m[i], t);
+      base[i] = m2 == -INFINITY ? 0.f : m2;
+      if (__any_sync(0xffffffffu, m2 > m[i])) {
+        const float f = exp2_approx(m[i] - base[i]);  // 0 while m is -inf
+        l[i] *= f;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          o[n][2 * i] *= f;
+          o[n][2 * i + 1] *= f;
+        }
+      }
+      m[i] = m2;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = exp2_approx(s[n][e] - base[e >> 1]);
+        l[e >> 1] += x;
+        s[n][e] = x;
+      }
+    // ---- O += P V; P is rounded to T, the one rounding before the output's ----
+#pragma unroll
+    for (int kg = 0; kg < NT / 2; ++kg) {
+      uint32_t a[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = s[2 * kg + (i >> 1)][2 * (i & 1)], y = s[2 * kg + (i >> 1)][2 * (i & 1) + 1];
+        if constexpr (Q8 && M::kWideRange) {
+          // V's factors are powers of two: bf16 takes them on P without loss.  A key that the
+          // row does not see stays 0 whatever its row holds.
+          const int j = kg * 16 + (i >> 1) * 8 + 2 * c;
+          x = x == 0.f ? 0.f : x * vf[j];
+          y = y == 0.f ? 0.f : y * vf[j + 1];
+        }
+        a[i] = M::pack(x, y);
+      }
+      if constexpr (Q8) {
+        uint32_t f0 = 0, f1 = 0, g0 = 0, g1 = 0;
+        if constexpr (!M::kWideRange) {
+          const int j = kg * 16 + 2 * c;
+          M::split_factors(vf[j], vf[j + 1], f0, g0);
+          M::split_factors(vf[j + 8], vf[j + 9], f1, g1);
+        }
+#pragma unroll
+        for (int ch = 0; ch < D / 16; ch += 2) {
+          uint32_t r[4];
+          // keys kg * 16 + 0-7, 8-15 of chunks ch, ch + 1
+          ldmatrix4_trans(r, vs + Tile::at(kg * 16 + (lane & 15), ch + (lane >> 4)));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t e0, d0, e1, d1;
+            M::unpack_codes(r[2 * h], e0, d0);
+            M::unpack_codes(r[2 * h + 1], e1, d1);
+            if constexpr (M::kWideRange) {
+              M::mma(o[2 * (ch + h)], a, M::code_scale(e0), M::code_scale(e1));
+              M::mma(o[2 * (ch + h) + 1], a, M::code_scale(d0), M::code_scale(d1));
+            } else {
+              M::mma(o[2 * (ch + h)], a, M::scale2(e0, f0, g0), M::scale2(e1, f1, g1));
+              M::mma(o[2 * (ch + h) + 1], a, M::scale2(d0, f0, g0), M::scale2(d1, f1, g1));
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int ch = 0; ch < D / 8; ch += 2) {
+          uint32_t r[4];
+          ldmatrix4_trans(r, vs + Tile::at(kg * 16 + (lane & 15), ch + (lane >> 4)));
+          M::mma(o[ch], a, r[0], r[1]);
+          M::mma(o[ch + 1], a, r[2], r[3]);
+        }
+      }
+    }
+    __syncwarp();  // the slot is free for the copies of the next turn
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // ---- join the warps ----------------------------------------------------------
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    const int r = g + 8 * i;
+    if (r < rows) {
+      if (c == 0) {
+        join_ml[(warp * 16 + r) * 2] = m[i];
+        join_ml[(warp * 16 + r) * 2 + 1] = l[i];
+      }
+      float* dst = reinterpret_cast<float*>(ring) + r * D;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        const int d = Q8 ? (n >> 1) * 16 + 4 * c + (n & 1) : n * 8 + 2 * c;
+        dst[d] = o[n][2 * i];
+        dst[d + (Q8 ? 2 : 1)] = o[n][2 * i + 1];
+      }
+    }
+  }
+  __syncthreads();
+  constexpr int V4 = D / 4;
+  const int64_t slot = (int64_t)(w.slot + w.split) * p.kv_heads + kvh;
+  for (int u = threadIdx.x; u < rows * V4; u += kFewWarps * 32) {
+    const int r = u / V4, d = (u - r * V4) * 4;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kFewWarps; ++k) mm = fmaxf(mm, join_ml[(k * 16 + r) * 2]);
+    const float b = mm == -INFINITY ? 0.f : mm;
+    float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kFewWarps; ++k) {
+      const float f = exp2_approx(join_ml[(k * 16 + r) * 2] - b);
+      sum += f * join_ml[(k * 16 + r) * 2 + 1];
+      const float4 x = *reinterpret_cast<const float4*>(smem + k * Tile::kWarpBytes + (r * D + d) * 4);
+      v[0] += f * x.x;
+      v[1] += f * x.y;
+      v[2] += f * x.z;
+      v[3] += f * x.w;
+    }
+    if (w.splits == 1) {
+      write_out<T>(p, w.tok0 + r / group, kvh * group + r % group, d, v, mm, sum);
+    } else {
+      __stcg(reinterpret_cast<float4*>(partial + (slot * 16 + r) * D + d),
+             make_float4(v[0], v[1], v[2], v[3]));
+      if (d == 0) __stcg(partial_ml + slot * 16 + r, make_float2(mm, sum));
+    }
+  }
+  if (w.splits == 1) return;
+
+  // ---- the last piece of these rows to arrive joins them all --------------------
+  __shared__ bool last;
+  if (!arrive_last(counters + (int64_t)w.tile * p.kv_heads + kvh, w.splits, &last)) return;
+  for (int u = threadIdx.x; u < rows * V4; u += kFewWarps * 32) {
+    const int r = u / V4, d = (u - r * V4) * 4;
+    join_pieces<T, 16>(p, partial, partial_ml, w, kvh, r, d, D, group);
+  }
+}
+
+template <typename T, int D, bool Q8>
+static int run_few(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+                   int32_t* counters, int device, cudaStream_t stream, const char* what) {
+  using Tile = FewTile<D, Q8>;
+  auto kernel = attention_few_kernel<T, D, Q8>;
+  cudaError_t err =
+      ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), device, Tile::kSmemBytes);
+  if (err != cudaSuccess) return cuda_fail(err, what);
+  const bool even = (reinterpret_cast<uintptr_t>(p.query) & 3) == 0 && p.q_stride % 2 == 0;
+  err = launch(kernel, dim3((unsigned)(num_items * p.kv_heads)), dim3(kFewWarps * 32),
+               Tile::kSmemBytes, stream, p, items, partial, ml, counters, even);
+  return err == cudaSuccess ? PACE_OK : cuda_fail(err, what);
+}
+
+int run_few_rows(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+                 int32_t* counters, bool bf16, int device, cudaStream_t stream, const char* what) {
+  auto pick = [&](auto t) -> int {
+    using T = decltype(t);
+    if (p.head_dim == 128)
+      return p.exponents ? run_few<T, 128, true>(p, items, num_items, partial, ml, counters, device,
+                                                 stream, what)
+                         : run_few<T, 128, false>(p, items, num_items, partial, ml, counters, device,
+                                                  stream, what);
+    return p.exponents ? run_few<T, 64, true>(p, items, num_items, partial, ml, counters, device,
+                                              stream, what)
+                       : run_few<T, 64, false>(p, items, num_items, partial, ml, counters, device,
+                                               stream, what);
+  };
+  return bf16 ? pick(__nv_bfloat16{}) : pick(__half{});
+}
+
+}  // namespace attn
+}  // namespace pace

@@ -13,7 +13,7 @@
 #include <exception>
 #include <vector>
 
-#include "attention.cuh"
+#include "attention_mma.cuh"
 
 namespace pace {
 namespace attn {
@@ -123,9 +123,14 @@ constexpr int kTileMinUnits = 4;
 constexpr int kPiecesPerSlot = 3;
 constexpr int kFewCtasPerSm = 2;
 
-// Cuts pieces longer than the even share of a slot, and orders all longest
-// first.  Returns the number of partial slots used.
-int cut_items(std::vector<Item>& items, int unit, int min_units, int64_t slots, int* tiles) {
+// Counters at the head of the workspace.  Their place must not move from plan to
+// plan: every launch leaves them zero, what lies behind them not.
+constexpr int kCounters = 16384;
+
+// Cuts pieces longer than the even share of a slot, at most max_tiles of them,
+// and orders all longest first.  Returns the number of partial slots used.
+int cut_items(std::vector<Item>& items, int unit, int min_units, int64_t slots, int max_tiles,
+              int* tiles) {
   int64_t total = 0;
   auto cost = [&](const Item& w) { return ceil_div(std::max(w.kv_end - w.kv_begin, 0), unit); };
   for (const Item& w : items) total += cost(w);
@@ -135,7 +140,7 @@ int cut_items(std::vector<Item>& items, int unit, int min_units, int64_t slots, 
   int slot = 0, tile = 0;
   for (Item w : items) {
     const int64_t n = cost(w);
-    const int64_t parts = n > share + share / 2 ? ceil_div(n, share) : 1;
+    const int64_t parts = n > share + share / 2 && tile < max_tiles ? ceil_div(n, share) : 1;
     w.tile = 0;
     w.slot = 0;
     w.splits = (int)parts;
@@ -167,7 +172,24 @@ int64_t plan_capacity(int64_t batch, int64_t total_q, int64_t num_indices, int s
   return 4 * total_q + num_indices + 12 * (2 * batch + total_q + slots) + 16;
 }
 
-size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+// The workspace: counters, then the two kernels' partial rows (fp32) and their
+// (maximum, sum) pairs, [slot][kv head][row].
+struct Workspace {
+  size_t few, few_ml, many, many_ml, bytes;
+};
+
+Workspace workspace_of(const pace_attention_plan& plan) {
+  auto align = [](size_t n) { return (n + 255) & ~(size_t)255; };
+  const size_t few = (size_t)plan.few_slots * plan.num_kv_heads * kFewRows;
+  const size_t many = (size_t)plan.many_slots * plan.num_kv_heads * kTileRows;
+  Workspace w;
+  w.few = (size_t)kCounters * sizeof(int32_t);
+  w.few_ml = align(w.few + few * plan.head_dim * sizeof(float));
+  w.many = align(w.few_ml + few * sizeof(float2));
+  w.many_ml = align(w.many + many * plan.head_dim * sizeof(float));
+  w.bytes = align(w.many_ml + many * sizeof(float2));
+  return w;
+}
 
 }  // namespace attn
 }  // namespace pace
@@ -286,8 +308,13 @@ extern "C" int pace_paged_attention_plan(
     }
     const int64_t few_slots = (int64_t)ceil_div((int64_t)num_sms * kFewCtasPerSm, num_kv_heads);
     const int64_t many_slots = ceil_div(num_sms, num_kv_heads);
-    plan->few_slots = cut_items(few, kFewKeys, kFewMinUnits, few_slots, &plan->few_tiles);
-    plan->many_slots = cut_items(many, kTileKeys, kTileMinUnits, many_slots, &plan->many_tiles);
+    const int max_tiles = kCounters / 2 / num_kv_heads;
+    plan->few_slots =
+        cut_items(few, kFewKeys, kFewMinUnits, few_slots, max_tiles, &plan->few_tiles);
+    plan->many_slots =
+        cut_items(many, kTileKeys, kTileMinUnits, many_slots, max_tiles, &plan->many_tiles);
+    const Workspace ws = workspace_of(*plan);
+    plan->workspace_bytes = ws.bytes;
     plan->total_q = total_q;
     plan->max_page = max_page;
     plan->num_few = (int)few.size();
@@ -358,6 +385,24 @@ extern "C" int pace_paged_attention(const pace_attention_plan* plan, const int32
   p.scale = sm_scale;
   p.cap = logits_soft_cap;
   StreamDeviceGuard guard(stream);
+  // The tensor-core kernels take 16-bit queries of 64 or 128 dimensions over a cache that 16-byte
+  // copies fit and whose rows 32 bits number; the CUDA-core kernel the rest.
+  const int64_t cache_rows = num_pages * 2 * plan->page_size * plan->num_kv_heads;
+  const bool tensor = (dtype == PACE_BF16 || dtype == PACE_F16) &&
+                      (plan->head_dim == 64 || plan->head_dim == 128) && aligned16(cache) &&
+                      cache_rows <= UINT32_MAX;
+  if (tensor && plan->num_many == 0) {
+    if (!workspace || workspace_bytes < plan->workspace_bytes || !aligned16(workspace))
+      return fail(PACE_ERR_INVALID_ARGUMENT, "%s: the plan needs %zu bytes of 16-byte aligned "
+                  "workspace", what, plan->workspace_bytes);
+    const Workspace ws = workspace_of(*plan);
+    uint8_t* base = static_cast<uint8_t*>(workspace);
+    int32_t* counters = reinterpret_cast<int32_t*>(base);
+    return run_few_rows(p, reinterpret_cast<const Item*>(plan_words + plan->few_offset),
+                        plan->num_few, reinterpret_cast<float*>(base + ws.few),
+                        reinterpret_cast<float2*>(base + ws.few_ml), counters, dtype == PACE_BF16,
+                        guard.device(), stream, what);
+  }
   return PACE_DISPATCH_FLOAT(dtype, what, [&] {
     using T = scalar_t;
     return exponents ? run_rows<T, uint8_t>(p, stream, what) : run_rows<T, T>(p, stream, what);

@@ -1,0 +1,217 @@
+// Warp-level pieces of the paged-attention kernels: asynchronous copies, the
+// 16 x 8 x 16 matrix instruction for both 16-bit types, unpacking of e4m3
+// codes, and the joining of pieces' results.
+#pragma once
+
+#include "attention.cuh"
+
+namespace pace {
+namespace attn {
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// 16 bytes to shared memory; zeros where `there` is false (nothing is read).
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src),
+               "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_addr(p))
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_addr(p))
+               : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A word of four codes as two registers of two 16-bit values each, bytes 0, 2
+// and bytes 1, 3: sign to the top, exponent and mantissa below it, shifted to
+// the type's mantissa end.  The value is the code's times 2^-120 (bf16) or 2^-8
+// (fp16).
+template <int SHIFT>
+__device__ __forceinline__ void spread_codes(uint32_t w, uint32_t& even, uint32_t& odd) {
+  constexpr uint32_t kMag = 0x007f007fu << SHIFT;
+  even = ((w << 8) & 0x80008000u) | ((w << SHIFT) & kMag);
+  odd = (w & 0x80008000u) | ((w >> (8 - SHIFT)) & kMag);
+}
+
+template <typename T>
+struct Mma;
+
+template <>
+struct Mma<__nv_bfloat16> {
+  static constexpr bool kWideRange = true;  // fp32's exponents
+  __device__ static __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  __device__ static __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ uint32_t pair(__nv_bfloat16 x, __nv_bfloat16 y) {
+    const __nv_bfloat162 h = __halves2bfloat162(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ uint32_t mul2(uint32_t x, uint32_t f) {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  __device__ static __forceinline__ void unpack_codes(uint32_t w, uint32_t& even, uint32_t& odd) {
+    spread_codes<4>(w, even, odd);
+  }
+  // times 2^120
+  __device__ static __forceinline__ uint32_t code_scale(uint32_t x) { return mul2(x, 0x7b807b80u); }
+};
+
+template <>
+struct Mma<__half> {
+  static constexpr bool kWideRange = false;
+  __device__ static __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  __device__ static __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ uint32_t pair(__half x, __half y) {
+    const __half2 h = __halves2half2(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ uint32_t mul2(uint32_t x, uint32_t f) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&x),
+                              *reinterpret_cast<const __half2*>(&f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  __device__ static __forceinline__ void unpack_codes(uint32_t w, uint32_t& even, uint32_t& odd) {
+    spread_codes<7>(w, even, odd);
+  }
+  // times 2^8
+  __device__ static __forceinline__ uint32_t code_scale(uint32_t x) { return mul2(x, 0x5c005c00u); }
+  // Two rows' factors times 2^8, as a product f * g of which fp16 holds each: g is 1 unless a
+  // factor passes 2^7 (the product ends at 2^22, past which every value but a few subnormal codes
+  // is outside fp16's range).  Factors below 2^-32 vanish: so do their values, in fp16.
+  __device__ static __forceinline__ void split_factors(float x, float y, uint32_t& f, uint32_t& g) {
+    f = pack(x != x ? x : fminf(x, 128.f) * 256.f, y != y ? y : fminf(y, 128.f) * 256.f);
+    g = pack(fminf(fmaxf(x * 0.0078125f, 1.f), 32768.f), fminf(fmaxf(y * 0.0078125f, 1.f), 32768.f));
+  }
+  // Values past fp16's range saturate.
+  __device__ static __forceinline__ uint32_t scale2(uint32_t x, uint32_t f, uint32_t g) {
+    x = mul2(x, f);
+    if (g != 0x3c003c00u) {
+      x = mul2(x, g);
+      __half2 h = *reinterpret_cast<__half2*>(&x);
+      const __half2 top = __float2half2_rn(65504.f);
+      h = __hmin2_nan(__hmax2_nan(h, __hneg2(top)), top);
+      x = *reinterpret_cast<uint32_t*>(&h);
+    }
+    return x;
+  }
+};
+
+// Four outputs of one row from its unnormalised sums, and the row's lse (m in
+// powers of two).  A row that saw nothing (sum 0) is zero.
+template <typename T>
+__device__ __forceinline__ void write_out(const Problem& p, int64_t tok, int head, int d,
+                                          const float (&v)[4], float m, float sum) {
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* o = static_cast<T*>(p.out) + tok * p.out_stride + (int64_t)head * p.head_dim + d;
+  T y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = Traits<T>::from_f(sum == 0.f ? 0.f : v[i] * inv);
+  if ((reinterpret_cast<uintptr_t>(o) & 7) == 0) {
+    *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = y[i];
+  }
+  if (p.lse && d == 0)
+    p.lse[tok * p.heads + head] = sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
+}
+
+// Called by every thread of the CTA after it wrote its part of a piece's
+// result: true in the CTA that arrives last of `splits`, which then sees what
+// all of them wrote; the counter is zero again.
+__device__ __forceinline__ bool arrive_last(int32_t* counter, int splits, bool* last) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int before = atomicAdd(counter, 1);
+    *last = before == splits - 1;
+    if (*last) *counter = 0;
+  }
+  __syncthreads();
+  if (!*last) return false;
+  __threadfence();
+  return true;
+}
+
+// Joins columns d .. d + 3 of row r over the pieces of item w's rows and writes
+// the output.  ROWS: rows of a slot.
+template <typename T, int ROWS>
+__device__ __forceinline__ void join_pieces(const Problem& p, const float* partial,
+                                            const float2* partial_ml, const Item& w, int kvh, int r,
+                                            int d, int D, int group) {
+  const int64_t first = (int64_t)w.slot * p.kv_heads + kvh;
+  float mm = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = 0; k < w.splits; ++k)
+    mm = fmaxf(mm, __ldcg(partial_ml + (first + (int64_t)k * p.kv_heads) * ROWS + r).x);
+  const float b = mm == -INFINITY ? 0.f : mm;
+#pragma unroll 4
+  for (int k = 0; k < w.splits; ++k) {
+    const int64_t at = (first + (int64_t)k * p.kv_heads) * ROWS + r;
+    const float2 ml = __ldcg(partial_ml + at);
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(partial + at * D + d));
+    const float f = exp2_approx(ml.x - b);
+    sum += f * ml.y;
+    v[0] += f * x.x;
+    v[1] += f * x.y;
+    v[2] += f * x.z;
+    v[3] += f * x.w;
+  }
+  write_out<T>(p, w.tok0 + r / group, kvh * group + r % group, d, v, mm, sum);
+}
+
+// The two tensor-core kernels' launchers.
+int run_few_rows(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+                 int32_t* counters, bool bf16, int device, cudaStream_t stream, const char* what);
+
+}  // namespace attn
+}  // namespace pace

@@ -1,8 +1,8 @@
 """GPU: paged attention against the restatement in 64 bits.
 
 Tolerance, per element of the output o = sum p v (p the softmax): the output is
-rounded once to its type (half an ulp: u * |o|, u = 2^-9 for bf16, 2^-12 * 2 =
-2^-11 for fp16, 2^-24 for fp32), and the kernels round each p once to the
+rounded once to its type (half an ulp: u * |o|, u = eps / 2 of the type: 2^-8 for
+bf16, 2^-11 for fp16, 2^-24 for fp32), and the kernels round each p once to the
 query's type before it meets v (at most u * sum p|v| in the worst case).  The
 fp32 score of D products is off by at most (D + 3) * 2^-24 * scale * sum|q k|,
 here under 2e-4 with these inputs, and moves p by twice that.  fp16's subnormals
@@ -22,7 +22,7 @@ from tests.test_kv_quant_gpu import pages_of
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 TINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25, torch.float32: 0.0}
-U = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+U = {t: torch.finfo(t).eps / 2 for t in (torch.bfloat16, torch.float16, torch.float32)}
 
 
 class Step:
