@@ -51,6 +51,7 @@ CUDA_SOURCES = [
     "kv_quant_kernels.cu",
     "attention_kernels.cu",
     "attention_few_kernels.cu",
+    "attention_tile_kernels.cu",
     "gemm_rope_kernels.cu",
     "moe_gemm_kernels.cu",
 ]

@@ -27,11 +27,12 @@ struct TokenInfo {
 // A piece of work: `ntok` query tokens (all their heads of one kv head) over
 // keys [kv_begin, kv_end).  splits > 1: it is number `split` of that many
 // pieces of the same rows, which leave partial results in slots `slot`,
-// slot + 1, ... and count their arrivals in counter `tile`.
+// slot + 1, ... and count their arrivals in counter `tile`.  mixed: some row
+// does not see every key that another sees.
 struct Item {
   int tok0, ntok, kv_begin, kv_end;
   int page_base, tile, slot, split;
-  int splits, pad0, pad1, pad2;
+  int splits, mixed, pad0, pad1;
 };
 static_assert(sizeof(Item) == 48 && sizeof(TokenInfo) == 16, "plan records are int32 words");
 
@@ -64,6 +65,81 @@ __device__ __forceinline__ float score(float dot, float scale, float cap, float 
 // Whether drafted token `node` (0 .. 64 * words - 1) is visible.
 __device__ __forceinline__ bool tree_bit(const uint64_t* row, int node) {
   return (row[node >> 6] >> (node & 63)) & 1u;
+}
+
+template <typename KV>
+__device__ __forceinline__ float load_kv(const KV* p, float) {
+  return Traits<KV>::to_f(*p);
+}
+template <>
+__device__ __forceinline__ float load_kv<uint8_t>(const uint8_t* p, float factor) {
+  float f[4];
+  e4m3x4_to_floats(*p, f);
+  return f[0] * factor;
+}
+
+// One row by one warp on the CUDA cores: lane l holds dimensions l, l + 32, ...
+// (N of them); the keys it sees, and no others, are walked one by one with a
+// running maximum and sum in fp32.  Head sizes that the tensor-core kernels do
+// not take run on this; and those kernels call it for a row that came out
+// infinite or NaN while some of its piece's keys are hidden from it: a matrix
+// product multiplies a hidden key's value by 0, which an infinity or a NaN in
+// it survives.
+template <typename T, typename KV, int N>
+__device__ void attend_row(const Problem& p, int64_t tok, int head) {
+  const int lane = threadIdx.x & 31;
+  const int kvh = head / (p.heads / p.kv_heads);
+  const int D = p.head_dim;
+  const T* q = static_cast<const T*>(p.query) + tok * p.q_stride + (int64_t)head * D;
+  const KV* cache = static_cast<const KV*>(p.cache);
+  const TokenInfo info = p.tokens[tok];
+  float qv[N], acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int d = lane + 32 * i;
+    qv[i] = d < D ? Traits<T>::to_f(q[d]) : 0.f;
+    acc[i] = 0.f;
+  }
+  const float slope = p.slopes ? p.slopes[head] : 0.f;
+  const uint64_t* bits = p.tree_mask ? p.tree_mask + tok * p.tree_words : nullptr;
+  const int end = bits ? info.pos : info.hi;  // a tree's drafted keys are hi .. pos - 1
+  float m = -INFINITY, l = 0.f;
+  for (int j = info.lo; j < end; ++j) {
+    if (j >= info.hi && !tree_bit(bits, j - info.hi)) continue;
+    const int64_t page = p.kv_indices[info.page_base + j / p.page_size];
+    const int64_t krow = (page * 2 * p.page_size + j % p.page_size) * p.kv_heads + kvh;
+    const int64_t vrow = krow + (int64_t)p.page_size * p.kv_heads;
+    float kf = 1.f, vf = 1.f;
+    if (p.exponents) {
+      kf = exponent_factor(p.exponents[krow]);
+      vf = exponent_factor(p.exponents[vrow]);
+    }
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int d = lane + 32 * i;
+      if (d < D) dot += qv[i] * load_kv(cache + krow * D + d, kf);
+    }
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    const float s = score(dot, p.scale, p.cap, slope, abs(info.pos - j));
+    const float m2 = fmaxf(m, s);  // a NaN stays out of the maximum and enters the sum
+    const float c = m2 == -INFINITY ? 1.f : expf(m - m2);
+    const float e = s == -INFINITY ? 0.f : expf(s - m2);
+    l = l * c + e;
+    m = m2;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int d = lane + 32 * i;
+      if (d < D) acc[i] = acc[i] * c + e * load_kv(cache + vrow * D + d, vf);
+    }
+  }
+  T* o = static_cast<T*>(p.out) + tok * p.out_stride + (int64_t)head * D;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int d = lane + 32 * i;
+    if (d < D) o[d] = Traits<T>::from_f(l == 0.f ? 0.f : acc[i] / l);
+  }
+  if (p.lse && lane == 0) p.lse[tok * p.heads + head] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
 }  // namespace attn

@@ -360,39 +360,46 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   __syncthreads();
   constexpr int V4 = D / 4;
   const int64_t slot = (int64_t)(w.slot + w.split) * p.kv_heads + kvh;
-  for (int u = threadIdx.x; u < rows * V4; u += kFewWarps * 32) {
+  // whole warps stay in the loop, for redo_rows
+  for (int u = threadIdx.x; (u & ~31) < rows * V4; u += kFewWarps * 32) {
     const int r = u / V4, d = (u - r * V4) * 4;
-    float mm = -INFINITY;
+    bool fine = true;
+    if (u < rows * V4) {
+      float mm = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < kFewWarps; ++k) mm = fmaxf(mm, join_ml[(k * 16 + r) * 2]);
-    const float b = mm == -INFINITY ? 0.f : mm;
-    float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < kFewWarps; ++k) mm = fmaxf(mm, join_ml[(k * 16 + r) * 2]);
+      const float b = mm == -INFINITY ? 0.f : mm;
+      float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < kFewWarps; ++k) {
-      const float f = exp2_approx(join_ml[(k * 16 + r) * 2] - b);
-      sum += f * join_ml[(k * 16 + r) * 2 + 1];
-      const float4 x = *reinterpret_cast<const float4*>(smem + k * Tile::kWarpBytes + (r * D + d) * 4);
-      v[0] += f * x.x;
-      v[1] += f * x.y;
-      v[2] += f * x.z;
-      v[3] += f * x.w;
+      for (int k = 0; k < kFewWarps; ++k) {
+        const float f = exp2_approx(join_ml[(k * 16 + r) * 2] - b);
+        sum += f * join_ml[(k * 16 + r) * 2 + 1];
+        const float4 x = *reinterpret_cast<const float4*>(smem + k * Tile::kWarpBytes + (r * D + d) * 4);
+        v[0] += f * x.x;
+        v[1] += f * x.y;
+        v[2] += f * x.z;
+        v[3] += f * x.w;
+      }
+      if (w.splits == 1) {
+        fine = write_out<T>(p, w.tok0 + r / group, kvh * group + r % group, d, v, mm, sum);
+      } else {
+        __stcg(reinterpret_cast<float4*>(partial + (slot * 16 + r) * D + d),
+               make_float4(v[0], v[1], v[2], v[3]));
+        if (d == 0) __stcg(partial_ml + slot * 16 + r, make_float2(mm, sum));
+      }
     }
-    if (w.splits == 1) {
-      write_out<T>(p, w.tok0 + r / group, kvh * group + r % group, d, v, mm, sum);
-    } else {
-      __stcg(reinterpret_cast<float4*>(partial + (slot * 16 + r) * D + d),
-             make_float4(v[0], v[1], v[2], v[3]));
-      if (d == 0) __stcg(partial_ml + slot * 16 + r, make_float2(mm, sum));
-    }
+    if (w.mixed) redo_rows<T, D, Q8>(p, w, kvh, group, r, fine);
   }
   if (w.splits == 1) return;
 
   // ---- the last piece of these rows to arrive joins them all --------------------
   __shared__ bool last;
   if (!arrive_last(counters + (int64_t)w.tile * p.kv_heads + kvh, w.splits, &last)) return;
-  for (int u = threadIdx.x; u < rows * V4; u += kFewWarps * 32) {
+  for (int u = threadIdx.x; (u & ~31) < rows * V4; u += kFewWarps * 32) {
     const int r = u / V4, d = (u - r * V4) * 4;
-    join_pieces<T, 16>(p, partial, partial_ml, w, kvh, r, d, D, group);
+    const bool fine =
+        u >= rows * V4 || join_pieces<T, 16>(p, partial, partial_ml, w, kvh, r, d, D, group);
+    if (w.mixed) redo_rows<T, D, Q8>(p, w, kvh, group, r, fine);
   }
 }
 

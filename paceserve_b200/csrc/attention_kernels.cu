@@ -21,80 +21,14 @@ namespace attn {
 constexpr int kMaxHeadDim = 256;
 constexpr int kWarps = 4;
 
-template <typename KV>
-__device__ __forceinline__ float load_kv(const KV* p, float) {
-  return Traits<KV>::to_f(*p);
-}
-template <>
-__device__ __forceinline__ float load_kv<uint8_t>(const uint8_t* p, float factor) {
-  float f[4];
-  e4m3x4_to_floats(*p, f);
-  return f[0] * factor;
-}
-
-// One warp per (query token, head): lane l holds dimensions l, l + 32, ...
-// The keys are walked one by one with a running maximum and sum in fp32.
+// One warp per (query token, head).
 template <typename T, typename KV>
 __global__ void __launch_bounds__(kWarps * 32) attention_rows_kernel(const Problem p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (w >= p.total_q * p.heads) return;
-  const int64_t tok = w / p.heads;
-  const int head = (int)(w - tok * p.heads), kvh = head / (p.heads / p.kv_heads);
-  const int D = p.head_dim;
-  constexpr int N = kMaxHeadDim / 32;
-  const T* q = static_cast<const T*>(p.query) + tok * p.q_stride + (int64_t)head * D;
-  const KV* cache = static_cast<const KV*>(p.cache);
-  const TokenInfo info = p.tokens[tok];
-  float qv[N], acc[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int d = lane + 32 * i;
-    qv[i] = d < D ? Traits<T>::to_f(q[d]) : 0.f;
-    acc[i] = 0.f;
-  }
-  const float slope = p.slopes ? p.slopes[head] : 0.f;
-  const uint64_t* bits = p.tree_mask ? p.tree_mask + tok * p.tree_words : nullptr;
-  const int end = bits ? info.pos : info.hi;  // a tree's drafted keys are hi .. pos - 1
-  float m = -INFINITY, l = 0.f;
-  for (int j = info.lo; j < end; ++j) {
-    if (j >= info.hi && !tree_bit(bits, j - info.hi)) continue;
-    const int64_t page = p.kv_indices[info.page_base + j / p.page_size];
-    const int64_t krow = (page * 2 * p.page_size + j % p.page_size) * p.kv_heads + kvh;
-    const int64_t vrow = krow + (int64_t)p.page_size * p.kv_heads;
-    float kf = 1.f, vf = 1.f;
-    if (p.exponents) {
-      kf = exponent_factor(p.exponents[krow]);
-      vf = exponent_factor(p.exponents[vrow]);
-    }
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int d = lane + 32 * i;
-      if (d < D) dot += qv[i] * load_kv(cache + krow * D + d, kf);
-    }
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float s = score(dot, p.scale, p.cap, slope, abs(info.pos - j));
-    const float m2 = fmaxf(m, s);  // a NaN stays out of the maximum and enters the sum
-    const float c = m2 == -INFINITY ? 1.f : expf(m - m2);
-    const float e = s == -INFINITY ? 0.f : expf(s - m2);
-    l = l * c + e;
-    m = m2;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int d = lane + 32 * i;
-      if (d < D) acc[i] = acc[i] * c + e * load_kv(cache + vrow * D + d, vf);
-    }
-  }
-  T* o = static_cast<T*>(p.out) + tok * p.out_stride + (int64_t)head * D;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int d = lane + 32 * i;
-    if (d < D) o[d] = Traits<T>::from_f(l == 0.f ? 0.f : acc[i] / l);
-  }
-  if (p.lse && lane == 0) p.lse[tok * p.heads + head] = l == 0.f ? -INFINITY : m + logf(l);
+  attend_row<T, KV, kMaxHeadDim / 32>(p, w / p.heads, (int)(w % p.heads));
 }
 
 template <typename T, typename KV>
@@ -278,6 +212,7 @@ extern "C" int pace_paged_attention_plan(
       for (int t0 = 0; t0 < q; t0 += step) {
         const int n = std::min(step, q - t0);
         int first = len, end = 0;  // keys that some token of the piece sees
+        bool mixed = tree_words > 0 && n > 1;
         for (int i = t0; i < t0 + n; ++i) {
           const int pos = len - q + i;
           TokenInfo& w = tok[q0 + i];
@@ -297,7 +232,10 @@ extern "C" int pace_paged_attention_plan(
           }
         }
         if (end <= first) first = end = 0;
+        for (int i = t0; i < t0 + n && tree_words == 0; ++i)
+          mixed |= tok[q0 + i].lo != first || tok[q0 + i].hi != end;
         Item w{};
+        w.mixed = mixed;
         w.tok0 = q0 + t0;
         w.ntok = n;
         w.kv_begin = first;
@@ -391,16 +329,25 @@ extern "C" int pace_paged_attention(const pace_attention_plan* plan, const int32
   const bool tensor = (dtype == PACE_BF16 || dtype == PACE_F16) &&
                       (plan->head_dim == 64 || plan->head_dim == 128) && aligned16(cache) &&
                       cache_rows <= UINT32_MAX;
-  if (tensor && plan->num_many == 0) {
+  if (tensor) {
     if (!workspace || workspace_bytes < plan->workspace_bytes || !aligned16(workspace))
       return fail(PACE_ERR_INVALID_ARGUMENT, "%s: the plan needs %zu bytes of 16-byte aligned "
                   "workspace", what, plan->workspace_bytes);
     const Workspace ws = workspace_of(*plan);
     uint8_t* base = static_cast<uint8_t*>(workspace);
     int32_t* counters = reinterpret_cast<int32_t*>(base);
+    const bool bf16 = dtype == PACE_BF16;
+    if (plan->num_many > 0) {
+      const int st = run_tile_rows(
+          p, reinterpret_cast<const Item*>(plan_words + plan->many_offset), plan->num_many,
+          reinterpret_cast<float*>(base + ws.many), reinterpret_cast<float2*>(base + ws.many_ml),
+          counters + kCounters / 2, fault_flags, bf16, guard.device(), stream, what);
+      if (st != PACE_OK) return st;
+    }
+    if (plan->num_few == 0) return PACE_OK;
     return run_few_rows(p, reinterpret_cast<const Item*>(plan_words + plan->few_offset),
                         plan->num_few, reinterpret_cast<float*>(base + ws.few),
-                        reinterpret_cast<float2*>(base + ws.few_ml), counters, dtype == PACE_BF16,
+                        reinterpret_cast<float2*>(base + ws.few_ml), counters, bf16,
                         guard.device(), stream, what);
   }
   return PACE_DISPATCH_FLOAT(dtype, what, [&] {

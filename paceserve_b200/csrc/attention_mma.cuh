@@ -3,6 +3,8 @@
 // codes, and the joining of pieces' results.
 #pragma once
 
+#include <type_traits>
+
 #include "attention.cuh"
 
 namespace pace {
@@ -91,6 +93,24 @@ struct Mma<__nv_bfloat16> {
   __device__ static __forceinline__ void unpack_codes(uint32_t w, uint32_t& even, uint32_t& odd) {
     spread_codes<4>(w, even, odd);
   }
+  // Sixteen codes of a row with exponent byte `ex` as values, dimensions 0, 2, 1, 3 of each four.
+  __device__ static __forceinline__ void dequantise16(const uint32_t (&w)[4], uint32_t ex,
+                                                      uint32_t (&o)[8]) {
+    // 2^(ex - 127 + 120) while bf16 holds it; larger rows (and NaN ones) in two steps
+    const uint32_t f1 = (min(ex, 134u) + 120u) << 7, f = f1 | f1 << 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t a, b;
+      unpack_codes(w[i], a, b);
+      o[2 * i] = mul2(a, f);
+      o[2 * i + 1] = mul2(b, f);
+    }
+    if (ex > 134u) {
+      const uint32_t g1 = ex == (uint32_t)kNanExponent ? 0x7fc0u : (ex - 7u) << 7, g = g1 | g1 << 16;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = mul2(o[i], g);
+    }
+  }
   // times 2^120
   __device__ static __forceinline__ uint32_t code_scale(uint32_t x) { return mul2(x, 0x7b807b80u); }
 };
@@ -122,6 +142,20 @@ struct Mma<__half> {
   __device__ static __forceinline__ void unpack_codes(uint32_t w, uint32_t& even, uint32_t& odd) {
     spread_codes<7>(w, even, odd);
   }
+  // As above; values past fp16's range saturate.
+  __device__ static __forceinline__ void dequantise16(const uint32_t (&w)[4], uint32_t ex,
+                                                      uint32_t (&o)[8]) {
+    uint32_t f, g;
+    const float x = exponent_factor(ex);
+    split_factors(x, x, f, g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t a, b;
+      unpack_codes(w[i], a, b);
+      o[2 * i] = scale2(a, f, g);
+      o[2 * i + 1] = scale2(b, f, g);
+    }
+  }
   // times 2^8
   __device__ static __forceinline__ uint32_t code_scale(uint32_t x) { return mul2(x, 0x5c005c00u); }
   // Two rows' factors times 2^8, as a product f * g of which fp16 holds each: g is 1 unless a
@@ -146,9 +180,10 @@ struct Mma<__half> {
 };
 
 // Four outputs of one row from its unnormalised sums, and the row's lse (m in
-// powers of two).  A row that saw nothing (sum 0) is zero.
+// powers of two).  A row that saw nothing (sum 0) is zero.  Returns whether all
+// are finite.
 template <typename T>
-__device__ __forceinline__ void write_out(const Problem& p, int64_t tok, int head, int d,
+__device__ __forceinline__ bool write_out(const Problem& p, int64_t tok, int head, int d,
                                           const float (&v)[4], float m, float sum) {
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* o = static_cast<T*>(p.out) + tok * p.out_stride + (int64_t)head * p.head_dim + d;
@@ -163,6 +198,31 @@ __device__ __forceinline__ void write_out(const Problem& p, int64_t tok, int hea
   }
   if (p.lse && d == 0)
     p.lse[tok * p.heads + head] = sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
+  return fabsf(v[0] * inv) + fabsf(v[1] * inv) + fabsf(v[2] * inv) + fabsf(v[3] * inv) < INFINITY;
+}
+
+// attend_row out of line: it is rarely needed.
+template <typename T, typename KV, int N>
+__device__ __noinline__ void attend_row_again(const Problem& p, int64_t tok, int head) {
+  attend_row<T, KV, N>(p, tok, head);
+}
+
+// Redoes rows whose outputs, just written by this warp's lanes (lane u: four
+// columns of row `r`), are not all finite.  The whole warp calls it; lanes
+// without a row pass fine = true.
+template <typename T, int D, bool Q8>
+__device__ __forceinline__ void redo_rows(const Problem& p, const Item& w, int kvh, int group, int r,
+                                          bool fine) {
+  uint32_t bad = __ballot_sync(0xffffffffu, !fine);
+  if (bad) __syncwarp();  // their stores come before the ones below
+  constexpr uint32_t kRowLanes = D / 4 >= 32 ? 0xffffffffu : (1u << (D / 4 & 31)) - 1u;
+  while (bad) {
+    const int first = __ffs(bad) - 1;
+    const int row = __shfl_sync(0xffffffffu, r, first);
+    attend_row_again<T, std::conditional_t<Q8, uint8_t, T>, D / 32>(p, w.tok0 + row / group,
+                                                                    kvh * group + row % group);
+    bad &= ~(kRowLanes << (first / (D / 4) * (D / 4)));
+  }
 }
 
 // Called by every thread of the CTA after it wrote its part of a piece's
@@ -185,7 +245,7 @@ __device__ __forceinline__ bool arrive_last(int32_t* counter, int splits, bool* 
 // Joins columns d .. d + 3 of row r over the pieces of item w's rows and writes
 // the output.  ROWS: rows of a slot.
 template <typename T, int ROWS>
-__device__ __forceinline__ void join_pieces(const Problem& p, const float* partial,
+__device__ __forceinline__ bool join_pieces(const Problem& p, const float* partial,
                                             const float2* partial_ml, const Item& w, int kvh, int r,
                                             int d, int D, int group) {
   const int64_t first = (int64_t)w.slot * p.kv_heads + kvh;
@@ -206,10 +266,13 @@ __device__ __forceinline__ void join_pieces(const Problem& p, const float* parti
     v[2] += f * x.z;
     v[3] += f * x.w;
   }
-  write_out<T>(p, w.tok0 + r / group, kvh * group + r % group, d, v, mm, sum);
+  return write_out<T>(p, w.tok0 + r / group, kvh * group + r % group, d, v, mm, sum);
 }
 
 // The two tensor-core kernels' launchers.
+int run_tile_rows(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+                  int32_t* counters, int32_t* fault, bool bf16, int device, cudaStream_t stream,
+                  const char* what);
 int run_few_rows(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
                  int32_t* counters, bool bf16, int device, cudaStream_t stream, const char* what);
 

@@ -1,0 +1,628 @@
+// Paged attention of many query rows on the tensor cores (tcgen05): prompts,
+// prompt chunks, draft trees and wide groups of heads.
+//
+// A CTA takes one piece of the plan for one kv head: up to 256 query rows
+// (tokens x the group's heads, so that grouped heads share every key they
+// read) in two tiles of 128, over keys [kv_begin, kv_end) in steps of 128.
+//   S_t = Q_t K^T      128 x 128 per tile and step, accumulated in TMEM;
+//   softmax            one thread per row: the row's 128 scores come from TMEM
+//                      into registers, P goes back over them as 16-bit values;
+//   O_t += P_t V       A operand from TMEM, O_t stays in TMEM throughout.
+// Warps 0-3 and 4-7 are the two tiles' softmax, warp 8 issues the MMAs, the
+// others copy K and V from their pages into a ring of 128-key tiles.  While one
+// tile's rows are in softmax the tensor core works on the other tile.
+//
+// The running maximum m is allowed to lag: O and the sum l are scaled down only
+// when a row's maximum has risen by more than 2^8 (kLag), so P is at most 2^8,
+// which both 16-bit types hold with the same relative error, and O is read
+// back and rescaled in a step of a sequence or two instead of in every one.
+// S_t of step j + 1 is issued behind P_t V of step j, so its arrival also says
+// that O_t may be touched.
+//
+// Keys past kv_end are copied as zeros.  Every wait is bounded.
+#include "attention_mma.cuh"
+#include "tcgen05.cuh"
+
+namespace pace {
+namespace attn {
+
+constexpr uint64_t kWaitLimitNs = 1000000000ull;  // 1 s per wait
+constexpr int32_t kFaultTimeout = 1 << 30;
+constexpr int kTileRowsEach = 128;
+constexpr int kStepKeys = 128;
+constexpr float kLag = 8.f;  // in powers of two
+constexpr int kLoadBarrier = 1;
+
+template <int D, bool Q8>
+struct TileCfg {
+  static constexpr int kLoadWarp0 = Q8 ? 12 : 9;
+  static constexpr int kLoaders = Q8 ? 128 : 96;  // threads
+  static constexpr int kThreads = kLoadWarp0 * 32 + kLoaders;
+  static constexpr int kKvBytes = kStepKeys * D * 2;
+  static constexpr int kQBytes = kTileRowsEach * D * 2;
+  static constexpr int kStages = D == 128 ? 4 : 8;
+  static constexpr int kSmemBytes = 2 * kQBytes + kStages * kKvBytes + 1024 + 2048;
+  // registers per thread after the split; the sum over the warpgroups is what
+  // the block was launched with
+  static constexpr int kSoftmaxRegs = Q8 ? 176 : 208;
+  static constexpr int kOtherRegs = Q8 ? 80 : 88;
+};
+
+struct TileCtl {
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t kv_full[8], kv_empty[8];
+  uint64_t drain;
+  uint32_t tmem;
+  int abort;
+  uint32_t rows[2][kStepKeys];  // cache row (K part) of each key of a step; ~0: none
+};
+static_assert(sizeof(TileCtl) <= 2048, "");
+
+__device__ __forceinline__ void tile_fault(TileCtl* ctl, int32_t* fault) {
+  *reinterpret_cast<volatile int*>(&ctl->abort) = 1;
+  if (fault) atomicOr(fault, kFaultTimeout);
+}
+
+// Byte offset of 16-byte chunk `c` (8 dimensions) of row r of a 128-row tile:
+// 64 dimensions a half, 128-byte rows, the chunk swizzled by the row.
+__device__ __forceinline__ int tile_at(int r, int c) {
+  return (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+// The MN-major operand descriptor of a V tile: its rows are keys (the K axis of
+// P V) of 64 contiguous dimensions; groups of 8 keys 1024 bytes apart, the next
+// 64 dimensions 16 KB apart.
+__device__ __forceinline__ uint64_t umma_desc_v(uint32_t smem) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem >> 4) & 0x3FFFu);
+  d |= (uint64_t)(16384u >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+
+// D[tmem] (+)= A[tmem] * B[smem], B MN-major by its instruction descriptor.
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void fence_async_proxy() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Barrier of the copying threads that also ANDs `pred` over them.
+template <int N>
+__device__ __forceinline__ bool loaders_all(bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(pred ? 1u : 0u), "n"(kLoadBarrier), "n"(N)
+      : "memory");
+  return r != 0;
+}
+
+// Bits of the keys j0 .. j0 + 31 that a row sees: lo <= j < hi, and of the
+// drafted ones hi .. end - 1 those of its tree row.
+__device__ __forceinline__ uint32_t seen_bits(int j0, int lo, int hi, int end, const uint64_t* tree) {
+  auto below = [](int n) -> uint32_t {  // the first n bits
+    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+  };
+  uint32_t bits = below(hi - j0) & ~below(lo - j0);
+  if (tree && end > hi && j0 + 32 > hi && j0 < end) {
+    const int n0 = j0 - hi;  // node of bit 0
+    uint32_t t;
+    if (n0 < 0) {
+      t = (uint32_t)tree[0] << -n0;  // -n0 < 32
+    } else {
+      const uint64_t w = tree[n0 >> 6];
+      t = (uint32_t)(w >> (n0 & 63));
+      // the next word, where the sequence reaches into it
+      if ((n0 & 63) > 32 && hi + ((n0 >> 6) + 1) * 64 < end)
+        t |= (uint32_t)(tree[(n0 >> 6) + 1] << (64 - (n0 & 63)));
+    }
+    bits |= t & below(end - j0) & ~below(hi - j0);
+  }
+  return bits;
+}
+
+template <typename T, int D, bool Q8>
+__global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
+    attention_tile_kernel(const Problem p, const Item* __restrict__ items, float* partial,
+                          float2* partial_ml, int32_t* counters, int32_t* fault) {
+  using Cfg = TileCfg<D, Q8>;
+  using M = Mma<T>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ bool last;
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* ring = smem + 2 * Cfg::kQBytes;
+  TileCtl* ctl = reinterpret_cast<TileCtl*>(ring + Cfg::kStages * Cfg::kKvBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x % p.kv_heads;
+  const Item w = items[blockIdx.x / p.kv_heads];
+  const int group = p.heads / p.kv_heads;
+  const int rows = w.ntok * group;
+  const int tiles = rows > kTileRowsEach ? 2 : 1;
+  const int steps = (w.kv_end - w.kv_begin + kStepKeys - 1) / kStepKeys;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&ctl->q_full[i], 128);
+      tc::mbar_init(&ctl->s_full[i], 1);
+      tc::mbar_init(&ctl->p_full[i], 128);
+      tc::mbar_init(&ctl->o_full[i], 1);
+    }
+    for (int i = 0; i < Cfg::kStages; ++i) {
+      tc::mbar_init(&ctl->kv_full[i], Cfg::kLoaders);
+      tc::mbar_init(&ctl->kv_empty[i], 1);
+    }
+    tc::mbar_init(&ctl->drain, 1);
+    ctl->abort = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == 8) tc::tmem_alloc(&ctl->tmem, 512);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+  pdl_wait();
+
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kSoftmaxRegs));
+    // ---- softmax of tile t: thread = row ---------------------------------------
+    const int t = warp >> 2;
+    const int r = threadIdx.x & 127;      // row of the tile
+    const int row = t * kTileRowsEach + r;  // of the piece
+    const bool live = row < rows;
+    const int tok = w.tok0 + (live ? row / group : 0);
+    const int head = kvh * group + (live ? row % group : 0);
+    TokenInfo info{0, 0, 0, 0};
+    float slope = 0.f;
+    const uint64_t* tree = nullptr;
+    if (live) {
+      info = p.tokens[tok];
+      if (p.slopes) slope = p.slopes[head] * kLog2e;
+      if (p.tree_mask) tree = p.tree_mask + (int64_t)tok * p.tree_words;
+    }
+    const int end = tree ? min(info.pos, w.kv_end) : 0;  // of the drafted keys
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    if (t < tiles) {
+      // the row's query into the tile; negated where the scale is negative (and
+      // zero where it is), so that the largest product is the largest score
+      {
+        const T* q = static_cast<const T*>(p.query) + (int64_t)tok * p.q_stride + (int64_t)head * D;
+        uint8_t* qs = smem + t * Cfg::kQBytes;
+        const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+        const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint32_t v[4] = {0, 0, 0, 0};
+          if (live && p.scale != 0.f) {
+            if (vec) {
+              const uint4 x = ld_nc_v4(q + c * 8);
+              v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[i] = M::pair(q[c * 8 + 2 * i], q[c * 8 + 2 * i + 1]);
+            }
+          }
+          if constexpr (Q8) {
+            // quantised keys are unpacked as dimensions 0, 2, 1, 3 of each four
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const uint32_t a = v[i], b = v[i + 1];
+              v[i] = __byte_perm(a, b, 0x5410);
+              v[i + 1] = __byte_perm(a, b, 0x7632);
+            }
+          }
+          *reinterpret_cast<uint4*>(qs + tile_at(r, c)) =
+              make_uint4(v[0] ^ flip, v[1] ^ flip, v[2] ^ flip, v[3] ^ flip);
+        }
+        fence_async_proxy();
+        tc::mbar_arrive(&ctl->q_full[t]);
+      }
+      const float scale2 = (p.scale != 0.f ? fabsf(p.scale) : 1.f) * kLog2e;
+      const float cap2 = p.cap * kLog2e, cap_in = p.cap > 0.f ? 2.f * scale2 / p.cap : 0.f;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t ts = tmem + lanes + (uint32_t)(t * 128);
+      const uint32_t to = tmem + lanes + 256u + (uint32_t)(t * D);
+      for (int j = 0; j < steps; ++j) {
+        ok = __all_sync(0xffffffffu,
+                        tc::mbar_wait(&ctl->s_full[t], j & 1, kWaitLimitNs, &ctl->abort));
+        if (!ok) break;
+        tc::tc_fence_after();
+        uint32_t sr[128];
+        tmem_ld32(ts, sr);
+        tmem_ld32(ts + 32, sr + 32);
+        tmem_ld32(ts + 64, sr + 64);
+        tmem_ld32(ts + 96, sr + 96);
+        tc::tmem_wait_ld(sr);
+        float sc = scale2;
+        const int j0 = w.kv_begin + j * kStepKeys;
+        if (p.cap > 0.f) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            sr[i] = __float_as_uint(
+                cap2 - 2.f * cap2 * rcp_approx(1.f + exp2_approx(__uint_as_float(sr[i]) * cap_in)));
+          sc = 1.f;
+        }
+        if (p.slopes) {
+          const float d0 = (float)(info.pos - j0);
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            sr[i] = __float_as_uint(__uint_as_float(sr[i]) * sc - slope * fabsf(d0 - (float)i));
+          sc = 1.f;
+        }
+        const bool whole = j0 >= info.lo && j0 + kStepKeys <= min(info.hi, w.kv_end);
+        if (!__all_sync(0xffffffffu, whole)) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t bits =
+                seen_bits(j0 + 32 * k, info.lo, min(info.hi, w.kv_end), end, tree);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(bits >> i & 1)) sr[32 * k + i] = 0xff800000u;
+          }
+          __syncwarp();
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 128; ++i) top = fmaxf(top, __uint_as_float(sr[i]));
+        top *= sc;
+        if (j == 0) {
+          m = top;
+        } else {
+          const bool raise = top > m + kLag || (m == -INFINITY && top > m);
+          if (__any_sync(0xffffffffu, raise)) {
+            // O is complete up to the step before: S of this step was issued behind it
+            const float f = raise ? exp2_approx(m - top) : 1.f;
+            if (raise) m = top;
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(to + c, o);
+              tc::tmem_wait_ld(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st16(to + c, o);
+              tmem_st16(to + c + 16, o + 16);
+            }
+          }
+        }
+        const float b = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float x = exp2_approx(fmaf(__uint_as_float(sr[32 * k + 2 * i]), sc, -b));
+            const float y = exp2_approx(fmaf(__uint_as_float(sr[32 * k + 2 * i + 1]), sc, -b));
+            sum[2 * (i & 1)] += x;
+            sum[2 * (i & 1) + 1] += y;
+            pk[i] = M::pack(x, y);
+          }
+          tmem_st16(ts + 16 * k, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc::tc_fence_before();
+        tc::mbar_arrive(&ctl->p_full[t]);
+      }
+      // ---- the tile's output ----------------------------------------------------
+      if (ok && steps > 0)
+        ok = __all_sync(0xffffffffu,
+                        tc::mbar_wait(&ctl->o_full[t], 0, kWaitLimitNs, &ctl->abort));
+      if (!ok) tile_fault(ctl, fault);
+      if (ok) {
+        tc::tc_fence_after();
+        const int64_t slot = ((int64_t)(w.slot + w.split) * p.kv_heads + kvh) * 256 + row;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        T* out = static_cast<T*>(p.out) + (int64_t)tok * p.out_stride + (int64_t)head * D;
+        const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+        float size = 0.f;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          if (steps > 0) {
+            tmem_ld32(to + c, o);
+            tc::tmem_wait_ld(o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0;
+          }
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int s = Q8 ? (i & ~3) | ((i & 1) << 1) | ((i >> 1) & 1) : i;
+            v[i] = __uint_as_float(o[s]);
+          }
+          if (live && w.splits > 1) {
+            float* dst = partial + slot * D + c;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              __stcg(reinterpret_cast<float4*>(dst + i),
+                     make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+          } else if (live) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              v[i] = l == 0.f ? 0.f : v[i] * inv;
+              size += fabsf(v[i]);
+            }
+            if (vec) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) st_v4(out + c + i, Traits<T>::pack(v + i));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) out[c + i] = Traits<T>::from_f(v[i]);
+            }
+          }
+          __syncwarp();
+        }
+        if (live) {
+          if (w.splits > 1)
+            __stcg(partial_ml + slot, make_float2(m, l));
+          else if (p.lse)
+            p.lse[(int64_t)tok * p.heads + head] =
+                l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+        }
+        if (w.mixed && w.splits == 1) {
+          uint32_t bad = __ballot_sync(0xffffffffu, !(size < INFINITY));
+          if (bad) __syncwarp();  // their stores come before the ones below
+          for (; bad; bad &= bad - 1) {
+            const int at = row - lane + __ffs(bad) - 1;
+            attend_row_again<T, std::conditional_t<Q8, uint8_t, T>, D / 32>(
+                p, w.tok0 + at / group, kvh * group + at % group);
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kOtherRegs));
+    if (warp == 8) {
+      // ---- MMA issuer ------------------------------------------------------------
+      if (lane == 0 && steps > 0) {
+        constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+        constexpr uint32_t idesc_s = tc::umma_idesc_f16(kBf16, 128, kStepKeys);
+        constexpr uint32_t idesc_o = tc::umma_idesc_f16(kBf16, 128, D) | (1u << 16);  // B MN-major
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+          ok = ok && tc::mbar_wait(bar, parity, kWaitLimitNs, &ctl->abort);
+          tc::tc_fence_after();
+          return ok;
+        };
+        // ring slot i holds K of step i / 2 (i even) or V (i odd)
+        auto slot = [&](int i) { return tc::smem_u32(ring + (i % Cfg::kStages) * Cfg::kKvBytes); };
+        auto full = [&](int i) {
+          return wait(&ctl->kv_full[i % Cfg::kStages], (uint32_t)(i / Cfg::kStages) & 1u);
+        };
+        auto scores = [&](int t, int j) {
+          const uint32_t q = tc::smem_u32(smem + t * Cfg::kQBytes), k = slot(2 * j);
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            const uint32_t at = (uint32_t)((i >> 2) * 16384 + (i & 3) * 32);
+            tc::umma_f16(tmem + t * 128, tc::umma_desc_sw128(q + at), tc::umma_desc_sw128(k + at),
+                         idesc_s, i > 0);
+          }
+          tc::umma_commit(&ctl->s_full[t]);
+        };
+        auto output = [&](int t, int j) {
+          const uint32_t v = slot(2 * j + 1);
+#pragma unroll
+          for (int i = 0; i < kStepKeys / 16; ++i)
+            umma_ts(tmem + 256 + t * D, tmem + t * 128 + i * 8, umma_desc_v(v + i * 2048), idesc_o,
+                    j > 0 || i > 0);
+        };
+        for (int t = 0; t < tiles; ++t) {
+          if (!wait(&ctl->q_full[t], 0)) break;
+          if (t == 0 && !full(0)) break;
+          scores(t, 0);
+        }
+        if (ok) tc::umma_commit(&ctl->kv_empty[0]);
+        for (int j = 0; ok && j < steps; ++j) {
+          if (!full(2 * j + 1)) break;
+          for (int t = 0; t < tiles; ++t) {
+            if (!wait(&ctl->p_full[t], j & 1)) break;
+            output(t, j);
+            if (j + 1 < steps) {
+              if (t == 0 && !full(2 * j + 2)) break;
+              scores(t, j + 1);
+            } else {
+              tc::umma_commit(&ctl->o_full[t]);
+            }
+          }
+          if (!ok) break;
+          tc::umma_commit(&ctl->kv_empty[(2 * j + 1) % Cfg::kStages]);
+          if (j + 1 < steps) tc::umma_commit(&ctl->kv_empty[(2 * j + 2) % Cfg::kStages]);
+        }
+        if (!ok) tile_fault(ctl, fault);
+        tc::umma_commit(&ctl->drain);
+        tc::mbar_wait(&ctl->drain, 0, kWaitLimitNs, nullptr);
+      }
+    } else if (warp >= Cfg::kLoadWarp0) {
+      // ---- copies: slot 2j is K, slot 2j + 1 V of step j ----------------------------
+      constexpr int N = Cfg::kLoaders;
+      const int u = threadIdx.x - Cfg::kLoadWarp0 * 32;
+      const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
+      const int64_t v_rows = (int64_t)p.page_size * p.kv_heads;
+      auto row_of = [&](int j, int key) -> uint32_t {
+        const int pos = w.kv_begin + j * kStepKeys + key;
+        if (j >= steps || pos >= w.kv_end) return ~0u;
+        const int64_t page = p.kv_indices[w.page_base + pos / p.page_size];
+        return (uint32_t)((page * 2 * p.page_size + pos % p.page_size) * p.kv_heads + kvh);
+      };
+      constexpr int kOwn = (kStepKeys + N - 1) / N;  // keys whose row a thread looks up
+      uint32_t next[kOwn];
+      auto look_up = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) next[i] = u + i * N < kStepKeys ? row_of(j, u + i * N) : ~0u;
+      };
+      auto put = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+          if (u + i * N < kStepKeys) ctl->rows[j & 1][u + i * N] = next[i];
+      };
+      look_up(0);
+      put(0);
+      bool ok = loaders_all<N>(true);
+      // waits until slot i is free; the same answer for every thread
+      auto wait_empty = [&](int i) {
+        bool got = true;
+        if (i >= Cfg::kStages)
+          got = tc::mbar_wait(&ctl->kv_empty[i % Cfg::kStages],
+                              (uint32_t)(i / Cfg::kStages - 1) & 1u, kWaitLimitNs, &ctl->abort);
+        return loaders_all<N>(got);
+      };
+      for (int j = 0; ok && j < steps; ++j) {
+        look_up(j + 1);
+        const uint32_t* rws = ctl->rows[j & 1];
+#pragma unroll 1
+        for (int kind = 0; kind < 2; ++kind) {
+          const int i = 2 * j + kind;
+          ok = wait_empty(i);
+          if (!ok) break;
+          uint8_t* dst = ring + (i % Cfg::kStages) * Cfg::kKvBytes;
+          if constexpr (!Q8) {
+            constexpr int kChunks = D / 8;
+#pragma unroll 4
+            for (int x = u; x < kStepKeys * kChunks; x += N) {
+              const int key = x / kChunks, c = x % kChunks;
+              const uint32_t row = rws[key];
+              const bool there = row != ~0u;
+              const int64_t at = there ? (int64_t)row + kind * v_rows : 0;
+              cp_async16(dst + tile_at(key, c), cache + at * (2 * D) + c * 16, there);
+            }
+            cp_async_commit();
+            // the slot before this one has had a slot's time to arrive
+            cp_async_wait<1>();
+            fence_async_proxy();
+            if (i > 0) tc::mbar_arrive(&ctl->kv_full[(i - 1) % Cfg::kStages]);
+          } else {
+            constexpr int kChunks = D / 16;  // 16 codes each
+            constexpr int kEach = kStepKeys * kChunks / N;
+            uint4 v[kEach];
+            uint32_t ex[kEach];
+#pragma unroll
+            for (int x = 0; x < kEach; ++x) {
+              const int key = (x * N + u) / kChunks, c = (x * N + u) % kChunks;
+              const uint32_t row = rws[key];
+              v[x] = make_uint4(0, 0, 0, 0);
+              ex[x] = 127;
+              if (row != ~0u) {
+                const int64_t at = (int64_t)row + kind * v_rows;
+                v[x] = ld_nc_v4(cache + at * D + c * 16);
+                ex[x] = p.exponents[at];
+              }
+            }
+#pragma unroll
+            for (int x = 0; x < kEach; ++x) {
+              const int key = (x * N + u) / kChunks, c = (x * N + u) % kChunks;
+              const uint32_t codes[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+              uint32_t o[8];
+              M::dequantise16(codes, ex[x], o);
+              *reinterpret_cast<uint4*>(dst + tile_at(key, 2 * c)) =
+                  make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4*>(dst + tile_at(key, 2 * c + 1)) =
+                  make_uint4(o[4], o[5], o[6], o[7]);
+            }
+            fence_async_proxy();
+            tc::mbar_arrive(&ctl->kv_full[i % Cfg::kStages]);
+          }
+        }
+        if (!ok) break;
+        put(j + 1);  // read after the next slot's barrier
+      }
+      if constexpr (!Q8) {
+        cp_async_wait<0>();
+        fence_async_proxy();
+        if (ok && steps > 0) tc::mbar_arrive(&ctl->kv_full[(2 * steps - 1) % Cfg::kStages]);
+      }
+      if (!ok) tile_fault(ctl, fault);
+    }
+  }
+
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 8) tc::tmem_dealloc(tmem, 512);
+  if (w.splits == 1 || *reinterpret_cast<volatile int*>(&ctl->abort)) return;
+
+  // ---- the last piece of these rows to arrive joins them all --------------------
+  if (!arrive_last(counters + (int64_t)w.tile * p.kv_heads + kvh, w.splits, &last)) return;
+  if (warp >= 8) return;  // these gave their registers away
+  for (int u = threadIdx.x; (u & ~31) < rows * (D / 4); u += 256) {
+    const int r = u / (D / 4), d = (u - r * (D / 4)) * 4;
+    const bool fine = u >= rows * (D / 4) ||
+                      join_pieces<T, 256>(p, partial, partial_ml, w, kvh, r, d, D, group);
+    if (w.mixed) redo_rows<T, D, Q8>(p, w, kvh, group, r, fine);
+  }
+}
+
+template <typename T, int D, bool Q8>
+static int run_tile(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+                    int32_t* counters, int32_t* fault, int device, cudaStream_t stream,
+                    const char* what) {
+  using Cfg = TileCfg<D, Q8>;
+  auto kernel = attention_tile_kernel<T, D, Q8>;
+  cudaError_t err =
+      ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), device, Cfg::kSmemBytes);
+  if (err != cudaSuccess) return cuda_fail(err, what);
+  err = launch(kernel, dim3((unsigned)(num_items * p.kv_heads)), dim3(Cfg::kThreads),
+               Cfg::kSmemBytes, stream, p, items, partial, ml, counters, fault);
+  return err == cudaSuccess ? PACE_OK : cuda_fail(err, what);
+}
+
+int run_tile_rows(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+                  int32_t* counters, int32_t* fault, bool bf16, int device, cudaStream_t stream,
+                  const char* what) {
+  auto pick = [&](auto t) -> int {
+    using T = decltype(t);
+    auto go = [&](auto f) {
+      return f(p, items, num_items, partial, ml, counters, fault, device, stream, what);
+    };
+    if (p.head_dim == 128)
+      return p.exponents ? go(run_tile<T, 128, true>) : go(run_tile<T, 128, false>);
+    return p.exponents ? go(run_tile<T, 64, true>) : go(run_tile<T, 64, false>);
+  };
+  return bf16 ? pick(__nv_bfloat16{}) : pick(__half{});
+}
+
+}  // namespace attn
+}  // namespace pace
