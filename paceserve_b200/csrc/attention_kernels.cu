@@ -66,7 +66,10 @@ constexpr int kCounters = 16384;
 int cut_items(std::vector<Item>& items, int unit, int min_units, int64_t slots, int max_tiles,
               int* tiles) {
   int64_t total = 0;
-  auto cost = [&](const Item& w) { return ceil_div(std::max(w.kv_end - w.kv_begin, 0), unit); };
+  // cuts lie on multiples of the unit, so that only a sequence's first step is ragged
+  auto cost = [&](const Item& w) -> int64_t {
+    return w.kv_end > w.kv_begin ? ceil_div(w.kv_end, unit) - w.kv_begin / unit : 0;
+  };
   for (const Item& w : items) total += cost(w);
   const int64_t share = std::max<int64_t>(min_units, ceil_div(total, slots * kPiecesPerSlot));
   std::vector<Item> cut;
@@ -83,11 +86,11 @@ int cut_items(std::vector<Item>& items, int unit, int min_units, int64_t slots, 
       w.slot = slot;
       slot += (int)parts;
     }
-    const int begin = w.kv_begin, end = w.kv_end;
+    const int begin = w.kv_begin, end = w.kv_end, base = begin / unit * unit;
     for (int64_t k = 0; k < parts; ++k) {
       w.split = (int)k;
-      w.kv_begin = begin + (int)(n * k / parts) * unit;
-      w.kv_end = k + 1 < parts ? begin + (int)(n * (k + 1) / parts) * unit : end;
+      w.kv_begin = k > 0 ? base + (int)(n * k / parts) * unit : begin;
+      w.kv_end = k + 1 < parts ? base + (int)(n * (k + 1) / parts) * unit : end;
       cut.push_back(w);
     }
   }
@@ -339,7 +342,7 @@ extern "C" int pace_paged_attention(const pace_attention_plan* plan, const int32
     const bool bf16 = dtype == PACE_BF16;
     if (plan->num_many > 0) {
       const int st = run_tile_rows(
-          p, reinterpret_cast<const Item*>(plan_words + plan->many_offset), plan->num_many,
+          p, num_pages, reinterpret_cast<const Item*>(plan_words + plan->many_offset), plan->num_many,
           reinterpret_cast<float*>(base + ws.many), reinterpret_cast<float2*>(base + ws.many_ml),
           counters + kCounters / 2, fault_flags, bf16, guard.device(), stream, what);
       if (st != PACE_OK) return st;

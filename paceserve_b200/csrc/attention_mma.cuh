@@ -270,7 +270,7 @@ __device__ __forceinline__ bool join_pieces(const Problem& p, const float* parti
 }
 
 // The two tensor-core kernels' launchers.
-int run_tile_rows(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+int run_tile_rows(const Problem& p, int64_t num_pages, const Item* items, int num_items, float* partial, float2* ml,
                   int32_t* counters, int32_t* fault, bool bf16, int device, cudaStream_t stream,
                   const char* what);
 int run_few_rows(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,

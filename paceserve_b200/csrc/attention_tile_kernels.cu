@@ -49,7 +49,7 @@ struct TileCfg {
 };
 
 struct TileCtl {
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2];
   uint64_t kv_full[8], kv_empty[8];
   uint64_t drain;
   uint32_t tmem;
@@ -114,8 +114,39 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t u32x2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  return u32x2(__float_as_uint(lo), __float_as_uint(hi));
+}
+__device__ __forceinline__ float lo_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float hi_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// One box of a page: `slots` keys of one head, 64 dimensions, swizzled.
+__device__ __forceinline__ void tma_load_page(void* dst, const CUtensorMap* map, int dim, int head,
+                                              int slot, int page_kind, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(tc::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(dim), "r"(head), "r"(slot), "r"(page_kind),
+      "r"(tc::smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ void fence_async_proxy() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -137,14 +168,15 @@ __device__ __forceinline__ bool loaders_all(bool pred) {
 }
 
 // Bits of the keys j0 .. j0 + 31 that a row sees: lo <= j < hi, and of the
-// drafted ones hi .. end - 1 those of its tree row.
-__device__ __forceinline__ uint32_t seen_bits(int j0, int lo, int hi, int end, const uint64_t* tree) {
+// drafted ones base .. end - 1 those of its tree row.
+__device__ __forceinline__ uint32_t seen_bits(int j0, int lo, int hi, int base, int end,
+                                              const uint64_t* tree) {
   auto below = [](int n) -> uint32_t {  // the first n bits
     return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
   };
   uint32_t bits = below(hi - j0) & ~below(lo - j0);
-  if (tree && end > hi && j0 + 32 > hi && j0 < end) {
-    const int n0 = j0 - hi;  // node of bit 0
+  if (tree && j0 + 32 > base && j0 < end) {
+    const int n0 = j0 - base;  // node of bit 0
     uint32_t t;
     if (n0 < 0) {
       t = (uint32_t)tree[0] << -n0;  // -n0 < 32
@@ -152,18 +184,19 @@ __device__ __forceinline__ uint32_t seen_bits(int j0, int lo, int hi, int end, c
       const uint64_t w = tree[n0 >> 6];
       t = (uint32_t)(w >> (n0 & 63));
       // the next word, where the sequence reaches into it
-      if ((n0 & 63) > 32 && hi + ((n0 >> 6) + 1) * 64 < end)
+      if ((n0 & 63) > 32 && base + ((n0 >> 6) + 1) * 64 < end)
         t |= (uint32_t)(tree[(n0 >> 6) + 1] << (64 - (n0 & 63)));
     }
-    bits |= t & below(end - j0) & ~below(hi - j0);
+    bits |= t & below(end - j0) & ~below(max(base, lo) - j0);
   }
   return bits;
 }
 
 template <typename T, int D, bool Q8>
 __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
-    attention_tile_kernel(const Problem p, const Item* __restrict__ items, float* partial,
-                          float2* partial_ml, int32_t* counters, int32_t* fault) {
+    attention_tile_kernel(const Problem p, const __grid_constant__ CUtensorMap map, int box,
+                          const Item* __restrict__ items, float* partial, float2* partial_ml,
+                          int32_t* counters, int32_t* fault) {
   using Cfg = TileCfg<D, Q8>;
   using M = Mma<T>;
   extern __shared__ uint8_t smem_raw[];
@@ -178,14 +211,17 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   const int group = p.heads / p.kv_heads;
   const int rows = w.ntok * group;
   const int tiles = rows > kTileRowsEach ? 2 : 1;
-  const int steps = (w.kv_end - w.kv_begin + kStepKeys - 1) / kStepKeys;
+  // steps lie on multiples of 128 keys, so that pages do not straddle them
+  const int k_base = w.kv_begin & ~(kStepKeys - 1);
+  const int steps = w.kv_end > w.kv_begin ? (w.kv_end - k_base + kStepKeys - 1) / kStepKeys : 0;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&ctl->q_full[i], 128);
       tc::mbar_init(&ctl->s_full[i], 1);
-      tc::mbar_init(&ctl->p_full[i], 128);
+      tc::mbar_init(&ctl->p_full[i][0], 4);
+      tc::mbar_init(&ctl->p_full[i][1], 4);
       tc::mbar_init(&ctl->o_full[i], 1);
     }
     for (int i = 0; i < Cfg::kStages; ++i) {
@@ -221,6 +257,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
       if (p.tree_mask) tree = p.tree_mask + (int64_t)tok * p.tree_words;
     }
     const int end = tree ? min(info.pos, w.kv_end) : 0;  // of the drafted keys
+    const int lo = max(info.lo, w.kv_begin), hi = min(info.hi, w.kv_end);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     if (t < tiles) {
@@ -275,7 +312,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         tmem_ld32(ts + 96, sr + 96);
         tc::tmem_wait_ld(sr);
         float sc = scale2;
-        const int j0 = w.kv_begin + j * kStepKeys;
+        const int j0 = k_base + j * kStepKeys;
         if (p.cap > 0.f) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
@@ -290,21 +327,25 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
             sr[i] = __float_as_uint(__uint_as_float(sr[i]) * sc - slope * fabsf(d0 - (float)i));
           sc = 1.f;
         }
-        const bool whole = j0 >= info.lo && j0 + kStepKeys <= min(info.hi, w.kv_end);
+        const bool whole = j0 >= lo && j0 + kStepKeys <= hi;
         if (!__all_sync(0xffffffffu, whole)) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t bits =
-                seen_bits(j0 + 32 * k, info.lo, min(info.hi, w.kv_end), end, tree);
+            const uint32_t bits = seen_bits(j0 + 32 * k, lo, hi, info.hi, end, tree);
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!(bits >> i & 1)) sr[32 * k + i] = 0xff800000u;
           }
           __syncwarp();
         }
-        float top = -INFINITY;
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 128; ++i) top = fmaxf(top, __uint_as_float(sr[i]));
+        for (int i = 0; i < 128; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(sr[i + 2 * k])),
+                            __uint_as_float(sr[i + 2 * k + 1]));
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         top *= sc;
         if (j == 0) {
           m = top;
@@ -328,24 +369,29 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
           }
         }
         const float b = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t sum[2] = {0, 0};  // two pairs of partial sums
+        const uint64_t sc2 = f32x2(sc, sc), b2 = f32x2(-b, -b);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float x = exp2_approx(fmaf(__uint_as_float(sr[32 * k + 2 * i]), sc, -b));
-            const float y = exp2_approx(fmaf(__uint_as_float(sr[32 * k + 2 * i + 1]), sc, -b));
-            sum[2 * (i & 1)] += x;
-            sum[2 * (i & 1) + 1] += y;
+            const uint64_t z = fma2(u32x2(sr[32 * k + 2 * i], sr[32 * k + 2 * i + 1]), sc2, b2);
+            const float x = exp2_approx(lo_of(z)), y = exp2_approx(hi_of(z));
+            sum[i & 1] = add2(sum[i & 1], f32x2(x, y));
             pk[i] = M::pack(x, y);
           }
           tmem_st16(ts + 16 * k, pk);
+          if (k & 1) {
+            // half of P is in place: its product may begin
+            tmem_wait_st();
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&ctl->p_full[t][k >> 1]);
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-        tc::tc_fence_before();
-        tc::mbar_arrive(&ctl->p_full[t]);
+        sum[0] = add2(sum[0], sum[1]);
+        l += lo_of(sum[0]) + hi_of(sum[0]);
       }
       // ---- the tile's output ----------------------------------------------------
       if (ok && steps > 0)
@@ -444,12 +490,14 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
           }
           tc::umma_commit(&ctl->s_full[t]);
         };
-        auto output = [&](int t, int j) {
+        auto output = [&](int t, int j, int half) {
           const uint32_t v = slot(2 * j + 1);
 #pragma unroll
-          for (int i = 0; i < kStepKeys / 16; ++i)
+          for (int x = 0; x < kStepKeys / 32; ++x) {
+            const int i = half * (kStepKeys / 32) + x;
             umma_ts(tmem + 256 + t * D, tmem + t * 128 + i * 8, umma_desc_v(v + i * 2048), idesc_o,
                     j > 0 || i > 0);
+          }
         };
         for (int t = 0; t < tiles; ++t) {
           if (!wait(&ctl->q_full[t], 0)) break;
@@ -460,8 +508,10 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         for (int j = 0; ok && j < steps; ++j) {
           if (!full(2 * j + 1)) break;
           for (int t = 0; t < tiles; ++t) {
-            if (!wait(&ctl->p_full[t], j & 1)) break;
-            output(t, j);
+            if (!wait(&ctl->p_full[t][0], j & 1)) break;
+            output(t, j, 0);
+            if (!wait(&ctl->p_full[t][1], j & 1)) break;
+            output(t, j, 1);
             if (j + 1 < steps) {
               if (t == 0 && !full(2 * j + 2)) break;
               scores(t, j + 1);
@@ -484,8 +534,8 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
       const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
       const int64_t v_rows = (int64_t)p.page_size * p.kv_heads;
       auto row_of = [&](int j, int key) -> uint32_t {
-        const int pos = w.kv_begin + j * kStepKeys + key;
-        if (j >= steps || pos >= w.kv_end) return ~0u;
+        const int pos = k_base + j * kStepKeys + key;
+        if (j >= steps || pos < w.kv_begin || pos >= w.kv_end) return ~0u;
         const int64_t page = p.kv_indices[w.page_base + pos / p.page_size];
         return (uint32_t)((page * 2 * p.page_size + pos % p.page_size) * p.kv_heads + kvh);
       };
@@ -511,16 +561,43 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
                               (uint32_t)(i / Cfg::kStages - 1) & 1u, kWaitLimitNs, &ctl->abort);
         return loaders_all<N>(got);
       };
+      int pending = -1;  // slot whose cp.async copies are under way
       for (int j = 0; ok && j < steps; ++j) {
+        const int j0 = k_base + j * kStepKeys;
         look_up(j + 1);
         const uint32_t* rws = ctl->rows[j & 1];
+        // whole steps come box by box through TMA, where the pages allow (box > 0); ragged ones
+        // by 16-byte copies, which put zeros for the keys outside the piece
+        const bool by_tma = !Q8 && box > 0 && j0 >= w.kv_begin && j0 + kStepKeys <= w.kv_end;
 #pragma unroll 1
         for (int kind = 0; kind < 2; ++kind) {
           const int i = 2 * j + kind;
           ok = wait_empty(i);
           if (!ok) break;
           uint8_t* dst = ring + (i % Cfg::kStages) * Cfg::kKvBytes;
-          if constexpr (!Q8) {
+          if (by_tma) {
+            if (u < 32) {
+              if (u == 0)
+                tc::mbar_arrive_expect_tx(&ctl->kv_full[i % Cfg::kStages], Cfg::kKvBytes);
+              __syncwarp();
+              constexpr int kHalves = D / 64;
+              for (int x = u; x < kStepKeys / box * kHalves; x += 32) {
+                const int key = x / kHalves * box, half = x % kHalves;
+                const int pos = j0 + key;
+                tma_load_page(dst + half * 16384 + key * 128, &map, half * 64, kvh,
+                              pos % p.page_size,
+                              p.kv_indices[w.page_base + pos / p.page_size] * 2 + kind,
+                              &ctl->kv_full[i % Cfg::kStages]);
+              }
+            }
+            if (pending >= 0) {
+              cp_async_wait<0>();
+              fence_async_proxy();
+              tc::mbar_arrive(&ctl->kv_full[pending % Cfg::kStages]);
+              pending = -1;
+            }
+            if (u != 0) tc::mbar_arrive(&ctl->kv_full[i % Cfg::kStages]);
+          } else if constexpr (!Q8) {
             constexpr int kChunks = D / 8;
 #pragma unroll 4
             for (int x = u; x < kStepKeys * kChunks; x += N) {
@@ -532,9 +609,12 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
             }
             cp_async_commit();
             // the slot before this one has had a slot's time to arrive
-            cp_async_wait<1>();
-            fence_async_proxy();
-            if (i > 0) tc::mbar_arrive(&ctl->kv_full[(i - 1) % Cfg::kStages]);
+            if (pending >= 0) {
+              cp_async_wait<1>();
+              fence_async_proxy();
+              tc::mbar_arrive(&ctl->kv_full[pending % Cfg::kStages]);
+            }
+            pending = i;
           } else {
             constexpr int kChunks = D / 16;  // 16 codes each
             constexpr int kEach = kStepKeys * kChunks / N;
@@ -573,7 +653,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
       if constexpr (!Q8) {
         cp_async_wait<0>();
         fence_async_proxy();
-        if (ok && steps > 0) tc::mbar_arrive(&ctl->kv_full[(2 * steps - 1) % Cfg::kStages]);
+        if (pending >= 0) tc::mbar_arrive(&ctl->kv_full[pending % Cfg::kStages]);
       }
       if (!ok) tile_fault(ctl, fault);
     }
@@ -595,8 +675,30 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   }
 }
 
+// Tensor map of a 16-bit cache as [2 * pages, page_size, kv_heads, D], boxes of
+// `box` keys of one head's 64 dimensions.
+static int make_page_map(CUtensorMap* map, const Problem& p, bool bf16, int64_t num_pages, int box,
+                         const char* what) {
+  tc::EncodeTiledFn enc = tc::encode_tiled();
+  if (!enc) return fail(PACE_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", what);
+  const cuuint64_t row = (cuuint64_t)p.head_dim * 2;
+  const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.kv_heads,
+                              (cuuint64_t)p.page_size, (cuuint64_t)(2 * num_pages)};
+  const cuuint64_t strides[3] = {row, row * p.kv_heads, row * p.kv_heads * p.page_size};
+  const cuuint32_t boxes[4] = {64u, 1u, (cuuint32_t)box, 1u};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+          const_cast<void*>(p.cache), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(PACE_ERR_INVALID_ARGUMENT, "%s: tensor map rejected (CUresult %d)", what, (int)r);
+  return PACE_OK;
+}
+
 template <typename T, int D, bool Q8>
-static int run_tile(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+static int run_tile(const Problem& p, int64_t num_pages, const Item* items, int num_items, float* partial, float2* ml,
                     int32_t* counters, int32_t* fault, int device, cudaStream_t stream,
                     const char* what) {
   using Cfg = TileCfg<D, Q8>;
@@ -604,18 +706,28 @@ static int run_tile(const Problem& p, const Item* items, int num_items, float* p
   cudaError_t err =
       ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), device, Cfg::kSmemBytes);
   if (err != cudaSuccess) return cuda_fail(err, what);
+  // A TMA box is a page's share of a 128-key step, and its 8-row swizzle groups have to be the
+  // step's: pages of 8 to 128 keys that divide 128, or multiples of 128.
+  CUtensorMap map{};
+  int box = 0;
+  if (!Q8 && p.page_size >= 8 && (128 % p.page_size == 0 || p.page_size % 128 == 0) &&
+      num_pages < (1 << 30)) {
+    box = p.page_size < 128 ? p.page_size : 128;
+    const int st = make_page_map(&map, p, std::is_same<T, __nv_bfloat16>::value, num_pages, box, what);
+    if (st != PACE_OK) return st;
+  }
   err = launch(kernel, dim3((unsigned)(num_items * p.kv_heads)), dim3(Cfg::kThreads),
-               Cfg::kSmemBytes, stream, p, items, partial, ml, counters, fault);
+               Cfg::kSmemBytes, stream, p, map, box, items, partial, ml, counters, fault);
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, what);
 }
 
-int run_tile_rows(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+int run_tile_rows(const Problem& p, int64_t num_pages, const Item* items, int num_items, float* partial, float2* ml,
                   int32_t* counters, int32_t* fault, bool bf16, int device, cudaStream_t stream,
                   const char* what) {
   auto pick = [&](auto t) -> int {
     using T = decltype(t);
     auto go = [&](auto f) {
-      return f(p, items, num_items, partial, ml, counters, fault, device, stream, what);
+      return f(p, num_pages, items, num_items, partial, ml, counters, fault, device, stream, what);
     };
     if (p.head_dim == 128)
       return p.exponents ? go(run_tile<T, 128, true>) : go(run_tile<T, 128, false>);
