@@ -40,8 +40,13 @@ struct TileCfg {
   static constexpr int kThreads = kLoadWarp0 * 32 + kLoaders;
   static constexpr int kKvBytes = kStepKeys * D * 2;
   static constexpr int kQBytes = kTileRowsEach * D * 2;
-  static constexpr int kStages = D == 128 ? 4 : 8;
-  static constexpr int kSmemBytes = 2 * kQBytes + kStages * kKvBytes + 1024 + 2048;
+  static constexpr int kStages = D == 64 ? 8 : Q8 ? 3 : 4;
+  // a quantised cache's codes, as copied: K or V of a step
+  static constexpr int kCodeBytes = kStepKeys * D;
+  static constexpr int kCodeStages = 3;
+  static constexpr int kCodeRingBytes = Q8 ? kCodeStages * kCodeBytes : 0;
+  static constexpr int kSmemBytes =
+      2 * kQBytes + kStages * kKvBytes + kCodeRingBytes + 1024 + 2048;
   // registers per thread after the split; the sum over the warpgroups is what
   // the block was launched with
   static constexpr int kSoftmaxRegs = Q8 ? 176 : 208;
@@ -51,16 +56,34 @@ struct TileCfg {
 struct TileCtl {
   uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2];
   uint64_t kv_full[8], kv_empty[8];
+  uint64_t code_full[3], code_empty[3];
   uint64_t drain;
   uint32_t tmem;
   int abort;
-  uint32_t rows[2][kStepKeys];  // cache row (K part) of each key of a step; ~0: none
+  uint8_t exps[3][kStepKeys];   // exponents of the keys of a slot of codes
+  uint32_t rows[kStepKeys];     // cache row (K part) of each key of a step; ~0: none
 };
 static_assert(sizeof(TileCtl) <= 2048, "");
 
 __device__ __forceinline__ void tile_fault(TileCtl* ctl, int32_t* fault) {
   *reinterpret_cast<volatile int*>(&ctl->abort) = 1;
   if (fault) atomicOr(fault, kFaultTimeout);
+}
+
+// tc::mbar_wait with the timer out of the way: its read takes longer than most of
+// these waits, so it is looked at once in many tries.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, const TileCtl* ctl) {
+  if (tc::mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = 0;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 128; ++i)
+      if (tc::mbar_try_wait(bar, parity)) return true;
+    if (*reinterpret_cast<const volatile int*>(&ctl->abort)) return false;
+    const uint64_t t = tc::globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > kWaitLimitNs) return false;
+  }
 }
 
 // Byte offset of 16-byte chunk `c` (8 dimensions) of row r of a 128-row tile:
@@ -152,6 +175,11 @@ __device__ __forceinline__ void fence_async_proxy() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+__device__ __forceinline__ void mbar_arrive_many(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(count)
+               : "memory");
+}
+
 // Barrier of the copying threads that also ANDs `pred` over them.
 template <int N>
 __device__ __forceinline__ bool loaders_all(bool pred) {
@@ -204,7 +232,8 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* ring = smem + 2 * Cfg::kQBytes;
-  TileCtl* ctl = reinterpret_cast<TileCtl*>(ring + Cfg::kStages * Cfg::kKvBytes);
+  uint8_t* codes = ring + Cfg::kStages * Cfg::kKvBytes;
+  TileCtl* ctl = reinterpret_cast<TileCtl*>(codes + Cfg::kCodeRingBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.x % p.kv_heads;
   const Item w = items[blockIdx.x / p.kv_heads];
@@ -227,6 +256,10 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
     for (int i = 0; i < Cfg::kStages; ++i) {
       tc::mbar_init(&ctl->kv_full[i], Cfg::kLoaders);
       tc::mbar_init(&ctl->kv_empty[i], 1);
+    }
+    for (int i = 0; i < Cfg::kCodeStages; ++i) {
+      tc::mbar_init(&ctl->code_full[i], 3);  // the codes' warp, two of the exponents
+      tc::mbar_init(&ctl->code_empty[i], Cfg::kLoaders);
     }
     tc::mbar_init(&ctl->drain, 1);
     ctl->abort = 0;
@@ -302,7 +335,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
       const uint32_t to = tmem + lanes + 256u + (uint32_t)(t * D);
       for (int j = 0; j < steps; ++j) {
         ok = __all_sync(0xffffffffu,
-                        tc::mbar_wait(&ctl->s_full[t], j & 1, kWaitLimitNs, &ctl->abort));
+                        wait_for(&ctl->s_full[t], j & 1, ctl));
         if (!ok) break;
         tc::tc_fence_after();
         uint32_t sr[128];
@@ -396,7 +429,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
       // ---- the tile's output ----------------------------------------------------
       if (ok && steps > 0)
         ok = __all_sync(0xffffffffu,
-                        tc::mbar_wait(&ctl->o_full[t], 0, kWaitLimitNs, &ctl->abort));
+                        wait_for(&ctl->o_full[t], 0, ctl));
       if (!ok) tile_fault(ctl, fault);
       if (ok) {
         tc::tc_fence_after();
@@ -471,7 +504,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         constexpr uint32_t idesc_o = tc::umma_idesc_f16(kBf16, 128, D) | (1u << 16);  // B MN-major
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-          ok = ok && tc::mbar_wait(bar, parity, kWaitLimitNs, &ctl->abort);
+          ok = ok && wait_for(bar, parity, ctl);
           tc::tc_fence_after();
           return ok;
         };
@@ -527,12 +560,133 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         tc::umma_commit(&ctl->drain);
         tc::mbar_wait(&ctl->drain, 0, kWaitLimitNs, nullptr);
       }
+    } else if (Q8 && box > 0 && warp < Cfg::kLoadWarp0) {
+      // ---- quantised pages by TMA: codes (warp 9) and exponents (warps 10, 11) ------
+      // Keys outside the piece get the exponent 0: whatever codes lie there, they
+      // come out finite.
+      bool ok = true;
+      if (warp == 9) {
+        int page = 0;
+        constexpr int kBoxes = kStepKeys / 8;  // at most
+        static_assert(kBoxes <= 32, "");
+        const int key = lane * box;
+        auto look_up = [&](int j) {
+          const int pos = k_base + j * kStepKeys + key;
+          return key < kStepKeys && pos < w.kv_end ? p.kv_indices[w.page_base + pos / p.page_size] : -1;
+        };
+        page = look_up(0);
+        for (int i = 0; ok && i < 2 * steps; ++i) {
+          const int s = i % Cfg::kCodeStages;
+          if (i >= Cfg::kCodeStages)
+            ok = __all_sync(0xffffffffu, wait_for(&ctl->code_empty[s],
+                                                  (uint32_t)(i / Cfg::kCodeStages - 1) & 1u, ctl));
+          if (!ok) break;
+          const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+          if (lane == 0)
+            tc::mbar_arrive_expect_tx(&ctl->code_full[s], (uint32_t)(__popc(there) * box * D));
+          __syncwarp();
+          if (page >= 0) {
+            const int pos = k_base + (i >> 1) * kStepKeys + key;
+            tma_load_page(codes + s * Cfg::kCodeBytes + key * D, &map, 0, kvh, pos % p.page_size,
+                          page * 2 + (i & 1), &ctl->code_full[s]);
+          }
+          if (i & 1) page = look_up((i >> 1) + 1);
+        }
+      } else {
+        const int u = threadIdx.x - 10 * 32;  // keys u and u + 64 of each step
+        const int64_t v_rows = (int64_t)p.page_size * p.kv_heads;
+        auto row_of = [&](int j, int key) -> int64_t {
+          const int pos = k_base + j * kStepKeys + key;
+          if (j >= steps || pos < w.kv_begin || pos >= w.kv_end) return -1;
+          const int64_t page = p.kv_indices[w.page_base + pos / p.page_size];
+          return (page * 2 * p.page_size + pos % p.page_size) * p.kv_heads + kvh;
+        };
+        // rows two steps ahead, exponents one step ahead: their loads depend on each other
+        int64_t rows[2] = {row_of(0, u), row_of(0, u + 64)};
+        uint8_t ex[2][2];
+        auto load = [&]() {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int kind = 0; kind < 2; ++kind)
+              ex[kind][k] = rows[k] >= 0 ? p.exponents[rows[k] + kind * v_rows] : 0;
+        };
+        load();
+        rows[0] = row_of(1, u);
+        rows[1] = row_of(1, u + 64);
+        for (int i = 0; ok && i < 2 * steps; ++i) {
+          const int s = i % Cfg::kCodeStages;
+          if (i >= Cfg::kCodeStages)
+            ok = __all_sync(0xffffffffu, wait_for(&ctl->code_empty[s],
+                                                  (uint32_t)(i / Cfg::kCodeStages - 1) & 1u, ctl));
+          if (!ok) break;
+          ctl->exps[s][u] = ex[i & 1][0];
+          ctl->exps[s][u + 64] = ex[i & 1][1];
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&ctl->code_full[s]);
+          if (i & 1) {
+            load();
+            rows[0] = row_of((i >> 1) + 2, u);
+            rows[1] = row_of((i >> 1) + 2, u + 64);
+          }
+        }
+      }
+      if (!ok) tile_fault(ctl, fault);
+    } else if (Q8 && box > 0) {
+      // ---- codes to 16-bit values, slot by slot -------------------------------------
+      constexpr int N = Cfg::kLoaders;
+      constexpr int kChunks = D / 16;
+      constexpr int kEach = kStepKeys * kChunks / N;
+      const int u = threadIdx.x - Cfg::kLoadWarp0 * 32;
+      bool ok = true;
+      for (int i = 0; ok && i < 2 * steps; ++i) {
+        const int s = i % Cfg::kCodeStages, d = i % Cfg::kStages;
+        ok = wait_for(&ctl->code_full[s], (uint32_t)(i / Cfg::kCodeStages) & 1u, ctl);
+        if (ok && i >= Cfg::kStages)
+          ok = wait_for(&ctl->kv_empty[d], (uint32_t)(i / Cfg::kStages - 1) & 1u, ctl);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint8_t* src = codes + s * Cfg::kCodeBytes;
+        uint8_t* dst = ring + d * Cfg::kKvBytes;
+#pragma unroll 4
+        for (int x = 0; x < kEach; ++x) {
+          const int key = (x * N + u) / kChunks, c = (x * N + u) % kChunks;
+          const uint4 v = *reinterpret_cast<const uint4*>(src + key * D + c * 16);
+          const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
+          uint32_t o[8];
+          M::dequantise16(w4, ctl->exps[s][key], o);
+          *reinterpret_cast<uint4*>(dst + tile_at(key, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(dst + tile_at(key, 2 * c + 1)) =
+              make_uint4(o[4], o[5], o[6], o[7]);
+        }
+        fence_async_proxy();
+        tc::mbar_arrive(&ctl->code_empty[s]);
+        tc::mbar_arrive(&ctl->kv_full[d]);
+      }
+      if (!ok) tile_fault(ctl, fault);
     } else if (warp >= Cfg::kLoadWarp0) {
       // ---- copies: slot 2j is K, slot 2j + 1 V of step j ----------------------------
+      // Whole steps come box by box through TMA, issued by the first of these warps
+      // alone, where the pages allow it (box > 0).  The others, ragged ones among
+      // them, take all threads: 16-byte copies (zeros for keys outside the piece) of
+      // a 16-bit cache, loads and unpacking of a quantised one.
       constexpr int N = Cfg::kLoaders;
       const int u = threadIdx.x - Cfg::kLoadWarp0 * 32;
       const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
       const int64_t v_rows = (int64_t)p.page_size * p.kv_heads;
+      auto by_tma = [&](int j) {
+        const int j0 = k_base + j * kStepKeys;
+        return !Q8 && box > 0 && j0 >= w.kv_begin && j0 + kStepKeys <= w.kv_end;
+      };
+      constexpr int kHalves = D / 64;
+      const int box_key = u / kHalves * (box > 0 ? box : 1), box_half = u % kHalves;
+      const bool has_box = u < 32 && box > 0 && box_key < kStepKeys;
+      auto page_of = [&](int j) {  // of this lane's box
+        const int pos = k_base + j * kStepKeys + box_key;
+        return has_box && j < steps && pos < w.kv_end ? p.kv_indices[w.page_base + pos / p.page_size]
+                                                      : 0;
+      };
+      int page = u < 32 ? page_of(0) : 0;
       auto row_of = [&](int j, int key) -> uint32_t {
         const int pos = k_base + j * kStepKeys + key;
         if (j >= steps || pos < w.kv_begin || pos >= w.kv_end) return ~0u;
@@ -545,59 +699,67 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) next[i] = u + i * N < kStepKeys ? row_of(j, u + i * N) : ~0u;
       };
-      auto put = [&](int j) {
+      look_up(0);
+      bool ok = true;
+      int pending = -1;  // slot whose cp.async copies are under way
+      auto flush = [&](bool all) {
+        if (pending < 0) return;
+        if (all)
+          cp_async_wait<0>();
+        else
+          cp_async_wait<1>();
+        fence_async_proxy();
+        tc::mbar_arrive(&ctl->kv_full[pending % Cfg::kStages]);
+      };
+      for (int j = 0; j < steps; ++j) {
+        if (by_tma(j)) {
+          if (u < 32) {
+            const int pos = k_base + j * kStepKeys + box_key;
+            for (int kind = 0; ok && kind < 2; ++kind) {
+              const int i = 2 * j + kind, s = i % Cfg::kStages;
+              if (i >= Cfg::kStages)
+                ok = __all_sync(0xffffffffu, wait_for(&ctl->kv_empty[s],
+                                                      (uint32_t)(i / Cfg::kStages - 1) & 1u, ctl));
+              if (!ok) break;  // and on to the next step that all threads take, to say so
+              if (lane == 0) {
+                tc::mbar_arrive_expect_tx(&ctl->kv_full[s], Cfg::kKvBytes);
+                mbar_arrive_many(&ctl->kv_full[s], N - 1);
+              }
+              __syncwarp();
+              if (has_box)
+                tma_load_page(ring + s * Cfg::kKvBytes + box_half * 16384 + box_key * 128, &map,
+                              box_half * 64, kvh, pos % p.page_size, page * 2 + kind,
+                              &ctl->kv_full[s]);
+            }
+            page = page_of(j + 1);
+          }
+          if (pending >= 0) {
+            flush(true);
+            pending = -1;
+          }
+          if (j + 1 < steps && !by_tma(j + 1)) look_up(j + 1);
+          continue;
+        }
+        ok = loaders_all<N>(ok);  // the rows of the step before are read
+        if (!ok) break;
+        const uint32_t* rws = ctl->rows;
 #pragma unroll
         for (int i = 0; i < kOwn; ++i)
-          if (u + i * N < kStepKeys) ctl->rows[j & 1][u + i * N] = next[i];
-      };
-      look_up(0);
-      put(0);
-      bool ok = loaders_all<N>(true);
-      // waits until slot i is free; the same answer for every thread
-      auto wait_empty = [&](int i) {
-        bool got = true;
-        if (i >= Cfg::kStages)
-          got = tc::mbar_wait(&ctl->kv_empty[i % Cfg::kStages],
-                              (uint32_t)(i / Cfg::kStages - 1) & 1u, kWaitLimitNs, &ctl->abort);
-        return loaders_all<N>(got);
-      };
-      int pending = -1;  // slot whose cp.async copies are under way
-      for (int j = 0; ok && j < steps; ++j) {
-        const int j0 = k_base + j * kStepKeys;
-        look_up(j + 1);
-        const uint32_t* rws = ctl->rows[j & 1];
-        // whole steps come box by box through TMA, where the pages allow (box > 0); ragged ones
-        // by 16-byte copies, which put zeros for the keys outside the piece
-        const bool by_tma = !Q8 && box > 0 && j0 >= w.kv_begin && j0 + kStepKeys <= w.kv_end;
+          if (u + i * N < kStepKeys) ctl->rows[u + i * N] = next[i];
+        if (j + 1 < steps && !by_tma(j + 1))
+          look_up(j + 1);
+        else if (u < 32)
+          page = page_of(j + 1);
 #pragma unroll 1
         for (int kind = 0; kind < 2; ++kind) {
           const int i = 2 * j + kind;
-          ok = wait_empty(i);
+          if (ok && i >= Cfg::kStages)
+            ok = wait_for(&ctl->kv_empty[i % Cfg::kStages],
+                          (uint32_t)(i / Cfg::kStages - 1) & 1u, ctl);
+          ok = loaders_all<N>(ok);  // also: the step's rows are in place
           if (!ok) break;
           uint8_t* dst = ring + (i % Cfg::kStages) * Cfg::kKvBytes;
-          if (by_tma) {
-            if (u < 32) {
-              if (u == 0)
-                tc::mbar_arrive_expect_tx(&ctl->kv_full[i % Cfg::kStages], Cfg::kKvBytes);
-              __syncwarp();
-              constexpr int kHalves = D / 64;
-              for (int x = u; x < kStepKeys / box * kHalves; x += 32) {
-                const int key = x / kHalves * box, half = x % kHalves;
-                const int pos = j0 + key;
-                tma_load_page(dst + half * 16384 + key * 128, &map, half * 64, kvh,
-                              pos % p.page_size,
-                              p.kv_indices[w.page_base + pos / p.page_size] * 2 + kind,
-                              &ctl->kv_full[i % Cfg::kStages]);
-              }
-            }
-            if (pending >= 0) {
-              cp_async_wait<0>();
-              fence_async_proxy();
-              tc::mbar_arrive(&ctl->kv_full[pending % Cfg::kStages]);
-              pending = -1;
-            }
-            if (u != 0) tc::mbar_arrive(&ctl->kv_full[i % Cfg::kStages]);
-          } else if constexpr (!Q8) {
+          if constexpr (!Q8) {
             constexpr int kChunks = D / 8;
 #pragma unroll 4
             for (int x = u; x < kStepKeys * kChunks; x += N) {
@@ -608,12 +770,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
               cp_async16(dst + tile_at(key, c), cache + at * (2 * D) + c * 16, there);
             }
             cp_async_commit();
-            // the slot before this one has had a slot's time to arrive
-            if (pending >= 0) {
-              cp_async_wait<1>();
-              fence_async_proxy();
-              tc::mbar_arrive(&ctl->kv_full[pending % Cfg::kStages]);
-            }
+            flush(false);  // the slot before this one has had a slot's time to arrive
             pending = i;
           } else {
             constexpr int kChunks = D / 16;  // 16 codes each
@@ -635,9 +792,9 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
 #pragma unroll
             for (int x = 0; x < kEach; ++x) {
               const int key = (x * N + u) / kChunks, c = (x * N + u) % kChunks;
-              const uint32_t codes[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+              const uint32_t w4[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
               uint32_t o[8];
-              M::dequantise16(codes, ex[x], o);
+              M::dequantise16(w4, ex[x], o);
               *reinterpret_cast<uint4*>(dst + tile_at(key, 2 * c)) =
                   make_uint4(o[0], o[1], o[2], o[3]);
               *reinterpret_cast<uint4*>(dst + tile_at(key, 2 * c + 1)) =
@@ -648,12 +805,10 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
           }
         }
         if (!ok) break;
-        put(j + 1);  // read after the next slot's barrier
       }
       if constexpr (!Q8) {
         cp_async_wait<0>();
-        fence_async_proxy();
-        if (pending >= 0) tc::mbar_arrive(&ctl->kv_full[pending % Cfg::kStages]);
+        if (ok) flush(true);
       }
       if (!ok) tile_fault(ctl, fault);
     }
@@ -675,23 +830,25 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   }
 }
 
-// Tensor map of a 16-bit cache as [2 * pages, page_size, kv_heads, D], boxes of
-// `box` keys of one head's 64 dimensions.
-static int make_page_map(CUtensorMap* map, const Problem& p, bool bf16, int64_t num_pages, int box,
-                         const char* what) {
+// Tensor map of the cache as [2 * pages, page_size, kv_heads, D], boxes of `box`
+// keys of one head: 64 dimensions, swizzled, of a 16-bit cache, a quantised
+// one's whole rows as they are.
+static int make_page_map(CUtensorMap* map, const Problem& p, CUtensorMapDataType type,
+                         int64_t num_pages, int box, const char* what) {
   tc::EncodeTiledFn enc = tc::encode_tiled();
   if (!enc) return fail(PACE_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", what);
-  const cuuint64_t row = (cuuint64_t)p.head_dim * 2;
+  const bool codes = type == CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const cuuint64_t row = (cuuint64_t)p.head_dim * (codes ? 1 : 2);
   const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.kv_heads,
                               (cuuint64_t)p.page_size, (cuuint64_t)(2 * num_pages)};
   const cuuint64_t strides[3] = {row, row * p.kv_heads, row * p.kv_heads * p.page_size};
-  const cuuint32_t boxes[4] = {64u, 1u, (cuuint32_t)box, 1u};
+  const cuuint32_t boxes[4] = {codes ? (cuuint32_t)p.head_dim : 64u, 1u, (cuuint32_t)box, 1u};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r =
-      enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-          const_cast<void*>(p.cache), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      enc(map, type, 4, const_cast<void*>(p.cache), dims, strides, boxes, estr,
+          CU_TENSOR_MAP_INTERLEAVE_NONE,
+          codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(PACE_ERR_INVALID_ARGUMENT, "%s: tensor map rejected (CUresult %d)", what, (int)r);
   return PACE_OK;
@@ -710,10 +867,14 @@ static int run_tile(const Problem& p, int64_t num_pages, const Item* items, int 
   // step's: pages of 8 to 128 keys that divide 128, or multiples of 128.
   CUtensorMap map{};
   int box = 0;
-  if (!Q8 && p.page_size >= 8 && (128 % p.page_size == 0 || p.page_size % 128 == 0) &&
+  if (p.page_size >= 8 && (128 % p.page_size == 0 || p.page_size % 128 == 0) &&
       num_pages < (1 << 30)) {
     box = p.page_size < 128 ? p.page_size : 128;
-    const int st = make_page_map(&map, p, std::is_same<T, __nv_bfloat16>::value, num_pages, box, what);
+    const CUtensorMapDataType type = Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : std::is_same<T, __nv_bfloat16>::value
+                                         ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const int st = make_page_map(&map, p, type, num_pages, box, what);
     if (st != PACE_OK) return st;
   }
   err = launch(kernel, dim3((unsigned)(num_items * p.kv_heads)), dim3(Cfg::kThreads),
