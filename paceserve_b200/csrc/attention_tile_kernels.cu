@@ -40,7 +40,7 @@ struct TileCfg {
   static constexpr int kThreads = kLoadWarp0 * 32 + kLoaders;
   static constexpr int kKvBytes = kStepKeys * D * 2;
   static constexpr int kQBytes = kTileRowsEach * D * 2;
-  static constexpr int kStages = D == 64 ? 8 : Q8 ? 3 : 4;
+  static constexpr int kStages = D == 64 ? 8 : Q8 ? 3 : 5;
   // a quantised cache's codes, as copied: K or V of a step
   static constexpr int kCodeBytes = kStepKeys * D;
   static constexpr int kCodeStages = 3;
@@ -60,6 +60,7 @@ struct TileCtl {
   uint64_t drain;
   uint32_t tmem;
   int abort;
+  bool last;
   uint8_t exps[3][kStepKeys];   // exponents of the keys of a slot of codes
   uint32_t rows[kStepKeys];     // cache row (K part) of each key of a step; ~0: none
 };
@@ -228,7 +229,6 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   using Cfg = TileCfg<D, Q8>;
   using M = Mma<T>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ bool last;
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* ring = smem + 2 * Cfg::kQBytes;
@@ -337,6 +337,13 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         ok = __all_sync(0xffffffffu,
                         wait_for(&ctl->s_full[t], j & 1, ctl));
         if (!ok) break;
+        // the last tile's scores are the last reader of K of this step and come behind the last
+        // reader of V of the step before: their slots are free.  Said here, not by commits of the
+        // MMA thread, each of which would hold up its next MMA.
+        if (t == tiles - 1 && r == 0) {
+          tc::mbar_arrive(&ctl->kv_empty[(2 * j) % Cfg::kStages]);
+          if (j > 0) tc::mbar_arrive(&ctl->kv_empty[(2 * j - 1) % Cfg::kStages]);
+        }
         tc::tc_fence_after();
         uint32_t sr[128];
         tmem_ld32(ts, sr);
@@ -537,7 +544,6 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
           if (t == 0 && !full(0)) break;
           scores(t, 0);
         }
-        if (ok) tc::umma_commit(&ctl->kv_empty[0]);
         for (int j = 0; ok && j < steps; ++j) {
           if (!full(2 * j + 1)) break;
           for (int t = 0; t < tiles; ++t) {
@@ -552,9 +558,6 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
               tc::umma_commit(&ctl->o_full[t]);
             }
           }
-          if (!ok) break;
-          tc::umma_commit(&ctl->kv_empty[(2 * j + 1) % Cfg::kStages]);
-          if (j + 1 < steps) tc::umma_commit(&ctl->kv_empty[(2 * j + 2) % Cfg::kStages]);
         }
         if (!ok) tile_fault(ctl, fault);
         tc::umma_commit(&ctl->drain);
@@ -820,7 +823,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   if (w.splits == 1 || *reinterpret_cast<volatile int*>(&ctl->abort)) return;
 
   // ---- the last piece of these rows to arrive joins them all --------------------
-  if (!arrive_last(counters + (int64_t)w.tile * p.kv_heads + kvh, w.splits, &last)) return;
+  if (!arrive_last(counters + (int64_t)w.tile * p.kv_heads + kvh, w.splits, &ctl->last)) return;
   if (warp >= 8) return;  // these gave their registers away
   for (int u = threadIdx.x; (u & ~31) < rows * (D / 4); u += 256) {
     const int r = u / (D / 4), d = (u - r * (D / 4)) * 4;
