@@ -93,28 +93,45 @@ __device__ __forceinline__ int tile_at(int r, int c) {
   return (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// The MN-major operand descriptor of a V tile: its rows are keys (the K axis of
-// P V) of 64 contiguous dimensions; groups of 8 keys 1024 bytes apart, the next
-// 64 dimensions 16 KB apart.
-__device__ __forceinline__ uint64_t umma_desc_v(uint32_t smem) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem >> 4) & 0x3FFFu);
-  d |= (uint64_t)(16384u >> 4) << 16;
-  d |= (uint64_t)(1024u >> 4) << 32;
-  d |= (uint64_t)1u << 46;
-  d |= (uint64_t)2u << 61;
-  return d;
-}
+// Operand descriptors are passed as their low words (start address and leading
+// offset); the high words are constants: stride 1024 bytes (8 rows of 128),
+// version 1, 128-byte swizzle.  K-major tiles (Q, K) ignore the leading offset.
+// A V tile is MN-major: its rows are keys (the K axis of P V) of 64 contiguous
+// dimensions, groups of 8 keys 1024 bytes apart, the next 64 dimensions 16 KB
+// apart (the leading offset).
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+constexpr uint32_t kDescLeadK = 1u << 16, kDescLeadV = (16384u >> 4) << 16;
 
-// D[tmem] (+)= A[tmem] * B[smem], B MN-major by its instruction descriptor.
-__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc,
+// D[tmem] (+)= A[smem] * B[smem]^T
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint32_t a_low, uint32_t b_low,
                                         uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
       : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem], B MN-major by its instruction descriptor.
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_low,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)::"memory");
+  return r != 0;
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
@@ -339,7 +356,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         if (!ok) break;
         // the last tile's scores are the last reader of K of this step and come behind the last
         // reader of V of the step before: their slots are free.  Said here, not by commits of the
-        // MMA thread, each of which would hold up its next MMA.
+        // MMA warp, each of which would hold up its next MMA.
         if (t == tiles - 1 && r == 0) {
           tc::mbar_arrive(&ctl->kv_empty[(2 * j) % Cfg::kStages]);
           if (j > 0) tc::mbar_arrive(&ctl->kv_empty[(2 * j - 1) % Cfg::kStages]);
@@ -504,64 +521,87 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kOtherRegs));
     if (warp == 8) {
-      // ---- MMA issuer ------------------------------------------------------------
-      if (lane == 0 && steps > 0) {
+      // ---- MMA issuer: the whole warp walks the steps, so that descriptors and
+      // addresses stay in uniform registers; one lane issues ---------------------------
+      if (steps > 0) {
         constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
         constexpr uint32_t idesc_s = tc::umma_idesc_f16(kBf16, 128, kStepKeys);
         constexpr uint32_t idesc_o = tc::umma_idesc_f16(kBf16, 128, D) | (1u << 16);  // B MN-major
+        constexpr uint32_t kSlot = Cfg::kKvBytes >> 4;
+        const uint32_t q0 = (tc::smem_u32(smem) >> 4) | kDescLeadK;
+        const uint32_t r0 = tc::smem_u32(ring) >> 4;
+        const uint32_t ubase = __shfl_sync(0xffffffffu, tmem, 0);
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
           ok = ok && wait_for(bar, parity, ctl);
+          ok = __all_sync(0xffffffffu, ok);
           tc::tc_fence_after();
           return ok;
         };
-        // ring slot i holds K of step i / 2 (i even) or V (i odd)
-        auto slot = [&](int i) { return tc::smem_u32(ring + (i % Cfg::kStages) * Cfg::kKvBytes); };
-        auto full = [&](int i) {
-          return wait(&ctl->kv_full[i % Cfg::kStages], (uint32_t)(i / Cfg::kStages) & 1u);
-        };
-        auto scores = [&](int t, int j) {
-          const uint32_t q = tc::smem_u32(smem + t * Cfg::kQBytes), k = slot(2 * j);
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            const uint32_t at = (uint32_t)((i >> 2) * 16384 + (i & 3) * 32);
-            tc::umma_f16(tmem + t * 128, tc::umma_desc_sw128(q + at), tc::umma_desc_sw128(k + at),
-                         idesc_s, i > 0);
+        // ring slots in order: K of step 0, V of step 0, K of step 1, ...
+        int ks = 0, vs = 1 % Cfg::kStages;  // slots of the next K and V
+        uint32_t kp = 0, vp = 0;            // their phases
+        auto step_slot = [](int& s, uint32_t& phase) {
+          s += 2;
+          if (s >= Cfg::kStages) {
+            s -= Cfg::kStages;
+            phase ^= 1u;
           }
-          tc::umma_commit(&ctl->s_full[t]);
         };
-        auto output = [&](int t, int j, int half) {
-          const uint32_t v = slot(2 * j + 1);
+        auto scores = [&](int t, int slot) {
+          if (elect_one()) {
+            const uint32_t q = q0 + (uint32_t)t * (Cfg::kQBytes >> 4);
+            const uint32_t k = (r0 + (uint32_t)slot * kSlot) | kDescLeadK;
 #pragma unroll
-          for (int x = 0; x < kStepKeys / 32; ++x) {
-            const int i = half * (kStepKeys / 32) + x;
-            umma_ts(tmem + 256 + t * D, tmem + t * 128 + i * 8, umma_desc_v(v + i * 2048), idesc_o,
-                    j > 0 || i > 0);
+            for (int i = 0; i < D / 16; ++i) {
+              const uint32_t at = (uint32_t)((i >> 2) * 16384 + (i & 3) * 32) >> 4;
+              umma_ss(ubase + t * 128, q + at, k + at, idesc_s, i > 0);
+            }
+            tc::umma_commit(&ctl->s_full[t]);
           }
+          __syncwarp();
+        };
+        auto output = [&](int t, int slot, int half, bool add) {
+          if (elect_one()) {
+            const uint32_t v = (r0 + (uint32_t)slot * kSlot) | kDescLeadV;
+#pragma unroll
+            for (int x = 0; x < kStepKeys / 32; ++x) {
+              const int i = half * (kStepKeys / 32) + x;
+              umma_ts(ubase + 256 + t * D, ubase + t * 128 + i * 8, v + (i * 2048 >> 4), idesc_o,
+                      x > 0 || add);
+            }
+          }
+          __syncwarp();
         };
         for (int t = 0; t < tiles; ++t) {
           if (!wait(&ctl->q_full[t], 0)) break;
-          if (t == 0 && !full(0)) break;
+          if (t == 0 && !wait(&ctl->kv_full[0], 0)) break;
           scores(t, 0);
         }
+        step_slot(ks, kp);
         for (int j = 0; ok && j < steps; ++j) {
-          if (!full(2 * j + 1)) break;
+          if (!wait(&ctl->kv_full[vs], vp)) break;
           for (int t = 0; t < tiles; ++t) {
             if (!wait(&ctl->p_full[t][0], j & 1)) break;
-            output(t, j, 0);
+            output(t, vs, 0, j > 0);
             if (!wait(&ctl->p_full[t][1], j & 1)) break;
-            output(t, j, 1);
+            output(t, vs, 1, true);
             if (j + 1 < steps) {
-              if (t == 0 && !full(2 * j + 2)) break;
-              scores(t, j + 1);
-            } else {
+              if (t == 0 && !wait(&ctl->kv_full[ks], kp)) break;
+              scores(t, ks);
+            } else if (elect_one()) {
               tc::umma_commit(&ctl->o_full[t]);
             }
           }
+          step_slot(ks, kp);
+          step_slot(vs, vp);
         }
         if (!ok) tile_fault(ctl, fault);
-        tc::umma_commit(&ctl->drain);
-        tc::mbar_wait(&ctl->drain, 0, kWaitLimitNs, nullptr);
+        if (elect_one()) {
+          tc::umma_commit(&ctl->drain);
+          tc::mbar_wait(&ctl->drain, 0, kWaitLimitNs, nullptr);
+        }
+        __syncwarp();
       }
     } else if (Q8 && box > 0 && warp < Cfg::kLoadWarp0) {
       // ---- quantised pages by TMA: codes (warp 9) and exponents (warps 10, 11) ------
