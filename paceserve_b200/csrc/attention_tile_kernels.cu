@@ -176,6 +176,29 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// The largest of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t both(float x) { return f32x2(x, x); }
+
+// tanh(u) / u on |u| <= 1 as a polynomial in z = u^2, fitted for the least
+// largest error of tanh (2.3e-8).
+__device__ __forceinline__ uint64_t tanh_ratio_pair(uint64_t z) {
+  uint64_t y = fma2(both(0.000964018632657826f), z, both(-0.005952119827270508f));
+  y = fma2(y, z, both(0.019974395632743835f));
+  y = fma2(y, z, both(-0.053266558796167374f));
+  y = fma2(y, z, both(0.13319607079029083f));
+  y = fma2(y, z, both(-0.33332133293151855f));
+  return fma2(y, z, both(0.9999997019767761f));
+}
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -298,36 +321,31 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
     const bool live = row < rows;
     const int tok = w.tok0 + (live ? row / group : 0);
     const int head = kvh * group + (live ? row % group : 0);
-    TokenInfo info{0, 0, 0, 0};
-    float slope = 0.f;
-    const uint64_t* tree = nullptr;
-    if (live) {
-      info = p.tokens[tok];
-      if (p.slopes) slope = p.slopes[head] * kLog2e;
-      if (p.tree_mask) tree = p.tree_mask + (int64_t)tok * p.tree_words;
-    }
-    const int end = tree ? min(info.pos, w.kv_end) : 0;  // of the drafted keys
-    const int lo = max(info.lo, w.kv_begin), hi = min(info.hi, w.kv_end);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     if (t < tiles) {
-      // the row's query into the tile; negated where the scale is negative (and
-      // zero where it is), so that the largest product is the largest score
+      // the tile's queries, a row by 8 or 16 neighbouring threads; negated where the scale is
+      // negative (and zero where it is), so that the largest product is the largest score
       {
-        const T* q = static_cast<const T*>(p.query) + (int64_t)tok * p.q_stride + (int64_t)head * D;
         uint8_t* qs = smem + t * Cfg::kQBytes;
         const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-        const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+        const bool vec = p.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.query) & 15) == 0;
+        constexpr int kChunks = D / 8;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
+        for (int x = 0; x < kChunks; ++x) {
+          const int qr = (x * 128 + r) / kChunks, c = (x * 128 + r) % kChunks;
+          const int at = t * kTileRowsEach + qr;
           uint32_t v[4] = {0, 0, 0, 0};
-          if (live && p.scale != 0.f) {
+          if (at < rows && p.scale != 0.f) {
+            const T* q = static_cast<const T*>(p.query) +
+                         (int64_t)(w.tok0 + at / group) * p.q_stride +
+                         (int64_t)(kvh * group + at % group) * D + c * 8;
             if (vec) {
-              const uint4 x = ld_nc_v4(q + c * 8);
-              v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+              const uint4 y = ld_nc_v4(q);
+              v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
             } else {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) v[i] = M::pair(q[c * 8 + 2 * i], q[c * 8 + 2 * i + 1]);
+              for (int i = 0; i < 4; ++i) v[i] = M::pair(q[2 * i], q[2 * i + 1]);
             }
           }
           if constexpr (Q8) {
@@ -339,12 +357,22 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
               v[i + 1] = __byte_perm(a, b, 0x7632);
             }
           }
-          *reinterpret_cast<uint4*>(qs + tile_at(r, c)) =
+          *reinterpret_cast<uint4*>(qs + tile_at(qr, c)) =
               make_uint4(v[0] ^ flip, v[1] ^ flip, v[2] ^ flip, v[3] ^ flip);
         }
         fence_async_proxy();
         tc::mbar_arrive(&ctl->q_full[t]);
       }
+      TokenInfo info{0, 0, 0, 0};
+      float slope = 0.f;
+      const uint64_t* tree = nullptr;
+      if (live) {
+        info = p.tokens[tok];
+        if (p.slopes) slope = p.slopes[head] * kLog2e;
+        if (p.tree_mask) tree = p.tree_mask + (int64_t)tok * p.tree_words;
+      }
+      const int end = tree ? min(info.pos, w.kv_end) : 0;  // of the drafted keys
+      const int lo = max(info.lo, w.kv_begin), hi = min(info.hi, w.kv_end);
       const float scale2 = (p.scale != 0.f ? fabsf(p.scale) : 1.f) * kLog2e;
       const float cap2 = p.cap * kLog2e, cap_in = p.cap > 0.f ? 2.f * scale2 / p.cap : 0.f;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -371,17 +399,59 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         float sc = scale2;
         const int j0 = k_base + j * kStepKeys;
         if (p.cap > 0.f) {
+          float size[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            sr[i] = __float_as_uint(
-                cap2 - 2.f * cap2 * rcp_approx(1.f + exp2_approx(__uint_as_float(sr[i]) * cap_in)));
+          for (int i = 0; i < kStepKeys; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              size[k] = max3(size[k], fabsf(__uint_as_float(sr[i + 2 * k])),
+                             fabsf(__uint_as_float(sr[i + 2 * k + 1])));
+          size[0] = fmaxf(fmaxf(size[0], size[1]), fmaxf(size[2], size[3]));
+          if (__all_sync(0xffffffffu, size[0] * scale2 <= cap2)) {
+            // no score passes the cap: tanh by a polynomial.  The special-function unit, which
+            // two calls a score keep busy for longer than the exponentials do, has none of it.
+            const uint64_t in2 = both(scale2 / cap2), out2 = both(scale2);
+#pragma unroll
+            for (int i = 0; i < kStepKeys; i += 2) {
+              const uint64_t x = u32x2(sr[i], sr[i + 1]), u = mul2(x, in2);
+              const uint64_t y = mul2(mul2(x, out2), tanh_ratio_pair(mul2(u, u)));
+              sr[i] = (uint32_t)y;
+              sr[i + 1] = (uint32_t)(y >> 32);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kStepKeys; ++i)
+              sr[i] = __float_as_uint(
+                  cap2 -
+                  2.f * cap2 * rcp_approx(1.f + exp2_approx(__uint_as_float(sr[i]) * cap_in)));
+          }
           sc = 1.f;
         }
         if (p.slopes) {
           const float d0 = (float)(info.pos - j0);
+          if (__all_sync(0xffffffffu, d0 >= (float)(kStepKeys - 1))) {
+            // all keys lie before the row's token: the bias rises by the slope from key to key
+            const uint64_t sc2 = both(sc);
+            uint64_t rise[4];
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            sr[i] = __float_as_uint(__uint_as_float(sr[i]) * sc - slope * fabsf(d0 - (float)i));
+            for (int k = 0; k < 4; ++k)
+              rise[k] = f32x2(slope * (2.f * k - d0), slope * (2.f * k + 1.f - d0));
+            const uint64_t by = both(8.f * slope);
+#pragma unroll
+            for (int i = 0; i < kStepKeys; i += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int x = i + 2 * k;
+                const uint64_t y = fma2(u32x2(sr[x], sr[x + 1]), sc2, rise[k]);
+                rise[k] = add2(rise[k], by);
+                sr[x] = (uint32_t)y;
+                sr[x + 1] = (uint32_t)(y >> 32);
+              }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kStepKeys; ++i)
+              sr[i] = __float_as_uint(__uint_as_float(sr[i]) * sc - slope * fabsf(d0 - (float)i));
+          }
           sc = 1.f;
         }
         const bool whole = j0 >= lo && j0 + kStepKeys <= hi;
@@ -400,8 +470,8 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         for (int i = 0; i < 128; i += 8)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            tops[k] = fmaxf(fmaxf(tops[k], __uint_as_float(sr[i + 2 * k])),
-                            __uint_as_float(sr[i + 2 * k + 1]));
+            tops[k] = max3(tops[k], __uint_as_float(sr[i + 2 * k]),
+                           __uint_as_float(sr[i + 2 * k + 1]));
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         top *= sc;
         if (j == 0) {
