@@ -279,6 +279,9 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   const Item w = items[blockIdx.x / p.kv_heads];
   const int group = p.heads / p.kv_heads;
   const int rows = w.ntok * group;
+  // row / group for rows below 256 and groups up to 128: the fraction added stays below 1 / group
+  const uint32_t group_inv = 65536u / (uint32_t)group + 1u;
+  auto div_group = [&](int row) { return (int)((uint32_t)row * group_inv >> 16); };
   const int tiles = rows > kTileRowsEach ? 2 : 1;
   // steps lie on multiples of 128 keys, so that pages do not straddle them
   const int k_base = w.kv_begin & ~(kStepKeys - 1);
@@ -319,8 +322,9 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
     const int r = threadIdx.x & 127;      // row of the tile
     const int row = t * kTileRowsEach + r;  // of the piece
     const bool live = row < rows;
-    const int tok = w.tok0 + (live ? row / group : 0);
-    const int head = kvh * group + (live ? row % group : 0);
+    const int tok_of = live ? div_group(row) : 0;
+    const int tok = w.tok0 + tok_of;
+    const int head = kvh * group + (live ? row - tok_of * group : 0);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     if (t < tiles) {
@@ -330,24 +334,25 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         uint8_t* qs = smem + t * Cfg::kQBytes;
         const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
         const bool vec = p.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.query) & 15) == 0;
-        constexpr int kChunks = D / 8;
+        constexpr int kChunks = D / 8, kRowStep = 128 / kChunks;
+        const int c = r % kChunks;
+        uint4 q[kChunks];  // all loads first, then the stores
 #pragma unroll
         for (int x = 0; x < kChunks; ++x) {
-          const int qr = (x * 128 + r) / kChunks, c = (x * 128 + r) % kChunks;
-          const int at = t * kTileRowsEach + qr;
-          uint32_t v[4] = {0, 0, 0, 0};
+          const int at = t * kTileRowsEach + x * kRowStep + r / kChunks;
+          q[x] = make_uint4(0, 0, 0, 0);
           if (at < rows && p.scale != 0.f) {
-            const T* q = static_cast<const T*>(p.query) +
-                         (int64_t)(w.tok0 + at / group) * p.q_stride +
-                         (int64_t)(kvh * group + at % group) * D + c * 8;
-            if (vec) {
-              const uint4 y = ld_nc_v4(q);
-              v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) v[i] = M::pair(q[2 * i], q[2 * i + 1]);
-            }
+            const int tk = div_group(at);
+            const T* src = static_cast<const T*>(p.query) + (int64_t)(w.tok0 + tk) * p.q_stride +
+                           (int64_t)(kvh * group + at - tk * group) * D + c * 8;
+            q[x] = vec ? ld_nc_v4(src)
+                       : make_uint4(M::pair(src[0], src[1]), M::pair(src[2], src[3]),
+                                    M::pair(src[4], src[5]), M::pair(src[6], src[7]));
           }
+        }
+#pragma unroll
+        for (int x = 0; x < kChunks; ++x) {
+          uint32_t v[4] = {q[x].x, q[x].y, q[x].z, q[x].w};
           if constexpr (Q8) {
             // quantised keys are unpacked as dimensions 0, 2, 1, 3 of each four
 #pragma unroll
@@ -357,7 +362,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
               v[i + 1] = __byte_perm(a, b, 0x7632);
             }
           }
-          *reinterpret_cast<uint4*>(qs + tile_at(qr, c)) =
+          *reinterpret_cast<uint4*>(qs + tile_at(x * kRowStep + r / kChunks, c)) =
               make_uint4(v[0] ^ flip, v[1] ^ flip, v[2] ^ flip, v[3] ^ flip);
         }
         fence_async_proxy();
@@ -529,8 +534,9 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         tc::tc_fence_after();
         const int64_t slot = ((int64_t)(w.slot + w.split) * p.kv_heads + kvh) * 256 + row;
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        T* out = static_cast<T*>(p.out) + (int64_t)tok * p.out_stride + (int64_t)head * D;
-        const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+        // whole rows go out through the query tile's place, so that a warp writes rows and not
+        // 16 bytes of each of 32 rows
+        uint8_t* os = smem + t * Cfg::kQBytes;
         float size = 0.f;
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
@@ -548,27 +554,52 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
             const int s = Q8 ? (i & ~3) | ((i & 1) << 1) | ((i >> 1) & 1) : i;
             v[i] = __uint_as_float(o[s]);
           }
-          if (live && w.splits > 1) {
+          if (w.splits > 1) {
             float* dst = partial + slot * D + c;
+            if (live) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              __stcg(reinterpret_cast<float4*>(dst + i),
-                     make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
-          } else if (live) {
+              for (int i = 0; i < 32; i += 8)
+                st_v8(dst + i,
+                      make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]),
+                                 __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3])),
+                      make_uint4(__float_as_uint(v[i + 4]), __float_as_uint(v[i + 5]),
+                                 __float_as_uint(v[i + 6]), __float_as_uint(v[i + 7])));
+            }
+          } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               v[i] = l == 0.f ? 0.f : v[i] * inv;
               size += fabsf(v[i]);
             }
-            if (vec) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 8) st_v4(out + c + i, Traits<T>::pack(v + i));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) out[c + i] = Traits<T>::from_f(v[i]);
-            }
+            for (int i = 0; i < 32; i += 8)
+              *reinterpret_cast<uint4*>(os + tile_at(r, (c + i) / 8)) = Traits<T>::pack(v + i);
           }
           __syncwarp();
+        }
+        if (w.splits == 1) {
+          // a warp's 32 rows are its own
+          constexpr int kChunks = D / 8, kRowStep = 32 / kChunks;
+          const int c = lane % kChunks;
+          const bool vec = p.out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+#pragma unroll 4
+          for (int x = 0; x < kChunks; ++x) {
+            const int qr = (warp & 3) * 32 + x * kRowStep + lane / kChunks;
+            const int at = t * kTileRowsEach + qr;
+            if (at < rows) {
+              const int tk = div_group(at);
+              T* dst = static_cast<T*>(p.out) + (int64_t)(w.tok0 + tk) * p.out_stride +
+                       (int64_t)(kvh * group + at - tk * group) * D + c * 8;
+              const uint4 y = *reinterpret_cast<const uint4*>(os + tile_at(qr, c));
+              if (vec) {
+                st_v4(dst, y);
+              } else {
+                const T* e = reinterpret_cast<const T*>(&y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dst[i] = e[i];
+              }
+            }
+          }
         }
         if (live) {
           if (w.splits > 1)
