@@ -14,6 +14,10 @@
 //
 // Both kernels move bytes and little else.  Append, per token: 4 * kv_heads *
 // head_dim bytes of 16-bit input read, half of that plus 2 * kv_heads written.
+#include <string.h>
+
+#include <type_traits>
+
 #include "fp8.cuh"
 #include "paged.cuh"
 
@@ -22,6 +26,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHeadDim = 256;
+constexpr int kResident = 4;  // CTAs that an SM holds
 
 struct QuantJob : PageTable {
   int64_t rows;  // tokens appended or read back
@@ -51,28 +56,108 @@ __device__ __forceinline__ void stage_requests(const PageTable& t, int32_t* sh,
   indptr = s_ai;
 }
 
-// Eight elements of a row as floats; elements at or past `valid` are zero.
+// Eight elements of a row as they are; elements at or past `valid` are zero.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int valid, float* f) {
-  if constexpr (VEC) {
-    if (valid >= 8) {
-      if constexpr (sizeof(T) == 4) {
-        Traits<T>::unpack(ld_nc_v4(p), f);
-        Traits<T>::unpack(ld_nc_v4(p + 4), f + 4);
-      } else {
-        Traits<T>::unpack(ld_nc_v4(p), f);
-      }
-      return;
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, int valid) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0, 0, 0, 0);
+    if (valid <= 0) return;
+    if constexpr (VEC) {  // head_dim is a multiple of 8: all of them or none
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = ld_nc_v4(p + i * Traits<T>::kVec);
+    } else {
+      T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
+      memcpy(v, e, sizeof(v));
     }
   }
+};
+
+// Eight elements' codes and their row's exponent byte; the row is spread over
+// `group` neighbouring lanes, all of which call.  In fp32, whatever the elements.
+__device__ __forceinline__ uint32_t quantise_floats(const float (&x)[8], int group, uint2& code) {
+  float amax = 0.f;
+  bool nan = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = i < valid ? Traits<T>::to_f(p[i]) : 0.f;
+  for (int e = 0; e < 8; ++e) {
+    const float a = fabsf(x[e]);
+    nan |= a != a;
+    if (a < INFINITY) amax = fmaxf(amax, a);
+  }
+  // NaN travels as a value above every finite magnitude
+  if (nan) amax = INFINITY;
+  for (int o = group >> 1; o > 0; o >>= 1)
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const bool row_nan = amax == INFINITY;
+  const uint32_t ex = row_nan ? (uint32_t)kNanExponent : row_exponent(amax);
+  // 2^-e: an exact power of two, since e lies in [-126, 120]
+  const float inv = row_nan ? 0.f : __uint_as_float((254u - ex) << 23);
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = row_nan ? 0.f : x[e] * inv;
+  code = make_uint2(floats_to_e4m3x4(y), floats_to_e4m3x4(y + 4));
+  return ex;
 }
 
-// One CTA: U tokens.  A row is quantised by a group of 2^lanes_log2 lanes, 8
-// elements each; the maximum is a shuffle reduction, so every element is read
-// once.  All of a pass's loads are issued before the token -> page lookups,
-// which only the first U threads do.
+// The same from the elements' bits.  16-bit types find the maximum on pairs of
+// magnitudes as integers; only a warp that holds an infinity or a NaN takes the
+// way above (which at 110 instructions for 8 elements bound the kernel: 16167
+// fp16 tokens 39 us).
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8(const uint4 (&v)[sizeof(T) / 2], int group,
+                                              uint2& code) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) Traits<T>::unpack(v[i], x + i * Traits<T>::kVec);
+  if constexpr (sizeof(T) == 2) {
+    constexpr uint32_t kMag = 0x7fff7fffu;
+    uint32_t m = __vmaxu2(__vmaxu2(v[0].x & kMag, v[0].y & kMag),
+                          __vmaxu2(v[0].z & kMag, v[0].w & kMag));
+    for (int o = group >> 1; o > 0; o >>= 1)
+      m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = max(m & 0xffffu, m >> 16);
+    constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    if (__all_sync(0xffffffffu, m < kInf)) {
+      const uint16_t bits = (uint16_t)m;
+      const uint32_t ex = row_exponent(Traits<T>::to_f(*reinterpret_cast<const T*>(&bits)));
+      const float inv = __uint_as_float((254u - ex) << 23);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= inv;
+      code = make_uint2(floats_to_e4m3x4(x), floats_to_e4m3x4(x + 4));
+      return ex;
+    }
+  }
+  return quantise_floats(x, group, code);
+}
+
+// Where this thread works: as many tokens as fit the CTA side by side, `lanes`
+// threads each; a token with more than kThreads units takes the CTA in turns.
+constexpr int kMaxSide = kThreads / 4;  // of four rounds: a CTA looks up at most kThreads places
+struct Place {
+  int side;    // tokens side by side
+  int sub;     // this thread's among them; >= side: idle
+  int first;   // its first unit of the token
+};
+__device__ __forceinline__ Place place_of(int per_token) {
+  if (per_token >= kThreads) return {1, 0, (int)threadIdx.x};
+  Place p;
+  p.side = min(kThreads / per_token, kMaxSide);
+  p.sub = (int)threadIdx.x / per_token;
+  p.first = (int)threadIdx.x - p.sub * per_token;
+  return p;
+}
+
+// The tokens of a CTA: `batches` of U rounds of the tokens side by side.  A row is
+// quantised by a group of 2^lanes_log2 lanes, 8 elements each; the maximum is a
+// shuffle reduction, so every element is read once.  A batch's loads are issued
+// before the batch in front of it is worked on, the first one's before the token
+// -> page lookups, which the first threads do for all batches: the lookups are
+// two loads that depend on each other, and with CTAs of one batch they were most
+// of the time (16167 fp16 tokens: 59 us with one load after the other, 39 us
+// with a batch of four a CTA).
 template <typename T, int U, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     kv_quant_append_kernel(const T* __restrict__ key, const T* __restrict__ value,
@@ -80,39 +165,42 @@ __global__ void __launch_bounds__(kThreads)
                            uint8_t* __restrict__ exponents, const int32_t* __restrict__ kv_indices,
                            const int32_t* __restrict__ kv_indptr,
                            const int32_t* __restrict__ kv_last_page_len, QuantJob job,
-                           int32_t* bad) {
+                           int batches, int32_t* bad) {
   extern __shared__ int32_t sh[];
-  __shared__ int64_t s_slot[U];  // K row slot of the token's page (V: + page_size), or -1
+  __shared__ int64_t s_slot[kThreads];  // K row slot of the token's page (V: + page_size), or -1
+  const int group = 1 << job.lanes_log2;
+  const int per_token = (2 * job.heads) << job.lanes_log2;
+  const Place at = place_of(per_token);
+  const int each = U * at.side;  // tokens of a batch
+  const int64_t tok0 = (int64_t)blockIdx.x * each * batches;
+  const int ntok = (int)min((int64_t)each * batches, job.rows - tok0);
+  const int32_t *ai = append_indptr, *ip = kv_indptr, *last = kv_last_page_len;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t tok0 = (int64_t)blockIdx.x * U;
-  const int ntok = (int)min((int64_t)U, job.rows - tok0);
-  const int group = 1 << job.lanes_log2;
-  const int rows_per_token = 2 * job.heads;
-  const int units = (ntok * rows_per_token) << job.lanes_log2;
-  const int32_t *ai = append_indptr, *ip = kv_indptr, *last = kv_last_page_len;
-  for (int base = 0; base < units; base += U * kThreads) {
-    float x[U][8];
+  for (int base = 0; base < per_token; base += kThreads) {
+    const int u = base + at.first;
+    const int kh = u >> job.lanes_log2, c = (u & (group - 1)) * 8;
+    const bool is_v = kh >= job.heads;
+    const int head = is_v ? kh - job.heads : kh;
+    const bool mine = at.sub < at.side && u < per_token && c < job.head_dim;
+    const T* src = (is_v ? value : key) + (int64_t)head * job.head_dim + c;
+    const int64_t stride = is_v ? job.value_stride : job.key_stride;
+    Raw8<T, VEC> raw[U], next[U];
+    auto load = [&](Raw8<T, VEC>(&r)[U], int t0) {
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int u = base + k * kThreads + (int)threadIdx.x;
-      const int row = u >> job.lanes_log2;
-      const int t = row / rows_per_token, kh = row - t * rows_per_token;
-      const int c = (u & (group - 1)) * 8;
-      const bool is_v = kh >= job.heads;
-      const int valid = u < units ? job.head_dim - c : 0;  // <= 0: an idle lane
-      const T* src = (is_v ? value + (tok0 + t) * job.value_stride
-                           : key + (tok0 + t) * job.key_stride) +
-                     (int64_t)(is_v ? kh - job.heads : kh) * job.head_dim + c;
-      load8<T, VEC>(src, valid, x[k]);
-    }
+      for (int k = 0; k < U; ++k) {
+        const int t = t0 + k * at.side + at.sub;
+        r[k].load(src + (tok0 + t) * stride, mine && t < ntok ? 8 : 0);
+      }
+    };
+    load(raw, 0);
     if (base == 0) {
       stage_requests(job, sh, ai, ip, last);
       __syncthreads();
       if ((int)threadIdx.x < ntok) {
         const int64_t i = tok0 + threadIdx.x;
         const int b = find_request(ai, job.batch, i);
-        int64_t page, at = -1;
+        int64_t page, where = -1;
         int slot;
         // i lies outside [ai[b], ai[b + 1]) where append_indptr does not cover it
         if (i >= (int64_t)ai[b] && i < (int64_t)ai[b + 1]) {
@@ -120,46 +208,29 @@ __global__ void __launch_bounds__(kThreads)
               ((int64_t)ip[b + 1] - ip[b] - 1) * job.page_size + last[b];
           const int64_t pos = seq_len - ai[b + 1] + i;
           if (locate_token(job, b, pos, kv_indices, ip, last, &page, &slot))
-            at = page * 2 * job.page_size + slot;
+            where = page * 2 * job.page_size + slot;
         }
-        s_slot[threadIdx.x] = at;
-        if (at < 0 && bad) atomicAdd(bad, 1);
+        s_slot[threadIdx.x] = where;
+        if (where < 0 && bad) atomicAdd(bad, 1);
       }
       __syncthreads();
     }
+    for (int t0 = 0; t0 < ntok; t0 += each) {
+      load(next, t0 + each);
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int u = base + k * kThreads + (int)threadIdx.x;
-      float amax = 0.f;
-      bool nan = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = fabsf(x[k][e]);
-        nan |= a != a;
-        if (a < INFINITY) amax = fmaxf(amax, a);
+      for (int k = 0; k < U; ++k) {
+          uint2 code;
+        const uint32_t ex = quantise8<T>(raw[k].v, group, code);
+        const int t = t0 + k * at.side + at.sub;
+        const int64_t where = mine && t < ntok ? s_slot[t] : -1;
+        if (where >= 0) {
+          const int64_t dst = (where + (is_v ? job.page_size : 0)) * job.heads + head;
+          *reinterpret_cast<uint2*>(codes + dst * job.head_dim + c) = code;
+          if (c == 0) exponents[dst] = (uint8_t)ex;
+        }
       }
-      // NaN travels as a value above every finite magnitude
-      if (nan) amax = INFINITY;
-      for (int o = group >> 1; o > 0; o >>= 1)
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      const bool row_nan = amax == INFINITY;
-      const uint32_t ex = row_nan ? (uint32_t)kNanExponent : row_exponent(amax);
-      // 2^-e: an exact power of two, since e lies in [-126, 120]
-      const float inv = row_nan ? 0.f : __uint_as_float((254u - ex) << 23);
-      const int row = u >> job.lanes_log2;
-      const int t = row / rows_per_token, kh = row - t * rows_per_token;
-      const int c = (u & (group - 1)) * 8;
-      if (u >= units || c >= job.head_dim) continue;
-      const int64_t at = s_slot[t];
-      if (at < 0) continue;
-      const bool is_v = kh >= job.heads;
-      const int64_t dst = (at + (is_v ? job.page_size : 0)) * job.heads + (is_v ? kh - job.heads : kh);
-      float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = row_nan ? 0.f : x[k][e] * inv;
-      const uint2 w = make_uint2(floats_to_e4m3x4(y), floats_to_e4m3x4(y + 4));
-      *reinterpret_cast<uint2*>(codes + dst * job.head_dim + c) = w;
-      if (c == 0) exponents[dst] = (uint8_t)ex;
+      for (int k = 0; k < U; ++k) raw[k] = next[k];
     }
   }
 }
@@ -173,17 +244,25 @@ __device__ __forceinline__ void store_values(T* dst, const uint32_t (&codes)[V /
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] *= factor;
   if constexpr (VEC) {
+    constexpr int kVec = Traits<T>::kVec;
+    if (V >= 2 * kVec && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
 #pragma unroll
-    for (int i = 0; i < V; i += Traits<T>::kVec) st_v4(dst + i, Traits<T>::pack(f + i));
+      for (int i = 0; i < V / kVec; i += 2)
+        st_v8(dst + i * kVec, Traits<T>::pack(f + i * kVec),
+              Traits<T>::pack(f + (V >= 2 * kVec ? (i + 1) * kVec : 0)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i += kVec) st_v4(dst + i, Traits<T>::pack(f + i));
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) dst[i] = Traits<T>::from_f(f[i]);
   }
 }
 
-// One CTA: `tokens` output rows (K and V of every head), V codes per thread
-// and step.  The rows' places are looked up by the first threads; then each
-// thread issues its U code loads together.
+// The output rows of a CTA: `batches` of U rounds of the tokens side by side, V
+// codes per thread.  The rows' places are looked up by the first threads; a
+// batch's loads are issued before the batch in front of it is written.
 template <typename T, int V, int U, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     kv_quant_read_kernel(T* __restrict__ key, T* __restrict__ value,
@@ -191,76 +270,93 @@ __global__ void __launch_bounds__(kThreads)
                          const uint8_t* __restrict__ exponents,
                          const int32_t* __restrict__ kv_indices,
                          const int32_t* __restrict__ kv_indptr,
-                         const int32_t* __restrict__ kv_last_page_len, QuantJob job, int tokens,
+                         const int32_t* __restrict__ kv_last_page_len, QuantJob job, int batches,
                          int32_t* bad) {
   extern __shared__ int32_t sh[];
   __shared__ int64_t s_slot[kThreads];
+  const int per_row = job.head_dim / V;
+  const int per_token = 2 * job.heads * per_row;
+  const Place at = place_of(per_token);
+  const int each = U * at.side;  // tokens of a batch
+  const int64_t tok0 = (int64_t)blockIdx.x * each * batches;
+  const int ntok = (int)min((int64_t)each * batches, job.rows - tok0);
+  const int32_t *oi = out_indptr, *ip = kv_indptr, *last = kv_last_page_len;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t tok0 = (int64_t)blockIdx.x * tokens;
-  const int ntok = (int)min((int64_t)tokens, job.rows - tok0);
-  const int32_t *oi = out_indptr, *ip = kv_indptr, *last = kv_last_page_len;
   stage_requests(job, sh, oi, ip, last);
   __syncthreads();
   if ((int)threadIdx.x < ntok) {
     const int64_t i = tok0 + threadIdx.x;
     const int b = find_request(oi, job.batch, i);
-    int64_t page, at = -1;
+    int64_t page, where = -1;
     int slot;
     if (i >= (int64_t)oi[b] && i < (int64_t)oi[b + 1] &&
         locate_token(job, b, i - oi[b], kv_indices, ip, last, &page, &slot))
-      at = page * 2 * job.page_size + slot;
-    s_slot[threadIdx.x] = at;
-    if (at < 0 && bad) atomicAdd(bad, 1);
+      where = page * 2 * job.page_size + slot;
+    s_slot[threadIdx.x] = where;
+    if (where < 0 && bad) atomicAdd(bad, 1);
   }
   __syncthreads();
-  const int per_row = job.head_dim / V;
-  const int per_token = 2 * job.heads * per_row;
-  const int units = ntok * per_token;
-  for (int base = 0; base < units; base += U * kThreads) {
-    uint32_t w[U][V / 4];
-    uint32_t ex[U];
+  for (int u = at.first; u < per_token && at.sub < at.side; u += kThreads) {
+    const int kh = u / per_row, c = (u - kh * per_row) * V;
+    const bool is_v = kh >= job.heads;
+    const int head = is_v ? kh - job.heads : kh;
+    struct Codes {
+      uint32_t w[V / 4];
+      uint32_t ex;
+      bool there;
+    };
+    Codes cur[U], next[U];
+    auto load = [&](Codes(&r)[U], int t0) {
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int u = base + k * kThreads + (int)threadIdx.x;
-      const int t = u / per_token, r = u - t * per_token;
-      const int kh = r / per_row, c = (r - kh * per_row) * V;
-      const int64_t at = u < units ? s_slot[t] : -1;
-      ex[k] = 0;
-#pragma unroll
-      for (int i = 0; i < V / 4; ++i) w[k][i] = 0;
-      if (at >= 0) {
-        const bool is_v = kh >= job.heads;
-        const int64_t src =
-            (at + (is_v ? job.page_size : 0)) * job.heads + (is_v ? kh - job.heads : kh);
-        const uint8_t* p = codes + src * job.head_dim + c;
-        if constexpr (V == 16) {
-          const uint4 q = ld_nc_v4(p);
-          w[k][0] = q.x;
-          w[k][1] = q.y;
-          w[k][2] = q.z;
-          w[k][3] = q.w;
-        } else {
-          const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
-          w[k][0] = q.x;
-          w[k][1] = q.y;
+      for (int k = 0; k < U; ++k) {
+        const int t = t0 + k * at.side + at.sub;
+        const int64_t where = t < ntok ? s_slot[t] : -1;
+        r[k].there = where >= 0;
+        if (where >= 0) {
+          const int64_t src = (where + (is_v ? job.page_size : 0)) * job.heads + head;
+          const uint8_t* p = codes + src * job.head_dim + c;
+          if constexpr (V == 16) {
+            const uint4 q = ld_nc_v4(p);
+            r[k].w[0] = q.x;
+            r[k].w[1] = q.y;
+            r[k].w[2] = q.z;
+            r[k].w[3] = q.w;
+          } else {
+            const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
+            r[k].w[0] = q.x;
+            r[k].w[1] = q.y;
+          }
+          r[k].ex = __ldg(exponents + src);
         }
-        ex[k] = __ldg(exponents + src);
+      }
+    };
+    T* dst = (is_v ? value : key) + (int64_t)head * job.head_dim + c;
+    const int64_t stride = is_v ? job.value_stride : job.key_stride;
+    load(cur, 0);
+    for (int t0 = 0; t0 < ntok; t0 += each) {
+      load(next, t0 + each);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (cur[k].there)
+          store_values<T, V, VEC>(dst + (tok0 + t0 + k * at.side + at.sub) * stride, cur[k].w,
+                                  exponent_factor(cur[k].ex));
+        cur[k] = next[k];
       }
     }
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int u = base + k * kThreads + (int)threadIdx.x;
-      if (u >= units) continue;
-      const int t = u / per_token, r = u - t * per_token;
-      const int kh = r / per_row, c = (r - kh * per_row) * V;
-      if (s_slot[t] < 0) continue;
-      const bool is_v = kh >= job.heads;
-      T* dst = (is_v ? value + (tok0 + t) * job.value_stride : key + (tok0 + t) * job.key_stride) +
-               (int64_t)(is_v ? kh - job.heads : kh) * job.head_dim + c;
-      store_values<T, V, VEC>(dst, w[k], exponent_factor(ex[k]));
-    }
   }
+}
+
+// Tokens of a batch, and batches of a CTA: as many as leave every SM about
+// `resident` CTAs, so that all run at once.
+int64_t tokens_per_batch(int u, int per_token) {
+  const int side = kThreads / per_token;
+  return (int64_t)u * (side < 1 ? 1 : side > kMaxSide ? kMaxSide : side);
+}
+int batches_per_cta(int64_t rows, int64_t batch, int sms, int resident) {
+  const int64_t n = ceil_div(rows, batch * sms * resident);
+  const int64_t most = kThreads / batch;  // places that a CTA looks up
+  return (int)(n < 1 ? 1 : n > most ? most : n);
 }
 
 // Checks shared by the two entry points; PACE_OK with rows == 0 means nothing
@@ -315,11 +411,15 @@ extern "C" int pace_append_quantised_paged_kv_cache(
     constexpr int V = Traits<T>::kVec;
     const bool vec = key_row_stride % V == 0 && value_row_stride % V == 0 && aligned16(key) &&
                      aligned16(value);
-    auto go = [&](auto kernel, int per_cta) {
-      return launch(kernel, dim3((unsigned)ceil_div(nnz, per_cta)), dim3(kThreads), smem, stream,
+    const int per_token = (2 * num_kv_heads) << lanes_log2;
+    auto go = [&](auto kernel, int u) {
+      const int64_t batch = tokens_per_batch(u, per_token);
+      const int batches = batches_per_cta(nnz, batch, sms, kResident);
+      return launch(kernel, dim3((unsigned)ceil_div(nnz, batch * batches)), dim3(kThreads), smem,
+                    stream,
                     static_cast<const T*>(key), static_cast<const T*>(value), append_indptr,
                     static_cast<uint8_t*>(codes), static_cast<uint8_t*>(exponents), kv_indices,
-                    kv_indptr, kv_last_page_len, job, bad_tokens);
+                    kv_indptr, kv_last_page_len, job, batches, bad_tokens);
     };
     cudaError_t err;
     if (!vec)
@@ -358,12 +458,13 @@ extern "C" int pace_read_quantised_paged_kv_cache(
     const int codes_per = head_dim % 16 == 0 ? 16 : 8;
     const int per_token = 2 * num_kv_heads * (head_dim / codes_per);
     auto go = [&](auto kernel, int u) {
-      int64_t tokens = (int64_t)u * kThreads / per_token;  // one pass of the CTA
-      tokens = tokens < 1 ? 1 : tokens > kThreads ? kThreads : tokens;
-      return launch(kernel, dim3((unsigned)ceil_div(rows, tokens)), dim3(kThreads), smem, stream,
+      const int64_t batch = tokens_per_batch(u, per_token);
+      const int batches = batches_per_cta(rows, batch, sms, kResident);
+      return launch(kernel, dim3((unsigned)ceil_div(rows, batch * batches)), dim3(kThreads), smem,
+                    stream,
                     static_cast<T*>(key), static_cast<T*>(value), out_indptr,
                     static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(exponents),
-                    kv_indices, kv_indptr, kv_last_page_len, job, (int)tokens, bad_tokens);
+                    kv_indices, kv_indptr, kv_last_page_len, job, batches, bad_tokens);
     };
     const bool few = rows * per_token <= (int64_t)8 * kThreads * sms;
     cudaError_t err;
