@@ -521,6 +521,7 @@ typedef struct {
   int num_few, num_many;      /* pieces of the few-row and of the tile kernel */
   int few_slots, many_slots;  /* their partial results */
   int few_tiles, many_tiles;  /* their cut groups of rows */
+  int few_rows;               /* query rows of the few-row kernel's largest piece */
   int max_page;
 } pace_attention_plan;
 

@@ -42,7 +42,7 @@ class AttentionPlan(ctypes.Structure):
                     (name, c_int) for name in (
                         "num_heads", "num_kv_heads", "head_dim", "page_size", "tree_words",
                         "num_few", "num_many", "few_slots", "many_slots", "few_tiles",
-                        "many_tiles", "max_page")]
+                        "many_tiles", "few_rows", "max_page")]
 
 
 _P = c_void_p  # device pointer / stream

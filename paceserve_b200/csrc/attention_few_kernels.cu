@@ -17,10 +17,16 @@
 // order of arrival.
 //
 // A quantised cache is copied as it is and unpacked between shared memory and
-// the matrix instruction: an e4m3 code moved to the top of the target type's
-// bits is the code's value times a power of two (2^-120 in bf16, 2^-8 in fp16),
-// subnormals included, so one multiplication restores it exactly.
-#include "attention.cuh"
+// the matrix instruction, which then works in fp16 whatever the query's type: a
+// code moved to the top of 16 bits is its value times 2^-8 as fp16 holds it,
+// subnormals included, and no multiplication touches it.  (The conversion
+// instruction is slower: 64 requests of up to 8191 tokens took 238 us with it.)
+// K's factor multiplies the scores.  V's factor 2^e goes with P, as 2^(e - E) for
+// the largest exponent E among the values so far, so that P stays at most 1 (the
+// output is in units of 2^(E - 8) and is scaled down when E rises, as it is when
+// the maximum does).  Queries are scaled by a power of two
+// to the top of fp16's range: a bf16 query keeps all its bits down to 2^-29 of
+// its largest element.
 #include "attention_mma.cuh"
 
 namespace pace {
@@ -38,7 +44,8 @@ struct FewTile {
   static constexpr int kRingBytes = kStages * 2 * kKvBytes;
   static constexpr int kJoinBytes = 16 * D * 4;  // a warp's output, over its ring
   static constexpr int kWarpBytes = kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes;
-  static constexpr int kFactorBytes = Q8 ? kStages * 2 * kKeys * 4 : 0;
+  // K's factors (fp32) and V's exponents of the keys in the ring
+  static constexpr int kFactorBytes = Q8 ? kStages * kKeys * 8 : 0;
   static constexpr int kSmemBytes = kFewWarps * (kWarpBytes + kFactorBytes) + kFewWarps * 32 * 4;
   // 16-byte chunk c of row r, placed so that eight rows' same chunk, and one
   // row's eight chunks, lie in different banks
@@ -48,12 +55,22 @@ struct FewTile {
   }
 };
 
-template <typename T, int D, bool Q8>
+// 2^-n, 0 where that is no normal number.
+__device__ __forceinline__ float pow2_down(int n) {
+  return n < 127 ? __uint_as_float((uint32_t)(127 - n) << 23) : 0.f;
+}
+// A value row's factor in units of 2^(top - 127); NaN for a row that is.
+__device__ __forceinline__ float v_factor(int exponent, int top) {
+  return exponent == kNanExponent ? __uint_as_float(0x7fc00000u) : pow2_down(top - exponent);
+}
+
+// R: 1 where the rows fit the matrix instruction's first eight, else 2.
+template <typename T, int D, bool Q8, int R>
 __global__ void __launch_bounds__(kFewWarps * 32, 2)
     attention_few_kernel(const Problem p, const Item* __restrict__ items, float* partial,
                          float2* partial_ml, int32_t* counters, bool q_even) {
   using Tile = FewTile<D, Q8>;
-  using M = Mma<T>;
+  using M = Mma<std::conditional_t<Q8, __half, T>>;
   constexpr int KEYS = Tile::kKeys, NT = KEYS / 8, KB = D / 16, STAGES = Tile::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -65,18 +82,19 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   uint8_t* ring = smem + warp * Tile::kWarpBytes;
   float* factors = reinterpret_cast<float*>(smem + kFewWarps * Tile::kWarpBytes +
                                             warp * Tile::kFactorBytes);
+  int* v_exps = reinterpret_cast<int*>(factors + Tile::kStages * KEYS);
   float* join_ml = reinterpret_cast<float*>(
       smem + kFewWarps * (Tile::kWarpBytes + Tile::kFactorBytes));  // [warp][16][m, l]
   pdl_launch_dependents();
   pdl_wait();
 
   // ---- rows g and g + 8 of this thread: visible keys, slope, queries --------
-  int lo[2], hi[2], pos[2];
-  float slope[2];
-  const uint64_t* bits[2] = {nullptr, nullptr};
+  int lo[R], hi[R], pos[R];
+  float slope[R];
+  const uint64_t* bits[R] = {};
   int all_lo = 0, all_hi = INT32_MAX;  // keys that every row sees
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < R; ++i) {
     const int r = g + 8 * i;
     lo[i] = 0;
     hi[i] = INT32_MAX;
@@ -113,18 +131,46 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const T* row = q[i & 1];
+        const T* row = (i & 1) < R ? q[i & 1] : nullptr;
         // the two dimensions of this register: those that the keys' register of the same
         // index holds (a quantised key's registers hold bytes 0, 2 and 1, 3 of four)
         const int d0 = Q8 ? kb * 16 + 4 * c + (i >> 1) : kb * 16 + 2 * c + 8 * (i >> 1);
-        const int d1 = d0 + (Q8 ? 2 : 1);
         if (!row)
           qf[kb][i] = 0;
         else if (!Q8 && q_even)
           qf[kb][i] = *reinterpret_cast<const uint32_t*>(row + d0);
         else
-          qf[kb][i] = M::pair(row[d0], row[d1]);
+          qf[kb][i] = Mma<T>::pair(row[d0], row[d0 + (Q8 ? 2 : 1)]);
       }
+  }
+  float row_scale[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) row_scale[i] = p.scale * kLog2e;
+  if constexpr (Q8) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float top = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int k = i; k < 4; k += 2) {
+          const float2 x = Mma<T>::floats(qf[kb][k]);
+          top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the power of two that brings `top` to 2^14 .. 2^15
+      const uint32_t up = min(268u - (__float_as_uint(top) >> 23), 254u);
+      const float f = __uint_as_float(up << 23);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int k = i; k < 4; k += 2) {
+          const float2 x = Mma<T>::floats(qf[kb][k]);
+          qf[kb][k] = M::pack(x.x * f, x.y * f);
+        }
+      row_scale[i] *= 256.f / f;  // and the codes' 2^-8
+    }
   }
 
   // ---- the ring ---------------------------------------------------------------
@@ -164,9 +210,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   };
   auto put_factors = [&](int step) {
     if constexpr (Q8) {
-      float* f = factors + (step % STAGES) * 2 * KEYS;
-      f[lane] = exponent_factor(ex & 0xff);
-      f[KEYS + lane] = exponent_factor(ex >> 8);
+      factors[(step % STAGES) * KEYS + lane] = exponent_factor(ex & 0xff);
+      v_exps[(step % STAGES) * KEYS + lane] = (int)(ex >> 8);
     }
   };
 
@@ -175,9 +220,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   for (int i = 0; i < D / 8; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const float scale2 = p.scale * kLog2e;
-  const float cap2 = p.cap * kLog2e, cap_in = p.cap > 0.f ? 2.f * scale2 / p.cap : 0.f;
+  float m[R], l[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+  }
+  int v_top = 0;  // the largest of V's exponents so far; O is in units of 2^(v_top - 127)
+  const float cap2 = p.cap * kLog2e, cap_in = p.cap > 0.f ? 2.f / p.cap : 0.f;
 
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {
@@ -195,8 +245,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
     __syncwarp();
     const uint8_t* ks = ring + (step % STAGES) * 2 * Tile::kKvBytes;
     const uint8_t* vs = ks + Tile::kKvBytes;
-    const float* kf = factors + (step % STAGES) * 2 * KEYS;
-    const float* vf = kf + KEYS;
+    const float* kf = factors + (step % STAGES) * KEYS;
+    const int* ve = v_exps + (step % STAGES) * KEYS;
     // ---- S = Q K^T ------------------------------------------------------------
     float s[NT][4];
 #pragma unroll
@@ -212,7 +262,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         for (int n = 0; n < NT; ++n) {
           uint32_t b0, b1;
           M::unpack_codes(r[n], b0, b1);
-          M::mma(s[n], qf[kb], M::code_scale(b0), M::code_scale(b1));
+          M::mma(s[n], qf[kb], b0, b1);
         }
       } else {
 #pragma unroll
@@ -226,34 +276,45 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
     }
     // ---- scores in powers of two, masks ---------------------------------------
     const int j0 = begin + step * kFewWarps * KEYS;
+    float away[R];  // from each row's token to the thread's first key
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int i = 0; i < R; ++i) away[i] = (float)(pos[i] - j0 - 2 * c);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x = s[n][e];
-        if constexpr (Q8) x *= kf[n * 8 + 2 * c + (e & 1)];
+    for (int n = 0; n < NT; ++n) {
+      float2 f = make_float2(1.f, 1.f);
+      if constexpr (Q8) f = *reinterpret_cast<const float2*>(kf + n * 8 + 2 * c);
+#pragma unroll
+      for (int e = 0; e < 2 * R; ++e) {
+        float x = s[n][e] * row_scale[e >> 1];
+        if constexpr (Q8) x *= e & 1 ? f.y : f.x;
         if (p.cap > 0.f)
           x = cap2 - 2.f * cap2 * rcp_approx(1.f + exp2_approx(x * cap_in));  // cap tanh
-        else
-          x *= scale2;
-        if (p.slopes) x -= slope[e >> 1] * fabsf((float)(pos[e >> 1] - (j0 + n * 8 + 2 * c + (e & 1))));
+        if (p.slopes) x -= slope[e >> 1] * fabsf(away[e >> 1] - (float)(n * 8 + (e & 1)));
         s[n][e] = x;
       }
+    }
     if (j0 < all_lo || j0 + KEYS > min(all_hi, w.kv_end)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 2 * R; ++e) {
           const int j = j0 + n * 8 + 2 * c + (e & 1), i = e >> 1;
           bool see = j >= lo[i] && j < hi[i] && j < w.kv_end;
           if (bits[i] && j >= hi[i]) see = j < min(pos[i], w.kv_end) && tree_bit(bits[i], j - hi[i]);
           if (!see) s[n][e] = -INFINITY;
         }
     }
+    float v_down = 1.f;  // what a rise of V's largest exponent does to O
+    if constexpr (Q8) {
+      const int x = ve[lane];
+      const int top = max(v_top, (int)__reduce_max_sync(0xffffffffu, x == kNanExponent ? 0 : x));
+      if (top > v_top) v_down = pow2_down(top - v_top);
+      v_top = top;
+    }
     // ---- running maximum and sum ----------------------------------------------
-    float base[2];
+    float base[R];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < R; ++i) {
       float t = -INFINITY;
 #pragma unroll
       for (int n = 0; n < NT; ++n) t = fmaxf(t, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
@@ -261,9 +322,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
       t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
       const float m2 = fmaxf(m[i], t);
       base[i] = m2 == -INFINITY ? 0.f : m2;
-      if (__any_sync(0xffffffffu, m2 > m[i])) {
-        const float f = exp2_approx(m[i] - base[i]);  // 0 while m is -inf
+      if (v_down != 1.f || __any_sync(0xffffffffu, m2 > m[i])) {
+        float f = exp2_approx(m[i] - base[i]);  // 0 while m is -inf
         l[i] *= f;
+        f *= v_down;
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) {
           o[n][2 * i] *= f;
@@ -275,7 +337,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 2 * R; ++e) {
         const float x = exp2_approx(s[n][e] - base[e >> 1]);
         l[e >> 1] += x;
         s[n][e] = x;
@@ -286,40 +348,30 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
       uint32_t a[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        a[i] = 0;
+        if ((i & 1) >= R) continue;
         float x = s[2 * kg + (i >> 1)][2 * (i & 1)], y = s[2 * kg + (i >> 1)][2 * (i & 1) + 1];
-        if constexpr (Q8 && M::kWideRange) {
-          // V's factors are powers of two: bf16 takes them on P without loss.  A key that the
-          // row does not see stays 0 whatever its row holds.
-          const int j = kg * 16 + (i >> 1) * 8 + 2 * c;
-          x = x == 0.f ? 0.f : x * vf[j];
-          y = y == 0.f ? 0.f : y * vf[j + 1];
+        if constexpr (Q8) {
+          // a key that the row does not see stays 0 whatever its row holds
+          const int2 e = *reinterpret_cast<const int2*>(ve + kg * 16 + (i >> 1) * 8 + 2 * c);
+          x = x == 0.f ? 0.f : x * v_factor(e.x, v_top);
+          y = y == 0.f ? 0.f : y * v_factor(e.y, v_top);
         }
         a[i] = M::pack(x, y);
       }
       if constexpr (Q8) {
-        uint32_t f0 = 0, f1 = 0, g0 = 0, g1 = 0;
-        if constexpr (!M::kWideRange) {
-          const int j = kg * 16 + 2 * c;
-          M::split_factors(vf[j], vf[j + 1], f0, g0);
-          M::split_factors(vf[j + 8], vf[j + 9], f1, g1);
-        }
 #pragma unroll
         for (int ch = 0; ch < D / 16; ch += 2) {
           uint32_t r[4];
-          // keys kg * 16 + 0-7, 8-15 of chunks ch, ch + 1
+          // keys kg * 16 + 0-7, 8-15 of chunks ch, ch + 1: two keys' pairs of dimensions
           ldmatrix4_trans(r, vs + Tile::at(kg * 16 + (lane & 15), ch + (lane >> 4)));
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t e0, d0, e1, d1;
             M::unpack_codes(r[2 * h], e0, d0);
             M::unpack_codes(r[2 * h + 1], e1, d1);
-            if constexpr (M::kWideRange) {
-              M::mma(o[2 * (ch + h)], a, M::code_scale(e0), M::code_scale(e1));
-              M::mma(o[2 * (ch + h) + 1], a, M::code_scale(d0), M::code_scale(d1));
-            } else {
-              M::mma(o[2 * (ch + h)], a, M::scale2(e0, f0, g0), M::scale2(e1, f1, g1));
-              M::mma(o[2 * (ch + h) + 1], a, M::scale2(d0, f0, g0), M::scale2(d1, f1, g1));
-            }
+            M::mma(o[2 * (ch + h)], a, e0, e1);
+            M::mma(o[2 * (ch + h) + 1], a, d0, d1);
           }
         }
       } else {
@@ -339,7 +391,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 
   // ---- join the warps ----------------------------------------------------------
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < R; ++i) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     const int r = g + 8 * i;
@@ -349,11 +401,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
         join_ml[(warp * 16 + r) * 2 + 1] = l[i];
       }
       float* dst = reinterpret_cast<float*>(ring) + r * D;
+      const float up = Q8 ? 256.f : 1.f, unit = Q8 ? exponent_factor(v_top) : 1.f;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
         const int d = Q8 ? (n >> 1) * 16 + 4 * c + (n & 1) : n * 8 + 2 * c;
-        dst[d] = o[n][2 * i];
-        dst[d + (Q8 ? 2 : 1)] = o[n][2 * i + 1];
+        dst[d] = o[n][2 * i] * up * unit;
+        dst[d + (Q8 ? 2 : 1)] = o[n][2 * i + 1] * up * unit;
       }
     }
   }
@@ -404,10 +457,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 }
 
 template <typename T, int D, bool Q8>
-static int run_few(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+static int run_few(const Problem& p, int max_rows, const Item* items, int num_items, float* partial, float2* ml,
                    int32_t* counters, int device, cudaStream_t stream, const char* what) {
   using Tile = FewTile<D, Q8>;
-  auto kernel = attention_few_kernel<T, D, Q8>;
+  auto kernel = max_rows <= 8 ? attention_few_kernel<T, D, Q8, 1> : attention_few_kernel<T, D, Q8, 2>;
   cudaError_t err =
       ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), device, Tile::kSmemBytes);
   if (err != cudaSuccess) return cuda_fail(err, what);
@@ -417,19 +470,16 @@ static int run_few(const Problem& p, const Item* items, int num_items, float* pa
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, what);
 }
 
-int run_few_rows(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
-                 int32_t* counters, bool bf16, int device, cudaStream_t stream, const char* what) {
+int run_few_rows(const Problem& p, int max_rows, const Item* items, int num_items, float* partial,
+                 float2* ml, int32_t* counters, bool bf16, int device, cudaStream_t stream,
+                 const char* what) {
   auto pick = [&](auto t) -> int {
     using T = decltype(t);
-    if (p.head_dim == 128)
-      return p.exponents ? run_few<T, 128, true>(p, items, num_items, partial, ml, counters, device,
-                                                 stream, what)
-                         : run_few<T, 128, false>(p, items, num_items, partial, ml, counters, device,
-                                                  stream, what);
-    return p.exponents ? run_few<T, 64, true>(p, items, num_items, partial, ml, counters, device,
-                                              stream, what)
-                       : run_few<T, 64, false>(p, items, num_items, partial, ml, counters, device,
-                                               stream, what);
+    auto go = [&](auto f) {
+      return f(p, max_rows, items, num_items, partial, ml, counters, device, stream, what);
+    };
+    if (p.head_dim == 128) return p.exponents ? go(run_few<T, 128, true>) : go(run_few<T, 128, false>);
+    return p.exponents ? go(run_few<T, 64, true>) : go(run_few<T, 64, false>);
   };
   return bf16 ? pick(__nv_bfloat16{}) : pick(__half{});
 }

@@ -245,6 +245,7 @@ extern "C" int pace_paged_attention_plan(
         w.kv_end = end;
         w.page_base = kv_indptr[b];
         (is_few ? few : many).push_back(w);
+        if (is_few) plan->few_rows = std::max(plan->few_rows, n * group);
       }
     }
     const int64_t few_slots = (int64_t)ceil_div((int64_t)num_sms * kFewCtasPerSm, num_kv_heads);
@@ -348,8 +349,8 @@ extern "C" int pace_paged_attention(const pace_attention_plan* plan, const int32
       if (st != PACE_OK) return st;
     }
     if (plan->num_few == 0) return PACE_OK;
-    return run_few_rows(p, reinterpret_cast<const Item*>(plan_words + plan->few_offset),
-                        plan->num_few, reinterpret_cast<float*>(base + ws.few),
+    return run_few_rows(p, plan->few_rows,
+                        reinterpret_cast<const Item*>(plan_words + plan->few_offset), plan->num_few, reinterpret_cast<float*>(base + ws.few),
                         reinterpret_cast<float2*>(base + ws.few_ml), counters, bf16,
                         guard.device(), stream, what);
   }

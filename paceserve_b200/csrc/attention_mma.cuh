@@ -68,7 +68,6 @@ struct Mma;
 
 template <>
 struct Mma<__nv_bfloat16> {
-  static constexpr bool kWideRange = true;  // fp32's exponents
   __device__ static __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                              uint32_t b1) {
     asm volatile(
@@ -84,6 +83,9 @@ struct Mma<__nv_bfloat16> {
   __device__ static __forceinline__ uint32_t pair(__nv_bfloat16 x, __nv_bfloat16 y) {
     const __nv_bfloat162 h = __halves2bfloat162(x, y);
     return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ float2 floats(uint32_t x) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
   }
   __device__ static __forceinline__ uint32_t mul2(uint32_t x, uint32_t f) {
     const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x),
@@ -111,13 +113,10 @@ struct Mma<__nv_bfloat16> {
       for (int i = 0; i < 8; ++i) o[i] = mul2(o[i], g);
     }
   }
-  // times 2^120
-  __device__ static __forceinline__ uint32_t code_scale(uint32_t x) { return mul2(x, 0x7b807b80u); }
 };
 
 template <>
 struct Mma<__half> {
-  static constexpr bool kWideRange = false;
   __device__ static __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                              uint32_t b1) {
     asm volatile(
@@ -133,6 +132,9 @@ struct Mma<__half> {
   __device__ static __forceinline__ uint32_t pair(__half x, __half y) {
     const __half2 h = __halves2half2(x, y);
     return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ float2 floats(uint32_t x) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
   }
   __device__ static __forceinline__ uint32_t mul2(uint32_t x, uint32_t f) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&x),
@@ -156,8 +158,6 @@ struct Mma<__half> {
       o[2 * i + 1] = scale2(b, f, g);
     }
   }
-  // times 2^8
-  __device__ static __forceinline__ uint32_t code_scale(uint32_t x) { return mul2(x, 0x5c005c00u); }
   // Two rows' factors times 2^8, as a product f * g of which fp16 holds each: g is 1 unless a
   // factor passes 2^7 (the product ends at 2^22, past which every value but a few subnormal codes
   // is outside fp16's range).  Factors below 2^-32 vanish: so do their values, in fp16.
@@ -273,8 +273,9 @@ __device__ __forceinline__ bool join_pieces(const Problem& p, const float* parti
 int run_tile_rows(const Problem& p, int64_t num_pages, const Item* items, int num_items, float* partial, float2* ml,
                   int32_t* counters, int32_t* fault, bool bf16, int device, cudaStream_t stream,
                   const char* what);
-int run_few_rows(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
-                 int32_t* counters, bool bf16, int device, cudaStream_t stream, const char* what);
+int run_few_rows(const Problem& p, int max_rows, const Item* items, int num_items, float* partial,
+                 float2* ml, int32_t* counters, bool bf16, int device, cudaStream_t stream,
+                 const char* what);
 
 }  // namespace attn
 }  // namespace pace

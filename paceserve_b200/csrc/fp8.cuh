@@ -18,13 +18,18 @@ __device__ __forceinline__ float exponent_factor(uint32_t exponent) {
   return __uint_as_float(exponent << 23);
 }
 
+// Two codes as two fp16 values, exactly.
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t codes) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)codes));
+  return r;
+}
+
 // Four codes (little endian) as floats, exactly.
 __device__ __forceinline__ void e4m3x4_to_floats(uint32_t codes, float* f) {
-  uint32_t lo, hi;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)(codes & 0xffffu)));
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(codes >> 16)));
-  const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo));
-  const float2 b = __half22float2(*reinterpret_cast<__half2*>(&hi));
+  const uint32_t lo = e4m3x2_to_half2(codes & 0xffffu), hi = e4m3x2_to_half2(codes >> 16);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   f[0] = a.x;
   f[1] = a.y;
   f[2] = b.x;
