@@ -51,6 +51,7 @@ struct Problem {
   int64_t q_stride, out_stride;
   int64_t total_q;
   int heads, kv_heads, head_dim, page_size, tree_words;
+  int page_shift;  // log2 of the page size; -1: no power of two
   float scale;  // of q . k
   float cap;    // 0: none
 };
@@ -60,6 +61,14 @@ __device__ __forceinline__ float score(float dot, float scale, float cap, float 
   float s = dot * scale;
   if (cap > 0.f) s = cap * tanhf(s / cap);
   return s - slope * (float)distance;
+}
+
+// Page and slot of a position, without the division where there need be none.
+__device__ __forceinline__ int page_number(const Problem& p, int pos) {
+  return p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+}
+__device__ __forceinline__ int page_slot(const Problem& p, int pos) {
+  return p.page_shift >= 0 ? pos & (p.page_size - 1) : pos % p.page_size;
 }
 
 // Whether drafted token `node` (0 .. 64 * words - 1) is visible.
@@ -106,8 +115,8 @@ __device__ void attend_row(const Problem& p, int64_t tok, int head) {
   float m = -INFINITY, l = 0.f;
   for (int j = info.lo; j < end; ++j) {
     if (j >= info.hi && !tree_bit(bits, j - info.hi)) continue;
-    const int64_t page = p.kv_indices[info.page_base + j / p.page_size];
-    const int64_t krow = (page * 2 * p.page_size + j % p.page_size) * p.kv_heads + kvh;
+    const int64_t page = p.kv_indices[info.page_base + page_number(p, j)];
+    const int64_t krow = (page * 2 * p.page_size + page_slot(p, j)) * p.kv_heads + kvh;
     const int64_t vrow = krow + (int64_t)p.page_size * p.kv_heads;
     float kf = 1.f, vf = 1.f;
     if (p.exponents) {

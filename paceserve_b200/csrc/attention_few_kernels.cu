@@ -175,43 +175,45 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
 
   // ---- the ring ---------------------------------------------------------------
   const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
-  const int64_t v_rows = (int64_t)p.page_size * p.kv_heads;
+  const int64_t v_rows = (int64_t)p.page_size * p.kv_heads, v_bytes = v_rows * Tile::kRowBytes;
   const int begin = w.kv_begin + warp * KEYS;
   const int steps = begin < w.kv_end ? (w.kv_end - begin + kFewWarps * KEYS - 1) / (kFewWarps * KEYS) : 0;
   const int my_key = lane % KEYS;
   auto page_of = [&](int step) -> int {
     const int j = begin + step * kFewWarps * KEYS + my_key;
-    return step < steps && j < w.kv_end ? p.kv_indices[w.page_base + j / p.page_size] : -1;
+    return step < steps && j < w.kv_end ? p.kv_indices[w.page_base + page_number(p, j)] : -1;
   };
-  // row number (of the whole cache, K part) of this lane's key of a step
-  auto row_of = [&](int step, int page) -> uint32_t {
-    const int j = begin + step * kFewWarps * KEYS + my_key;
-    return (uint32_t)(((int64_t)page * 2 * p.page_size + j % p.page_size) * p.kv_heads + kvh);
-  };
-  uint32_t ex = 0;  // exponents (K | V << 8) of this lane's key of the step issued last
+  uint32_t k_ex = 0, v_ex = 0;  // exponents of this lane's key of the step issued last
   auto issue = [&](int step, int page) {
-    const uint32_t row = page >= 0 ? row_of(step, page) : 0;
+    // row number (of the whole cache, K part) of this lane's key; ~0: none
+    uint32_t row = ~0u;
+    if (page >= 0) {
+      const int j = begin + step * kFewWarps * KEYS + my_key;
+      row = (uint32_t)(((int64_t)page * 2 * p.page_size + page_slot(p, j)) * p.kv_heads + kvh);
+    }
     uint8_t* slot = ring + (step % STAGES) * 2 * Tile::kKvBytes;
 #pragma unroll
     for (int i = 0; i < KEYS * Tile::kChunks / 32; ++i) {
       const int r = (i * 32 + lane) / Tile::kChunks, ch = (i * 32 + lane) % Tile::kChunks;
-      const uint32_t src_row = __shfl_sync(0xffffffffu, row, r);
-      const bool there = __shfl_sync(0xffffffffu, page, r) >= 0;
-      const uint8_t* k = cache + (int64_t)src_row * Tile::kRowBytes + ch * 16;
+      const uint32_t src = __shfl_sync(0xffffffffu, row, r);
+      const bool there = src != ~0u;
+      const uint8_t* k = cache + (there ? (int64_t)src * Tile::kRowBytes + ch * 16 : 0);
       const int at = Tile::at(r, ch);
       cp_async16(slot + at, k, there);
-      cp_async16(slot + Tile::kKvBytes + at, k + (there ? v_rows * Tile::kRowBytes : 0), there);
+      cp_async16(slot + Tile::kKvBytes + at, k + (there ? v_bytes : 0), there);
     }
     if constexpr (Q8) {
-      ex = 0;
-      if (page >= 0)
-        ex = (uint32_t)p.exponents[row] | (uint32_t)p.exponents[row + v_rows] << 8;
+      k_ex = v_ex = 0;
+      if (row != ~0u) {
+        k_ex = p.exponents[row];
+        v_ex = p.exponents[row + v_rows];
+      }
     }
   };
   auto put_factors = [&](int step) {
     if constexpr (Q8) {
-      factors[(step % STAGES) * KEYS + lane] = exponent_factor(ex & 0xff);
-      v_exps[(step % STAGES) * KEYS + lane] = (int)(ex >> 8);
+      factors[(step % STAGES) * KEYS + lane] = exponent_factor(k_ex);
+      v_exps[(step % STAGES) * KEYS + lane] = (int)v_ex;
     }
   };
 

@@ -324,6 +324,9 @@ extern "C" int pace_paged_attention(const pace_attention_plan* plan, const int32
   p.head_dim = plan->head_dim;
   p.page_size = plan->page_size;
   p.tree_words = plan->tree_words;
+  p.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (plan->page_size == 1 << s) p.page_shift = s;
   p.scale = sm_scale;
   p.cap = logits_soft_cap;
   StreamDeviceGuard guard(stream);

@@ -716,7 +716,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         const int key = lane * box;
         auto look_up = [&](int j) {
           const int pos = k_base + j * kStepKeys + key;
-          return key < kStepKeys && pos < w.kv_end ? p.kv_indices[w.page_base + pos / p.page_size] : -1;
+          return key < kStepKeys && pos < w.kv_end ? p.kv_indices[w.page_base + page_number(p, pos)] : -1;
         };
         page = look_up(0);
         for (int i = 0; ok && i < 2 * steps; ++i) {
@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
           __syncwarp();
           if (page >= 0) {
             const int pos = k_base + (i >> 1) * kStepKeys + key;
-            tma_load_page(codes + s * Cfg::kCodeBytes + key * D, &map, 0, kvh, pos % p.page_size,
+            tma_load_page(codes + s * Cfg::kCodeBytes + key * D, &map, 0, kvh, page_slot(p, pos),
                           page * 2 + (i & 1), &ctl->code_full[s]);
           }
           if (i & 1) page = look_up((i >> 1) + 1);
@@ -742,8 +742,8 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         auto row_of = [&](int j, int key) -> int64_t {
           const int pos = k_base + j * kStepKeys + key;
           if (j >= steps || pos < w.kv_begin || pos >= w.kv_end) return -1;
-          const int64_t page = p.kv_indices[w.page_base + pos / p.page_size];
-          return (page * 2 * p.page_size + pos % p.page_size) * p.kv_heads + kvh;
+          const int64_t page = p.kv_indices[w.page_base + page_number(p, pos)];
+          return (page * 2 * p.page_size + page_slot(p, pos)) * p.kv_heads + kvh;
         };
         // rows two steps ahead, exponents one step ahead: their loads depend on each other
         int64_t rows[2] = {row_of(0, u), row_of(0, u + 64)};
@@ -827,15 +827,15 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
       const bool has_box = u < 32 && box > 0 && box_key < kStepKeys;
       auto page_of = [&](int j) {  // of this lane's box
         const int pos = k_base + j * kStepKeys + box_key;
-        return has_box && j < steps && pos < w.kv_end ? p.kv_indices[w.page_base + pos / p.page_size]
+        return has_box && j < steps && pos < w.kv_end ? p.kv_indices[w.page_base + page_number(p, pos)]
                                                       : 0;
       };
       int page = u < 32 ? page_of(0) : 0;
       auto row_of = [&](int j, int key) -> uint32_t {
         const int pos = k_base + j * kStepKeys + key;
         if (j >= steps || pos < w.kv_begin || pos >= w.kv_end) return ~0u;
-        const int64_t page = p.kv_indices[w.page_base + pos / p.page_size];
-        return (uint32_t)((page * 2 * p.page_size + pos % p.page_size) * p.kv_heads + kvh);
+        const int64_t page = p.kv_indices[w.page_base + page_number(p, pos)];
+        return (uint32_t)((page * 2 * p.page_size + page_slot(p, pos)) * p.kv_heads + kvh);
       };
       constexpr int kOwn = (kStepKeys + N - 1) / N;  // keys whose row a thread looks up
       uint32_t next[kOwn];
@@ -872,7 +872,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
               __syncwarp();
               if (has_box)
                 tma_load_page(ring + s * Cfg::kKvBytes + box_half * 16384 + box_key * 128, &map,
-                              box_half * 64, kvh, pos % p.page_size, page * 2 + kind,
+                              box_half * 64, kvh, page_slot(p, pos), page * 2 + kind,
                               &ctl->kv_full[s]);
             }
             page = page_of(j + 1);
