@@ -34,13 +34,16 @@ namespace attn {
 
 constexpr int kFewWarps = 4;
 
-template <int D, bool Q8>
+template <int D, bool Q8, int R>
 struct FewTile {
   static constexpr int kKeys = D == 128 && !Q8 ? 16 : 32;  // of a warp's turn
   static constexpr int kRowBytes = Q8 ? D : 2 * D;
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kKvBytes = kKeys * kRowBytes;
-  static constexpr int kStages = 3;
+  // One row half of a quantised cache fits three CTAs an SM with two slots each (64 requests: 170
+  // us, two CTAs with three slots 180 us).
+  static constexpr int kCtas = Q8 && R == 1 ? 3 : 2;
+  static constexpr int kStages = Q8 && R == 1 ? 2 : 3;
   static constexpr int kRingBytes = kStages * 2 * kKvBytes;
   static constexpr int kJoinBytes = 16 * D * 4;  // a warp's output, over its ring
   static constexpr int kWarpBytes = kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes;
@@ -66,10 +69,10 @@ __device__ __forceinline__ float v_factor(int exponent, int top) {
 
 // R: 1 where the rows fit the matrix instruction's first eight, else 2.
 template <typename T, int D, bool Q8, int R>
-__global__ void __launch_bounds__(kFewWarps * 32, 2)
+__global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
     attention_few_kernel(const Problem p, const Item* __restrict__ items, float* partial,
-                         float2* partial_ml, int32_t* counters, bool q_even) {
-  using Tile = FewTile<D, Q8>;
+                         float2* partial_ml, int32_t* counters, bool q_even, bool beside) {
+  using Tile = FewTile<D, Q8, R>;
   using M = Mma<std::conditional_t<Q8, __half, T>>;
   constexpr int KEYS = Tile::kKeys, NT = KEYS / 8, KB = D / 16, STAGES = Tile::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -85,8 +88,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   int* v_exps = reinterpret_cast<int*>(factors + Tile::kStages * KEYS);
   float* join_ml = reinterpret_cast<float*>(
       smem + kFewWarps * (Tile::kWarpBytes + Tile::kFactorBytes));  // [warp][16][m, l]
+  // `beside`: the kernel before this one in the stream is the tile kernel of the same call, which
+  // this one reads nothing of and which let it start only when all before both was complete.  It
+  // then waits for that kernel at its end, for the sake of what comes after.
   pdl_launch_dependents();
-  pdl_wait();
+  if (!beside) pdl_wait();
 
   // ---- rows g and g + 8 of this thread: visible keys, slope, queries --------
   int lo[R], hi[R], pos[R];
@@ -445,40 +451,52 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
     }
     if (w.mixed) redo_rows<T, D, Q8>(p, w, kvh, group, r, fine);
   }
-  if (w.splits == 1) return;
+  if (w.splits == 1) {
+    if (beside) pdl_wait();
+    return;
+  }
 
   // ---- the last piece of these rows to arrive joins them all --------------------
   __shared__ bool last;
-  if (!arrive_last(counters + (int64_t)w.tile * p.kv_heads + kvh, w.splits, &last)) return;
-  for (int u = threadIdx.x; (u & ~31) < rows * V4; u += kFewWarps * 32) {
-    const int r = u / V4, d = (u - r * V4) * 4;
-    const bool fine =
-        u >= rows * V4 || join_pieces<T, 16>(p, partial, partial_ml, w, kvh, r, d, D, group);
-    if (w.mixed) redo_rows<T, D, Q8>(p, w, kvh, group, r, fine);
-  }
+  if (arrive_last(counters + (int64_t)w.tile * p.kv_heads + kvh, w.splits, &last))
+    join_pieces<T, 16, D, Q8, kFewWarps * 32>(p, partial, partial_ml, w, kvh, group, rows,
+                                              reinterpret_cast<float*>(smem),
+                                              kFewWarps * Tile::kWarpBytes / 4);
+  if (beside) pdl_wait();
 }
 
-template <typename T, int D, bool Q8>
-static int run_few(const Problem& p, int max_rows, const Item* items, int num_items, float* partial, float2* ml,
-                   int32_t* counters, int device, cudaStream_t stream, const char* what) {
-  using Tile = FewTile<D, Q8>;
-  auto kernel = max_rows <= 8 ? attention_few_kernel<T, D, Q8, 1> : attention_few_kernel<T, D, Q8, 2>;
+template <typename T, int D, bool Q8, int R>
+static int run_few_r(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
+                     int32_t* counters, bool beside, int device, cudaStream_t stream,
+                     const char* what) {
+  using Tile = FewTile<D, Q8, R>;
+  auto kernel = attention_few_kernel<T, D, Q8, R>;
   cudaError_t err =
       ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), device, Tile::kSmemBytes);
   if (err != cudaSuccess) return cuda_fail(err, what);
   const bool even = (reinterpret_cast<uintptr_t>(p.query) & 3) == 0 && p.q_stride % 2 == 0;
   err = launch(kernel, dim3((unsigned)(num_items * p.kv_heads)), dim3(kFewWarps * 32),
-               Tile::kSmemBytes, stream, p, items, partial, ml, counters, even);
+               Tile::kSmemBytes, stream, p, items, partial, ml, counters, even, beside);
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, what);
 }
 
+template <typename T, int D, bool Q8>
+static int run_few(const Problem& p, int max_rows, const Item* items, int num_items, float* partial,
+                   float2* ml, int32_t* counters, bool beside, int device, cudaStream_t stream,
+                   const char* what) {
+  return max_rows <= 8 ? run_few_r<T, D, Q8, 1>(p, items, num_items, partial, ml, counters, beside,
+                                                device, stream, what)
+                       : run_few_r<T, D, Q8, 2>(p, items, num_items, partial, ml, counters, beside,
+                                                device, stream, what);
+}
+
 int run_few_rows(const Problem& p, int max_rows, const Item* items, int num_items, float* partial,
-                 float2* ml, int32_t* counters, bool bf16, int device, cudaStream_t stream,
-                 const char* what) {
+                 float2* ml, int32_t* counters, bool beside, bool bf16, int device,
+                 cudaStream_t stream, const char* what) {
   auto pick = [&](auto t) -> int {
     using T = decltype(t);
     auto go = [&](auto f) {
-      return f(p, max_rows, items, num_items, partial, ml, counters, device, stream, what);
+      return f(p, max_rows, items, num_items, partial, ml, counters, beside, device, stream, what);
     };
     if (p.head_dim == 128) return p.exponents ? go(run_few<T, 128, true>) : go(run_few<T, 128, false>);
     return p.exponents ? go(run_few<T, 64, true>) : go(run_few<T, 64, false>);

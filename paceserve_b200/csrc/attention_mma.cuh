@@ -242,31 +242,81 @@ __device__ __forceinline__ bool arrive_last(int32_t* counter, int splits, bool* 
   return true;
 }
 
-// Joins columns d .. d + 3 of row r over the pieces of item w's rows and writes
-// the output.  ROWS: rows of a slot.
-template <typename T, int ROWS>
-__device__ __forceinline__ bool join_pieces(const Problem& p, const float* partial,
-                                            const float2* partial_ml, const Item& w, int kvh, int r,
-                                            int d, int D, int group) {
+template <int NT>
+__device__ __forceinline__ void join_sync() {
+  asm volatile("bar.sync 2, %0;" ::"n"(NT) : "memory");
+}
+
+// Joins the pieces of item w's rows and writes the output: threads 0 .. NT - 1.
+// ROWS: rows of a slot; scratch: `room` floats of shared memory.  The pieces'
+// weights 2^(m_k - M) are found once per row; then every thread keeps four
+// columns of four units, a piece of each, in flight (one unit at a time, each
+// waiting for its own loads, 32 trees took 155 us instead of 105 uncut).
+template <typename T, int ROWS, int D, bool Q8, int NT>
+__device__ __forceinline__ void join_pieces(const Problem& p, const float* partial,
+                                            const float2* partial_ml, const Item& w, int kvh,
+                                            int group, int rows, float* scratch, int room) {
+  constexpr int V4 = D / 4, U = 4;
   const int64_t first = (int64_t)w.slot * p.kv_heads + kvh;
-  float mm = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int k = 0; k < w.splits; ++k)
-    mm = fmaxf(mm, __ldcg(partial_ml + (first + (int64_t)k * p.kv_heads) * ROWS + r).x);
-  const float b = mm == -INFINITY ? 0.f : mm;
-#pragma unroll 4
-  for (int k = 0; k < w.splits; ++k) {
-    const int64_t at = (first + (int64_t)k * p.kv_heads) * ROWS + r;
-    const float2 ml = __ldcg(partial_ml + at);
-    const float4 x = __ldcg(reinterpret_cast<const float4*>(partial + at * D + d));
-    const float f = exp2_approx(ml.x - b);
-    sum += f * ml.y;
-    v[0] += f * x.x;
-    v[1] += f * x.y;
-    v[2] += f * x.z;
-    v[3] += f * x.w;
+  const int most = min(rows, room / (2 * w.splits + 2));  // rows of a pass
+  for (int r0 = 0; r0 < rows; r0 += most) {
+    const int n = min(most, rows - r0);
+    float *ms = scratch, *ls = ms + n * w.splits, *top = ls + n * w.splits, *total = top + n;
+    for (int x = threadIdx.x; x < n * w.splits; x += NT) {
+      const int k = x / n, r = x - k * n;
+      const float2 ml = __ldcg(partial_ml + (first + (int64_t)k * p.kv_heads) * ROWS + r0 + r);
+      ms[x] = ml.x;
+      ls[x] = ml.y;
+    }
+    join_sync<NT>();
+    for (int r = threadIdx.x; r < n; r += NT) {
+      float mm = -INFINITY, sum = 0.f;
+      for (int k = 0; k < w.splits; ++k) mm = fmaxf(mm, ms[k * n + r]);
+      const float b = mm == -INFINITY ? 0.f : mm;
+      for (int k = 0; k < w.splits; ++k) {
+        const float f = exp2_approx(ms[k * n + r] - b);
+        sum += f * ls[k * n + r];
+        ms[k * n + r] = f;
+      }
+      top[r] = mm;
+      total[r] = sum;
+    }
+    join_sync<NT>();
+    // whole warps stay in the loop, for redo_rows
+    for (int u0 = threadIdx.x; (u0 & ~31) < n * V4; u0 += U * NT) {
+      float v[U][4];
+#pragma unroll
+      for (int i = 0; i < U; ++i) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+#pragma unroll 2
+      for (int k = 0; k < w.splits; ++k) {
+        const float* piece = partial + ((first + (int64_t)k * p.kv_heads) * ROWS + r0) * D;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int u = u0 + i * NT;
+          if (u < n * V4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(piece) + u);
+            const float f = ms[k * n + u / V4];
+            v[i][0] += f * x.x;
+            v[i][1] += f * x.y;
+            v[i][2] += f * x.z;
+            v[i][3] += f * x.w;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int u = u0 + i * NT;
+        if ((u & ~31) >= n * V4) break;
+        const int r = u / V4;
+        bool fine = true;
+        if (u < n * V4)
+          fine = write_out<T>(p, w.tok0 + (r0 + r) / group, kvh * group + (r0 + r) % group,
+                              (u - r * V4) * 4, v[i], top[r], total[r]);
+        if (w.mixed) redo_rows<T, D, Q8>(p, w, kvh, group, r0 + r, fine);
+      }
+    }
+    join_sync<NT>();
   }
-  return write_out<T>(p, w.tok0 + r / group, kvh * group + r % group, d, v, mm, sum);
 }
 
 // The two tensor-core kernels' launchers.
@@ -274,8 +324,8 @@ int run_tile_rows(const Problem& p, int64_t num_pages, const Item* items, int nu
                   int32_t* counters, int32_t* fault, bool bf16, int device, cudaStream_t stream,
                   const char* what);
 int run_few_rows(const Problem& p, int max_rows, const Item* items, int num_items, float* partial,
-                 float2* ml, int32_t* counters, bool bf16, int device, cudaStream_t stream,
-                 const char* what);
+                 float2* ml, int32_t* counters, bool beside, bool bf16, int device,
+                 cudaStream_t stream, const char* what);
 
 }  // namespace attn
 }  // namespace pace

@@ -287,7 +287,6 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   const int k_base = w.kv_begin & ~(kStepKeys - 1);
   const int steps = w.kv_end > w.kv_begin ? (w.kv_end - k_base + kStepKeys - 1) / kStepKeys : 0;
 
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&ctl->q_full[i], 128);
@@ -314,6 +313,9 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   tc::tc_fence_after();
   const uint32_t tmem = ctl->tmem;
   pdl_wait();
+  // not earlier: the few-row kernel of the same call starts beside this one without a wait of its
+  // own, on what is complete here
+  pdl_launch_dependents();
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kSoftmaxRegs));
@@ -966,12 +968,9 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   // ---- the last piece of these rows to arrive joins them all --------------------
   if (!arrive_last(counters + (int64_t)w.tile * p.kv_heads + kvh, w.splits, &ctl->last)) return;
   if (warp >= 8) return;  // these gave their registers away
-  for (int u = threadIdx.x; (u & ~31) < rows * (D / 4); u += 256) {
-    const int r = u / (D / 4), d = (u - r * (D / 4)) * 4;
-    const bool fine = u >= rows * (D / 4) ||
-                      join_pieces<T, 256>(p, partial, partial_ml, w, kvh, r, d, D, group);
-    if (w.mixed) redo_rows<T, D, Q8>(p, w, kvh, group, r, fine);
-  }
+  join_pieces<T, 256, D, Q8, 256>(p, partial, partial_ml, w, kvh, group, rows,
+                                  reinterpret_cast<float*>(ring),
+                                  Cfg::kStages * Cfg::kKvBytes / 4);
 }
 
 // Tensor map of the cache as [2 * pages, page_size, kv_heads, D], boxes of `box`
