@@ -55,11 +55,10 @@ class PagedAttention:
             device = torch.device("cuda", torch.cuda.current_device())
         self.device = device
         self.num_sms = torch.cuda.get_device_properties(device).multi_processor_count
-        self.plan = None
-        self._tree_mask: Optional[torch.Tensor] = None
+        self._scale = 1.0 / math.sqrt(head_dim)
         self._workspace = torch.zeros(0, dtype=torch.uint8, device=device)
-        self._words: Optional[torch.Tensor] = None
-        self._planned: Optional[torch.cuda.Event] = None
+        self._step = None
+        self.plan = None
 
     def begin_forward(self, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, *,
                       window_left: int = -1, prefix_lens=None, doc_starts=None) -> None:
@@ -76,7 +75,6 @@ class PagedAttention:
         zeros."""
         self._begin(qo_indptr, kv_indptr, kv_indices, kv_last_page_len, window_left=window_left,
                     prefix_lens=prefix_lens, doc_starts=doc_starts)
-        self._tree_mask = None
 
     def begin_tree_forward(self, qo_indptr, kv_indptr, kv_indices, kv_last_page_len,
                            tree_mask: torch.Tensor) -> None:
@@ -87,29 +85,28 @@ class PagedAttention:
         int64 [tokens, words], 64 drafted tokens a word."""
         if tree_mask.dim() != 2 or tree_mask.dtype != torch.int64 or tree_mask.shape[1] == 0:
             raise RuntimeError("begin_tree_forward: tree_mask must be int64 [tokens, words]")
-        self._begin(qo_indptr, kv_indptr, kv_indices, kv_last_page_len,
-                    tree_words=tree_mask.shape[1])
-        if tree_mask.shape[0] != self.plan.total_q:
-            self.plan = None
-            raise RuntimeError("begin_tree_forward: tree_mask needs a row for each new token")
-        self._tree_mask = tree_mask.to(self.device, non_blocking=True).contiguous()
+        self._begin(qo_indptr, kv_indptr, kv_indices, kv_last_page_len, tree_mask=tree_mask)
 
     def _begin(self, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, *, window_left=-1,
-               prefix_lens=None, doc_starts=None, tree_words=0) -> None:
-        self.plan = None
+               prefix_lens=None, doc_starts=None, tree_mask=None) -> None:
+        self._step = self.plan = None
         plan = attention_ops.plan_paged_attention(
             _host_ints(qo_indptr), _host_ints(kv_indptr), _host_ints(kv_indices),
             _host_ints(kv_last_page_len), self.num_heads, self.num_kv_heads, self.head_dim,
             self.page_size, window_left,
             None if prefix_lens is None else _host_ints(prefix_lens),
-            None if doc_starts is None else _host_ints(doc_starts), tree_words, self.num_sms)
+            None if doc_starts is None else _host_ints(doc_starts),
+            0 if tree_mask is None else tree_mask.shape[1], self.num_sms)
+        if tree_mask is not None and tree_mask.shape[0] != plan.total_q:
+            raise RuntimeError("begin_tree_forward: tree_mask needs a row for each new token")
         with torch.cuda.device(self.device):
-            self._words = plan.words.to(self.device, non_blocking=True)
             if self._workspace.numel() < plan.workspace_bytes:
                 self._workspace = torch.zeros(plan.workspace_bytes, dtype=torch.uint8,
                                               device=self.device)
-            self._planned = torch.cuda.current_stream().record_event()
-            self._stream = torch.cuda.current_stream().cuda_stream
+            if tree_mask is not None:
+                tree_mask = tree_mask.to(self.device, non_blocking=True).contiguous()
+            self._step = attention_ops.AttentionStep(
+                plan, plan.words.to(self.device, non_blocking=True), self._workspace, tree_mask)
         self.plan = plan
 
     def forward(self, query: torch.Tensor, paged_kv_cache: torch.Tensor, *,
@@ -122,23 +119,8 @@ class PagedAttention:
         [pages, 2, page_size, num_kv_heads, head_dim], or over a quantised
         cache's codes with its ``exponents``.  ``lse`` (float32 [tokens,
         num_heads]) receives each row's log-sum-exp."""
-        if self.plan is None:
+        if self._step is None:
             raise RuntimeError("PagedAttention.forward: begin_forward has not planned a step")
-        if out is None:
-            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        if query.is_cuda:
-            stream = torch.cuda.current_stream(query.device)
-            if stream.cuda_stream != self._stream and not torch.cuda.is_current_stream_capturing():
-                # another stream than the plan's: its copy to the device comes first, and the
-                # plan's memory is kept from reuse until this stream is done with it.  A graph
-                # keeps to neither: torch.cuda.graph waits for the GPU before it captures, and
-                # the object has to outlive the graph.
-                stream.wait_event(self._planned)
-                for t in (self._words, self._workspace, self._tree_mask):
-                    if t is not None:
-                        t.record_stream(stream)
-        attention_ops.paged_attention(
-            out, query, paged_kv_cache, self.plan, self._words, self._workspace,
-            1.0 / math.sqrt(self.head_dim) if sm_scale is None else sm_scale, logits_soft_cap,
-            exponents, alibi_slopes, self._tree_mask, lse, fault_flags)
-        return out
+        return self._step.forward(query, paged_kv_cache, exponents,
+                                  self._scale if sm_scale is None else sm_scale, logits_soft_cap,
+                                  alibi_slopes, out, lse, fault_flags)

@@ -10,6 +10,8 @@
 // through the C ABI on the current stream of the tensors' device, and a
 // non-zero status becomes a RuntimeError carrying pace_last_error().
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAEvent.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -1124,6 +1126,48 @@ void paged_attention(Tensor& out, const Tensor& query, const Tensor& paged_kv_ca
                op);
 }
 
+// A plan with its words on the device, its workspace and (for a tree) its mask:
+// what every layer of the step runs on.
+struct AttentionStep {
+  AttentionPlan plan;
+  Tensor words, workspace;
+  c10::optional<Tensor> tree_mask;
+  cudaStream_t stream;
+  at::cuda::CUDAEvent ready;
+
+  AttentionStep(const AttentionPlan& p, const Tensor& w, const Tensor& ws,
+                const c10::optional<Tensor>& mask)
+      : plan(p), words(w), workspace(ws), tree_mask(mask) {
+    check_cuda(words, "AttentionStep", "words");
+    const at::cuda::CUDAGuard guard(words.device());
+    const auto cur = at::cuda::getCurrentCUDAStream(words.device().index());
+    stream = cur.stream();
+    ready.record(cur);
+  }
+
+  Tensor forward(const Tensor& query, const Tensor& paged_kv_cache,
+                 const c10::optional<Tensor>& exponents, double sm_scale, double logits_soft_cap,
+                 const c10::optional<Tensor>& alibi_slopes, const c10::optional<Tensor>& out,
+                 const c10::optional<Tensor>& lse, const c10::optional<Tensor>& fault_flags) {
+    check_cuda(query, "paged_attention", "query");
+    const auto cur = at::cuda::getCurrentCUDAStream(query.device().index());
+    if (cur.stream() != stream && query.device() == words.device() &&
+        at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) {
+      // another stream than the plan's: its copy to the device comes first, and its memory is
+      // kept from reuse until this stream is done with it.  A graph keeps to neither: it is
+      // captured with the GPU idle, and the step has to outlive it.
+      ready.block(cur);
+      words.record_stream(cur);
+      workspace.record_stream(cur);
+      if (tree_mask.has_value()) tree_mask->record_stream(cur);
+    }
+    Tensor o = out.has_value() ? *out : torch::empty(query.sizes(), query.options());
+    paged_attention(o, query, paged_kv_cache, plan, words, workspace, sm_scale, logits_soft_cap,
+                    exponents, alibi_slopes, tree_mask, lse, fault_flags);
+    return o;
+  }
+};
+
 py::tuple ipc_get_handle(const Tensor& t) {
   TORCH_CHECK(t.is_cuda(), "ipc_get_handle: tensor must be on a CUDA device");
   const at::cuda::CUDAGuard guard(t.device());
@@ -1276,6 +1320,15 @@ PYBIND11_MODULE(_C, m) {
           py::arg("logits_soft_cap") = 0.0, py::arg("exponents") = py::none(),
           py::arg("alibi_slopes") = py::none(), py::arg("tree_mask") = py::none(),
           py::arg("lse") = py::none(), py::arg("fault_flags") = py::none());
+
+  py::class_<AttentionStep>(at_, "AttentionStep")
+      .def(py::init<const AttentionPlan&, const Tensor&, const Tensor&,
+                    const c10::optional<Tensor>&>(),
+           py::arg("plan"), py::arg("words"), py::arg("workspace"),
+           py::arg("tree_mask") = py::none())
+      .def("forward", &AttentionStep::forward, py::arg("query"), py::arg("paged_kv_cache"),
+           py::arg("exponents"), py::arg("sm_scale"), py::arg("logits_soft_cap"),
+           py::arg("alibi_slopes"), py::arg("out"), py::arg("lse"), py::arg("fault_flags"));
 
   auto kv = m.def_submodule("kv_transfer_ops");
   kv.def("copy_blocks_p2p", &copy_blocks_p2p,
