@@ -33,6 +33,7 @@ namespace pace {
 namespace attn {
 
 constexpr int kFewWarps = 4;
+constexpr float kLag = 8.f;  // in powers of two
 
 template <int D, bool Q8, int R>
 struct FewTile {
@@ -284,9 +285,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
     }
     // ---- scores in powers of two, masks ---------------------------------------
     const int j0 = begin + step * kFewWarps * KEYS;
-    float away[R];  // from each row's token to the thread's first key
-#pragma unroll
-    for (int i = 0; i < R; ++i) away[i] = (float)(pos[i] - j0 - 2 * c);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float2 f = make_float2(1.f, 1.f);
@@ -297,8 +295,24 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
         if constexpr (Q8) x *= e & 1 ? f.y : f.x;
         if (p.cap > 0.f)
           x = cap2 - 2.f * cap2 * rcp_approx(1.f + exp2_approx(x * cap_in));  // cap tanh
-        if (p.slopes) x -= slope[e >> 1] * fabsf(away[e >> 1] - (float)(n * 8 + (e & 1)));
         s[n][e] = x;
+      }
+    }
+    if (p.slopes) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        // from the row's token to the thread's first key; it is before the token in most steps,
+        // where the bias rises by the slope from key to key
+        const float away = (float)(pos[i] - j0 - 2 * c);
+        const float first = -slope[i] * away;
+        const bool before = away >= (float)KEYS;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float k = (float)(n * 8 + e);
+            s[n][2 * i + e] += before ? fmaf(slope[i], k, first) : -slope[i] * fabsf(away - k);
+          }
       }
     }
     if (j0 < all_lo || j0 + KEYS > min(all_hi, w.kv_end)) {
@@ -312,26 +326,37 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
           if (!see) s[n][e] = -INFINITY;
         }
     }
-    float v_down = 1.f;  // what a rise of V's largest exponent does to O
-    if constexpr (Q8) {
-      const int x = ve[lane];
-      const int top = max(v_top, (int)__reduce_max_sync(0xffffffffu, x == kNanExponent ? 0 : x));
-      if (top > v_top) v_down = pow2_down(top - v_top);
-      v_top = top;
-    }
-    // ---- running maximum and sum ----------------------------------------------
-    float base[R];
+    // ---- running maximum and sum: the maximum may lag by 2^kLag, so that most steps
+    // need neither the row's maximum, which its lanes share by shuffles, nor a new scale
+    float most[R];
+    bool rise = false;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      float t = -INFINITY;
+      most[i] = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) t = fmaxf(t, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
-      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-      const float m2 = fmaxf(m[i], t);
-      base[i] = m2 == -INFINITY ? 0.f : m2;
-      if (v_down != 1.f || __any_sync(0xffffffffu, m2 > m[i])) {
-        float f = exp2_approx(m[i] - base[i]);  // 0 while m is -inf
+      for (int n = 0; n < NT; ++n) most[i] = fmaxf(most[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]));
+      rise |= most[i] > m[i] + kLag || (m[i] == -INFINITY && most[i] > m[i]);
+    }
+    int v_new = v_top;
+    if constexpr (Q8) {
+      const int x = ve[lane];
+      v_new = max(v_top, x == kNanExponent ? 0 : x);
+      rise |= v_new > v_top;
+    }
+    if (__any_sync(0xffffffffu, rise)) {
+      float v_down = 1.f;  // what a rise of V's largest exponent does to O
+      if constexpr (Q8) {
+        v_new = (int)__reduce_max_sync(0xffffffffu, v_new);
+        v_down = pow2_down(v_new - v_top);
+        v_top = v_new;
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        float t = most[i];
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+        const float m2 = fmaxf(m[i], t);
+        float f = exp2_approx(m[i] - (m2 == -INFINITY ? 0.f : m2));  // 0 while m is -inf
         l[i] *= f;
         f *= v_down;
 #pragma unroll
@@ -339,9 +364,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
           o[n][2 * i] *= f;
           o[n][2 * i + 1] *= f;
         }
+        m[i] = m2;
       }
-      m[i] = m2;
     }
+    float base[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -190,14 +190,13 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint64_t both(float x) { return f32x2(x, x); }
 
 // tanh(u) / u on |u| <= 1 as a polynomial in z = u^2, fitted for the least
-// largest error of tanh (2.3e-8).
+// largest error of tanh (2.5e-7: in the score, 1.3e-5 of a cap of 50).
 __device__ __forceinline__ uint64_t tanh_ratio_pair(uint64_t z) {
-  uint64_t y = fma2(both(0.000964018632657826f), z, both(-0.005952119827270508f));
-  y = fma2(y, z, both(0.019974395632743835f));
-  y = fma2(y, z, both(-0.053266558796167374f));
-  y = fma2(y, z, both(0.13319607079029083f));
-  y = fma2(y, z, both(-0.33332133293151855f));
-  return fma2(y, z, both(0.9999997019767761f));
+  uint64_t y = fma2(both(-0.002840145258232951f), z, both(0.016116151586174965f));
+  y = fma2(y, z, both(-0.05097497999668121f));
+  y = fma2(y, z, both(0.13253627717494965f));
+  y = fma2(y, z, both(-0.33324024081230164f));
+  return fma2(y, z, both(0.9999968409538269f));
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");

@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHeadDim = 256;
-constexpr int kResident = 4;  // CTAs that an SM holds
+constexpr int kResident = 6;  // CTAs that an SM holds
 
 struct QuantJob : PageTable {
   int64_t rows;  // tokens appended or read back
@@ -427,7 +427,7 @@ extern "C" int pace_append_quantised_paged_kv_cache(
     else if (nnz <= 16 * sms)
       err = go(kv_quant_append_kernel<T, 1, true>, 1);
     else
-      err = go(kv_quant_append_kernel<T, 4, true>, 4);
+      err = go(kv_quant_append_kernel<T, 2, true>, 2);
     if (err != cudaSuccess) return cuda_fail(err, what);
     return (int)PACE_OK;
   });
@@ -473,9 +473,9 @@ extern "C" int pace_read_quantised_paged_kv_cache(
                             : go(kv_quant_read_kernel<T, 8, 1, false>, 1);
     else if (codes_per == 16)
       err = few ? go(kv_quant_read_kernel<T, 16, 1, true>, 1)
-                : go(kv_quant_read_kernel<T, 16, 4, true>, 4);
+                : go(kv_quant_read_kernel<T, 16, 2, true>, 2);
     else
-      err = go(kv_quant_read_kernel<T, 8, 4, true>, 4);
+      err = go(kv_quant_read_kernel<T, 8, 2, true>, 2);
     if (err != cudaSuccess) return cuda_fail(err, what);
     return (int)PACE_OK;
   });
