@@ -40,10 +40,10 @@ struct TileCfg {
   static constexpr int kThreads = kLoadWarp0 * 32 + kLoaders;
   static constexpr int kKvBytes = kStepKeys * D * 2;
   static constexpr int kQBytes = kTileRowsEach * D * 2;
-  static constexpr int kStages = D == 64 ? 8 : Q8 ? 3 : 5;
+  static constexpr int kStages = D == 64 ? 8 : Q8 ? 4 : 5;
   // a quantised cache's codes, as copied: K or V of a step
   static constexpr int kCodeBytes = kStepKeys * D;
-  static constexpr int kCodeStages = 3;
+  static constexpr int kCodeStages = 2;  // of TileCtl
   static constexpr int kCodeRingBytes = Q8 ? kCodeStages * kCodeBytes : 0;
   static constexpr int kSmemBytes =
       2 * kQBytes + kStages * kKvBytes + kCodeRingBytes + 1024 + 2048;
@@ -56,12 +56,12 @@ struct TileCfg {
 struct TileCtl {
   uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2];
   uint64_t kv_full[8], kv_empty[8];
-  uint64_t code_full[3], code_empty[3];
+  uint64_t code_full[2], code_empty[2];
   uint64_t drain;
   uint32_t tmem;
   int abort;
   bool last;
-  uint8_t exps[3][kStepKeys];   // exponents of the keys of a slot of codes
+  uint8_t exps[2][kStepKeys];   // exponents of the keys of a slot of codes
   uint32_t rows[kStepKeys];     // cache row (K part) of each key of a step; ~0: none
 };
 static_assert(sizeof(TileCtl) <= 2048, "");
@@ -378,7 +378,9 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         if (p.tree_mask) tree = p.tree_mask + (int64_t)tok * p.tree_words;
       }
       const int end = tree ? min(info.pos, w.kv_end) : 0;  // of the drafted keys
-      const int lo = max(info.lo, w.kv_begin), hi = min(info.hi, w.kv_end);
+      // a row that is none sees everything, which saves its warp the masks; nothing is made of it
+      const int lo = live ? max(info.lo, w.kv_begin) : 0;
+      const int hi = live ? min(info.hi, w.kv_end) : INT32_MAX;
       const float scale2 = (p.scale != 0.f ? fabsf(p.scale) : 1.f) * kLog2e;
       const float cap2 = p.cap * kLog2e, cap_in = p.cap > 0.f ? 2.f * scale2 / p.cap : 0.f;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         if (!__all_sync(0xffffffffu, whole)) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t bits = seen_bits(j0 + 32 * k, lo, hi, info.hi, end, tree);
+            const uint32_t bits = seen_bits(j0 + 32 * k, lo, min(hi, w.kv_end), info.hi, end, tree);
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!(bits >> i & 1)) sr[32 * k + i] = 0xff800000u;
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
                 l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
         }
         if (w.mixed && w.splits == 1) {
-          uint32_t bad = __ballot_sync(0xffffffffu, !(size < INFINITY));
+          uint32_t bad = __ballot_sync(0xffffffffu, live && !(size < INFINITY));
           if (bad) __syncwarp();  // their stores come before the ones below
           for (; bad; bad &= bad - 1) {
             const int at = row - lane + __ffs(bad) - 1;
@@ -779,10 +781,11 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
       if (!ok) tile_fault(ctl, fault);
     } else if (Q8 && box > 0) {
       // ---- codes to 16-bit values, slot by slot -------------------------------------
-      constexpr int N = Cfg::kLoaders;
+      // A thread has one key, whose factor it finds once; the chunk it begins with goes
+      // by the key, so that neighbours meet in no bank.
       constexpr int kChunks = D / 16;
-      constexpr int kEach = kStepKeys * kChunks / N;
-      const int u = threadIdx.x - Cfg::kLoadWarp0 * 32;
+      static_assert(Cfg::kLoaders == kStepKeys || !Q8, "");
+      const int key = threadIdx.x - Cfg::kLoadWarp0 * 32;
       bool ok = true;
       for (int i = 0; ok && i < 2 * steps; ++i) {
         const int s = i % Cfg::kCodeStages, d = i % Cfg::kStages;
@@ -791,15 +794,19 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
           ok = wait_for(&ctl->kv_empty[d], (uint32_t)(i / Cfg::kStages - 1) & 1u, ctl);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint8_t* src = codes + s * Cfg::kCodeBytes;
+        const uint8_t* src = codes + s * Cfg::kCodeBytes + key * D;
         uint8_t* dst = ring + d * Cfg::kKvBytes;
-#pragma unroll 4
-        for (int x = 0; x < kEach; ++x) {
-          const int key = (x * N + u) / kChunks, c = (x * N + u) % kChunks;
-          const uint4 v = *reinterpret_cast<const uint4*>(src + key * D + c * 16);
-          const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t ex = ctl->exps[s][key];
+        uint4 v[kChunks];
+#pragma unroll
+        for (int x = 0; x < kChunks; ++x)
+          v[x] = *reinterpret_cast<const uint4*>(src + ((x + key) % kChunks) * 16);
+#pragma unroll
+        for (int x = 0; x < kChunks; ++x) {
+          const int c = (x + key) % kChunks;
+          const uint32_t w4[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
           uint32_t o[8];
-          M::dequantise16(w4, ctl->exps[s][key], o);
+          M::dequantise16(w4, ex, o);
           *reinterpret_cast<uint4*>(dst + tile_at(key, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
           *reinterpret_cast<uint4*>(dst + tile_at(key, 2 * c + 1)) =
               make_uint4(o[4], o[5], o[6], o[7]);
