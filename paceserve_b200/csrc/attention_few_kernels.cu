@@ -59,6 +59,22 @@ struct FewTile {
   }
 };
 
+// A quantised word's two pairs of values as fp16: every other one by the
+// conversion instruction, as they are, the rest by shifts, times 2^-8.  The two
+// run on different units, neither of which alone keeps up with the memory.
+__device__ __forceinline__ constexpr bool by_conversion(int n) { return n & 1; }
+template <typename M>
+__device__ __forceinline__ void unpack_by(bool conversion, uint32_t w, uint32_t& even,
+                                          uint32_t& odd) {
+  if (conversion) {
+    const uint32_t x = __byte_perm(w, 0, 0x3120);
+    even = e4m3x2_to_half2(x & 0xffffu);
+    odd = e4m3x2_to_half2(x >> 16);
+  } else {
+    M::unpack_codes(w, even, odd);
+  }
+}
+
 // 2^-n, 0 where that is no normal number.
 __device__ __forceinline__ float pow2_down(int n) {
   return n < 127 ? __uint_as_float((uint32_t)(127 - n) << 23) : 0.f;
@@ -176,7 +192,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
           const float2 x = Mma<T>::floats(qf[kb][k]);
           qf[kb][k] = M::pack(x.x * f, x.y * f);
         }
-      row_scale[i] *= 256.f / f;  // and the codes' 2^-8
+      row_scale[i] *= 1.f / f;
     }
   }
 
@@ -270,7 +286,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           uint32_t b0, b1;
-          M::unpack_codes(r[n], b0, b1);
+          unpack_by<M>(by_conversion(n), r[n], b0, b1);
           M::mma(s[n], qf[kb], b0, b1);
         }
       } else {
@@ -288,7 +304,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float2 f = make_float2(1.f, 1.f);
-      if constexpr (Q8) f = *reinterpret_cast<const float2*>(kf + n * 8 + 2 * c);
+      if constexpr (Q8) {
+        f = *reinterpret_cast<const float2*>(kf + n * 8 + 2 * c);
+        if (!by_conversion(n)) {  // the shifted codes' 2^-8
+          f.x *= 256.f;
+          f.y *= 256.f;
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 2 * R; ++e) {
         float x = s[n][e] * row_scale[e >> 1];
@@ -404,8 +426,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t e0, d0, e1, d1;
-            M::unpack_codes(r[2 * h], e0, d0);
-            M::unpack_codes(r[2 * h + 1], e1, d1);
+            unpack_by<M>(by_conversion(ch + h), r[2 * h], e0, d0);
+            unpack_by<M>(by_conversion(ch + h), r[2 * h + 1], e1, d1);
             M::mma(o[2 * (ch + h)], a, e0, e1);
             M::mma(o[2 * (ch + h) + 1], a, d0, d1);
           }
@@ -437,9 +459,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
         join_ml[(warp * 16 + r) * 2 + 1] = l[i];
       }
       float* dst = reinterpret_cast<float*>(ring) + r * D;
-      const float up = Q8 ? 256.f : 1.f, unit = Q8 ? exponent_factor(v_top) : 1.f;
+      const float unit = Q8 ? exponent_factor(v_top) : 1.f;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
+        const float up = Q8 && !by_conversion(n >> 1) ? 256.f : 1.f;
         const int d = Q8 ? (n >> 1) * 16 + 4 * c + (n & 1) : n * 8 + 2 * c;
         dst[d] = o[n][2 * i] * up * unit;
         dst[d + (Q8 ? 2 : 1)] = o[n][2 * i + 1] * up * unit;
