@@ -380,6 +380,102 @@ def test_append_then_attend():
     step.check()
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.05, 0.7])
+def test_any_scale(scale):
+    Step([(1, 70), (90, 200)], 8, 2, 128, seed=14, spread=0.3).check(sm_scale=scale)
+    Step([(1, 70), (90, 200)], 8, 2, 64, seed=14, spread=0.3, quantised=True).check(
+        sm_scale=scale, logits_soft_cap=3.0)
+
+
+def test_cache_at_an_odd_address():
+    """A cache that no 16-byte access fits: the CUDA-core kernel takes it."""
+    step = Step([(1, 70), (30, 60)], 8, 2, 128, seed=15)
+    flat = torch.zeros(step.cache.numel() + 1, dtype=torch.bfloat16, device=DEV)
+    flat[1:] = step.cache.flatten().to(DEV)
+    attn = PagedAttention(8, 2, 128, 16, DEV)
+    attn.begin_forward(step.qp, step.kp, step.ki, step.kl)
+    got = attn.forward(step.query.to(DEV), flat[1:].view(step.cache.shape)).cpu()
+    out, _, size = step.want()
+    u = U[torch.bfloat16]
+    assert bool(((got.double() - out).abs() <= u * out.abs() + (u + 4e-4) * size).all())
+
+
+def test_the_widest_group():
+    Step([(1, 300), (5, 130)], 128, 1, 64, seed=16).check()
+    Step([(1, 300), (5, 130)], 256, 2, 128, seed=16, quantised=True).check()
+
+
+def test_without_programmatic_launch():
+    """A step with few and many rows, whose two kernels otherwise run beside each
+    other, in plain order."""
+    import paceserve_b200
+
+    step = Step([(1, 900), (100, 300), (1, 40)], 8, 2, 128, seed=17)
+    first, _ = step.run()
+    paceserve_b200.set_pdl(False)
+    try:
+        second, _ = step.run()
+    finally:
+        paceserve_b200.set_pdl(True)
+    assert torch.equal(first, second)
+    step.check()
+
+
+def test_append_and_attention_in_one_stream_order():
+    """Layer after layer without a wait: each attention sees its layer's append, and
+    the next append does not overtake it."""
+    lens = [(1, 200), (120, 300)]
+    step = Step(lens, 8, 2, 128, seed=18)
+    t = int(step.qp[-1])
+    g = torch.Generator().manual_seed(1)
+    keys = [torch.randn(2, t, 2 * 128, generator=g).bfloat16() for _ in range(4)]
+    on = [k.to(DEV) for k in keys]
+    cache = step.cache.to(DEV)
+    attn = PagedAttention(8, 2, 128, 16, DEV)
+    attn.begin_forward(step.qp, step.kp, step.ki, step.kl)
+    q, meta = step.query.to(DEV), [x.to(DEV) for x in (step.qp, step.ki, step.kp, step.kl)]
+    outs = []
+    for k in on:  # the same cache again and again
+        kv.append_paged_kv_cache_by_indptr(k[0], k[1], meta[0], cache, *meta[1:])
+        outs.append(attn.forward(q, cache))
+    torch.cuda.synchronize()
+    for k, got in zip(keys, outs):
+        for b, (n, length) in enumerate(lens):
+            for i in range(n):
+                pos = length - n + i
+                page = step.ki[int(step.kp[b]) + pos // 16]
+                step.cache[page, :, pos % 16] = k[:, int(step.qp[b]) + i].view(2, 2, 128)
+        out, _, size = step.want()
+        u = U[torch.bfloat16]
+        assert bool(((got.cpu().double() - out).abs() <= u * out.abs() + (u + 4e-4) * size).all())
+
+
+def test_example_steps():
+    """examples/paged_attention_steps.py: every step's output and the rows read back."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "paged_attention_steps.py")
+    spec = importlib.util.spec_from_file_location("paged_attention_steps", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    steps, rows = example.main(DEV)
+    u = U[torch.bfloat16]
+    for s in steps:
+        values = ref.dequantise(s["codes"].cpu(), s["exponents"].cpu())
+        args = dict(sm_scale=1 / math.sqrt(128), soft_cap=s["options"].get("logits_soft_cap", 0.0),
+                    tree_mask=s["tree_mask"])
+        out, _ = ref.attention(s["query"].cpu(), values, *s["meta"], **args)
+        size = values.clone()
+        size[:, 1] = size[:, 1].abs()
+        size, _ = ref.attention(s["query"].cpu(), size, *s["meta"], **args)
+        err = (s["out"].cpu().double() - out).abs()
+        assert bool((err <= u * out.abs() + (u + 4e-4) * size).all())
+    k, v = ref.gather_rows(values, rows["kv_indices"], rows["kv_indptr"], rows["kv_last_page_len"], 0)
+    assert torch.equal(rows["key"].cpu(), k.bfloat16()) and torch.equal(rows["value"].cpu(), v.bfloat16())
+
+
 def test_refusals():
     step = Step([(1, 30)], 8, 2, 128)
     attn = PagedAttention(8, 2, 128, 16, DEV)
