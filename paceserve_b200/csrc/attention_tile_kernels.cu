@@ -415,7 +415,22 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
               size[k] = max3(size[k], fabsf(__uint_as_float(sr[i + 2 * k])),
                              fabsf(__uint_as_float(sr[i + 2 * k + 1])));
           size[0] = fmaxf(fmaxf(size[0], size[1]), fmaxf(size[2], size[3]));
-          if (__all_sync(0xffffffffu, size[0] * scale2 <= cap2)) {
+          if (__all_sync(0xffffffffu, size[0] * scale2 <= 0.25f * cap2)) {
+            // all scores well within the cap, as they mostly are: three terms of the polynomial
+            // (largest error of tanh 5.0e-8), the factors in its coefficients.  8192 tokens, capped:
+            // 631 us, 740 with the six terms below, 1026 with the special-function unit.
+            const float in = scale2 / cap2, z1 = in * in;
+            const uint64_t a0 = both(0.9999986290931702f * scale2);
+            const uint64_t a1 = both(-0.3331570625305176f * scale2 * z1);
+            const uint64_t a2 = both(0.12762290239334106f * scale2 * z1 * z1);
+#pragma unroll
+            for (int i = 0; i < kStepKeys; i += 2) {
+              const uint64_t x = u32x2(sr[i], sr[i + 1]), z = mul2(x, x);
+              const uint64_t y = mul2(x, fma2(fma2(a2, z, a1), z, a0));
+              sr[i] = (uint32_t)y;
+              sr[i + 1] = (uint32_t)(y >> 32);
+            }
+          } else if (__all_sync(0xffffffffu, size[0] * scale2 <= cap2)) {
             // no score passes the cap: tanh by a polynomial.  The special-function unit, which
             // two calls a score keep busy for longer than the exponentials do, has none of it.
             const uint64_t in2 = both(scale2 / cap2), out2 = both(scale2);

@@ -380,6 +380,15 @@ def test_append_then_attend():
     step.check()
 
 
+@pytest.mark.parametrize("cap", [0.3, 1.5, 6.0, 40.0, 3000.0])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_caps_above_among_and_below_the_scores(cap, hd):
+    """The capped score has a form for scores well below the cap, one for scores
+    below it, and one for any."""
+    Step([(1, 300), (130, 400)], 8, 2, hd, seed=19).check(logits_soft_cap=cap)
+    Step([(1, 300), (130, 400)], 8, 2, hd, seed=19, dtype=torch.float16).check(logits_soft_cap=cap)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.05, 0.7])
 def test_any_scale(scale):
     Step([(1, 70), (90, 200)], 8, 2, 128, seed=14, spread=0.3).check(sm_scale=scale)
