@@ -21,12 +21,12 @@
 // code moved to the top of 16 bits is its value times 2^-8 as fp16 holds it,
 // subnormals included, and no multiplication touches it.  (The conversion
 // instruction is slower: 64 requests of up to 8191 tokens took 238 us with it.)
-// K's factor multiplies the scores.  V's factor 2^e goes with P, as 2^(e - E) for
-// the largest exponent E among the values so far, so that P stays at most 1 (the
-// output is in units of 2^(E - 8) and is scaled down when E rises, as it is when
-// the maximum does).  Queries are scaled by a power of two
-// to the top of fp16's range: a bf16 query keeps all its bits down to 2^-29 of
-// its largest element.
+// K's factor multiplies the scores.  V's factor 2^e goes into P: the output has a
+// running maximum of its own, of score + e, and is built from 2^(score + e - it), so
+// that the row's largest contribution is about 1 in fp16 whatever the factors are;
+// the sum l keeps the maximum of the scores alone.  Queries are scaled by a power
+// of two to the top of fp16's range: a bf16 query keeps all its bits down to 2^-29
+// of its largest element.
 #include "attention_mma.cuh"
 
 namespace pace {
@@ -48,7 +48,7 @@ struct FewTile {
   static constexpr int kRingBytes = kStages * 2 * kKvBytes;
   static constexpr int kJoinBytes = 16 * D * 4;  // a warp's output, over its ring
   static constexpr int kWarpBytes = kRingBytes > kJoinBytes ? kRingBytes : kJoinBytes;
-  // K's factors (fp32) and V's exponents of the keys in the ring
+  // K's factors and V's exponents (both fp32) of the keys in the ring
   static constexpr int kFactorBytes = Q8 ? kStages * kKeys * 8 : 0;
   static constexpr int kSmemBytes = kFewWarps * (kWarpBytes + kFactorBytes) + kFewWarps * 32 * 4;
   // 16-byte chunk c of row r, placed so that eight rows' same chunk, and one
@@ -75,15 +75,6 @@ __device__ __forceinline__ void unpack_by(bool conversion, uint32_t w, uint32_t&
   }
 }
 
-// 2^-n, 0 where that is no normal number.
-__device__ __forceinline__ float pow2_down(int n) {
-  return n < 127 ? __uint_as_float((uint32_t)(127 - n) << 23) : 0.f;
-}
-// A value row's factor in units of 2^(top - 127); NaN for a row that is.
-__device__ __forceinline__ float v_factor(int exponent, int top) {
-  return exponent == kNanExponent ? __uint_as_float(0x7fc00000u) : pow2_down(top - exponent);
-}
-
 // R: 1 where the rows fit the matrix instruction's first eight, else 2.
 template <typename T, int D, bool Q8, int R>
 __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
@@ -102,7 +93,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
   uint8_t* ring = smem + warp * Tile::kWarpBytes;
   float* factors = reinterpret_cast<float*>(smem + kFewWarps * Tile::kWarpBytes +
                                             warp * Tile::kFactorBytes);
-  int* v_exps = reinterpret_cast<int*>(factors + Tile::kStages * KEYS);
+  float* v_exps = factors + Tile::kStages * KEYS;
   float* join_ml = reinterpret_cast<float*>(
       smem + kFewWarps * (Tile::kWarpBytes + Tile::kFactorBytes));  // [warp][16][m, l]
   // `beside`: the kernel before this one in the stream is the tile kernel of the same call, which
@@ -236,7 +227,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
   auto put_factors = [&](int step) {
     if constexpr (Q8) {
       factors[(step % STAGES) * KEYS + lane] = exponent_factor(k_ex);
-      v_exps[(step % STAGES) * KEYS + lane] = (int)v_ex;
+      v_exps[(step % STAGES) * KEYS + lane] =
+          v_ex == (uint32_t)kNanExponent ? exponent_factor(kNanExponent) : (float)v_ex - 127.f;
     }
   };
 
@@ -251,7 +243,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
     m[i] = -INFINITY;
     l[i] = 0.f;
   }
-  int v_top = 0;  // the largest of V's exponents so far; O is in units of 2^(v_top - 127)
+  // over a quantised cache: the running maximum of score + V's exponent; O is in units of 2^mo
+  float mo[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) mo[i] = -INFINITY;
   const float cap2 = p.cap * kLog2e, cap_in = p.cap > 0.f ? 2.f / p.cap : 0.f;
 
 #pragma unroll
@@ -271,7 +266,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
     const uint8_t* ks = ring + (step % STAGES) * 2 * Tile::kKvBytes;
     const uint8_t* vs = ks + Tile::kKvBytes;
     const float* kf = factors + (step % STAGES) * KEYS;
-    const int* ve = v_exps + (step % STAGES) * KEYS;
+    const float* ve = v_exps + (step % STAGES) * KEYS;
     // ---- S = Q K^T ------------------------------------------------------------
     float s[NT][4];
 #pragma unroll
@@ -350,55 +345,67 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
     }
     // ---- running maximum and sum: the maximum may lag by 2^kLag, so that most steps
     // need neither the row's maximum, which its lanes share by shuffles, nor a new scale
-    float most[R];
+    float most[R], most_o[R];
     bool rise = false;
+    float2 v_e[NT];
+    if constexpr (Q8) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) v_e[n] = *reinterpret_cast<const float2*>(ve + n * 8 + 2 * c);
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      most[i] = -INFINITY;
+      most[i] = most_o[i] = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) most[i] = fmaxf(most[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]));
+      for (int n = 0; n < NT; ++n) {
+        most[i] = fmaxf(most[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]));
+        if constexpr (Q8)
+          most_o[i] = fmaxf(most_o[i], fmaxf(s[n][2 * i] + v_e[n].x, s[n][2 * i + 1] + v_e[n].y));
+      }
       rise |= most[i] > m[i] + kLag || (m[i] == -INFINITY && most[i] > m[i]);
-    }
-    int v_new = v_top;
-    if constexpr (Q8) {
-      const int x = ve[lane];
-      v_new = max(v_top, x == kNanExponent ? 0 : x);
-      rise |= v_new > v_top;
+      if constexpr (Q8)
+        rise |= most_o[i] > mo[i] + kLag || (mo[i] == -INFINITY && most_o[i] > mo[i]);
     }
     if (__any_sync(0xffffffffu, rise)) {
-      float v_down = 1.f;  // what a rise of V's largest exponent does to O
-      if constexpr (Q8) {
-        v_new = (int)__reduce_max_sync(0xffffffffu, v_new);
-        v_down = pow2_down(v_new - v_top);
-        v_top = v_new;
-      }
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        float t = most[i];
+      auto raise = [](float& old, float t) {  // to the row's maximum; returns what that scales by
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-        const float m2 = fmaxf(m[i], t);
-        float f = exp2_approx(m[i] - (m2 == -INFINITY ? 0.f : m2));  // 0 while m is -inf
+        const float now = fmaxf(old, t);
+        const float f = exp2_approx(old - (now == -INFINITY ? 0.f : now));  // 0 while old is -inf
+        old = now;
+        return f;
+      };
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        float f = raise(m[i], most[i]);
         l[i] *= f;
-        f *= v_down;
+        if constexpr (Q8) f = raise(mo[i], most_o[i]);
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) {
           o[n][2 * i] *= f;
           o[n][2 * i + 1] *= f;
         }
-        m[i] = m2;
       }
     }
-    float base[R];
+    float base[R], base_o[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i];
+    for (int i = 0; i < R; ++i) {
+      base[i] = m[i] == -INFINITY ? 0.f : m[i];
+      base_o[i] = mo[i] == -INFINITY ? 0.f : mo[i];
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2 * R; ++e) {
-        const float x = exp2_approx(s[n][e] - base[e >> 1]);
+        const float y = s[n][e];
+        const float x = exp2_approx(y - base[e >> 1]);
         l[e >> 1] += x;
-        s[n][e] = x;
+        if constexpr (Q8) {
+          // a key that the row does not see stays 0 whatever its row holds
+          const float z = y + ((e & 1 ? v_e[n].y : v_e[n].x) - base_o[e >> 1]);
+          s[n][e] = y == -INFINITY ? 0.f : exp2_approx(z);
+        } else {
+          s[n][e] = x;
+        }
       }
     // ---- O += P V; P is rounded to T, the one rounding before the output's ----
 #pragma unroll
@@ -408,13 +415,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
       for (int i = 0; i < 4; ++i) {
         a[i] = 0;
         if ((i & 1) >= R) continue;
-        float x = s[2 * kg + (i >> 1)][2 * (i & 1)], y = s[2 * kg + (i >> 1)][2 * (i & 1) + 1];
-        if constexpr (Q8) {
-          // a key that the row does not see stays 0 whatever its row holds
-          const int2 e = *reinterpret_cast<const int2*>(ve + kg * 16 + (i >> 1) * 8 + 2 * c);
-          x = x == 0.f ? 0.f : x * v_factor(e.x, v_top);
-          y = y == 0.f ? 0.f : y * v_factor(e.y, v_top);
-        }
+        const float x = s[2 * kg + (i >> 1)][2 * (i & 1)], y = s[2 * kg + (i >> 1)][2 * (i & 1) + 1];
         a[i] = M::pack(x, y);
       }
       if constexpr (Q8) {
@@ -459,7 +460,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
         join_ml[(warp * 16 + r) * 2 + 1] = l[i];
       }
       float* dst = reinterpret_cast<float*>(ring) + r * D;
-      const float unit = Q8 ? exponent_factor(v_top) : 1.f;
+      // in the joined output's units, 2^m
+      const float unit = Q8 ? (mo[i] == -INFINITY ? 0.f : exp2_approx(mo[i] - m[i])) : 1.f;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
         const float up = Q8 && !by_conversion(n >> 1) ? 256.f : 1.f;

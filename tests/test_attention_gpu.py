@@ -278,6 +278,25 @@ def test_quantised_extremes():
     step.check()  # values up to 2^117: bf16 holds them
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+def test_a_large_value_of_a_small_weight(dtype):
+    """A key whose weight is 2^-20 and whose value row is 2^20 times the others':
+    both parts of the output count."""
+    for tokens in (1, 40):
+        step = Step([(tokens, 100)], 4, 2, 128, dtype=dtype, quantised=True, seed=21)
+        step.exponents[:] = 119
+        # every key scores 0 but the one in question, which scores 20 powers of two below
+        page, slot = step.ki[3], 7
+        step.query[:] = 0
+        step.query[..., 0] = 1.0
+        step.cache[:, 0] = 0
+        step.cache[page, 0, slot, :, 0] = 0x80 | 0x70  # -128
+        step.exponents[page, 0, slot] = 127
+        step.exponents[page, 1, slot] = 139
+        kw = {"sm_scale": 20.0 / 128 / math.log2(math.e)}
+        step.check(**kw)
+
+
 @pytest.mark.parametrize("hd,dtype,quantised", [(96, torch.bfloat16, False), (256, torch.float16, True),
                                                 (8, torch.bfloat16, True), (128, torch.float32, False),
                                                 (64, torch.float32, True)])
