@@ -19,7 +19,14 @@
 // S_t of step j + 1 is issued behind P_t V of step j, so its arrival also says
 // that O_t may be touched.
 //
-// Keys past kv_end are copied as zeros.  Every wait is bounded.
+// Keys outside the piece are copied as zeros, or as whatever codes lie there with
+// a factor that makes them finite.  Every wait is bounded.
+//
+// What bounds it is the chain of a tile's step (scores out of TMEM, maximum,
+// exponentials, P into TMEM, its product, the next scores): 3870 cycles for a step
+// of both tiles, whose MMAs take about 2300.  One 8192-token prompt of 32 / 8 heads
+// of 128, causal: 510 us, 1.08 PFLOP/s, 0.64 of cuBLAS's measured rate; with capped
+// scores 631 us, with distance bias 641, over a quantised cache 677.
 #include "attention_mma.cuh"
 #include "tcgen05.cuh"
 
@@ -1027,8 +1034,9 @@ static int run_tile(const Problem& p, int64_t num_pages, const Item* items, int 
   cudaError_t err =
       ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), device, Cfg::kSmemBytes);
   if (err != cudaSuccess) return cuda_fail(err, what);
-  // A TMA box is a page's share of a 128-key step, and its 8-row swizzle groups have to be the
-  // step's: pages of 8 to 128 keys that divide 128, or multiples of 128.
+  // TMA where the pages allow it (8192 tokens: 528 us against 813 by 16-byte copies, quantised 706
+  // against 881).  A box is a page's share of a 128-key step, and its 8-row swizzle groups have to
+  // be the step's: pages of 8 to 128 keys that divide 128, or multiples of 128.
   CUtensorMap map{};
   int box = 0;
   if (p.page_size >= 8 && (128 % p.page_size == 0 || p.page_size % 128 == 0) &&
