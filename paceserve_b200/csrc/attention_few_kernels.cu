@@ -105,6 +105,61 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
   pdl_launch_dependents();
   if (!beside) pdl_wait();
 
+  // ---- the ring: its first copies are under way while the queries are fetched --------
+  const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
+  const int64_t v_rows = (int64_t)p.page_size * p.kv_heads, v_bytes = v_rows * Tile::kRowBytes;
+  const int begin = w.kv_begin + warp * KEYS;
+  const int steps = begin < w.kv_end ? (w.kv_end - begin + kFewWarps * KEYS - 1) / (kFewWarps * KEYS) : 0;
+  const int my_key = lane % KEYS;
+  auto page_of = [&](int step) -> int {
+    const int j = begin + step * kFewWarps * KEYS + my_key;
+    return step < steps && j < w.kv_end ? p.kv_indices[w.page_base + page_number(p, j)] : -1;
+  };
+  uint32_t k_ex = 0, v_ex = 0;  // exponents of this lane's key of the step issued last
+  auto issue = [&](int step, int page) {
+    // row number (of the whole cache, K part) of this lane's key; ~0: none
+    uint32_t row = ~0u;
+    if (page >= 0) {
+      const int j = begin + step * kFewWarps * KEYS + my_key;
+      row = (uint32_t)(((int64_t)page * 2 * p.page_size + page_slot(p, j)) * p.kv_heads + kvh);
+    }
+    uint8_t* slot = ring + (step % STAGES) * 2 * Tile::kKvBytes;
+#pragma unroll
+    for (int i = 0; i < KEYS * Tile::kChunks / 32; ++i) {
+      const int r = (i * 32 + lane) / Tile::kChunks, ch = (i * 32 + lane) % Tile::kChunks;
+      const uint32_t src = __shfl_sync(0xffffffffu, row, r);
+      const bool there = src != ~0u;
+      const uint8_t* k = cache + (there ? (int64_t)src * Tile::kRowBytes + ch * 16 : 0);
+      const int at = Tile::at(r, ch);
+      cp_async16(slot + at, k, there);
+      cp_async16(slot + Tile::kKvBytes + at, k + (there ? v_bytes : 0), there);
+    }
+    if constexpr (Q8) {
+      k_ex = v_ex = 0;
+      if (row != ~0u) {
+        k_ex = p.exponents[row];
+        v_ex = p.exponents[row + v_rows];
+      }
+    }
+  };
+  auto put_factors = [&](int step) {
+    if constexpr (Q8) {
+      factors[(step % STAGES) * KEYS + lane] = exponent_factor(k_ex);
+      v_exps[(step % STAGES) * KEYS + lane] =
+          v_ex == (uint32_t)kNanExponent ? exponent_factor(kNanExponent) : (float)v_ex - 127.f;
+    }
+  };
+
+  uint32_t k_first[STAGES - 1], v_first[STAGES - 1];
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    issue(s, page_of(s));
+    cp_async_commit();
+    k_first[s] = k_ex;
+    v_first[s] = v_ex;
+  }
+  int page = page_of(STAGES - 1);
+
   // ---- rows g and g + 8 of this thread: visible keys, slope, queries --------
   int lo[R], hi[R], pos[R];
   float slope[R];
@@ -190,51 +245,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
     }
   }
 
-  // ---- the ring ---------------------------------------------------------------
-  const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
-  const int64_t v_rows = (int64_t)p.page_size * p.kv_heads, v_bytes = v_rows * Tile::kRowBytes;
-  const int begin = w.kv_begin + warp * KEYS;
-  const int steps = begin < w.kv_end ? (w.kv_end - begin + kFewWarps * KEYS - 1) / (kFewWarps * KEYS) : 0;
-  const int my_key = lane % KEYS;
-  auto page_of = [&](int step) -> int {
-    const int j = begin + step * kFewWarps * KEYS + my_key;
-    return step < steps && j < w.kv_end ? p.kv_indices[w.page_base + page_number(p, j)] : -1;
-  };
-  uint32_t k_ex = 0, v_ex = 0;  // exponents of this lane's key of the step issued last
-  auto issue = [&](int step, int page) {
-    // row number (of the whole cache, K part) of this lane's key; ~0: none
-    uint32_t row = ~0u;
-    if (page >= 0) {
-      const int j = begin + step * kFewWarps * KEYS + my_key;
-      row = (uint32_t)(((int64_t)page * 2 * p.page_size + page_slot(p, j)) * p.kv_heads + kvh);
-    }
-    uint8_t* slot = ring + (step % STAGES) * 2 * Tile::kKvBytes;
 #pragma unroll
-    for (int i = 0; i < KEYS * Tile::kChunks / 32; ++i) {
-      const int r = (i * 32 + lane) / Tile::kChunks, ch = (i * 32 + lane) % Tile::kChunks;
-      const uint32_t src = __shfl_sync(0xffffffffu, row, r);
-      const bool there = src != ~0u;
-      const uint8_t* k = cache + (there ? (int64_t)src * Tile::kRowBytes + ch * 16 : 0);
-      const int at = Tile::at(r, ch);
-      cp_async16(slot + at, k, there);
-      cp_async16(slot + Tile::kKvBytes + at, k + (there ? v_bytes : 0), there);
-    }
-    if constexpr (Q8) {
-      k_ex = v_ex = 0;
-      if (row != ~0u) {
-        k_ex = p.exponents[row];
-        v_ex = p.exponents[row + v_rows];
-      }
-    }
-  };
-  auto put_factors = [&](int step) {
-    if constexpr (Q8) {
-      factors[(step % STAGES) * KEYS + lane] = exponent_factor(k_ex);
-      v_exps[(step % STAGES) * KEYS + lane] =
-          v_ex == (uint32_t)kNanExponent ? exponent_factor(kNanExponent) : (float)v_ex - 127.f;
-    }
-  };
-
+  for (int s = 0; s < STAGES - 1; ++s) {
+    k_ex = k_first[s];
+    v_ex = v_first[s];
+    put_factors(s);
+  }
   float o[D / 8][4];
 #pragma unroll
   for (int i = 0; i < D / 8; ++i)
@@ -252,13 +268,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
   for (int i = 0; i < R; ++i) mo[i] = -INFINITY;
   const float cap2 = p.cap * kLog2e, cap_in = p.cap > 0.f ? 2.f / p.cap : 0.f;
 
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
-    issue(s, page_of(s));
-    put_factors(s);
-    cp_async_commit();
-  }
-  int page = page_of(STAGES - 1);
   for (int step = 0; step < steps; ++step) {
     if (step > 0) put_factors(step + STAGES - 2);  // their loads had a step's time
     issue(step + STAGES - 1, page);
