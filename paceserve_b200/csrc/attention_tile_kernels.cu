@@ -337,8 +337,10 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
     bool ok = true;
     if (t < tiles) {
       // the tile's queries, a row by 8 or 16 neighbouring threads; negated where the scale is
-      // negative (and zero where it is), so that the largest product is the largest score
-      {
+      // negative (and zero where it is), so that the largest product is the largest score.  A piece
+      // without a step leaves them: nothing would order these stores, all over the tile, before the
+      // warps' outputs, which pass through the same memory.
+      if (steps > 0) {
         uint8_t* qs = smem + t * Cfg::kQBytes;
         const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
         const bool vec = p.q_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.query) & 15) == 0;
