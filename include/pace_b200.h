@@ -540,7 +540,7 @@ int pace_paged_attention_plan(pace_attention_plan* plan, int32_t* words, int64_t
  * contiguous, token strides in elements.  cache: the paged cache of `dtype`, or
  * with `exponents` the codes of a quantised one.  lse ([total_q, heads], may be
  * NULL) receives the natural log of each row's sum of e^s (-inf where nothing is
- * visible).  workspace: plan.workspace_bytes bytes, zeroed once by the caller
+ * visible).  workspace: plan.workspace_bytes bytes, 32-byte aligned, zeroed once by the caller
  * before its first use (each call leaves its counters zero again); calls that
  * may overlap need one each.  A kernel wait that runs out sets bit 30 of
  * *fault_flags (device int32, may be NULL); the outputs are then undefined and

@@ -333,17 +333,19 @@ extern "C" int pace_paged_attention(const pace_attention_plan* plan, const int32
     if (plan->page_size == 1 << s) p.page_shift = s;
   p.scale = sm_scale;
   p.cap = logits_soft_cap;
-  StreamDeviceGuard guard(stream);
   // The tensor-core kernels take 16-bit queries of 64 or 128 dimensions over a cache that 16-byte
   // copies fit and whose rows 32 bits number; the CUDA-core kernel the rest.
   const int64_t cache_rows = num_pages * 2 * plan->page_size * plan->num_kv_heads;
   const bool tensor = (dtype == PACE_BF16 || dtype == PACE_F16) &&
                       (plan->head_dim == 64 || plan->head_dim == 128) && aligned16(cache) &&
                       cache_rows <= UINT32_MAX;
+  // partial rows are written 32 bytes at a time
+  if (tensor && (!workspace || workspace_bytes < plan->workspace_bytes ||
+                 (reinterpret_cast<uintptr_t>(workspace) & 31) != 0))
+    return fail(PACE_ERR_INVALID_ARGUMENT, "%s: the plan needs %zu bytes of 32-byte aligned "
+                "workspace", what, plan->workspace_bytes);
+  StreamDeviceGuard guard(stream);
   if (tensor) {
-    if (!workspace || workspace_bytes < plan->workspace_bytes || !aligned16(workspace))
-      return fail(PACE_ERR_INVALID_ARGUMENT, "%s: the plan needs %zu bytes of 16-byte aligned "
-                  "workspace", what, plan->workspace_bytes);
     const Workspace ws = workspace_of(*plan);
     uint8_t* base = static_cast<uint8_t*>(workspace);
     int32_t* counters = reinterpret_cast<int32_t*>(base);

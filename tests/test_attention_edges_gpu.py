@@ -5,7 +5,7 @@ Tolerances are those derived in ``test_attention_gpu.py``.
 import pytest
 import torch
 
-from paceserve_b200.attention import PagedAttention
+from paceserve_b200.attention import PagedAttention, attention_ops
 from tests.test_attention_gpu import DEV, Step
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +42,22 @@ def test_pieces_without_a_key_are_zero(dtype, hd, quantised):
             assert not bool(out.cpu()[~want].any())
             assert bool((lse.cpu()[~want] == -float("inf")).all())
     step.check(doc_starts=starts)
+
+
+def test_workspace_at_an_odd_address_is_refused():
+    step = Step([(70, 20000)], 8, 2, 128, seed=1)
+    plan = attention_ops.plan_paged_attention(step.qp, step.kp, step.ki, step.kl, 8, 2, 128, 16)
+    assert plan.many_slots > 0
+    workspace = torch.zeros(plan.workspace_bytes + 64, dtype=torch.uint8, device=DEV)
+    query, cache = step.query.to(DEV), step.cache.to(DEV)
+    outs = []
+    for shift in (0, 16, 32, 8):
+        args = (query, cache, plan, plan.words.to(DEV), workspace[shift:], 0.1)
+        outs.append(torch.zeros_like(query))
+        if shift % 32:
+            with pytest.raises(RuntimeError, match="32-byte aligned workspace"):
+                attention_ops.paged_attention(outs[-1], *args)
+        else:
+            attention_ops.paged_attention(outs[-1], *args)
+            workspace.zero_()  # the next one's counters lie elsewhere
+    assert bool(outs[0].any()) and torch.equal(outs[0], outs[2])
