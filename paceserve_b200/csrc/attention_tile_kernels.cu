@@ -746,6 +746,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
           return key < kStepKeys && pos < w.kv_end ? p.kv_indices[w.page_base + page_number(p, pos)] : -1;
         };
         page = look_up(0);
+        int sent = 0;
         for (int i = 0; ok && i < 2 * steps; ++i) {
           const int s = i % Cfg::kCodeStages;
           if (i >= Cfg::kCodeStages)
@@ -761,8 +762,13 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
             tma_load_page(codes + s * Cfg::kCodeBytes + key * D, &map, 0, kvh, page_slot(p, pos),
                           page * 2 + (i & 1), &ctl->code_full[s]);
           }
+          sent = i + 1;
           if (i & 1) page = look_up((i >> 1) + 1);
         }
+        // whatever ended the steps, no copy outlives the CTA
+        for (int i = max(sent - Cfg::kCodeStages, 0); i < sent; ++i)
+          tc::mbar_wait(&ctl->code_full[i % Cfg::kCodeStages],
+                        (uint32_t)(i / Cfg::kCodeStages) & 1u, kWaitLimitNs, nullptr);
       } else {
         const int u = threadIdx.x - 10 * 32;  // keys u and u + 64 of each step
         const int64_t v_rows = (int64_t)p.page_size * p.kv_heads;
@@ -878,6 +884,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
       look_up(0);
       bool ok = true;
       int pending = -1;  // slot whose cp.async copies are under way
+      int sent = 0;      // behind the last slot filled, as the warp of the boxes counts them
       auto flush = [&](bool all) {
         if (pending < 0) return;
         if (all)
@@ -906,6 +913,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
                 tma_load_page(ring + s * Cfg::kKvBytes + box_half * 16384 + box_key * 128, &map,
                               box_half * 64, kvh, page_slot(p, pos), page * 2 + kind,
                               &ctl->kv_full[s]);
+              sent = i + 1;
             }
             page = page_of(j + 1);
           }
@@ -934,6 +942,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
                           (uint32_t)(i / Cfg::kStages - 1) & 1u, ctl);
           ok = loaders_all<N>(ok);  // also: the step's rows are in place
           if (!ok) break;
+          sent = i + 1;
           uint8_t* dst = ring + (i % Cfg::kStages) * Cfg::kKvBytes;
           if constexpr (!Q8) {
             constexpr int kChunks = D / 8;
@@ -985,6 +994,11 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
       if constexpr (!Q8) {
         cp_async_wait<0>();
         if (ok) flush(true);
+        // whatever ended the steps, no copy outlives the CTA; slots filled since then hold none
+        for (int i = max(sent - Cfg::kStages, 0); u < 32 && i < sent; ++i)
+          if (by_tma(i >> 1))
+            tc::mbar_wait(&ctl->kv_full[i % Cfg::kStages], (uint32_t)(i / Cfg::kStages) & 1u,
+                          kWaitLimitNs, nullptr);
       }
       if (!ok) tile_fault(ctl, fault);
     }
