@@ -81,6 +81,7 @@ def main(device: str = "cuda:0", pages: int = 256, seed: int = 0):
     # a tree of five drafted tokens: 0 - 1 - 2, 1 - 3, 0 - 4
     mask = torch.tensor([0b00001, 0b00011, 0b00111, 0b01011, 0b10001], dtype=torch.int64)[:, None]
     step({"a": 5}, tree_mask=mask)
+    attention.check()
     # request a's rows, in sequence order
     _, kp, ki, kl = requests.metadata({"a": 0})
     n = requests.length["a"]

@@ -543,8 +543,8 @@ int pace_paged_attention_plan(pace_attention_plan* plan, int32_t* words, int64_t
  * visible).  workspace: plan.workspace_bytes bytes, 32-byte aligned, zeroed once by the caller
  * before its first use (each call leaves its counters zero again); calls that
  * may overlap need one each.  A kernel wait that runs out sets bit 30 of
- * *fault_flags (device int32, may be NULL); the outputs are then undefined and
- * the workspace has to be zeroed again. */
+ * *fault_flags (device int32, may be NULL); the call's outputs are then undefined,
+ * later calls are not touched by it. */
 int pace_paged_attention(const pace_attention_plan* plan, const int32_t* plan_words, void* out,
                          const void* query, int64_t query_token_stride, int64_t out_token_stride,
                          const void* cache, const void* exponents, int64_t num_pages,

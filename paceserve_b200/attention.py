@@ -57,6 +57,7 @@ class PagedAttention:
         self.num_sms = torch.cuda.get_device_properties(device).multi_processor_count
         self._scale = 1.0 / math.sqrt(head_dim)
         self._workspace = torch.zeros(0, dtype=torch.uint8, device=device)
+        self._fault = torch.zeros(1, dtype=torch.int32, device=device)
         self._step = None
         self.plan = None
 
@@ -118,9 +119,23 @@ class PagedAttention:
         rows may be strided views of the qkv projection) over the layer's cache
         [pages, 2, page_size, num_kv_heads, head_dim], or over a quantised
         cache's codes with its ``exponents``.  ``lse`` (float32 [tokens,
-        num_heads]) receives each row's log-sum-exp."""
+        num_heads]) receives each row's log-sum-exp.  Every wait in the kernels
+        is bounded; one that runs out sets bit 30 of ``fault_flags`` (int32 on
+        the device), or of the object's own flag, which ``check`` reads."""
         if self._step is None:
             raise RuntimeError("PagedAttention.forward: begin_forward has not planned a step")
         return self._step.forward(query, paged_kv_cache, exponents,
                                   self._scale if sm_scale is None else sm_scale, logits_soft_cap,
-                                  alibi_slopes, out, lse, fault_flags)
+                                  alibi_slopes, out, lse,
+                                  self._fault if fault_flags is None else fault_flags)
+
+    def check(self) -> None:
+        """Raise if a kernel's wait ran out in a ``forward`` since the last call:
+        the outputs since then are undefined.  Waits for the current stream,
+        which has to come after those calls.  Afterwards the object is as new."""
+        if int(self._fault) == 0:
+            return
+        self._fault.zero_()
+        self._workspace.zero_()
+        raise RuntimeError("PagedAttention: a kernel wait ran out; the outputs since the last "
+                           "check are undefined")

@@ -1007,10 +1007,12 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   tc::tc_fence_before();
   __syncthreads();
   if (warp == 8) tc::tmem_dealloc(tmem, 512);
-  if (w.splits == 1 || *reinterpret_cast<volatile int*>(&ctl->abort)) return;
+  if (w.splits == 1) return;
 
   // ---- the last piece of these rows to arrive joins them all --------------------
+  // A piece whose waits ran out arrives too, so that the counter is zero again for the next call.
   if (!arrive_last(counters + (int64_t)w.tile * p.kv_heads + kvh, w.splits, &ctl->last)) return;
+  if (*reinterpret_cast<volatile int*>(&ctl->abort)) return;
   if (warp >= 8) return;  // these gave their registers away
   join_pieces<T, 256, D, Q8, 256>(p, partial, partial_ml, w, kvh, group, rows,
                                   reinterpret_cast<float*>(ring),

@@ -61,3 +61,27 @@ def test_workspace_at_an_odd_address_is_refused():
             attention_ops.paged_attention(outs[-1], *args)
             workspace.zero_()  # the next one's counters lie elsewhere
     assert bool(outs[0].any()) and torch.equal(outs[0], outs[2])
+
+
+def test_a_wait_that_ran_out_is_told_and_forgotten():
+    """The object's own flag, as a kernel would leave it (no wait runs out here), and a
+    workspace whose counters are not zero: ``check`` raises once, and what follows is right."""
+    step = Step([(70, 9000), (1, 5000)], 8, 2, 128, seed=11)
+    attn = PagedAttention(8, 2, 128, 16, DEV)
+    attn.begin_forward(step.qp, step.kp, step.ki, step.kl)
+    assert attn.plan.many_slots > 0 and attn.plan.few_slots > 0
+    query, cache = step.query.to(DEV), step.cache.to(DEV)
+    want = attn.forward(query, cache)
+    attn.check()
+    attn._fault.fill_(1 << 30)
+    attn._workspace[:65536].view(torch.int32).fill_(1)
+    with pytest.raises(RuntimeError, match="wait ran out"):
+        attn.check()
+    attn.check()
+    assert torch.equal(attn.forward(query, cache), want)
+    attn.begin_forward(step.qp, step.kp, step.ki, step.kl)
+    assert torch.equal(attn.forward(query, cache), want)
+    # a caller's own flag takes its place
+    mine = torch.zeros(1, dtype=torch.int32, device=DEV)
+    attn.forward(query, cache, fault_flags=mine)
+    assert mine.item() == 0
