@@ -81,7 +81,7 @@ __device__ __forceinline__ void unpack_by(bool conversion, uint32_t w, uint32_t&
 // R: 1 where the rows fit the matrix instruction's first eight, else 2.
 template <typename T, int D, bool Q8, int R>
 __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
-    attention_few_kernel(const Problem p, const Item* __restrict__ items, float* partial,
+    attention_few_kernel(const Problem p, const Item* items, float* partial,
                          float2* partial_ml, int32_t* counters, bool q_even, bool beside) {
   using Tile = FewTile<D, Q8, R>;
   using M = Mma<std::conditional_t<Q8, __half, T>>;
@@ -90,9 +90,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.x % p.kv_heads;
-  const Item w = items[blockIdx.x / p.kv_heads];
   const int group = p.heads / p.kv_heads;
-  const int rows = w.ntok * group;
   uint8_t* ring = smem + warp * Tile::kWarpBytes;
   float* factors = reinterpret_cast<float*>(smem + kFewWarps * Tile::kWarpBytes +
                                             warp * Tile::kFactorBytes);
@@ -104,6 +102,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
   // then waits for that kernel at its end, for the sake of what comes after.
   pdl_launch_dependents();
   if (!beside) pdl_wait();
+  const Item w = items[blockIdx.x / p.kv_heads];  // not earlier: a kernel may have written the plan
+  const int rows = w.ntok * group;
 
   // ---- the ring: its first copies are under way while the queries are fetched --------
   const uint8_t* cache = static_cast<const uint8_t*>(p.cache);

@@ -270,7 +270,7 @@ __device__ __forceinline__ uint32_t seen_bits(int j0, int lo, int hi, int base, 
 template <typename T, int D, bool Q8>
 __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
     attention_tile_kernel(const Problem p, const __grid_constant__ CUtensorMap map, int box,
-                          const Item* __restrict__ items, float* partial, float2* partial_ml,
+                          const Item* items, float* partial, float2* partial_ml,
                           int32_t* counters, int32_t* fault) {
   using Cfg = TileCfg<D, Q8>;
   using M = Mma<T>;
@@ -282,16 +282,6 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   TileCtl* ctl = reinterpret_cast<TileCtl*>(codes + Cfg::kCodeRingBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.x % p.kv_heads;
-  const Item w = items[blockIdx.x / p.kv_heads];
-  const int group = p.heads / p.kv_heads;
-  const int rows = w.ntok * group;
-  // row / group for rows below 256 and groups up to 128: the fraction added stays below 1 / group
-  const uint32_t group_inv = 65536u / (uint32_t)group + 1u;
-  auto div_group = [&](int row) { return (int)((uint32_t)row * group_inv >> 16); };
-  const int tiles = rows > kTileRowsEach ? 2 : 1;
-  // steps lie on multiples of 128 keys, so that pages do not straddle them
-  const int k_base = w.kv_begin & ~(kStepKeys - 1);
-  const int steps = w.kv_end > w.kv_begin ? (w.kv_end - k_base + kStepKeys - 1) / kStepKeys : 0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -314,14 +304,25 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
     tc::fence_barrier_init();
   }
   if (warp == 8) tc::tmem_alloc(&ctl->tmem, 512);
+  pdl_wait();
+  // not earlier: a kernel may have written the plan.  The barrier below hides its latency.
+  const Item w = items[blockIdx.x / p.kv_heads];
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = ctl->tmem;
-  pdl_wait();
-  // not earlier: the few-row kernel of the same call starts beside this one without a wait of its
-  // own, on what is complete here
+  // not before the wait: the few-row kernel of the same call starts beside this one without a wait
+  // of its own, on what is complete here
   pdl_launch_dependents();
+  const int group = p.heads / p.kv_heads;
+  const int rows = w.ntok * group;
+  // row / group for rows below 256 and groups up to 128: the fraction added stays below 1 / group
+  const uint32_t group_inv = 65536u / (uint32_t)group + 1u;
+  auto div_group = [&](int row) { return (int)((uint32_t)row * group_inv >> 16); };
+  const int tiles = rows > kTileRowsEach ? 2 : 1;
+  // steps lie on multiples of 128 keys, so that pages do not straddle them
+  const int k_base = w.kv_begin & ~(kStepKeys - 1);
+  const int steps = w.kv_end > w.kv_begin ? (w.kv_end - k_base + kStepKeys - 1) / kStepKeys : 0;
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kSoftmaxRegs));

@@ -85,3 +85,36 @@ def test_a_wait_that_ran_out_is_told_and_forgotten():
     mine = torch.zeros(1, dtype=torch.int32, device=DEV)
     attn.forward(query, cache, fault_flags=mine)
     assert mine.item() == 0
+
+
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_a_plan_written_by_the_kernel_before(tokens):
+    """Plan words that a kernel writes right before the call, over another step's: the call sees
+    the new ones, also where it may start before that kernel has ended."""
+    steps = [Step(lens, 8, 2, 128, seed=3) for lens in ([(tokens, 900), (tokens, 130)],
+                                                       [(tokens, 130), (tokens, 900)])]
+    cache = steps[0].cache.to(DEV)
+    assert steps[0].total == steps[1].total
+    plans = [attention_ops.plan_paged_attention(s.qp, s.kp, s.ki, s.kl, 8, 2, 128, 16) for s in steps]
+    n = plans[0].words.numel()
+    assert plans[1].words.numel() == n and not torch.equal(plans[0].words, plans[1].words)
+    workspace = torch.zeros(max(p.workspace_bytes for p in plans), dtype=torch.uint8, device=DEV)
+    query = steps[0].query.to(DEV)
+    # both at the end of a buffer whose writing takes a while
+    source = [torch.zeros(1 << 24, dtype=torch.int32, device=DEV) for _ in plans]
+    for s, p in zip(source, plans):
+        s[-n:] = p.words.to(DEV)
+    words = source[0].clone()
+    want = []
+    for p in plans:
+        want.append(torch.empty_like(query))
+        attention_ops.paged_attention(want[-1], query, cache, p, p.words.to(DEV), workspace, 0.1)
+    torch.cuda.synchronize()
+    assert not torch.equal(want[0], want[1])
+    outs = []
+    for i in range(40):
+        torch.add(source[i % 2], 0, out=words)
+        outs.append(torch.empty_like(query))
+        attention_ops.paged_attention(outs[-1], query, cache, plans[i % 2], words[-n:], workspace, 0.1)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i % 2]) for i, o in enumerate(outs))
