@@ -28,7 +28,7 @@ struct TokenInfo {
 // keys [kv_begin, kv_end).  splits > 1: it is number `split` of that many
 // pieces of the same rows, which leave partial results in slots `slot`,
 // slot + 1, ... and count their arrivals in counter `tile`.  mixed: some row
-// does not see every key that another sees.
+// may not see every key of the piece's rows.
 struct Item {
   int tok0, ntok, kv_begin, kv_end;
   int page_base, tile, slot, split;

@@ -219,7 +219,7 @@ extern "C" int pace_paged_attention_plan(
       for (int t0 = 0; t0 < q; t0 += step) {
         const int n = std::min(step, q - t0);
         int first = len, end = 0;  // keys that some token of the piece sees
-        bool mixed = tree_words > 0 && n > 1;
+        bool mixed = tree_words > 0;  // a node may not even see itself
         for (int i = t0; i < t0 + n; ++i) {
           const int pos = len - q + i;
           TokenInfo& w = tok[q0 + i];

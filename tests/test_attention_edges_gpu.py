@@ -118,3 +118,16 @@ def test_a_plan_written_by_the_kernel_before(tokens):
         attention_ops.paged_attention(outs[-1], query, cache, plans[i % 2], words[-n:], workspace, 0.1)
     torch.cuda.synchronize()
     assert all(torch.equal(o, want[i % 2]) for i, o in enumerate(outs))
+
+
+@pytest.mark.parametrize("heads", [8, 64])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_tree_of_one_hidden_node(heads, hd, bad):
+    """A drafted token that does not see itself, whose value row is not finite: the few-row
+    kernel (8 heads of 2) and the tile kernel (64)."""
+    lens = [(1, 300), (1, 1), (1, 40), (1, 5000)]
+    step = Step(lens, heads, 2, hd, seed=6)
+    for b, (_, n) in enumerate(lens):
+        step.cache[step.ki[int(step.kp[b]) + (n - 1) // 16], 1, (n - 1) % 16] = bad
+    step.check(tree_mask=torch.zeros(len(lens), 1, dtype=torch.int64))

@@ -1,7 +1,9 @@
 """CPU: what paged attention plans and refuses where arguments are at an edge."""
 import ctypes
 
-from paceserve_b200 import cabi
+import torch
+
+from paceserve_b200 import attention_ops, cabi
 
 
 def ints(*v):
@@ -33,3 +35,15 @@ def test_workspace_alignment_is_checked():
     for args in ((4096 + 16,), (4096 + 8,), (4096, plan.workspace_bytes - 1), (None,)):
         assert run(*args) == cabi.PACE_ERR_INVALID_ARGUMENT, args
         assert b"32-byte aligned workspace" in lib.pace_last_error()
+
+
+def test_every_piece_of_a_tree_may_hide_keys():
+    """Also a tree of one node: its own bit may be clear, and its key is in its piece."""
+    ints32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    for heads, words in ((8, 1), (64, 2)):
+        plan = attention_ops.plan_paged_attention(ints32(0, 1, 4), ints32(0, 2, 4), ints32(0, 1, 2, 3),
+                                                  ints32(5, 16), heads, 2, 128, 16, tree_words=words)
+        at = 4 * plan.total_q
+        items = [plan.words[at + 12 * i:at + 12 * i + 12].tolist()
+                 for i in range(plan.num_few + plan.num_many)]
+        assert len(items) == 2 and all(w[9] == 1 for w in items)
