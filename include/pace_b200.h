@@ -458,10 +458,12 @@ int pace_append_paged_kv_cache_by_indptr(const void* key, const void* value, int
  *   exponents [num_pages, 2, page_size, kv_heads]            uint8
  * A row x (one token's K or V of one head) is held as code = e4m3(x * 2^-e),
  * exponent = e + 127, with e the smallest integer >= -126 that has
- * max|x| <= 448 * 2^e (0 for a row of zeros), so value = code * 2^e and each
- * element is rounded once, to nearest even.  Infinities saturate at the
- * largest code and stay out of the maximum; a row with a NaN has exponent 255
- * and reads as NaN.  head_dim: a multiple of 8 up to 256.
+ * max|x| <= 448 * 2^e (so -126 for a row of zeros); value = code * 2^e, and each
+ * element is rounded once, to nearest even.  Attention reads any cache of codes
+ * and exponents rightly, but fast only where rows hold that smallest e.
+ * Infinities saturate at the largest code and stay out of the maximum (e is 0
+ * where they are among zeros alone); a row with a NaN has exponent 255 and reads
+ * as NaN.  head_dim: a multiple of 8 up to 256.
  *
  * Quantise and append nnz new tokens; arguments as
  * pace_append_paged_kv_cache_by_indptr (key and value float32, float16 or

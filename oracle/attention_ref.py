@@ -37,7 +37,7 @@ def quantise_row(x: torch.Tensor):
         return torch.zeros(x.shape, dtype=torch.uint8), 255
     finite = x[x.isfinite()].abs()
     top = float(finite.max()) if finite.numel() else 0.0
-    e = 0
+    e = 0 if bool(x.isinf().any()) else -126
     if top > 0:
         m, k = math.frexp(top)  # top = m * 2^k, 448 = 0.875 * 2^9
         e = max(k - 9 + (1 if m > 0.875 else 0), -126)

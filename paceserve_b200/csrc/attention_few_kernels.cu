@@ -27,7 +27,9 @@
 // K's factor multiplies the scores.  V's factor 2^e goes into P: the output has a
 // running maximum of its own, of score + e, and is built from 2^(score + e - it), so
 // that the row's largest contribution is about 1 in fp16 whatever the factors are;
-// the sum l keeps the maximum of the scores alone.  Queries are scaled by a power
+// the sum l keeps the maximum of the scores alone.  That holds for rows whose largest
+// code is near 448, as the append makes them; where another cache's rows break it, the
+// output shows it and the row is done again on the CUDA cores.  Queries are scaled by a power
 // of two to the top of fp16's range: a bf16 query keeps all its bits down to 2^-29
 // of its largest element.
 #include "attention_mma.cuh"
@@ -37,6 +39,11 @@ namespace attn {
 
 constexpr int kFewWarps = 4;
 constexpr float kLag = 8.f;  // in powers of two
+// Over a quantised cache: the least size of an output, in units of its largest contribution's
+// weight times one code, that its products in fp16 are trusted with.
+constexpr float kLeastOutput = 32.f;
+// Exponents of V below this are those of zeros: 448 * 2^-100 * 2^-25 times any length is nothing.
+constexpr float kFaintExponent = -100.f;
 
 template <int D, bool Q8, int R>
 struct FewTile {
@@ -78,6 +85,13 @@ __device__ __forceinline__ void unpack_by(bool conversion, uint32_t w, uint32_t&
   }
 }
 
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // R: 1 where the rows fit the matrix instruction's first eight, else 2.
 template <typename T, int D, bool Q8, int R>
 __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
@@ -87,6 +101,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
   using M = Mma<std::conditional_t<Q8, __half, T>>;
   constexpr int KEYS = Tile::kKeys, NT = KEYS / 8, KB = D / 16, STAGES = Tile::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint32_t faint;  // rows to be done again
+  if (threadIdx.x == 0) faint = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.x % p.kv_heads;
@@ -466,6 +482,23 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     const int r = g + 8 * i;
+    if constexpr (Q8) {
+      // The key that set the output's maximum adds its weight of 1 times its largest code, 224 or
+      // more of a row as the append writes it.  An output that stays far below had its maximum
+      // set by a row that adds little or nothing (zeros under a large exponent), and what counts
+      // may have been lost below fp16.  Not where that row's factor is next to nothing itself, as
+      // the append gives it to zeros: then so is all that is lost.  NaN is left as it is.
+      float top = 0.f;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        const float up = by_conversion(n >> 1) ? 1.f : 256.f;
+        top = max_nan(top, max_nan(fabsf(o[n][2 * i]), fabsf(o[n][2 * i + 1])) * up);
+      }
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if (c == 0 && r < rows && mo[i] > m[i] + kFaintExponent && top < kLeastOutput)
+        atomicOr(&faint, 1u << r);
+    }
     if (r < rows) {
       if (c == 0) {
         join_ml[(warp * 16 + r) * 2] = m[i];
@@ -486,6 +519,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
   __syncthreads();
   constexpr int V4 = D / 4;
   const int64_t slot = (int64_t)(w.slot + w.split) * p.kv_heads + kvh;
+  const uint32_t redo = Q8 ? *reinterpret_cast<volatile uint32_t*>(&faint) : 0;
   // whole warps stay in the loop, for redo_rows
   for (int u = threadIdx.x; (u & ~31) < rows * V4; u += kFewWarps * 32) {
     const int r = u / V4, d = (u - r * V4) * 4;
@@ -508,13 +542,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
       }
       if (w.splits == 1) {
         fine = write_out<T>(p, w.tok0 + r / group, kvh * group + r % group, d, v, mm, sum);
+        fine = (fine || !w.mixed) && !(redo >> r & 1);
       } else {
         __stcg(reinterpret_cast<float4*>(partial + (slot * 16 + r) * D + d),
                make_float4(v[0], v[1], v[2], v[3]));
-        if (d == 0) __stcg(partial_ml + slot * 16 + r, make_float2(mm, sum));
+        // the sign of the sum tells the piece that joins
+        if (d == 0) __stcg(partial_ml + slot * 16 + r, make_float2(mm, redo >> r & 1 ? -sum : sum));
       }
     }
-    if (w.mixed) redo_rows<T, D, Q8>(p, w, kvh, group, r, fine);
+    if (w.mixed || redo) redo_rows<T, D, Q8>(p, w, kvh, group, r, fine);
   }
   if (w.splits == 1) {
     if (beside) pdl_wait();

@@ -208,8 +208,8 @@ __device__ __noinline__ void attend_row_again(const Problem& p, int64_t tok, int
 }
 
 // Redoes rows whose outputs, just written by this warp's lanes (lane u: four
-// columns of row `r`), are not all finite.  The whole warp calls it; lanes
-// without a row pass fine = true.
+// columns of row `r`), are not fine: not all finite, or marked as too faint.  The
+// whole warp calls it; lanes without a row pass fine = true.
 template <typename T, int D, bool Q8>
 __device__ __forceinline__ void redo_rows(const Problem& p, const Item& w, int kvh, int group, int r,
                                           bool fine) {
@@ -251,7 +251,8 @@ __device__ __forceinline__ void join_sync() {
 // ROWS: rows of a slot; scratch: `room` floats of shared memory.  The pieces'
 // weights 2^(m_k - M) are found once per row; then every thread keeps four
 // columns of four units, a piece of each, in flight (one unit at a time, each
-// waiting for its own loads, 32 trees took 155 us instead of 105 uncut).
+// waiting for its own loads, 32 trees took 155 us instead of 105 uncut).  A
+// negative sum asks for the row to be done again.
 template <typename T, int ROWS, int D, bool Q8, int NT>
 __device__ __forceinline__ void join_pieces(const Problem& p, const float* partial,
                                             const float2* partial_ml, const Item& w, int kvh,
@@ -271,15 +272,17 @@ __device__ __forceinline__ void join_pieces(const Problem& p, const float* parti
     join_sync<NT>();
     for (int r = threadIdx.x; r < n; r += NT) {
       float mm = -INFINITY, sum = 0.f;
+      bool redo = false;
       for (int k = 0; k < w.splits; ++k) mm = fmaxf(mm, ms[k * n + r]);
       const float b = mm == -INFINITY ? 0.f : mm;
       for (int k = 0; k < w.splits; ++k) {
         const float f = exp2_approx(ms[k * n + r] - b);
-        sum += f * ls[k * n + r];
+        sum += f * fabsf(ls[k * n + r]);
+        redo |= ls[k * n + r] < 0.f;
         ms[k * n + r] = f;
       }
       top[r] = mm;
-      total[r] = sum;
+      total[r] = redo ? -sum : sum;
     }
     join_sync<NT>();
     // whole warps stay in the loop, for redo_rows
@@ -309,10 +312,12 @@ __device__ __forceinline__ void join_pieces(const Problem& p, const float* parti
         if ((u & ~31) >= n * V4) break;
         const int r = u / V4;
         bool fine = true;
-        if (u < n * V4)
+        if (u < n * V4) {
           fine = write_out<T>(p, w.tok0 + (r0 + r) / group, kvh * group + (r0 + r) % group,
-                              (u - r * V4) * 4, v[i], top[r], total[r]);
-        if (w.mixed) redo_rows<T, D, Q8>(p, w, kvh, group, r0 + r, fine);
+                              (u - r * V4) * 4, v[i], top[r], fabsf(total[r]));
+          fine = (fine || !w.mixed) && !(Q8 && total[r] < 0.f);
+        }
+        if (w.mixed || Q8) redo_rows<T, D, Q8>(p, w, kvh, group, r0 + r, fine);
       }
     }
     join_sync<NT>();

@@ -47,10 +47,9 @@ __device__ __forceinline__ uint32_t floats_to_e4m3x4(const float* f) {
 // The exponent byte of a row whose largest finite magnitude is `amax`: the
 // smallest e >= -126 with amax <= 448 * 2^e, plus 127.  448 = 1.75 * 2^8, so
 // with amax = 1.f * 2^(E - 127) it is e = E - 135, one more if 1.f > 1.75.
-// A row of zeros has e = 0.
+// A row of zeros so has e = -126, and no weight beside rows that are not.
 __device__ __forceinline__ uint32_t row_exponent(float amax) {
   const uint32_t bits = __float_as_uint(amax);
-  if (bits == 0) return 127;
   const int e = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return (uint32_t)(e < 1 ? 1 : e);
 }

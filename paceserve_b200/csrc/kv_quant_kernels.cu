@@ -10,7 +10,8 @@
 //   code = e4m3(x * 2^-e) (nearest, ties to even), exponent = e + 127,
 // where the scaling is exact, so each code has one rounding.  Infinities
 // saturate at the largest code and do not enter the maximum; a row that holds
-// a NaN gets exponent 255 and reads back as NaN.
+// a NaN gets exponent 255 and reads back as NaN.  Infinities among zeros alone
+// have e = 0.
 //
 // Both kernels move bytes and little else.  Append, per token: 4 * kv_heads *
 // head_dim bytes of 16-bit input read, half of that plus 2 * kv_heads written.
@@ -80,19 +81,25 @@ struct Raw8 {
 // `group` neighbouring lanes, all of which call.  In fp32, whatever the elements.
 __device__ __forceinline__ uint32_t quantise_floats(const float (&x)[8], int group, uint2& code) {
   float amax = 0.f;
-  bool nan = false;
+  bool nan = false, inf = false;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float a = fabsf(x[e]);
     nan |= a != a;
+    inf |= a == INFINITY;
     if (a < INFINITY) amax = fmaxf(amax, a);
   }
   // NaN travels as a value above every finite magnitude
   if (nan) amax = INFINITY;
-  for (int o = group >> 1; o > 0; o >>= 1)
+  for (int o = group >> 1; o > 0; o >>= 1) {
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    inf |= __shfl_xor_sync(0xffffffffu, inf, o);
+  }
   const bool row_nan = amax == INFINITY;
-  const uint32_t ex = row_nan ? (uint32_t)kNanExponent : row_exponent(amax);
+  // an infinity among zeros alone saturates at 448, not at 448 times next to nothing
+  const uint32_t ex = row_nan               ? (uint32_t)kNanExponent
+                      : inf && amax == 0.f ? 127u
+                                           : row_exponent(amax);
   // 2^-e: an exact power of two, since e lies in [-126, 120]
   const float inv = row_nan ? 0.f : __uint_as_float((254u - ex) << 23);
   float y[8];

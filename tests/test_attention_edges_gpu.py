@@ -2,11 +2,14 @@
 
 Tolerances are those derived in ``test_attention_gpu.py``.
 """
+import math
+
 import pytest
 import torch
 
+from paceserve_b200 import kv_transfer_ops as kv
 from paceserve_b200.attention import PagedAttention, attention_ops
-from tests.test_attention_gpu import DEV, Step
+from tests.test_attention_gpu import DEV, Step, random_trees
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +134,58 @@ def test_a_tree_of_one_hidden_node(heads, hd, bad):
     for b, (_, n) in enumerate(lens):
         step.cache[step.ki[int(step.kp[b]) + (n - 1) // 16], 1, (n - 1) % 16] = bad
     step.check(tree_mask=torch.zeros(len(lens), 1, dtype=torch.int64))
+
+
+def zero_row_step(tokens, length, key, above, exponent, zero_exponent, hd=128, dtype=torch.bfloat16,
+                  heads=8):
+    """Requests whose key `key` has a value row of zeros and a score `above` powers of two over the
+    others', which are near 0; the values' exponent byte, and the zero row's."""
+    step = Step([(q, n) for q, n in zip(tokens, length)], heads, 2, hd, dtype=dtype, quantised=True,
+                seed=41)
+    step.exponents[:, 1] = exponent
+    step.query[..., 0] = 1.0  # times the key's 128
+    step.exponents[:, 0] = 114  # the others' keys are up to 448 * 2^-13
+    for b in range(len(tokens)):
+        page, slot = step.ki[int(step.kp[b]) + key // step.page], key % step.page
+        step.cache[page, :, slot] = 0
+        step.exponents[page, 0, slot] = 127
+        step.cache[page, 0, slot, :, 0] = 0x70 if above else 0
+        step.exponents[page, 1, slot] = zero_exponent
+    return step, {"sm_scale": above / 128 / math.log2(math.e)} if above else {}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("above", [0, 6, 10])
+@pytest.mark.parametrize("exponent", [118, 113, 108, 90])  # values up to 0.9, 0.03, 9e-4, 3e-9
+@pytest.mark.parametrize("zero_exponent", [1, 127, 140])
+def test_a_value_row_of_zeros(dtype, above, exponent, zero_exponent):
+    """A visible key with a value row of zeros adds to the softmax's sum alone, whatever the row's
+    exponent and however high its score: few rows and many, whole and cut, in trees."""
+    for tokens, lengths, heads in (((1, 1, 1), (300, 33, 20), 8), ((1, 4), (6000, 5000), 8),
+                                   ((2, 1), (70, 300), 16), ((80, 40), (300, 200), 8),
+                                   ((70,), (6000,), 8)):
+        if dtype == torch.float16 and exponent == 90:
+            continue  # no values of fp16
+        step, kw = zero_row_step(tokens, lengths, 17, above, exponent, zero_exponent, dtype=dtype,
+                                 heads=heads)
+        step.check(**kw)
+    step, kw = zero_row_step((5, 3), (300, 90), 17, above, max(exponent, 100), zero_exponent, hd=64)
+    step.check(tree_mask=random_trees(step.lens, 1), **kw)
+
+
+def test_nothing_but_zeros():
+    """A cache as it is allocated, and zero rows as the append leaves them."""
+    for zero_exponent in (0, 1, 127):
+        step = Step([(1, 300), (1, 4000), (50, 200)], 8, 2, 128, quantised=True, seed=1)
+        step.cache[:] = 0
+        step.exponents[:] = zero_exponent
+        step.check()
+    key = torch.zeros(3, 2 * 128, dtype=torch.bfloat16)
+    key[1, 5] = 1.0
+    codes = torch.zeros(4, 2, 16, 2, 128, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    exps = torch.zeros(4, 2, 16, 2, dtype=torch.uint8, device=DEV)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    kv.append_quantised_paged_kv_cache(key.to(DEV), key.to(DEV), i32(0, 3), codes, exps, i32(2),
+                                       i32(0, 1), i32(3))
+    # e = -126 for zeros; 1 is 256 * 2^-8
+    assert exps[2, :, :3].cpu().tolist() == [[[1, 1], [119, 1], [1, 1]]] * 2
