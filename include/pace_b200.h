@@ -462,8 +462,9 @@ int pace_append_paged_kv_cache_by_indptr(const void* key, const void* value, int
  * element is rounded once, to nearest even.  Attention reads any cache of codes
  * and exponents rightly, but fast only where rows hold that smallest e.
  * Infinities saturate at the largest code and stay out of the maximum (e is 0
- * where they are among zeros alone); a row with a NaN has exponent 255 and reads
- * as NaN.  head_dim: a multiple of 8 up to 256.
+ * where they are among zeros alone); finite elements never take a code whose value
+ * their type does not hold, but the one below it; a row with a NaN has exponent 255
+ * and reads as NaN.  head_dim: a multiple of 8 up to 256.
  *
  * Quantise and append nnz new tokens; arguments as
  * pace_append_paged_kv_cache_by_indptr (key and value float32, float16 or

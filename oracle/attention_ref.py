@@ -32,6 +32,7 @@ E4M3_VALUES = torch.tensor([e4m3_value(c) for c in range(256)], dtype=torch.floa
 
 def quantise_row(x: torch.Tensor):
     """(codes uint8, exponent byte) of one row of floats."""
+    most = torch.finfo(x.dtype).max
     x = x.double()
     if bool(x.isnan().any()):
         return torch.zeros(x.shape, dtype=torch.uint8), 255
@@ -48,6 +49,8 @@ def quantise_row(x: torch.Tensor):
     lo = (hi - 1).clamp(min=0)
     dl, dh = y.abs() - grid[lo], grid[hi] - y.abs()
     code = torch.where((dl < dh) | ((dl == dh) & (lo % 2 == 0)), lo, hi)
+    # what is finite in its type stays so
+    code = torch.where(x.isfinite() & (grid[code] * 2.0 ** e > most), code - 1, code)
     return (code + 128 * torch.signbit(y).long()).to(torch.uint8), e + 127
 
 

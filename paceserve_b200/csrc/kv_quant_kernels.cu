@@ -11,7 +11,8 @@
 // where the scaling is exact, so each code has one rounding.  Infinities
 // saturate at the largest code and do not enter the maximum; a row that holds
 // a NaN gets exponent 255 and reads back as NaN.  Infinities among zeros alone
-// have e = 0.
+// have e = 0.  A finite element never takes a code whose value its type does not
+// hold (256 * 2^8 of float16, 256 * 2^120 of the others), but the one below it.
 //
 // Both kernels move bytes and little else.  Append, per token: 4 * kv_heads *
 // head_dim bytes of 16-bit input read, half of that plus 2 * kv_heads written.
@@ -77,8 +78,18 @@ struct Raw8 {
   }
 };
 
+// The exponent byte at which the type's largest magnitudes, from 248 * 2^e, would
+// round to 256 * 2^e, which it does not hold: they take the code below it, 240, so
+// that what was finite reads back finite.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t top_exponent() {
+  return std::is_same<T, __half>::value ? 127 + 16 - 8 : 127 + 128 - 8;
+}
+__device__ __forceinline__ float below_256(float y) { return fminf(fmaxf(y, -240.f), 240.f); }
+
 // Eight elements' codes and their row's exponent byte; the row is spread over
 // `group` neighbouring lanes, all of which call.  In fp32, whatever the elements.
+template <typename T>
 __device__ __forceinline__ uint32_t quantise_floats(const float (&x)[8], int group, uint2& code) {
   float amax = 0.f;
   bool nan = false, inf = false;
@@ -104,15 +115,18 @@ __device__ __forceinline__ uint32_t quantise_floats(const float (&x)[8], int gro
   const float inv = row_nan ? 0.f : __uint_as_float((254u - ex) << 23);
   float y[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = row_nan ? 0.f : x[e] * inv;
+  for (int e = 0; e < 8; ++e) {
+    y[e] = row_nan ? 0.f : x[e] * inv;
+    if (ex == top_exponent<T>() && fabsf(x[e]) < INFINITY) y[e] = below_256(y[e]);
+  }
   code = make_uint2(floats_to_e4m3x4(y), floats_to_e4m3x4(y + 4));
   return ex;
 }
 
 // The same from the elements' bits.  16-bit types find the maximum on pairs of
-// magnitudes as integers; only a warp that holds an infinity or a NaN takes the
-// way above (which at 110 instructions for 8 elements bound the kernel: 16167
-// fp16 tokens 39 us).
+// magnitudes as integers; only a warp that holds an infinity, a NaN or one of the
+// type's largest magnitudes takes the way above (which at 110 instructions for 8
+// elements bound the kernel: 16167 fp16 tokens 39 us).
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const uint4 (&v)[sizeof(T) / 2], int group,
                                               uint2& code) {
@@ -126,8 +140,9 @@ __device__ __forceinline__ uint32_t quantise8(const uint4 (&v)[sizeof(T) / 2], i
     for (int o = group >> 1; o > 0; o >>= 1)
       m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
     m = max(m & 0xffffu, m >> 16);
-    constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    if (__all_sync(0xffffffffu, m < kInf)) {
+    // 248 * 2^e of the top exponent, past which lie infinities and NaN too
+    constexpr uint32_t kTop = std::is_same<T, __half>::value ? 0x7bc0u : 0x7f78u;
+    if (__all_sync(0xffffffffu, m < kTop)) {
       const uint16_t bits = (uint16_t)m;
       const uint32_t ex = row_exponent(Traits<T>::to_f(*reinterpret_cast<const T*>(&bits)));
       const float inv = __uint_as_float((254u - ex) << 23);
@@ -137,7 +152,7 @@ __device__ __forceinline__ uint32_t quantise8(const uint4 (&v)[sizeof(T) / 2], i
       return ex;
     }
   }
-  return quantise_floats(x, group, code);
+  return quantise_floats<T>(x, group, code);
 }
 
 // Where this thread works: as many tokens as fit the CTA side by side, `lanes`

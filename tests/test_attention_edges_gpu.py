@@ -7,6 +7,7 @@ import math
 import pytest
 import torch
 
+from oracle import attention_ref as ref
 from paceserve_b200 import kv_transfer_ops as kv
 from paceserve_b200.attention import PagedAttention, attention_ops
 from tests.test_attention_gpu import DEV, Step, random_trees
@@ -189,3 +190,33 @@ def test_nothing_but_zeros():
                                        i32(0, 1), i32(3))
     # e = -126 for zeros; 1 is 256 * 2^-8
     assert exps[2, :, :3].cpu().tolist() == [[[1, 1], [119, 1], [1, 1]]] * 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_finite_rows_read_back_finite(dtype):
+    """The type's largest magnitudes, within 2^-4 as any other value; beside infinities too."""
+    heads, hd, most = 2, 64, torch.finfo(dtype).max
+    x = torch.full((4, heads * hd), most, dtype=dtype)
+    x[1] = -most
+    # 247 and 249 of 256 parts either side of the last tie, and smaller ones
+    x[2] = (torch.tensor([247.0, 249.0, 240.0, -249.0, 17.0, 1.0, 0.0, -255.0]) / 256).to(dtype).repeat(
+        heads * hd // 8) * (most / 2) * 2
+    x[3, ::3] = most
+    x[3, 1] = float("inf")
+    codes = torch.zeros(4, 2, 16, heads, hd, dtype=torch.uint8)
+    exps = torch.zeros(4, 2, 16, heads, dtype=torch.uint8)
+    got_c, got_e = codes.to(DEV).view(torch.float8_e4m3fn), exps.to(DEV)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    meta = [i32(2), i32(0, 1), i32(4)]
+    on = [t.to(DEV) for t in meta]
+    kv.append_quantised_paged_kv_cache(x.to(DEV), x.to(DEV), i32(0, 4).to(DEV), got_c, got_e, *on)
+    ref.append_quantised(x, x, i32(0, 4), codes, exps, *meta)
+    assert torch.equal(got_c.view(torch.uint8).cpu(), codes) and torch.equal(got_e.cpu(), exps)
+    out = torch.zeros(2, 4, heads * hd, dtype=dtype, device=DEV)
+    kv.read_quantised_paged_kv_cache(out[0], out[1], i32(0, 4).to(DEV), got_c, got_e, *on)
+    for got in out.cpu():
+        finite = x.isfinite()
+        assert bool(got[finite].isfinite().all())
+        # relative to the row's largest, which bounds the subnormal codes' error too
+        err = (got.double() - x.double()).abs()[finite]
+        assert bool((err <= 2.0 ** -4 * x.double().abs()[finite] + 2.0 ** -18 * most).all())
