@@ -41,7 +41,7 @@ constexpr int kFewWarps = 4;
 constexpr float kLag = 8.f;  // in powers of two
 // Over a quantised cache: the least size of an output, in units of its largest contribution's
 // weight times one code, that its products in fp16 are trusted with.
-constexpr float kLeastOutput = 32.f;
+constexpr float kLeastOutput = 32.f * 128;
 // Exponents of V below this are those of zeros: 448 * 2^-100 * 2^-25 times any length is nothing.
 constexpr float kFaintExponent = -100.f;
 
@@ -99,6 +99,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
                          float2* partial_ml, int32_t* counters, bool q_even, bool beside) {
   using Tile = FewTile<D, Q8, R>;
   using M = Mma<std::conditional_t<Q8, __half, T>>;
+  // what P, and with it the sum, is scaled up by; over a quantised cache P alone, see base_o
+  constexpr float kUp = !Q8 && std::is_same<T, __half>::value ? kHeadroom : 0.f;
   constexpr int KEYS = Tile::kKeys, NT = KEYS / 8, KB = D / 16, STAGES = Tile::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t faint;  // rows to be done again
@@ -417,8 +419,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
     float base[R], base_o[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      base[i] = m[i] == -INFINITY ? 0.f : m[i];
-      base_o[i] = mo[i] == -INFINITY ? 0.f : mo[i];
+      base[i] = m[i] == -INFINITY ? 0.f : m[i] - kUp;
+      base_o[i] = mo[i] == -INFINITY ? 0.f : mo[i] - kHeadroom;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -501,12 +503,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
     }
     if (r < rows) {
       if (c == 0) {
-        join_ml[(warp * 16 + r) * 2] = m[i];
+        join_ml[(warp * 16 + r) * 2] = m[i] - kUp;
         join_ml[(warp * 16 + r) * 2 + 1] = l[i];
       }
       float* dst = reinterpret_cast<float*>(ring) + r * D;
       // in the joined output's units, 2^m
-      const float unit = Q8 ? (mo[i] == -INFINITY ? 0.f : exp2_approx(mo[i] - m[i])) : 1.f;
+      const float unit =
+          Q8 ? (mo[i] == -INFINITY ? 0.f : exp2_approx(mo[i] - kHeadroom - m[i])) : 1.f;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) {
         const float up = Q8 && !by_conversion(n >> 1) ? 256.f : 1.f;

@@ -52,6 +52,12 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
+// Where P is fp16 it is built as 2^(s - m + kHeadroom): with a maximum that lags by
+// up to 2^8 it stays below 2^16, and weights down to 2^-21 of the largest keep all
+// their bits, where fp16 would else give out at 2^-14.  The sum has the same units,
+// and what leaves the kernel as the maximum is m - kHeadroom.
+constexpr float kHeadroom = 7.f;
+
 // A word of four codes as two registers of two 16-bit values each, bytes 0, 2
 // and bytes 1, 3: sign to the top, exponent and mantissa below it, shifted to
 // the type's mantissa end.  The value is the code's times 2^-120 (bf16) or 2^-8

@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
                           int32_t* counters, int32_t* fault) {
   using Cfg = TileCfg<D, Q8>;
   using M = Mma<T>;
+  constexpr float kUp = std::is_same<T, __half>::value ? kHeadroom : 0.f;  // of P and its sum
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
             }
           }
         }
-        const float b = m == -INFINITY ? 0.f : m;
+        const float b = m == -INFINITY ? 0.f : m - kUp;
         uint64_t sum[2] = {0, 0};  // two pairs of partial sums
         const uint64_t sc2 = f32x2(sc, sc), b2 = f32x2(-b, -b);
 #pragma unroll
@@ -554,6 +555,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
         l += lo_of(sum[0]) + hi_of(sum[0]);
       }
       // ---- the tile's output ----------------------------------------------------
+      m -= kUp;
       if (ok && steps > 0)
         ok = __all_sync(0xffffffffu,
                         wait_for(&ctl->o_full[t], 0, ctl));

@@ -220,3 +220,30 @@ def test_finite_rows_read_back_finite(dtype):
         # relative to the row's largest, which bounds the subnormal codes' error too
         err = (got.double() - x.double()).abs()[finite]
         assert bool((err <= 2.0 ** -4 * x.double().abs()[finite] + 2.0 ** -18 * most).all())
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_small_weights_keep_their_bits(dtype, quantised):
+    """Few rows and many, scores spread so far that one key has nearly all of the weight, and a
+    value row of that key that is zero in half of the dimensions: what the others, down to 2^-20
+    of it, give there is as exact as anything else."""
+    for tokens in (1, 3, 70):
+        for length in (200, 6000):
+            step = Step([(tokens, length)], 8, 2, 128, dtype=dtype, quantised=quantised, seed=25)
+            page, slot = step.ki[2], 5  # key 37
+            step.query[..., 0] = 4.0
+            step.cache[:, 0, :, :, 0] = 0
+            if quantised:
+                step.exponents[page, 0, slot] = 121
+                step.cache[page, 0, slot] = 0
+                step.cache[page, 0, slot, :, 0] = 0x7e  # 448 / 64 = 7
+                step.cache[page, 1, slot, :, :64] = 0
+                k = 7.0
+            else:
+                step.cache[page, 0, slot] = 0
+                step.cache[page, 0, slot, :, 0] = k = 7.0
+                step.cache[page, 1, slot, :, :64] = 0
+            # the others' scores are near 0 for a scale so small but for this key's
+            step.query[..., 1:] *= 0.02
+            step.check(sm_scale=20.0 / (4.0 * k) / math.log2(math.e))
