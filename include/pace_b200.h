@@ -497,7 +497,7 @@ int pace_read_quantised_paged_kv_cache(void* key, void* value, int64_t rows, int
 /* ---- paged attention ------------------------------------------------------
  * Attention of each request's newest tokens over its paged sequence.  For query
  * token i of a request (position p = kv_len - q_len + i), head h and key j
- *   s = cap * tanh(sm_scale * q.k / cap)   (cap 0: sm_scale * q.k)
+ *   s = cap * tanh(sm_scale * q.k / cap)   (cap 0 or from 1e30: sm_scale * q.k)
  *       - slope[h] * |p - j|               (with alibi_slopes)
  *   out = sum_j softmax_j(s) v_j over the visible keys; 0 where there is none.
  * Visible are the keys j <= p and, with a prefix, j < prefix_lens[request], of

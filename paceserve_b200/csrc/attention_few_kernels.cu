@@ -92,8 +92,25 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// R: 1 where the rows fit the matrix instruction's first eight, else 2.
-template <typename T, int D, bool Q8, int R>
+// cap * tanh(x / cap) as a difference, off by about cap * 2^-22.
+__device__ __forceinline__ float cap_score(float x, float cap, float cap_in) {
+  return cap - 2.f * cap * rcp_approx(1.f + exp2_approx(x * cap_in));
+}
+// Scores well within a cap larger than this would not bear that.  Up to a quarter
+// of it they take four terms of the series of tanh(u) / u instead (the fifth is
+// 3.3e-7 there), whose error goes with the score.  Choosing in the one kernel for
+// all caps took 64 requests over a quantised cache without any from 163 to 189 us.
+constexpr float kLargeCap = 512.f;
+__device__ __forceinline__ float large_cap_score(float x, float cap, float inv_cap,
+                                                 float cap_in) {
+  const float u = x * inv_cap, z = u * u;
+  const float near = x * fmaf(z, fmaf(z, fmaf(z, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+  return fabsf(u) <= 0.25f ? near : cap_score(x, cap, cap_in);
+}
+
+// R: 1 where the rows fit the matrix instruction's first eight, else 2.  LARGE:
+// the cap is a large one.
+template <typename T, int D, bool Q8, int R, bool LARGE>
 __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
     attention_few_kernel(const Problem p, const Item* items, float* partial,
                          float2* partial_ml, int32_t* counters, bool q_even, bool beside) {
@@ -285,6 +302,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
 #pragma unroll
   for (int i = 0; i < R; ++i) mo[i] = -INFINITY;
   const float cap2 = p.cap * kLog2e, cap_in = p.cap > 0.f ? 2.f / p.cap : 0.f;
+  const float inv_cap2 = LARGE ? 1.f / cap2 : 0.f;
 
   for (int step = 0; step < steps; ++step) {
     if (step > 0) put_factors(step + STAGES - 2);  // their loads had a step's time
@@ -340,8 +358,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
       for (int e = 0; e < 2 * R; ++e) {
         float x = s[n][e] * row_scale[e >> 1];
         if constexpr (Q8) x *= e & 1 ? f.y : f.x;
-        if (p.cap > 0.f)
-          x = cap2 - 2.f * cap2 * rcp_approx(1.f + exp2_approx(x * cap_in));  // cap tanh
+        if constexpr (LARGE)
+          x = large_cap_score(x, cap2, inv_cap2, cap_in);
+        else if (p.cap > 0.f)
+          x = cap_score(x, cap2, cap_in);
         s[n][e] = x;
       }
     }
@@ -569,12 +589,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
   if (beside) pdl_wait();
 }
 
-template <typename T, int D, bool Q8, int R>
+template <typename T, int D, bool Q8, int R, bool LARGE>
 static int run_few_r(const Problem& p, const Item* items, int num_items, float* partial, float2* ml,
                      int32_t* counters, bool beside, int device, cudaStream_t stream,
                      const char* what) {
   using Tile = FewTile<D, Q8, R>;
-  auto kernel = attention_few_kernel<T, D, Q8, R>;
+  auto kernel = attention_few_kernel<T, D, Q8, R, LARGE>;
   cudaError_t err =
       ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), device, Tile::kSmemBytes);
   if (err != cudaSuccess) return cuda_fail(err, what);
@@ -588,10 +608,11 @@ template <typename T, int D, bool Q8>
 static int run_few(const Problem& p, int max_rows, const Item* items, int num_items, float* partial,
                    float2* ml, int32_t* counters, bool beside, int device, cudaStream_t stream,
                    const char* what) {
-  return max_rows <= 8 ? run_few_r<T, D, Q8, 1>(p, items, num_items, partial, ml, counters, beside,
-                                                device, stream, what)
-                       : run_few_r<T, D, Q8, 2>(p, items, num_items, partial, ml, counters, beside,
-                                                device, stream, what);
+  auto go = [&](auto f) {
+    return f(p, items, num_items, partial, ml, counters, beside, device, stream, what);
+  };
+  if (p.cap > kLargeCap) return go(run_few_r<T, D, Q8, 2, true>);
+  return max_rows <= 8 ? go(run_few_r<T, D, Q8, 1, false>) : go(run_few_r<T, D, Q8, 2, false>);
 }
 
 int run_few_rows(const Problem& p, int max_rows, const Item* items, int num_items, float* partial,

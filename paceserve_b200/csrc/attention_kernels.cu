@@ -332,7 +332,7 @@ extern "C" int pace_paged_attention(const pace_attention_plan* plan, const int32
   for (int s = 0; s < 31; ++s)
     if (plan->page_size == 1 << s) p.page_shift = s;
   p.scale = sm_scale;
-  p.cap = logits_soft_cap;
+  p.cap = logits_soft_cap < 1e30f ? logits_soft_cap : 0.f;  // such a cap bends no score
   // The tensor-core kernels take 16-bit queries of 64 or 128 dimensions over a cache that 16-byte
   // copies fit and whose rows 32 bits number; the CUDA-core kernel the rest.
   const int64_t cache_rows = num_pages * 2 * plan->page_size * plan->num_kv_heads;

@@ -10,7 +10,7 @@ import torch
 from oracle import attention_ref as ref
 from paceserve_b200 import kv_transfer_ops as kv
 from paceserve_b200.attention import PagedAttention, attention_ops
-from tests.test_attention_gpu import DEV, Step, random_trees
+from tests.test_attention_gpu import DEV, U, Step, random_trees
 
 pytestmark = pytest.mark.gpu
 
@@ -247,3 +247,31 @@ def test_small_weights_keep_their_bits(dtype, quantised):
             # the others' scores are near 0 for a scale so small but for this key's
             step.query[..., 1:] *= 0.02
             step.check(sm_scale=20.0 / (4.0 * k) / math.log2(math.e))
+
+
+@pytest.mark.parametrize("cap", [513.0, 1e4, 1e5, 1e6, 1e9, 3e38, float("inf")])
+@pytest.mark.parametrize("quantised", [False, True])
+def test_large_caps(cap, quantised):
+    """A cap far above the scores hardly bends them, in whichever kernel; an infinite one is none."""
+    for hd, spread in ((64, 1.5), (128, 1.5), (128, 8.0)):
+        step = Step([(1, 300), (3, 90), (130, 400), (1, 6000)], 8, 2, hd, quantised=quantised, seed=23,
+                    spread=spread)
+        got, lse = step.run(logits_soft_cap=cap)
+        out, want_lse, size = step.want(logits_soft_cap=cap if cap < math.inf else 0.0)
+        u = U[torch.bfloat16]
+        assert bool(((got.double() - out).abs() <= u * out.abs() + (u + 4e-4) * size).all())
+        assert bool(((lse.double() - want_lse).abs() <= 5e-4 + 1e-6 * want_lse.abs()).all())
+
+
+@pytest.mark.parametrize("cap", [600.0, 1e4, 1e5])
+@pytest.mark.parametrize("tokens", [1, 5, 70])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_large_caps_beside_a_score_near_them(cap, tokens, hd):
+    """One key whose score is minus half the cap; the others' are ordinary and all that counts."""
+    step = Step([(tokens, 300), (tokens, 5000)], 8, 2, hd, seed=24)
+    step.query[..., 0] = 8.0
+    for b, (_, n) in enumerate(step.lens):
+        for j in (3, n - tokens - 2):
+            page, slot = step.ki[int(step.kp[b]) + j // 16], j % 16
+            step.cache[page, 0, slot, :, 0] = -0.5 * cap / 8 * math.sqrt(hd)
+    step.check(logits_soft_cap=cap)
