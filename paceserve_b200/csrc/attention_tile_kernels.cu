@@ -306,8 +306,11 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   }
   if (warp == 8) tc::tmem_alloc(&ctl->tmem, 512);
   pdl_wait();
-  // not earlier: a kernel may have written the plan.  The barrier below hides its latency.
-  const Item w = items[blockIdx.x / p.kv_heads];
+  // not earlier: a kernel may have written the plan.  Ahead of the barrier, which hides the latency
+  // (8192 tokens 498 us, behind it 513), but for a quantised cache, whose roles have no registers
+  // to spare for it (8192 tokens, capped: 846 us, behind it 832).
+  Item w;
+  if constexpr (!Q8) w = items[blockIdx.x / p.kv_heads];
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -315,6 +318,7 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
   // not before the wait: the few-row kernel of the same call starts beside this one without a wait
   // of its own, on what is complete here
   pdl_launch_dependents();
+  if constexpr (Q8) w = items[blockIdx.x / p.kv_heads];
   const int group = p.heads / p.kv_heads;
   const int rows = w.ntok * group;
   // row / group for rows below 256 and groups up to 128: the fraction added stays below 1 / group
