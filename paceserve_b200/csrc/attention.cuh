@@ -28,11 +28,12 @@ struct TokenInfo {
 // keys [kv_begin, kv_end).  splits > 1: it is number `split` of that many
 // pieces of the same rows, which leave partial results in slots `slot`,
 // slot + 1, ... and count their arrivals in counter `tile`.  mixed: some row
-// may not see every key of the piece's rows.
+// may not see every key of the piece's rows.  all_begin, all_end: the keys of all
+// pieces of these rows.
 struct Item {
   int tok0, ntok, kv_begin, kv_end;
   int page_base, tile, slot, split;
-  int splits, mixed, pad0, pad1;
+  int splits, mixed, all_begin, all_end;
 };
 static_assert(sizeof(Item) == 48 && sizeof(TokenInfo) == 16, "plan records are int32 words");
 

@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
       }
       if (w.splits == 1) {
         fine = write_out<T>(p, w.tok0 + r / group, kvh * group + r % group, d, v, mm, sum);
-        fine = (fine || !w.mixed) && !(redo >> r & 1);
+        fine |= !w.mixed;
       } else {
         __stcg(reinterpret_cast<float4*>(partial + (slot * 16 + r) * D + d),
                make_float4(v[0], v[1], v[2], v[3]));
@@ -573,7 +573,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewTile<D, Q8, R>::kCtas)
         if (d == 0) __stcg(partial_ml + slot * 16 + r, make_float2(mm, redo >> r & 1 ? -sum : sum));
       }
     }
-    if (w.mixed || redo) redo_rows<T, D, Q8>(p, w, kvh, group, r, fine);
+    if (w.splits == 1 && (w.mixed || redo))
+      redo_rows<T, D, Q8>(p, w, kvh, group, r, fine, u < rows * V4 && (redo >> r & 1));
   }
   if (w.splits == 1) {
     if (beside) pdl_wait();

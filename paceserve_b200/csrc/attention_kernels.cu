@@ -245,8 +245,8 @@ extern "C" int pace_paged_attention_plan(
         w.mixed = mixed;
         w.tok0 = q0 + t0;
         w.ntok = n;
-        w.kv_begin = first;
-        w.kv_end = end;
+        w.kv_begin = w.all_begin = first;
+        w.kv_end = w.all_end = end;
         w.page_base = kv_indptr[b];
         (is_few ? few : many).push_back(w);
         if (is_few) plan->few_rows = std::max(plan->few_rows, n * group);

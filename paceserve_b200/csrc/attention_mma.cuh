@@ -186,8 +186,9 @@ struct Mma<__half> {
 };
 
 // Four outputs of one row from its unnormalised sums, and the row's lse (m in
-// powers of two).  A row that saw nothing (sum 0) is zero.  Returns whether all
-// are finite.
+// powers of two).  A row that saw nothing (sum 0) is zero.  Returns false where a
+// hidden key may have spoilt one: some are infinite or NaN, and the sum, which no
+// hidden key enters, is not.
 template <typename T>
 __device__ __forceinline__ bool write_out(const Problem& p, int64_t tok, int head, int d,
                                           const float (&v)[4], float m, float sum) {
@@ -204,29 +205,73 @@ __device__ __forceinline__ bool write_out(const Problem& p, int64_t tok, int hea
   }
   if (p.lse && d == 0)
     p.lse[tok * p.heads + head] = sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
-  return fabsf(v[0] * inv) + fabsf(v[1] * inv) + fabsf(v[2] * inv) + fabsf(v[3] * inv) < INFINITY;
+  return !(sum < INFINITY) ||
+         fabsf(v[0] * inv) + fabsf(v[1] * inv) + fabsf(v[2] * inv) + fabsf(v[3] * inv) < INFINITY;
 }
 
-// attend_row out of line: it is rarely needed.
-template <typename T, typename KV, int N>
-__device__ __noinline__ void attend_row_again(const Problem& p, int64_t tok, int head) {
-  attend_row<T, KV, N>(p, tok, head);
+// Whether the value row of some key of [begin, end) that this row does not see
+// would spoil a product with 0: an infinity or a NaN in it (of a quantised row, as
+// either kernel may unpack it).  Lane by lane a key.
+template <typename T, bool Q8, int D>
+__device__ bool hidden_spoils(const Problem& p, int64_t tok, int head, int begin, int end) {
+  const TokenInfo info = p.tokens[tok];
+  const uint64_t* bits = p.tree_mask ? p.tree_mask + tok * p.tree_words : nullptr;
+  const int kvh = head / (p.heads / p.kv_heads);
+  const uint8_t* cache = static_cast<const uint8_t*>(p.cache);
+  constexpr int kRowBytes = Q8 ? D : 2 * D;
+  constexpr uint32_t kBad = Q8                                       ? 0x7f7f7f7fu
+                            : std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u
+                                                                    : 0x7c007c00u;
+  for (int j0 = begin; j0 < end; j0 += 32) {
+    const int j = j0 + (int)(threadIdx.x & 31);
+    bool see = j >= info.lo && j < info.hi;
+    if (bits && j >= info.hi) see = j < info.pos && tree_bit(bits, j - info.hi);
+    bool bad = false;
+    if (j < end && !see) {
+      const int64_t page = p.kv_indices[info.page_base + page_number(p, j)];
+      const int64_t row = ((page * 2 + 1) * p.page_size + page_slot(p, j)) * p.kv_heads + kvh;
+      // from 2^119 on a factor may take a code past bf16's range
+      if constexpr (Q8) bad = p.exponents[row] >= 127 + 119;
+#pragma unroll 4
+      for (int c = 0; c < kRowBytes; c += 16) {
+        const uint4 x = ld_v4(cache + row * kRowBytes + c);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          bad |= (Q8 ? __vcmpeq4(w[i] & kBad, kBad) : __vcmpeq2(w[i] & kBad, kBad)) != 0;
+      }
+    }
+    if (__any_sync(0xffffffffu, bad)) return true;
+  }
+  return false;
+}
+
+// A row that came out infinite or NaN, or (`faint`) as too little of what it was
+// scaled for, by attend_row; not where its own keys made it so, which NaN does to
+// whole prompts (8192 such rows and heads took 500 times a finite prompt's time).
+// Out of line: it is rarely needed.
+template <typename T, bool Q8, int D>
+__device__ __noinline__ void attend_row_again(const Problem& p, int64_t tok, int head, int begin,
+                                              int end, bool faint) {
+  if (faint || hidden_spoils<T, Q8, D>(p, tok, head, begin, end))
+    attend_row<T, std::conditional_t<Q8, uint8_t, T>, D / 32>(p, tok, head);
 }
 
 // Redoes rows whose outputs, just written by this warp's lanes (lane u: four
-// columns of row `r`), are not fine: not all finite, or marked as too faint.  The
-// whole warp calls it; lanes without a row pass fine = true.
+// columns of row `r`), are not fine.  The whole warp calls it; lanes without a row
+// pass fine = true.
 template <typename T, int D, bool Q8>
 __device__ __forceinline__ void redo_rows(const Problem& p, const Item& w, int kvh, int group, int r,
-                                          bool fine) {
-  uint32_t bad = __ballot_sync(0xffffffffu, !fine);
+                                          bool fine, bool faint) {
+  uint32_t bad = __ballot_sync(0xffffffffu, !fine || faint);
+  const uint32_t faint_lanes = __ballot_sync(0xffffffffu, faint);
   if (bad) __syncwarp();  // their stores come before the ones below
   constexpr uint32_t kRowLanes = D / 4 >= 32 ? 0xffffffffu : (1u << (D / 4 & 31)) - 1u;
   while (bad) {
     const int first = __ffs(bad) - 1;
     const int row = __shfl_sync(0xffffffffu, r, first);
-    attend_row_again<T, std::conditional_t<Q8, uint8_t, T>, D / 32>(p, w.tok0 + row / group,
-                                                                    kvh * group + row % group);
+    attend_row_again<T, Q8, D>(p, w.tok0 + row / group, kvh * group + row % group, w.all_begin,
+                               w.all_end, faint_lanes >> first & 1);
     bad &= ~(kRowLanes << (first / (D / 4) * (D / 4)));
   }
 }
@@ -317,13 +362,14 @@ __device__ __forceinline__ void join_pieces(const Problem& p, const float* parti
         const int u = u0 + i * NT;
         if ((u & ~31) >= n * V4) break;
         const int r = u / V4;
-        bool fine = true;
+        bool fine = true, faint = false;
         if (u < n * V4) {
           fine = write_out<T>(p, w.tok0 + (r0 + r) / group, kvh * group + (r0 + r) % group,
-                              (u - r * V4) * 4, v[i], top[r], fabsf(total[r]));
-          fine = (fine || !w.mixed) && !(Q8 && total[r] < 0.f);
+                              (u - r * V4) * 4, v[i], top[r], fabsf(total[r])) ||
+                 !w.mixed;
+          faint = Q8 && total[r] < 0.f;
         }
-        if (w.mixed || Q8) redo_rows<T, D, Q8>(p, w, kvh, group, r0 + r, fine);
+        if (w.mixed || Q8) redo_rows<T, D, Q8>(p, w, kvh, group, r0 + r, fine, faint);
       }
     }
     join_sync<NT>();

@@ -643,12 +643,13 @@ __global__ void __launch_bounds__(TileCfg<D, Q8>::kThreads, 1)
                 l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
         }
         if (w.mixed && w.splits == 1) {
-          uint32_t bad = __ballot_sync(0xffffffffu, live && !(size < INFINITY));
+          // not where the sum, which no hidden key enters, is infinite or NaN as well
+          uint32_t bad = __ballot_sync(0xffffffffu, live && l < INFINITY && !(size < INFINITY));
           if (bad) __syncwarp();  // their stores come before the ones below
           for (; bad; bad &= bad - 1) {
             const int at = row - lane + __ffs(bad) - 1;
-            attend_row_again<T, std::conditional_t<Q8, uint8_t, T>, D / 32>(
-                p, w.tok0 + at / group, kvh * group + at % group);
+            attend_row_again<T, Q8, D>(p, w.tok0 + at / group, kvh * group + at % group,
+                                       w.all_begin, w.all_end, false);
           }
         }
       }

@@ -275,3 +275,59 @@ def test_large_caps_beside_a_score_near_them(cap, tokens, hd):
             page, slot = step.ki[int(step.kp[b]) + j // 16], j % 16
             step.cache[page, 0, slot, :, 0] = -0.5 * cap / 8 * math.sqrt(hd)
     step.check(logits_soft_cap=cap)
+
+
+def test_infinite_and_nan_rows_cost_what_others_do():
+    """Rows that are not finite by what they see are not done again on the CUDA cores: NaN queries
+    and keys, and an infinite value that all rows but the first see."""
+    step = Step([(2048, 2048)], 32, 8, 128, seed=26)
+    attn = PagedAttention(32, 8, 128, 16, DEV)
+    attn.begin_forward(step.qp, step.kp, step.ki, step.kl)
+    query, cache = step.query.to(DEV), step.cache.to(DEV)
+
+    def ms(q, c):
+        times = []
+        for _ in range(5):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            attn.forward(q, c)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    base = ms(query, cache)
+    nan_query = query.clone()
+    nan_query[:] = math.nan
+    nan_key, inf_value = cache.clone(), cache.clone()
+    nan_key[step.ki[0], 0, 0] = math.nan
+    inf_value[step.ki[0], 1, 1] = math.inf
+    for q, c in ((nan_query, cache), (query, nan_key), (query, inf_value)):
+        assert ms(q, c) < 20 * base  # 500 times and more where every row was done again
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("lens", [[(1, 300), (4, 40)], [(90, 300), (300, 300)], [(70, 6000), (2, 9000)]])
+def test_values_not_finite_where_seen(hd, quantised, lens):
+    """An infinite (or, quantised, a NaN) value row in each sequence: seen by the later tokens,
+    whose outputs are not finite, hidden from the others, whose outputs are as without it."""
+    step = Step(lens, 8, 2, hd, quantised=quantised, seed=27, spread=0.3)
+    at = [max(n - q + q // 2, 0) for q, n in lens]
+    for b, j in enumerate(at):
+        page, slot = step.ki[int(step.kp[b]) + j // 16], j % 16
+        if quantised:
+            step.exponents[page, 1, slot] = 255
+            step.cache[page, 1, slot] = 0
+        else:
+            step.cache[page, 1, slot, :, ::3] = math.inf
+    got, _ = step.run()
+    out, _, _ = step.want()
+    assert torch.equal(got.isfinite(), out.isfinite()) and bool(got.isfinite().any())
+    assert not bool(got.isfinite().all())
+    hidden = torch.cat([torch.arange(n - q, n) < j for (q, n), j in zip(lens, at)])
+    clean = Step(lens, 8, 2, hd, quantised=quantised, seed=27, spread=0.3)
+    out, _, size = clean.want()
+    u = U[torch.bfloat16]
+    err = (got.double() - out).abs()
+    assert bool((err <= u * out.abs() + (u + 4e-4) * size)[hidden].all())
