@@ -200,7 +200,8 @@ extern "C" int pace_paged_attention_plan(
     return fail(PACE_ERR_INVALID_ARGUMENT, "%s: the plan needs %lld words", what,
                 (long long)plan_capacity(batch_size, total_q, num_kv_indices, num_sms));
   int32_t max_page = -1;
-  for (int64_t i = 0; i < num_kv_indices; ++i) {
+  // the requests' entries; what lies before and behind them is not read
+  for (int64_t i = kv_indptr[0]; i < kv_indptr[batch_size]; ++i) {
     if (kv_indices[i] < 0)
       return fail(PACE_ERR_INVALID_ARGUMENT, "%s: negative page in kv_indices", what);
     max_page = std::max(max_page, kv_indices[i]);

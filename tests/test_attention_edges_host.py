@@ -1,6 +1,7 @@
 """CPU: what paged attention plans and refuses where arguments are at an edge."""
 import ctypes
 
+import pytest
 import torch
 
 from paceserve_b200 import attention_ops, cabi
@@ -47,3 +48,26 @@ def test_every_piece_of_a_tree_may_hide_keys():
         items = [plan.words[at + 12 * i:at + 12 * i + 12].tolist()
                  for i in range(plan.num_few + plan.num_many)]
         assert len(items) == 2 and all(w[9] == 1 for w in items)
+
+
+def test_entries_of_no_request_are_not_looked_at():
+    """kv_indices of a fixed size, filled up with -1 or whatever was there: only the entries
+    between the first and the last kv_indptr name pages."""
+    ints32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    call = attention_ops.plan_paged_attention
+    rest = (ints32(5, 16), 8, 2, 128, 16)
+    plan = call(ints32(0, 1, 4), ints32(1, 3, 5), ints32(-1, 0, 7, 2, 3, -1, 1 << 30), *rest)
+    assert plan.words.tolist()[-7:] == [-1, 0, 7, 2, 3, -1, 1 << 30]
+    for bad in (1, 4):
+        indices = ints32(-1, 0, 7, 2, 3, -1, 1 << 30)
+        indices[bad] = -1
+        with pytest.raises(RuntimeError, match="negative page"):
+            call(ints32(0, 1, 4), ints32(1, 3, 5), indices, *rest)
+    lib = cabi.load()
+    c_plan = cabi.AttentionPlan()
+    n = lib.pace_paged_attention_plan_words(1, 1, 3, 148)
+    words = (ctypes.c_int32 * n)()
+    assert lib.pace_paged_attention_plan(ctypes.byref(c_plan), words, n, ints(0, 1), ints(0, 1),
+                                         ints(4, -1, 99), 3, ints(2), 1, 8, 2, 128, 16, -1, None, None,
+                                         0, 148) == cabi.PACE_OK
+    assert c_plan.max_page == 4
