@@ -39,7 +39,9 @@ class PagedAttention:
 
     The plan, its copy on the device and the workspace belong to the object: a
     new ``begin_forward`` replaces them, and calls of ``forward`` that may
-    overlap on the GPU (several streams) need an object each.
+    overlap on the GPU (several streams) need an object each.  A step that ran
+    while a CUDA graph was captured is kept as long as the object, which has to
+    outlive the graph.
     """
 
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
@@ -59,6 +61,7 @@ class PagedAttention:
         self._workspace = torch.zeros(0, dtype=torch.uint8, device=device)
         self._fault = torch.zeros(1, dtype=torch.int32, device=device)
         self._step = None
+        self._captured = []  # steps whose memory a CUDA graph reads
         self.plan = None
 
     def begin_forward(self, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, *,
@@ -90,6 +93,8 @@ class PagedAttention:
 
     def _begin(self, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, *, window_left=-1,
                prefix_lens=None, doc_starts=None, tree_mask=None) -> None:
+        if self._step is not None and self._step.captured:
+            self._captured.append(self._step)
         self._step = self.plan = None
         plan = attention_ops.plan_paged_attention(
             _host_ints(qo_indptr), _host_ints(kv_indptr), _host_ints(kv_indices),

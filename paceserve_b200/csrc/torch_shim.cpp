@@ -1134,6 +1134,7 @@ struct AttentionStep {
   c10::optional<Tensor> tree_mask;
   cudaStream_t stream;
   at::cuda::CUDAEvent ready;
+  bool captured = false;  // a CUDA graph holds the addresses of all three
 
   AttentionStep(const AttentionPlan& p, const Tensor& w, const Tensor& ws,
                 const c10::optional<Tensor>& mask)
@@ -1151,11 +1152,11 @@ struct AttentionStep {
                  const c10::optional<Tensor>& lse, const c10::optional<Tensor>& fault_flags) {
     check_cuda(query, "paged_attention", "query");
     const auto cur = at::cuda::getCurrentCUDAStream(query.device().index());
-    if (cur.stream() != stream && query.device() == words.device() &&
-        at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) {
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
+      captured = true;  // with the GPU idle; the step has to outlive the graph
+    } else if (cur.stream() != stream && query.device() == words.device()) {
       // another stream than the plan's: its copy to the device comes first, and its memory is
-      // kept from reuse until this stream is done with it.  A graph keeps to neither: it is
-      // captured with the GPU idle, and the step has to outlive it.
+      // kept from reuse until this stream is done with it
       ready.block(cur);
       words.record_stream(cur);
       workspace.record_stream(cur);
@@ -1326,6 +1327,7 @@ PYBIND11_MODULE(_C, m) {
                     const c10::optional<Tensor>&>(),
            py::arg("plan"), py::arg("words"), py::arg("workspace"),
            py::arg("tree_mask") = py::none())
+      .def_readonly("captured", &AttentionStep::captured)
       .def("forward", &AttentionStep::forward, py::arg("query"), py::arg("paged_kv_cache"),
            py::arg("exponents"), py::arg("sm_scale"), py::arg("logits_soft_cap"),
            py::arg("alibi_slopes"), py::arg("out"), py::arg("lse"), py::arg("fault_flags"));

@@ -331,3 +331,40 @@ def test_values_not_finite_where_seen(hd, quantised, lens):
     u = U[torch.bfloat16]
     err = (got.double() - out).abs()
     assert bool((err <= u * out.abs() + (u + 4e-4) * size)[hidden].all())
+
+
+def test_a_graph_outlives_the_plan_it_was_captured_with():
+    """Later steps on the same object, and whatever then takes freed memory, leave the captured
+    step's plan, workspace and tree mask as they were."""
+    step = Step([(1, 3000), (9, 4000), (40, 2000)], 8, 2, 128, seed=28)
+    mask = random_trees(step.lens, 1)
+    attn = PagedAttention(8, 2, 128, 16, DEV)
+    cache, q = step.cache.to(DEV), step.query.to(DEV)
+    for kw in ({}, {"tree": True}):
+        if kw:
+            attn.begin_tree_forward(step.qp, step.kp, step.ki, step.kl, mask)
+        else:
+            attn.begin_forward(step.qp, step.kp, step.ki, step.kl)
+        assert attn.plan.few_slots > 0 and attn.plan.many_slots > 0
+        want = attn.forward(q, cache)
+        torch.cuda.synchronize()
+        out = torch.zeros_like(want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            attn.forward(q, cache, out=out)
+        kept = attn._step
+        for n in (20000, 30000):  # needs a larger workspace
+            other = Step([(70, n), (1, 40)], 8, 2, 128, seed=29)
+            attn.begin_forward(other.qp, other.kp, other.ki, other.kl)
+            attn.forward(other.query.to(DEV), other.cache.to(DEV))
+        assert kept in attn._captured
+        del kept
+        filler = [torch.full((k,), -1, dtype=torch.uint8, device=DEV)
+                  for k in (512, 2048, 8192, 1 << 20, 1 << 22, 1 << 24) for _ in range(4)]
+        torch.cuda.synchronize()
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        del filler, graph
