@@ -86,7 +86,8 @@ class PagedAttention:
         already appended to its sequence, and token t sees the sequence before
         them and those drafted tokens k of its own request whose bit k of
         ``tree_mask[t]`` is set (its ancestors and itself).  ``tree_mask``:
-        int64 [tokens, words], 64 drafted tokens a word."""
+        int64 [tokens, words], 64 drafted tokens a word; on the host it may be
+        changed afterwards, on the GPU the step reads it as it is."""
         if tree_mask.dim() != 2 or tree_mask.dtype != torch.int64 or tree_mask.shape[1] == 0:
             raise RuntimeError("begin_tree_forward: tree_mask must be int64 [tokens, words]")
         self._begin(qo_indptr, kv_indptr, kv_indices, kv_last_page_len, tree_mask=tree_mask)
@@ -110,6 +111,8 @@ class PagedAttention:
                 self._workspace = torch.zeros(plan.workspace_bytes, dtype=torch.uint8,
                                               device=self.device)
             if tree_mask is not None:
+                if tree_mask.is_pinned():  # its copy would read the caller's memory later
+                    tree_mask = torch.empty(tree_mask.shape, dtype=torch.int64).copy_(tree_mask)
                 tree_mask = tree_mask.to(self.device, non_blocking=True).contiguous()
             self._step = attention_ops.AttentionStep(
                 plan, plan.words.to(self.device, non_blocking=True), self._workspace, tree_mask)

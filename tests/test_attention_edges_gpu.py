@@ -368,3 +368,19 @@ def test_a_graph_outlives_the_plan_it_was_captured_with():
             torch.cuda.synchronize()
             assert torch.equal(out, want)
         del filler, graph
+
+
+def test_a_page_locked_tree_mask_may_be_written_again():
+    """The engine fills the same page-locked buffer for the next step while the GPU is behind."""
+    step = Step([(40, 300), (3, 90)], 8, 2, 128, seed=30)
+    mask = random_trees(step.lens, 1)
+    want, _ = step.run(tree_mask=mask)
+    host = mask.clone().pin_memory()
+    attn = PagedAttention(8, 2, 128, 16, DEV)
+    cache, q = step.cache.to(DEV), step.query.to(DEV)
+    for _ in range(3):
+        host.copy_(mask)
+        torch.cuda._sleep(200_000_000)
+        attn.begin_tree_forward(step.qp, step.kp, step.ki, step.kl, host)
+        host.zero_()
+        assert torch.equal(attn.forward(q, cache).cpu(), want)
