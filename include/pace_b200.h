@@ -540,7 +540,7 @@ int pace_paged_attention_plan(pace_attention_plan* plan, int32_t* words, int64_t
                               int tree_words, int num_sms);
 
 /* Runs a plan.  query and out: [total_q, heads, head_dim] of `dtype`, heads
- * contiguous, token strides in elements.  cache: the paged cache of `dtype`, or
+ * contiguous, token strides in elements; they must not overlap.  cache: the paged cache of `dtype`, or
  * with `exponents` the codes of a quantised one.  lse ([total_q, heads], may be
  * NULL) receives the natural log of each row's sum of e^s (-inf where nothing is
  * visible).  workspace: plan.workspace_bytes bytes, 32-byte aligned, zeroed once by the caller

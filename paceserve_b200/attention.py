@@ -126,10 +126,11 @@ class PagedAttention:
         """One layer's attention: ``query`` [tokens, num_heads, head_dim] (token
         rows may be strided views of the qkv projection) over the layer's cache
         [pages, 2, page_size, num_kv_heads, head_dim], or over a quantised
-        cache's codes with its ``exponents``.  ``lse`` (float32 [tokens,
-        num_heads]) receives each row's log-sum-exp.  Every wait in the kernels
-        is bounded; one that runs out sets bit 30 of ``fault_flags`` (int32 on
-        the device), or of the object's own flag, which ``check`` reads."""
+        cache's codes with its ``exponents``.  ``out`` must not overlap the
+        query.  ``lse`` (float32 [tokens, num_heads]) receives each row's
+        log-sum-exp.  Every wait in the kernels is bounded; one that runs out
+        sets bit 30 of ``fault_flags`` (int32 on the device), or of the object's
+        own flag, which ``check`` reads."""
         if self._step is None:
             raise RuntimeError("PagedAttention.forward: begin_forward has not planned a step")
         return self._step.forward(query, paged_kv_cache, exponents,

@@ -345,6 +345,9 @@ extern "C" int pace_paged_attention(const pace_attention_plan* plan, const int32
                  (reinterpret_cast<uintptr_t>(workspace) & 31) != 0))
     return fail(PACE_ERR_INVALID_ARGUMENT, "%s: the plan needs %zu bytes of 32-byte aligned "
                 "workspace", what, plan->workspace_bytes);
+  // a row that is done again reads its query once more
+  if (out == query)
+    return fail(PACE_ERR_INVALID_ARGUMENT, "%s: out must not be the query", what);
   StreamDeviceGuard guard(stream);
   if (tensor) {
     const Workspace ws = workspace_of(*plan);

@@ -384,3 +384,13 @@ def test_a_page_locked_tree_mask_may_be_written_again():
         attn.begin_tree_forward(step.qp, step.kp, step.ki, step.kl, host)
         host.zero_()
         assert torch.equal(attn.forward(q, cache).cpu(), want)
+
+
+def test_output_over_the_query_is_refused():
+    step = Step([(1, 30)], 8, 2, 128)
+    attn = PagedAttention(8, 2, 128, 16, DEV)
+    attn.begin_forward(step.qp, step.kp, step.ki, step.kl)
+    q = step.query.to(DEV)
+    with pytest.raises(RuntimeError, match="out must not be the query"):
+        attn.forward(q, step.cache.to(DEV), out=q)
+    assert torch.equal(q.cpu(), step.query)
