@@ -3,8 +3,9 @@
 // drafts).  Every key and value is read once for so few products that memory
 // bounds it: the 16 x 8 x 16 matrix instructions of a warp are enough, and
 // what counts is the bytes in flight.  64 single tokens of 32 heads over up to
-// 8191 bf16 tokens each (1.2 GB) take 197 us, 6.0 TB/s, 93 % of a copy's rate; over
-// a quantised cache (597 MB) 149 us, 4.0 TB/s, where unpacking the codes bounds it.
+// 8191 bf16 tokens each (1.2 GB) take 182 us, 6.5 TB/s, a copy's rate; over a
+// quantised cache (597 MB) 166 us, 3.6 TB/s, where unpacking the codes bounds it
+// (a single call alone: 147).  Distance bias adds 2 and 10 us.
 //
 // A CTA takes one piece of the plan (keys [kv_begin, kv_end) of one request)
 // for one kv head.  Its four warps walk the keys in turns of KEYS each, every
@@ -23,7 +24,7 @@
 // code moved to the top of 16 bits is its value times 2^-8 as fp16 holds it,
 // subnormals included, and no multiplication touches it.  Every other word goes by
 // the conversion instruction instead, which runs on another unit (all by it: 238 us
-// for the 64 requests, all by shifts: 170, half and half: 166 then, 149 now).
+// for the 64 requests, all by shifts: 170, half and half: 166 then, 147 now).
 // K's factor multiplies the scores.  V's factor 2^e goes into P: the output has a
 // running maximum of its own, of score + e, and is built from 2^(score + e - it), so
 // that the row's largest contribution is about 1 in fp16 whatever the factors are;

@@ -25,8 +25,9 @@
 // What bounds it is the chain of a tile's step (scores out of TMEM, maximum,
 // exponentials, P into TMEM, its product, the next scores): 3870 cycles for a step
 // of both tiles, whose MMAs take about 2300.  One 8192-token prompt of 32 / 8 heads
-// of 128, causal: 510 us, 1.08 PFLOP/s, 0.64 of cuBLAS's measured rate; with capped
-// scores 631 us, with distance bias 641, over a quantised cache 677.
+// of 128, causal: 493 us in short runs, 1.12 PFLOP/s, 0.66 of cuBLAS's measured burst
+// rate (570 us in long runs, under the power cap); with capped scores or distance
+// bias 610 to 645 us (672), over a quantised cache 690 (703).
 #include "attention_mma.cuh"
 #include "tcgen05.cuh"
 

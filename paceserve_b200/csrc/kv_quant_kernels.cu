@@ -179,9 +179,9 @@ __device__ __forceinline__ Place place_of(int per_token) {
 // -> page lookups, which the first threads do for all batches: the lookups are
 // two loads that depend on each other, and with CTAs of one batch they were most
 // of the time.  What bounds it is the loads in flight: 16167 fp16 tokens (103.6
-// MB) take 25.4 us, 4.1 TB/s, in batches of two tokens with six CTAs an SM; 31 us
+// MB) take 25.6 us, 4.1 TB/s, in batches of two tokens with six CTAs an SM; 31 us
 // in batches of four with four, 28 us in batches of one with eight, 39 us with one
-// batch of four a CTA.
+// batch of four a CTA.  As float32 (172.5 MB) they take 44 us.
 template <typename T, int U, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     kv_quant_append_kernel(const T* __restrict__ key, const T* __restrict__ value,
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads)
       load(next, t0 + each);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-          uint2 code;
+        uint2 code;
         const uint32_t ex = quantise8<T>(raw[k].v, group, code);
         const int t = t0 + k * at.side + at.sub;
         const int64_t where = mine && t < ntok ? s_slot[t] : -1;
