@@ -94,6 +94,10 @@ class PagedAttention:
 
     def _begin(self, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, *, window_left=-1,
                prefix_lens=None, doc_starts=None, tree_mask=None) -> None:
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("PagedAttention: plan the step before the CUDA graph is captured: "
+                                   "a replay would copy the plan from host memory of this call")
         if self._step is not None and self._step.captured:
             self._captured.append(self._step)
         self._step = self.plan = None

@@ -394,3 +394,20 @@ def test_output_over_the_query_is_refused():
     with pytest.raises(RuntimeError, match="out must not be the query"):
         attn.forward(q, step.cache.to(DEV), out=q)
     assert torch.equal(q.cpu(), step.query)
+
+
+def test_planning_during_a_capture_is_refused():
+    step = Step([(1, 300)], 8, 2, 128, seed=32)
+    attn = PagedAttention(8, 2, 128, 16, DEV)
+    attn.begin_forward(step.qp, step.kp, step.ki, step.kl)
+    cache, q = step.cache.to(DEV), step.query.to(DEV)
+    want = attn.forward(q, cache)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before the CUDA graph"):
+            attn.begin_forward(step.qp, step.kp, step.ki, step.kl)
+        out = attn.forward(q, cache)  # the step planned before
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
