@@ -494,6 +494,136 @@ int pace_read_quantised_paged_kv_cache(void* key, void* value, int64_t rows, int
                                        int64_t batch_size, int32_t* bad_tokens, int dtype,
                                        cudaStream_t stream);
 
+/* ---- step tables ----------------------------------------------------------
+ * Block tables and index arrays of a step on the device, from the requests'
+ * lengths (the host's work at flashinfer_attention_wrapper.py:75-209).
+ *
+ * Request b (at most 8192 of them) holds seq_lens[b] tokens on the first
+ * ceil(seq_lens[b] / page_size) pages of its row of block_tables [num_requests,
+ * max_blocks] and gets new_lens[b] >= 0 more.  New pages are taken from the top
+ * of the stack free_pages[0 .. *free_count), in the requests' order: the k-th is
+ * free_pages[*free_count - 1 - k]; block_tables and *free_count are updated.
+ * Written: append_indptr, kv_indptr [num_requests + 1], kv_indices (room for
+ * num_kv_indices; what is past the last page stays), kv_last_page_len
+ * (page_size for a request without tokens), and for each new token its request,
+ * position and slot = page * page_size + place; token entries past the last, up
+ * to num_tokens, become -1.
+ *
+ * If something does not fit, a PACE_TABLES_* bit is set in *status, block_tables
+ * and the stack stay as they are, the indptr arrays and kv_last_page_len become
+ * 0 and all token entries -1, so that no later kernel writes to a page by them.
+ * *arrivals: a word of the caller's, zero, left zero; calls that share it, the
+ * tables or the stack must not overlap.  Page numbers are not looked at.
+ *
+ * pace_release_pages: request b keeps the pages of its first kept_lens[b] of
+ * held_lens[b] tokens and the others go back onto the stack, so that taking and
+ * releasing the same pages leaves it as it was.  block_tables is only read. */
+#define PACE_TABLES_BAD_LENGTH 1    /* negative, or more kept than held          */
+#define PACE_TABLES_SHORT_ROW 2     /* a request needs more than max_blocks      */
+#define PACE_TABLES_SHORT_INDICES 4 /* more pages than num_kv_indices            */
+#define PACE_TABLES_SHORT_TOKENS 8  /* more new tokens than num_tokens           */
+#define PACE_TABLES_NO_PAGES 16     /* the stack has too few pages (or no room)  */
+int pace_build_step_tables(int32_t* block_tables, int64_t table_row_stride, int64_t max_blocks,
+                           const int32_t* seq_lens, const int32_t* new_lens, int64_t num_requests,
+                           int64_t page_size, int32_t* free_pages, int64_t num_free_pages,
+                           int32_t* free_count, int32_t* append_indptr, int32_t* kv_indptr,
+                           int32_t* kv_indices, int64_t num_kv_indices, int32_t* kv_last_page_len,
+                           int32_t* batch_indices, int64_t* positions, int64_t* slot_mapping,
+                           int64_t num_tokens, int32_t* status, int32_t* arrivals,
+                           cudaStream_t stream);
+int pace_release_pages(const int32_t* block_tables, int64_t table_row_stride, int64_t max_blocks,
+                       const int32_t* held_lens, const int32_t* kept_lens, int64_t num_requests,
+                       int64_t page_size, int32_t* free_pages, int64_t num_free_pages,
+                       int32_t* free_count, int32_t* status, int32_t* arrivals,
+                       cudaStream_t stream);
+
+/* ---- 8-bit projections ----------------------------------------------------
+ * Rows as signed 8-bit integers with a scale each:
+ *   scales[t] = max(max_k |y[t, k]| / 127, 2^-126),
+ *   codes[t, k] = y[t, k] / scales[t] to the nearest integer, ties to even;
+ * a row with an infinity or a NaN gets the scale NaN and codes 0.  y is
+ *   pace_quantise_rows: input [rows, width] (activations, or a weight at load);
+ *   pace_rms_norm_quantise: r * rsqrt(mean r^2 + epsilon) * weight, where r is
+ *     input, or (T)(input + residual), which replaces residual (may be NULL);
+ *   pace_silu_and_mul_quantise: silu(input[:, :d]) * input[:, d:], codes [T, d].
+ * In fp32 throughout: y is not rounded to T, as rms_norm's and silu_and_mul's
+ * outputs are (layernorm_kernels.cu:33, activation_kernels.cu:8-25). */
+int pace_quantise_rows(int8_t* codes, float* scales, const void* input, int64_t rows,
+                       int64_t width, int64_t input_row_stride, int64_t codes_row_stride,
+                       int dtype, cudaStream_t stream);
+int pace_rms_norm_quantise(int8_t* codes, float* scales, const void* input, void* residual,
+                           const void* weight, float epsilon, int64_t num_tokens,
+                           int64_t hidden_size, int64_t input_row_stride,
+                           int64_t residual_row_stride, int64_t codes_row_stride, int dtype,
+                           cudaStream_t stream);
+int pace_silu_and_mul_quantise(int8_t* codes, float* scales, const void* input,
+                               int64_t num_tokens, int64_t d, int64_t input_row_stride,
+                               int64_t codes_row_stride, int dtype, cudaStream_t stream);
+
+/* Products of such rows with a weight quantised row by row (out_features or
+ * 2 * intermediate_size rows of k codes, a scale each):
+ *   y[t, n] = (sum_k codes[t, k] * weight[n, k]) * token_scales[t] * channel_scales[n]
+ * with the sum exact in 32 bits (k at most 131071) and the rest in fp32.
+ *   pace_int8_linear: out = (T)(y + bias + residual); bias [out_features] and
+ *     residual may be NULL, and residual may be out (the projections at
+ *     llama.py:101-106, 176-178, 240-254).
+ *   pace_int8_gate_up_silu: out[t, i] = (T)(silu(y[t, i]) * y[t, I + i]), as
+ *     pace_gate_up_silu.
+ * Out and residual are of `dtype`.  Workspace: 16-byte aligned, of
+ * pace_int8_linear_workspace_size bytes (gated: 1 for gate_up_silu; 0 bytes:
+ * NULL will do), its first 4096 bytes zero before the first call; calls leave
+ * them zero, and calls that may overlap need one each.  On the tensor cores
+ * where k, the row strides and the addresses of codes and weight are multiples
+ * of 16 bytes, on the CUDA cores (slowly, without a workspace) otherwise.  Every
+ * wait in the kernel is bounded by a second; one that runs out sets bit 30 of
+ * *fault_flags, leaves the output undefined, and the workspace to be zeroed. */
+size_t pace_int8_linear_workspace_size(int64_t num_tokens, int64_t out_features, int64_t k,
+                                       int gated, int device);
+int pace_int8_linear(void* out, const int8_t* codes, const float* token_scales,
+                     const int8_t* weight, const float* channel_scales, const void* bias,
+                     const void* residual, int64_t num_tokens, int64_t out_features, int64_t k,
+                     int64_t codes_row_stride, int64_t weight_row_stride, int64_t out_row_stride,
+                     int64_t residual_row_stride, int dtype, void* workspace,
+                     size_t workspace_bytes, int32_t* fault_flags, cudaStream_t stream);
+int pace_int8_gate_up_silu(void* out, const int8_t* codes, const float* token_scales,
+                           const int8_t* weight, const float* channel_scales, int64_t num_tokens,
+                           int64_t intermediate_size, int64_t k, int64_t codes_row_stride,
+                           int64_t weight_row_stride, int64_t out_row_stride, int dtype,
+                           void* workspace, size_t workspace_bytes, int32_t* fault_flags,
+                           cudaStream_t stream);
+
+/* ---- head norms with rotation ---------------------------------------------
+ * pace_qk_norm_rotary_embedding: every head x of query and key (head_size
+ *   dimensions) becomes rope(x * rsqrt(mean x^2 + epsilon) * w), w = q_weight or
+ *   k_weight [head_size], in place; rotation, cos_sin_cache and positions as
+ *   for pace_rotary_embedding (pos_encoding_kernels.cu:8-76), dimensions past
+ *   rot_dim only normalised.  In fp32, rounded once.  A token whose position is
+ *   outside [0, max_position) stays as it is.
+ * pace_qk_norm_rotary_append: query in place; key's result, and value as it is,
+ *   go to slot slot_mapping[t] of a paged cache [num_pages, 2, page_size,
+ *   num_kv_heads, head_size] (page slot / page_size, K then V); key and value
+ *   are only read.  Slot -1 leaves the token out of the cache; any other slot
+ *   outside it, and a slot of a token whose position is outside the table, is
+ *   counted into *bad_tokens (may be NULL) and left out.  No two tokens may have
+ *   the same slot.
+ * No reference kernel; RMSNorm per head, rotary_embedding and the append in one. */
+int pace_qk_norm_rotary_embedding(const int64_t* positions, void* query, void* key,
+                                  const void* q_weight, const void* k_weight, float epsilon,
+                                  int64_t num_tokens, int num_heads, int num_kv_heads,
+                                  int head_size, int64_t query_row_stride,
+                                  int64_t key_row_stride, const void* cos_sin_cache,
+                                  int cache_dtype, int rot_dim, int64_t max_position,
+                                  int is_neox, int dtype, cudaStream_t stream);
+int pace_qk_norm_rotary_append(const int64_t* positions, void* query, const void* key,
+                               const void* value, const void* q_weight, const void* k_weight,
+                               float epsilon, int64_t num_tokens, int num_heads, int num_kv_heads,
+                               int head_size, int64_t query_row_stride, int64_t key_row_stride,
+                               int64_t value_row_stride, const void* cos_sin_cache,
+                               int cache_dtype, int rot_dim, int64_t max_position, int is_neox,
+                               void* paged_cache, int64_t num_pages, int page_size,
+                               const int64_t* slot_mapping, int32_t* bad_tokens, int dtype,
+                               cudaStream_t stream);
+
 /* ---- paged attention ------------------------------------------------------
  * Attention of each request's newest tokens over its paged sequence.  For query
  * token i of a request (position p = kv_len - q_len + i), head h and key j

@@ -36,9 +36,10 @@ activation_ops = _C.activation_ops
 moe_ops = _C.moe_ops
 kv_transfer_ops = _C.kv_transfer_ops
 attention_ops = _C.attention_ops
+int8_ops = _C.int8_ops
 
 for _name in ("layernorm_ops", "pos_encoding_ops", "activation_ops", "moe_ops", "kv_transfer_ops",
-              "attention_ops"):
+              "attention_ops", "int8_ops"):
     sys.modules[f"{__name__}.{_name}"] = getattr(_C, _name)
 
 LIBRARY_PATH = os.path.join(_HERE, "libpace_b200.so")
@@ -60,6 +61,16 @@ def fold_rmsnorm_weight(linear_weight, norm_weight):
     (``pos_encoding_ops.qkv_proj_rmsnorm_rotary_embedding``).  Prepared once per
     model load."""
     return (linear_weight.float() * norm_weight.float()[None, :]).to(linear_weight.dtype).contiguous()
+
+
+def quantise_weight(weight):
+    """A linear weight [n, k] on the GPU as 8-bit integers with a scale for each
+    output channel, (codes, channel_scales), for ``int8_ops.linear``,
+    ``linear_residual`` and ``gate_up_silu``.  Prepared once per model load."""
+    codes = torch.empty(weight.shape, dtype=torch.int8, device=weight.device)
+    scales = torch.empty(weight.shape[0], dtype=torch.float32, device=weight.device)
+    int8_ops.quantise_rows(codes, scales, weight)
+    return codes, scales
 
 
 def install_as_paceserve() -> None:
@@ -92,6 +103,8 @@ __all__ = [
     "moe_ops",
     "kv_transfer_ops",
     "attention_ops",
+    "int8_ops",
+    "quantise_weight",
     "install_as_paceserve",
     "fold_rmsnorm_weight",
     "set_pdl",

@@ -4,8 +4,8 @@ Outputs, next to this file:
   * ``libpace_b200.so`` -- the C-ABI library (every kernel, ``include/pace_b200.h``),
     compiled with nvcc for ``sm_100a`` and linked against the static CUDA runtime;
   * ``_C.so`` -- the torch extension (pybind modules layernorm_ops, pos_encoding_ops,
-    activation_ops, moe_ops, kv_transfer_ops, attention_ops) that validates tensors and calls
-    the C ABI; it links ``libpace_b200.so`` through ``$ORIGIN``.
+    activation_ops, moe_ops, kv_transfer_ops, attention_ops, int8_ops) that validates tensors
+    and calls the C ABI; it links ``libpace_b200.so`` through ``$ORIGIN``.
 
 Objects go to ``<repo>/_build``.  Steps whose outputs are newer than every
 input are skipped.  Run ``python paceserve_b200/build.py`` (or
@@ -54,6 +54,10 @@ CUDA_SOURCES = [
     "attention_tile_kernels.cu",
     "gemm_rope_kernels.cu",
     "moe_gemm_kernels.cu",
+    "int8_quant_kernels.cu",
+    "int8_gemm_kernels.cu",
+    "qk_norm_rope_kernels.cu",
+    "step_tables_kernels.cu",
 ]
 
 

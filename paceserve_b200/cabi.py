@@ -24,6 +24,8 @@ PACE_U8, PACE_I8, PACE_I16, PACE_I32, PACE_I64 = 3, 4, 5, 6, 7
 PACE_IPC_HANDLE_BYTES = 64
 PACE_KV_TIMEOUT_FLAG = 1 << 30
 PACE_KV_DRAIN_TIMEOUT_FLAG = 1 << 29
+PACE_TABLES_BAD_LENGTH, PACE_TABLES_SHORT_ROW, PACE_TABLES_SHORT_INDICES = 1, 2, 4
+PACE_TABLES_SHORT_TOKENS, PACE_TABLES_NO_PAGES = 8, 16
 
 
 class KvCopyOpts(ctypes.Structure):
@@ -164,6 +166,44 @@ SIGNATURES: dict[str, tuple] = {
         c_int,
         [POINTER(AttentionPlan), _P, _P, _P, c_int64, c_int64, _P, _P, c_int64, c_float, c_float,
          _P, _P, _P, _P, c_size_t, _P, c_int, _P],
+    ),
+    "pace_build_step_tables": (
+        c_int,
+        [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, _P, c_int64, _P, _P, _P, _P, c_int64, _P,
+         _P, _P, _P, c_int64, _P, _P, _P],
+    ),
+    "pace_release_pages": (
+        c_int,
+        [_P, c_int64, c_int64, _P, _P, c_int64, c_int64, _P, c_int64, _P, _P, _P, _P],
+    ),
+    "pace_quantise_rows": (
+        c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int, _P]),
+    "pace_rms_norm_quantise": (
+        c_int,
+        [_P, _P, _P, _P, _P, c_float, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, _P],
+    ),
+    "pace_silu_and_mul_quantise": (
+        c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int, _P]),
+    "pace_int8_linear_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
+    "pace_int8_linear": (
+        c_int,
+        [_P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+         c_int, _P, c_size_t, _P, _P],
+    ),
+    "pace_int8_gate_up_silu": (
+        c_int,
+        [_P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, _P,
+         c_size_t, _P, _P],
+    ),
+    "pace_qk_norm_rotary_embedding": (
+        c_int,
+        [_P, _P, _P, _P, _P, c_float, c_int64, c_int, c_int, c_int, c_int64, c_int64, _P, c_int,
+         c_int, c_int64, c_int, c_int, _P],
+    ),
+    "pace_qk_norm_rotary_append": (
+        c_int,
+        [_P, _P, _P, _P, _P, _P, c_float, c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int64,
+         _P, c_int, c_int, c_int64, c_int, _P, c_int64, c_int, _P, _P, c_int, _P],
     ),
     "pace_enable_peer_access": (c_int, [c_int, c_int]),
     "pace_can_access_peer": (c_int, [c_int, c_int, POINTER(c_int)]),

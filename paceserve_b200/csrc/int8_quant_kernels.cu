@@ -1,0 +1,322 @@
+// Rows as 8-bit integers with a scale each, for sm_100a: of a tensor, of an
+// RMSNorm (with the residual added first), or of SiLU-and-mul.
+//
+//   scale_t = max(max_k |y_tk| / 127, 2^-126),   code_tk = rint(y_tk / scale_t)
+//   y = x;   y = r * rsqrt(mean r^2 + eps) * w with r = (T)(x + residual);   y = silu(g) * u
+//
+// y is fp32 and is never rounded to T: the code's half step is the one rounding
+// (and r's, since r is the residual stream that the next layer reads).  A row
+// with an infinity or a NaN in y has no scale: its scale is NaN and its codes 0,
+// so that all that is computed from it is NaN.
+//
+// The quotient is rounded as IEEE division gives it, without a division for
+// each element: y * (1 / scale) is off by less than 2^-15 at 127, so only where
+// it falls within 1e-4 of a half step can the nearest integer be another, and
+// there (one element in 5000) the division is done.
+//
+// Memory bounds it: a row is read once with 16-byte vectors, held in registers
+// over the one or two reductions, and stored as 8-byte groups of codes.
+#include "common.cuh"
+
+namespace pace {
+namespace {
+
+enum Source { kRows, kNorm, kAddNorm, kSilu };
+constexpr int kMaxThreads = 512;
+constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126
+
+struct QuantJob {
+  int8_t* codes;
+  float* scales;
+  const void* x;
+  void* residual;      // kAddNorm
+  const void* weight;  // kNorm, kAddNorm
+  float eps;
+  int width;  // codes per row
+  int64_t x_stride, residual_stride, codes_stride;
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+
+// Sum over the CTA, the same for every thread.
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = warp_sum(v);
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_sum(lane < warps ? red[lane] : 0.f);
+}
+
+// Largest over the CTA of the bit patterns of magnitudes: the order of the
+// floats, with infinity and NaN above all.
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return __reduce_max_sync(0xffffffffu, lane < warps ? red[lane] : 0u);
+}
+
+__device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
+
+// 16-bit inputs take the approximate exponential and quotient (a few units of
+// 2^-24, far below the code's half step), float32 the library's.
+template <typename T>
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  if constexpr (sizeof(T) == 2) return __fdividef(g, 1.f + __expf(-g)) * u;
+  return g / (1.f + expf(-g)) * u;
+}
+
+struct RowScale {
+  float scale, inverse;
+  bool finite;
+  __device__ __forceinline__ explicit RowScale(uint32_t top) {
+    finite = top < 0x7f800000u;
+    scale = finite ? fmaxf(__fdiv_rn(__uint_as_float(top), 127.f), kLeastScale)
+                   : __uint_as_float(0x7fc00000u);
+    inverse = __fdiv_rn(1.f, scale);
+  }
+  // The code in the low byte.
+  __device__ __forceinline__ uint32_t code(float y) const {
+    constexpr float kInteger = 12582912.f;  // 1.5 * 2^23: adding it leaves an integer in the low bits
+    const float q = y * inverse;
+    float r = q + kInteger;
+    if (fabsf(q - (r - kInteger)) > 0.4999f) r = __fdiv_rn(y, scale) + kInteger;
+    return finite ? __float_as_uint(r) & 0xffu : 0u;
+  }
+};
+
+template <typename T, int SRC, int NV>
+__global__ void __launch_bounds__(kMaxThreads) quantise_vec_kernel(const QuantJob job) {
+  using Tr = Traits<T>;
+  constexpr int V = Tr::kVec;
+  __shared__ float red_sum[32];
+  __shared__ uint32_t red_max[32];
+  const int64_t row = blockIdx.x;
+  const int nvec = job.width / V;
+  const T* xr = static_cast<const T*>(job.x) + row * job.x_stride;
+  T* rr = SRC == kAddNorm ? static_cast<T*>(job.residual) + row * job.residual_stride : nullptr;
+  const T* weight = static_cast<const T*>(job.weight);
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    const int64_t bytes = (int64_t)job.width * sizeof(T);
+    prefetch_l2(xr, SRC == kSilu ? 2 * bytes : bytes);
+    if (SRC == kAddNorm) prefetch_l2(rr, bytes);
+    if ((SRC == kNorm || SRC == kAddNorm) && row < 4) prefetch_l2(weight, bytes);
+  }
+  pdl_wait();
+  uint4 a[NV], b[NV], w[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = threadIdx.x + j * blockDim.x;
+    if (c < nvec) {
+      a[j] = ld_nc_v4(xr + (int64_t)c * V);
+      if (SRC == kSilu) b[j] = ld_nc_v4(xr + job.width + (int64_t)c * V);
+      if (SRC == kAddNorm) b[j] = ld_v4(rr + (int64_t)c * V);
+      if (SRC == kNorm || SRC == kAddNorm) w[j] = __ldg(reinterpret_cast<const uint4*>(weight) + c);
+    }
+  }
+  float y[NV][V];
+  float ss = 0.f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = threadIdx.x + j * blockDim.x;
+    if (c < nvec) {
+      Tr::unpack(a[j], y[j]);
+      if constexpr (SRC == kSilu || SRC == kAddNorm) {
+        float z[V];
+        Tr::unpack(b[j], z);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          y[j][e] = SRC == kSilu ? silu_mul<T>(y[j][e], z[e]) : Tr::round(y[j][e] + z[e]);
+        if (SRC == kAddNorm) st_v4(rr + (int64_t)c * V, Tr::pack(y[j]));
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (SRC == kNorm || SRC == kAddNorm)
+          ss += y[j][e] * y[j][e];
+        else
+          top = max(top, magnitude(y[j][e]));
+      }
+    }
+  }
+  if constexpr (SRC == kNorm || SRC == kAddNorm) {
+    const float inv = rsqrtf(block_sum(ss, red_sum) / (float)job.width + job.eps);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = threadIdx.x + j * blockDim.x;
+      if (c < nvec) {
+        float wf[V];
+        Tr::unpack(w[j], wf);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          y[j][e] = y[j][e] * inv * wf[e];
+          top = max(top, magnitude(y[j][e]));
+        }
+      }
+    }
+  }
+  const RowScale s(block_max(top, red_max));
+  if (threadIdx.x == 0) job.scales[row] = s.scale;
+  int8_t* codes = job.codes + row * job.codes_stride;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = threadIdx.x + j * blockDim.x;
+    if (c < nvec) {
+      uint32_t word[V / 4];
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i)
+        word[i] = s.code(y[j][4 * i]) | s.code(y[j][4 * i + 1]) << 8 |
+                  s.code(y[j][4 * i + 2]) << 16 | s.code(y[j][4 * i + 3]) << 24;
+      if constexpr (V == 8)
+        *reinterpret_cast<uint2*>(codes + (int64_t)c * V) = make_uint2(word[0], word[1]);
+      else
+        *reinterpret_cast<uint32_t*>(codes + (int64_t)c * V) = word[0];
+    }
+  }
+}
+
+// Any width, stride and alignment: a thread's elements are computed anew in
+// each pass, from what it read (and, with a residual, wrote) itself.
+template <typename T, int SRC>
+__global__ void __launch_bounds__(256) quantise_scalar_kernel(const QuantJob job) {
+  using Tr = Traits<T>;
+  __shared__ float red_sum[32];
+  __shared__ uint32_t red_max[32];
+  const int64_t row = blockIdx.x;
+  const T* xr = static_cast<const T*>(job.x) + row * job.x_stride;
+  T* rr = SRC == kAddNorm ? static_cast<T*>(job.residual) + row * job.residual_stride : nullptr;
+  const T* weight = static_cast<const T*>(job.weight);
+  pdl_launch_dependents();
+  pdl_wait();
+  float inv = 1.f;
+  if constexpr (SRC == kNorm || SRC == kAddNorm) {
+    float ss = 0.f;
+    for (int i = threadIdx.x; i < job.width; i += blockDim.x) {
+      float v = Tr::to_f(xr[i]);
+      if (SRC == kAddNorm) {
+        v = Tr::round(v + Tr::to_f(rr[i]));
+        rr[i] = Tr::from_f(v);
+      }
+      ss += v * v;
+    }
+    inv = rsqrtf(block_sum(ss, red_sum) / (float)job.width + job.eps);
+  }
+  auto value = [&](int i) -> float {
+    if constexpr (SRC == kSilu) return silu_mul<T>(Tr::to_f(xr[i]), Tr::to_f(xr[job.width + i]));
+    if constexpr (SRC == kNorm) return Tr::to_f(xr[i]) * inv * Tr::to_f(weight[i]);
+    if constexpr (SRC == kAddNorm) return Tr::to_f(rr[i]) * inv * Tr::to_f(weight[i]);
+    return Tr::to_f(xr[i]);
+  };
+  uint32_t top = 0;
+  for (int i = threadIdx.x; i < job.width; i += blockDim.x) top = max(top, magnitude(value(i)));
+  const RowScale s(block_max(top, red_max));
+  if (threadIdx.x == 0) job.scales[row] = s.scale;
+  int8_t* codes = job.codes + row * job.codes_stride;
+  for (int i = threadIdx.x; i < job.width; i += blockDim.x) codes[i] = (int8_t)s.code(value(i));
+}
+
+template <typename T, int SRC>
+int launch_quantise(const QuantJob& job, int64_t rows, cudaStream_t stream, const char* name) {
+  constexpr int V = Traits<T>::kVec;
+  const int64_t nvec = job.width / V;
+  bool vec = job.width % V == 0 && job.x_stride % V == 0 && job.codes_stride % V == 0 &&
+             aligned16(job.x) && (reinterpret_cast<uintptr_t>(job.codes) & (V - 1)) == 0 &&
+             nvec <= 4 * kMaxThreads;
+  if (SRC == kNorm || SRC == kAddNorm) vec = vec && aligned16(job.weight);
+  if (SRC == kAddNorm) vec = vec && job.residual_stride % V == 0 && aligned16(job.residual);
+  const dim3 grid((unsigned)rows);
+  cudaError_t err;
+  if (vec) {
+    int nv = 1;
+    while (nv < 4 && ceil_div(nvec, nv) > kMaxThreads) nv *= 2;
+    const dim3 threads((unsigned)(ceil_div(ceil_div(nvec, nv), 32) * 32));
+    err = nv == 1   ? launch(quantise_vec_kernel<T, SRC, 1>, grid, threads, 0, stream, job)
+          : nv == 2 ? launch(quantise_vec_kernel<T, SRC, 2>, grid, threads, 0, stream, job)
+                    : launch(quantise_vec_kernel<T, SRC, 4>, grid, threads, 0, stream, job);
+  } else {
+    err = launch(quantise_scalar_kernel<T, SRC>, grid, dim3(256), 0, stream, job);
+  }
+  return err == cudaSuccess ? PACE_OK : cuda_fail(err, name);
+}
+
+// What the entry points have in common: shapes, pointers, the number types.
+template <typename F>
+int checked(const QuantJob& job, int64_t rows, int64_t width, int64_t inputs, bool pointers,
+            const char* name, F run) {
+  if (rows < 0 || rows > INT32_MAX || width <= 0 || width > INT32_MAX)
+    return fail(PACE_ERR_INVALID_ARGUMENT, "%s: bad shape [%lld, %lld]", name, (long long)rows,
+                (long long)width);
+  if (job.x_stride < inputs * width || job.codes_stride < width)
+    return fail(PACE_ERR_INVALID_ARGUMENT, "%s: row stride smaller than the row", name);
+  if (rows == 0) return PACE_OK;
+  if (!job.codes || !job.scales || !job.x || !pointers)
+    return fail(PACE_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+  return run();
+}
+
+}  // namespace
+}  // namespace pace
+
+extern "C" int pace_quantise_rows(int8_t* codes, float* scales, const void* input, int64_t rows,
+                                  int64_t width, int64_t input_row_stride,
+                                  int64_t codes_row_stride, int dtype, cudaStream_t stream) {
+  using namespace pace;
+  const QuantJob job{codes, scales,     input,            nullptr, nullptr,
+                     0.f,   (int)width, input_row_stride, 0,       codes_row_stride};
+  return checked(job, rows, width, 1, true, "quantise_rows", [&] {
+    StreamDeviceGuard guard(stream);
+    return PACE_DISPATCH_FLOAT(dtype, "quantise_rows", [&] {
+      return launch_quantise<scalar_t, kRows>(job, rows, stream, "quantise_rows");
+    });
+  });
+}
+
+extern "C" int pace_rms_norm_quantise(int8_t* codes, float* scales, const void* input,
+                                      void* residual, const void* weight, float epsilon,
+                                      int64_t num_tokens, int64_t hidden_size,
+                                      int64_t input_row_stride, int64_t residual_row_stride,
+                                      int64_t codes_row_stride, int dtype, cudaStream_t stream) {
+  using namespace pace;
+  const QuantJob job{codes,
+                     scales,
+                     input,
+                     residual,
+                     weight,
+                     epsilon,
+                     (int)hidden_size,
+                     input_row_stride,
+                     residual_row_stride,
+                     codes_row_stride};
+  if (residual && residual_row_stride < hidden_size)
+    return fail(PACE_ERR_INVALID_ARGUMENT, "rms_norm_quantise: row stride smaller than the row");
+  return checked(job, num_tokens, hidden_size, 1, weight != nullptr, "rms_norm_quantise", [&] {
+    StreamDeviceGuard guard(stream);
+    return PACE_DISPATCH_FLOAT(dtype, "rms_norm_quantise", [&] {
+      return residual ? launch_quantise<scalar_t, kAddNorm>(job, num_tokens, stream,
+                                                            "rms_norm_quantise")
+                      : launch_quantise<scalar_t, kNorm>(job, num_tokens, stream,
+                                                         "rms_norm_quantise");
+    });
+  });
+}
+
+extern "C" int pace_silu_and_mul_quantise(int8_t* codes, float* scales, const void* input,
+                                          int64_t num_tokens, int64_t d, int64_t input_row_stride,
+                                          int64_t codes_row_stride, int dtype,
+                                          cudaStream_t stream) {
+  using namespace pace;
+  const QuantJob job{codes, scales, input,            nullptr, nullptr,
+                     0.f,   (int)d, input_row_stride, 0,       codes_row_stride};
+  return checked(job, num_tokens, d, 2, true, "silu_and_mul_quantise", [&] {
+    StreamDeviceGuard guard(stream);
+    return PACE_DISPATCH_FLOAT(dtype, "silu_and_mul_quantise", [&] {
+      return launch_quantise<scalar_t, kSilu>(job, num_tokens, stream, "silu_and_mul_quantise");
+    });
+  });
+}

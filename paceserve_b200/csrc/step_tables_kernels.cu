@@ -1,0 +1,326 @@
+// A step's page tables and index arrays from its requests' lengths, for
+// sm_100a: what PaceServe's block manager and attention wrapper build on the
+// host (flashinfer_attention_wrapper.py:75-209) and copy to the device.
+//
+// Request b holds ceil(seq_b / page) pages, the first of its row of the block
+// table, and gets new_b tokens more.  New pages come from the top of a stack of
+// free ones, in the requests' order: the k-th is free[count - 1 - k].  All else
+// follows from three prefix sums over the requests (new tokens, pages, new
+// pages).  Every CTA works them out for itself (they are a few KB, from L2) and
+// then takes its share of the outputs, finding an entry's request by bisection
+// in shared memory; so one launch does without a grid-wide barrier.  The one
+// value that is read by all and changed, the stack's height, is written by the
+// CTA that finishes last.  It is a matter of latency: a few dependent loads.
+#include "common.cuh"
+
+namespace pace {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int64_t kMaxRequests = 8192;  // three prefix sums of them in shared memory
+
+struct TableJob {
+  int32_t* block_tables;
+  const int32_t *lens_a, *lens_b;  // build: in the cache, new;  release: held, kept
+  int32_t *free_pages, *free_count;
+  int32_t *append_indptr, *kv_indptr, *kv_indices, *last_page_len, *batch_indices;
+  int64_t *positions, *slots;
+  int32_t *status, *arrivals;
+  int64_t table_stride, max_blocks, num_free_pages, num_indices, num_tokens;
+  int requests, page_size, page_shift;
+};
+
+__device__ __forceinline__ int64_t pages_of(const TableJob& j, int64_t tokens) {
+  const int64_t t = tokens + j.page_size - 1;
+  return j.page_shift >= 0 ? t >> j.page_shift : t / j.page_size;
+}
+
+// Exclusive prefix sums of three values over the CTA; totals in `all`.
+__device__ __forceinline__ void scan3(int64_t (&v)[3], int64_t (&all)[3], int64_t (*part)[3]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t mine[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    mine[k] = v[k];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, v[k], d);
+      if (lane >= d) v[k] += o;
+    }
+    if (lane == 31) part[warp][k] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    int64_t before = 0;
+    all[k] = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += part[w][k];
+      all[k] += part[w][k];
+    }
+    v[k] += before - mine[k];
+  }
+}
+
+// The request whose range of an ascending prefix sum holds `i`.
+__device__ __forceinline__ int owner_of(const int32_t* sum, int requests, int i) {
+  int lo = 0, hi = requests - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (sum[mid] <= i)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// Writes the stack's new height once every CTA has read the old one.
+__device__ __forceinline__ void leave(const TableJob& j, int64_t height, int32_t problems) {
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  uint32_t before;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+               : "=r"(before)
+               : "l"(j.arrivals)
+               : "memory");
+  if (before != gridDim.x - 1) return;
+  *j.arrivals = 0;
+  if (problems)
+    atomicOr(j.status, problems);
+  else
+    *j.free_count = (int32_t)height;
+}
+
+// BUILD: a step's arrays; otherwise pages go back onto the stack.
+template <bool BUILD>
+__global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j) {
+  extern __shared__ int32_t sums[];  // [requests + 1] each: first, pages, new pages
+  __shared__ int64_t part[kWarps][3];
+  __shared__ int problem_bits;
+  const int R = j.requests;
+  int32_t* ip = sums;              // BUILD: new tokens; release: pages kept
+  int32_t* kp = sums + R + 1;      // BUILD: pages
+  int32_t* np = sums + 2 * R + 2;  // BUILD: new pages; release: pages given back
+  if (threadIdx.x == 0) problem_bits = 0;
+  pdl_launch_dependents();
+  __syncthreads();
+  pdl_wait();
+  const int64_t height = *reinterpret_cast<volatile int32_t*>(j.free_count);
+  // requests of this thread: consecutive ones
+  const int per = (R + kThreads - 1) / kThreads;
+  const int b0 = threadIdx.x * per;
+  int64_t v[3] = {0, 0, 0}, all[3];
+  int32_t problems = 0;
+  // what request b adds to the three sums
+  auto shares = [&](int b, int64_t (&s)[3]) {
+    const int64_t x = j.lens_a[b], y = j.lens_b[b];
+    const int64_t most = BUILD ? x + y : x;
+    if (x < 0 || y < 0 || (!BUILD && y > x)) {
+      problems |= PACE_TABLES_BAD_LENGTH;
+      s[0] = s[1] = s[2] = 0;
+      return;
+    }
+    const int64_t pages = pages_of(j, most), less = pages_of(j, BUILD ? x : y);
+    if (pages > j.max_blocks) problems |= PACE_TABLES_SHORT_ROW;
+    s[0] = BUILD ? y : 0;
+    s[1] = BUILD ? pages : 0;
+    s[2] = pages - less;
+  };
+  for (int i = 0; i < per && b0 + i < R; ++i) {
+    int64_t s[3];
+    shares(b0 + i, s);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) v[k] += s[k];
+  }
+  scan3(v, all, part);
+  if (BUILD) {
+    if (all[1] > j.num_indices) problems |= PACE_TABLES_SHORT_INDICES;
+    if (all[0] > j.num_tokens) problems |= PACE_TABLES_SHORT_TOKENS;
+    if (height < 0 || height > j.num_free_pages || all[2] > height) problems |= PACE_TABLES_NO_PAGES;
+  } else if (height < 0 || height + all[2] > j.num_free_pages) {
+    problems |= PACE_TABLES_NO_PAGES;
+  }
+  if (problems) atomicOr(&problem_bits, problems);
+  __syncthreads();
+  problems = problem_bits;
+  const int64_t step = (int64_t)gridDim.x * kThreads;
+  const int64_t me = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (problems) {
+    // nothing is taken or given; tables that no token gets through
+    if (BUILD) {
+      for (int64_t i = me; i <= R; i += step) {
+        j.append_indptr[i] = j.kv_indptr[i] = 0;
+        if (i < R) j.last_page_len[i] = 0;
+      }
+      for (int64_t i = me; i < j.num_tokens; i += step) {
+        j.batch_indices[i] = -1;
+        j.positions[i] = j.slots[i] = -1;
+      }
+    }
+    leave(j, height, problems);
+    return;
+  }
+  for (int i = 0; i < per && b0 + i < R; ++i) {
+    int64_t s[3];
+    const int b = b0 + i;
+    shares(b, s);
+    ip[b] = BUILD ? (int32_t)v[0] : (int32_t)pages_of(j, j.lens_b[b]);
+    kp[b] = (int32_t)v[1];
+    np[b] = (int32_t)v[2];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) v[k] += s[k];
+  }
+  if (threadIdx.x == 0) {
+    ip[R] = (int32_t)all[0];
+    kp[R] = (int32_t)all[1];
+    np[R] = (int32_t)all[2];
+  }
+  __syncthreads();
+  if constexpr (BUILD) {
+    // page k of request b, old or new
+    auto page_at = [&](int b, int k, bool* fresh) -> int32_t {
+      const int held = (kp[b + 1] - kp[b]) - (np[b + 1] - np[b]);
+      *fresh = k >= held;
+      return *fresh ? j.free_pages[height - 1 - (np[b] + k - held)]
+                    : j.block_tables[(int64_t)b * j.table_stride + k];
+    };
+    for (int64_t i = me; i <= R; i += step) {
+      j.append_indptr[i] = ip[i];
+      j.kv_indptr[i] = kp[i];
+      if (i < R) {
+        // 1 .. page_size; page_size for a request without tokens, whose length is then 0
+        const int64_t n = (int64_t)j.lens_a[i] + j.lens_b[i];
+        j.last_page_len[i] = (int32_t)(n - (pages_of(j, n) - 1) * j.page_size);
+      }
+    }
+    const int pages = (int)all[1], tokens = (int)all[0];
+    for (int64_t i = me; i < pages; i += step) {
+      const int b = owner_of(kp, R, (int)i), k = (int)i - kp[b];
+      bool fresh;
+      const int32_t page = page_at(b, k, &fresh);
+      j.kv_indices[i] = page;
+      if (fresh) j.block_tables[(int64_t)b * j.table_stride + k] = page;
+    }
+    for (int64_t i = me; i < j.num_tokens; i += step) {
+      if (i >= tokens) {  // padding
+        j.batch_indices[i] = -1;
+        j.positions[i] = j.slots[i] = -1;
+        continue;
+      }
+      const int b = owner_of(ip, R, (int)i);
+      const int64_t pos = (int64_t)j.lens_a[b] + ((int)i - ip[b]);
+      const int k = (int)(j.page_shift >= 0 ? pos >> j.page_shift : pos / j.page_size);
+      bool fresh;
+      const int64_t page = page_at(b, k, &fresh);
+      j.batch_indices[i] = b;
+      j.positions[i] = pos;
+      j.slots[i] = page * j.page_size + (pos - (int64_t)k * j.page_size);
+    }
+    leave(j, height - all[2], 0);
+  } else {
+    const int given = (int)all[2];
+    for (int64_t i = me; i < given; i += step) {
+      const int b = owner_of(np, R, (int)i), k = ip[b] + ((int)i - np[b]);
+      j.free_pages[height + given - 1 - i] = j.block_tables[(int64_t)b * j.table_stride + k];
+    }
+    leave(j, height + given, 0);
+  }
+}
+
+template <bool BUILD>
+int run_tables(TableJob& j, int64_t requests, int64_t page_size, cudaStream_t stream,
+               const char* name) {
+  if (requests < 0 || page_size <= 0 || page_size > INT32_MAX || j.max_blocks < 0 ||
+      j.num_free_pages < 0 || j.num_indices < 0 || j.num_tokens < 0)
+    return fail(PACE_ERR_INVALID_ARGUMENT, "%s: bad shape", name);
+  if (requests > 1 && j.table_stride < j.max_blocks)
+    return fail(PACE_ERR_INVALID_ARGUMENT, "%s: row stride smaller than the row", name);
+  if (requests > kMaxRequests)
+    return fail(PACE_ERR_TOO_LARGE, "%s: %lld requests, at most %lld", name, (long long)requests,
+                (long long)kMaxRequests);
+  if (j.num_free_pages > INT32_MAX || j.num_indices > INT32_MAX || j.num_tokens > INT32_MAX ||
+      j.max_blocks > INT32_MAX)
+    return fail(PACE_ERR_TOO_LARGE, "%s: index arrays longer than 2^31 - 1", name);
+  if (!j.free_count || !j.status || !j.arrivals || (j.num_free_pages > 0 && !j.free_pages) ||
+      (requests > 0 && (!j.lens_a || !j.lens_b || (j.max_blocks > 0 && !j.block_tables))) ||
+      (BUILD && (!j.append_indptr || !j.kv_indptr || (requests > 0 && !j.last_page_len) ||
+                 (j.num_indices > 0 && !j.kv_indices) ||
+                 (j.num_tokens > 0 && (!j.batch_indices || !j.positions || !j.slots)))))
+    return fail(PACE_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+  j.requests = (int)requests;
+  j.page_size = (int)page_size;
+  j.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctzll(page_size) : -1;
+  StreamDeviceGuard guard(stream);
+  const int smem = (int)(3 * (requests + 1) * sizeof(int32_t));
+  cudaError_t err = cudaSuccess;
+  if (smem > 48 * 1024) {
+    err = ensure_dynamic_smem(reinterpret_cast<const void*>(step_tables_kernel<BUILD>),
+                              guard.device(), (int)(3 * (kMaxRequests + 1) * sizeof(int32_t)));
+    if (err != cudaSuccess) return cuda_fail(err, name);
+  }
+  // a few entries a thread, of the arrays' full length: how much of it a step needs is known on
+  // the device only
+  const int64_t entries = BUILD ? j.num_indices + j.num_tokens
+                                : (j.max_blocks < 1 ? 0 : requests * j.max_blocks);
+  int64_t ctas = ceil_div(entries, 4 * kThreads);
+  if (ctas < 1) ctas = 1;
+  if (ctas > sm_count(guard.device())) ctas = sm_count(guard.device());
+  err = launch(step_tables_kernel<BUILD>, dim3((unsigned)ctas), dim3(kThreads), (size_t)smem,
+               stream, j);
+  return err == cudaSuccess ? PACE_OK : cuda_fail(err, name);
+}
+
+}  // namespace
+}  // namespace pace
+
+extern "C" int pace_build_step_tables(
+    int32_t* block_tables, int64_t table_row_stride, int64_t max_blocks, const int32_t* seq_lens,
+    const int32_t* new_lens, int64_t num_requests, int64_t page_size, int32_t* free_pages,
+    int64_t num_free_pages, int32_t* free_count, int32_t* append_indptr, int32_t* kv_indptr,
+    int32_t* kv_indices, int64_t num_kv_indices, int32_t* kv_last_page_len,
+    int32_t* batch_indices, int64_t* positions, int64_t* slot_mapping, int64_t num_tokens,
+    int32_t* status, int32_t* arrivals, cudaStream_t stream) {
+  pace::TableJob j = {};
+  j.block_tables = block_tables;
+  j.table_stride = table_row_stride;
+  j.max_blocks = max_blocks;
+  j.lens_a = seq_lens;
+  j.lens_b = new_lens;
+  j.free_pages = free_pages;
+  j.num_free_pages = num_free_pages;
+  j.free_count = free_count;
+  j.append_indptr = append_indptr;
+  j.kv_indptr = kv_indptr;
+  j.kv_indices = kv_indices;
+  j.num_indices = num_kv_indices;
+  j.last_page_len = kv_last_page_len;
+  j.batch_indices = batch_indices;
+  j.positions = positions;
+  j.slots = slot_mapping;
+  j.num_tokens = num_tokens;
+  j.status = status;
+  j.arrivals = arrivals;
+  return pace::run_tables<true>(j, num_requests, page_size, stream, "build_step_tables");
+}
+
+extern "C" int pace_release_pages(const int32_t* block_tables, int64_t table_row_stride,
+                                  int64_t max_blocks, const int32_t* held_lens,
+                                  const int32_t* kept_lens, int64_t num_requests,
+                                  int64_t page_size, int32_t* free_pages, int64_t num_free_pages,
+                                  int32_t* free_count, int32_t* status, int32_t* arrivals,
+                                  cudaStream_t stream) {
+  pace::TableJob j = {};
+  j.block_tables = const_cast<int32_t*>(block_tables);
+  j.table_stride = table_row_stride;
+  j.max_blocks = max_blocks;
+  j.lens_a = held_lens;
+  j.lens_b = kept_lens;
+  j.free_pages = free_pages;
+  j.num_free_pages = num_free_pages;
+  j.free_count = free_count;
+  j.status = status;
+  j.arrivals = arrivals;
+  return pace::run_tables<false>(j, num_requests, page_size, stream, "release_pages");
+}

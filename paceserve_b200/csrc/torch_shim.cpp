@@ -5,8 +5,8 @@
 // layernorm_ops / pos_encoding_ops / activation_ops / moe_ops of
 // paceserve_b200._C, adds the new ops (fused_add_rms_norm, gelu_and_mul,
 // gelu_tanh_and_mul) in the same style, a kv_transfer_ops submodule for the
-// paged-KV block copy, append and quantised cache, and an attention_ops
-// submodule for paged attention.  Tensors are validated here; every launch goes
+// paged-KV block copy, append, quantised cache and step tables, an attention_ops
+// submodule for paged attention and an int8_ops submodule for 8-bit projections.  Tensors are validated here; every launch goes
 // through the C ABI on the current stream of the tensors' device, and a
 // non-zero status becomes a RuntimeError carrying pace_last_error().
 #include <ATen/cuda/CUDAContext.h>
@@ -1169,6 +1169,384 @@ struct AttentionStep {
   }
 };
 
+// ------------------------------------------------------------- step tables --
+// A tensor that the kernel writes (or reads) in place: int32 or int64, 1-D,
+// contiguous, on the tables' device, with at least n entries.
+template <typename I>
+I* entries_of(const Tensor& t, const Tensor& like, int64_t n, const char* op, const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.dim() == 1 && t.is_contiguous() &&
+                  t.scalar_type() == c10::CppTypeToScalarType<I>::value && t.numel() >= n,
+              op, ": ", name, " must be a contiguous 1-D ",
+              c10::toString(c10::CppTypeToScalarType<I>::value), " tensor of at least ", n,
+              " entries on ", like.device());
+  return t.data_ptr<I>();
+}
+
+// Rows of block_tables.
+int64_t table_rows(const Tensor& t, int64_t requests, const char* op) {
+  check_cuda(t, op, "block_tables");
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 2 &&
+                  (t.size(1) <= 1 || t.stride(1) == 1) && t.size(0) >= requests,
+              op, ": block_tables must be int32 [at least ", requests,
+              ", max_blocks], contiguous in its rows");
+  TORCH_CHECK(requests <= 1 || t.stride(0) >= t.size(1), op, ": block_tables' rows overlap");
+  return t.size(0) <= 1 ? t.size(1) : t.stride(0);
+}
+
+void build_step_tables(Tensor& block_tables, const Tensor& seq_lens, const Tensor& new_lens,
+                       int64_t page_size, Tensor& free_pages, Tensor& free_count,
+                       Tensor& append_indptr, Tensor& kv_indptr, Tensor& kv_indices,
+                       Tensor& kv_last_page_len, Tensor& batch_indices, Tensor& positions,
+                       Tensor& slot_mapping, Tensor& status, Tensor& arrivals) {
+  const char* op = "build_step_tables";
+  const int64_t r = seq_lens.numel(), tokens = slot_mapping.numel();
+  const int64_t stride = table_rows(block_tables, r, op);
+  const Tensor& like = block_tables;
+  TORCH_CHECK(new_lens.numel() == r, op, ": seq_lens and new_lens differ in length");
+  TORCH_CHECK(batch_indices.numel() == tokens && positions.numel() == tokens, op,
+              ": batch_indices, positions and slot_mapping differ in length");
+  const at::cuda::CUDAGuard guard(like.device());
+  check_status(
+      pace_build_step_tables(
+          block_tables.data_ptr<int32_t>(), stride, block_tables.size(1),
+          entries_of<int32_t>(seq_lens, like, r, op, "seq_lens"),
+          entries_of<int32_t>(new_lens, like, r, op, "new_lens"), r, page_size,
+          entries_of<int32_t>(free_pages, like, 0, op, "free_pages"), free_pages.numel(),
+          entries_of<int32_t>(free_count, like, 1, op, "free_count"),
+          entries_of<int32_t>(append_indptr, like, r + 1, op, "append_indptr"),
+          entries_of<int32_t>(kv_indptr, like, r + 1, op, "kv_indptr"),
+          entries_of<int32_t>(kv_indices, like, 0, op, "kv_indices"), kv_indices.numel(),
+          entries_of<int32_t>(kv_last_page_len, like, r, op, "kv_last_page_len"),
+          entries_of<int32_t>(batch_indices, like, 0, op, "batch_indices"),
+          entries_of<int64_t>(positions, like, 0, op, "positions"),
+          entries_of<int64_t>(slot_mapping, like, 0, op, "slot_mapping"), tokens,
+          entries_of<int32_t>(status, like, 1, op, "status"),
+          entries_of<int32_t>(arrivals, like, 1, op, "arrivals"), stream_of(like)),
+      op);
+}
+
+void release_pages(const Tensor& block_tables, const Tensor& held_lens, const Tensor& kept_lens,
+                   int64_t page_size, Tensor& free_pages, Tensor& free_count, Tensor& status,
+                   Tensor& arrivals) {
+  const char* op = "release_pages";
+  const int64_t r = held_lens.numel();
+  const int64_t stride = table_rows(block_tables, r, op);
+  const Tensor& like = block_tables;
+  TORCH_CHECK(kept_lens.numel() == r, op, ": held_lens and kept_lens differ in length");
+  const at::cuda::CUDAGuard guard(like.device());
+  check_status(pace_release_pages(block_tables.data_ptr<int32_t>(), stride, block_tables.size(1),
+                                  entries_of<int32_t>(held_lens, like, r, op, "held_lens"),
+                                  entries_of<int32_t>(kept_lens, like, r, op, "kept_lens"), r,
+                                  page_size,
+                                  entries_of<int32_t>(free_pages, like, 0, op, "free_pages"),
+                                  free_pages.numel(),
+                                  entries_of<int32_t>(free_count, like, 1, op, "free_count"),
+                                  entries_of<int32_t>(status, like, 1, op, "status"),
+                                  entries_of<int32_t>(arrivals, like, 1, op, "arrivals"),
+                                  stream_of(like)),
+               op);
+}
+
+// ----------------------------------------------- head norms with rotation --
+struct HeadArgs {
+  Rows q, k;
+  int num_heads, num_kv_heads;
+};
+
+HeadArgs check_heads(const Tensor& positions, const Tensor& query, const Tensor& key,
+                     const Tensor& q_weight, const Tensor& k_weight, int64_t head_size,
+                     const Tensor& cos_sin_cache, const char* op) {
+  check_cuda(query, op, "query");
+  check_same_device(positions, query, op);
+  check_same_device(key, query, op);
+  check_same_device(q_weight, query, op);
+  check_same_device(k_weight, query, op);
+  check_same_device(cos_sin_cache, query, op);
+  TORCH_CHECK(head_size > 0 && head_size <= INT32_MAX, op, ": head_size must be positive");
+  TORCH_CHECK(is_float_type(query) && key.scalar_type() == query.scalar_type() &&
+                  q_weight.scalar_type() == query.scalar_type() &&
+                  k_weight.scalar_type() == query.scalar_type(),
+              op, ": query, key and the weights must share a float dtype");
+  TORCH_CHECK(q_weight.is_contiguous() && q_weight.numel() == head_size &&
+                  k_weight.is_contiguous() && k_weight.numel() == head_size,
+              op, ": q_weight and k_weight must be [", head_size, "] and contiguous");
+  TORCH_CHECK(positions.scalar_type() == at::kLong && positions.is_contiguous(), op,
+              ": positions must be a contiguous int64 tensor");
+  TORCH_CHECK(cos_sin_cache.dim() == 2 && cos_sin_cache.is_contiguous(), op,
+              ": cos_sin_cache must be a contiguous [max_position, rot_dim] tensor");
+  TORCH_CHECK(cos_sin_cache.scalar_type() == at::kFloat ||
+                  cos_sin_cache.scalar_type() == query.scalar_type(),
+              op, ": cos_sin_cache must be float32 or the query dtype");
+  HeadArgs a{qk_rows(query, head_size, op, "query"), qk_rows(key, head_size, op, "key"), 0, 0};
+  TORCH_CHECK(a.k.rows == a.q.rows, op, ": query and key token counts differ");
+  TORCH_CHECK(positions.numel() >= a.q.rows, op, ": positions has ", positions.numel(),
+              " entries for ", a.q.rows, " tokens");
+  a.num_heads = (int)(a.q.width / head_size);
+  a.num_kv_heads = (int)(a.k.width / head_size);
+  return a;
+}
+
+void qk_norm_rotary_embedding(Tensor& positions, Tensor& query, Tensor& key, Tensor& q_weight,
+                              Tensor& k_weight, double epsilon, int64_t head_size,
+                              Tensor& cos_sin_cache, bool is_neox) {
+  const char* op = "qk_norm_rotary_embedding";
+  const HeadArgs a =
+      check_heads(positions, query, key, q_weight, k_weight, head_size, cos_sin_cache, op);
+  const at::cuda::CUDAGuard guard(query.device());
+  check_status(pace_qk_norm_rotary_embedding(
+                   positions.data_ptr<int64_t>(), query.data_ptr(), key.data_ptr(),
+                   q_weight.data_ptr(), k_weight.data_ptr(), (float)epsilon, a.q.rows, a.num_heads,
+                   a.num_kv_heads, (int)head_size, a.q.stride, a.k.stride,
+                   cos_sin_cache.data_ptr(), pace_dtype(cos_sin_cache),
+                   (int)cos_sin_cache.size(1), cos_sin_cache.size(0), is_neox ? 1 : 0,
+                   pace_dtype(query), stream_of(query)),
+               op);
+}
+
+void qk_norm_rotary_append(Tensor& positions, Tensor& query, const Tensor& key,
+                           const Tensor& value, Tensor& q_weight, Tensor& k_weight, double epsilon,
+                           int64_t head_size, Tensor& cos_sin_cache, bool is_neox,
+                           Tensor& paged_kv_cache, const Tensor& slot_mapping,
+                           const c10::optional<Tensor>& bad_tokens) {
+  const char* op = "qk_norm_rotary_append";
+  const HeadArgs a =
+      check_heads(positions, query, key, q_weight, k_weight, head_size, cos_sin_cache, op);
+  check_same_device(value, query, op);
+  check_same_device(paged_kv_cache, query, op);
+  check_same_device(slot_mapping, query, op);
+  const PagedCache pc = paged_cache_of(paged_kv_cache, "NHD", op);
+  TORCH_CHECK(value.scalar_type() == query.scalar_type() &&
+                  paged_kv_cache.scalar_type() == query.scalar_type(),
+              op, ": query, key, value and cache must share a dtype");
+  const Rows v = qk_rows(value, head_size, op, "value");
+  TORCH_CHECK(v.rows == a.q.rows && v.width == a.k.width, op, ": key and value differ in shape");
+  TORCH_CHECK(pc.heads == a.num_kv_heads && pc.hd == head_size, op, ": the cache holds ", pc.heads,
+              " heads of ", pc.hd, ", the keys are ", a.num_kv_heads, " of ", head_size);
+  TORCH_CHECK(slot_mapping.scalar_type() == at::kLong && slot_mapping.is_contiguous() &&
+                  slot_mapping.numel() >= a.q.rows,
+              op, ": slot_mapping must be a contiguous int64 tensor with an entry for each token");
+  int32_t* bad = counter_ptr(bad_tokens, query.device(), op, "bad_tokens");
+  const at::cuda::CUDAGuard guard(query.device());
+  check_status(pace_qk_norm_rotary_append(
+                   positions.data_ptr<int64_t>(), query.data_ptr(), key.data_ptr(),
+                   value.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), (float)epsilon,
+                   a.q.rows, a.num_heads, a.num_kv_heads, (int)head_size, a.q.stride, a.k.stride,
+                   v.stride, cos_sin_cache.data_ptr(), pace_dtype(cos_sin_cache),
+                   (int)cos_sin_cache.size(1), cos_sin_cache.size(0), is_neox ? 1 : 0,
+                   paged_kv_cache.data_ptr(), pc.pages, (int)pc.page_size,
+                   slot_mapping.data_ptr<int64_t>(), bad, pace_dtype(query), stream_of(query)),
+               op);
+}
+
+// ------------------------------------------------------- 8-bit projections --
+// Codes [rows, width] int8 and their scales [rows], on the device of `like`.
+Rows codes_of(const Tensor& codes, const Tensor& scales, const Tensor& like, const char* op,
+              const char* name, const char* scales_name) {
+  check_same_device(codes, like, op);
+  check_same_device(scales, like, op);
+  TORCH_CHECK(codes.scalar_type() == at::kChar && codes.dim() == 2, op, ": ", name,
+              " must be int8 [rows, k]");
+  const Rows r = rows_of(codes, op, name);
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous() &&
+                  scales.numel() == r.rows,
+              op, ": ", scales_name, " must be a contiguous float32 tensor with an entry for each of ",
+              name, "'s ", r.rows, " rows");
+  return r;
+}
+
+void quantise_rows(Tensor& codes, Tensor& scales, const Tensor& input) {
+  const char* op = "quantise_rows";
+  check_cuda(input, op, "input");
+  TORCH_CHECK(is_float_type(input), op, ": input dtype must be float32, float16 or bfloat16");
+  const Rows in = rows_of(input, op, "input");
+  const Rows c = codes_of(codes, scales, input, op, "codes", "scales");
+  TORCH_CHECK(c.rows == in.rows && c.width == in.width, op, ": codes ", codes.sizes(),
+              " do not match input ", input.sizes());
+  const at::cuda::CUDAGuard guard(input.device());
+  check_status(pace_quantise_rows(codes.data_ptr<int8_t>(), scales.data_ptr<float>(),
+                                  input.data_ptr(), in.rows, in.width, in.stride, c.stride,
+                                  pace_dtype(input), stream_of(input)),
+               op);
+}
+
+void rms_norm_quantise(Tensor& codes, Tensor& scales, const Tensor& input, const Tensor& weight,
+                       double epsilon, const c10::optional<Tensor>& residual) {
+  const char* op = "rms_norm_quantise";
+  check_cuda(input, op, "input");
+  check_same_device(weight, input, op);
+  TORCH_CHECK(is_float_type(input) && weight.scalar_type() == input.scalar_type(), op,
+              ": input and weight must share one of float32, float16 and bfloat16");
+  const Rows in = rows_of(input, op, "input");
+  const Rows c = codes_of(codes, scales, input, op, "codes", "scales");
+  TORCH_CHECK(c.rows == in.rows && c.width == in.width, op, ": codes ", codes.sizes(),
+              " do not match input ", input.sizes());
+  TORCH_CHECK(weight.is_contiguous() && weight.numel() == in.width, op, ": weight must be [",
+              in.width, "] and contiguous");
+  Rows r{0, 0, 0};
+  if (residual.has_value()) {
+    check_same_device(*residual, input, op);
+    TORCH_CHECK(residual->scalar_type() == input.scalar_type(), op,
+                ": residual must have the input's dtype");
+    r = rows_of(*residual, op, "residual");
+    TORCH_CHECK(r.rows == in.rows && r.width == in.width, op, ": residual shape ",
+                residual->sizes(), " does not match input ", input.sizes());
+  }
+  const at::cuda::CUDAGuard guard(input.device());
+  check_status(pace_rms_norm_quantise(codes.data_ptr<int8_t>(), scales.data_ptr<float>(),
+                                      input.data_ptr(),
+                                      residual.has_value() ? residual->data_ptr() : nullptr,
+                                      weight.data_ptr(), (float)epsilon, in.rows, in.width,
+                                      in.stride, r.stride, c.stride, pace_dtype(input),
+                                      stream_of(input)),
+               op);
+}
+
+void silu_and_mul_quantise(Tensor& codes, Tensor& scales, const Tensor& input) {
+  const char* op = "silu_and_mul_quantise";
+  check_cuda(input, op, "input");
+  TORCH_CHECK(is_float_type(input), op, ": input dtype must be float32, float16 or bfloat16");
+  const Rows in = rows_of(input, op, "input");
+  const Rows c = codes_of(codes, scales, input, op, "codes", "scales");
+  TORCH_CHECK(c.rows == in.rows && 2 * c.width == in.width, op, ": codes ", codes.sizes(),
+              " do not match input ", input.sizes());
+  const at::cuda::CUDAGuard guard(input.device());
+  check_status(pace_silu_and_mul_quantise(codes.data_ptr<int8_t>(), scales.data_ptr<float>(),
+                                          input.data_ptr(), in.rows, c.width, in.stride, c.stride,
+                                          pace_dtype(input), stream_of(input)),
+               op);
+}
+
+// The partial sums' workspace where the caller passes none.  Outside of a
+// capture: one for each (device, stream), large enough for any shape, so that
+// it is never exchanged under a kernel that uses it.  Inside: one for each
+// capture and stream, zeroed by the graph itself at its first use, so that no
+// two graphs share one; it lives in the graph's memory.
+Tensor int8_workspace(const at::Device& dev, cudaStream_t stream, size_t bytes) {
+  constexpr int64_t kCounterBytes = 4096;  // as the C ABI asks: zero before the first call
+  struct Entry {
+    unsigned long long capture = 0;
+    Tensor ws;
+  };
+  static std::mutex mu;
+  static std::map<std::pair<int, cudaStream_t>, Entry> eager, captured;
+  const auto bytes_of = at::TensorOptions().dtype(at::kByte).device(dev);
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id));
+  std::lock_guard<std::mutex> lock(mu);
+  const bool capturing = status == cudaStreamCaptureStatusActive;
+  Entry& e = (capturing ? captured : eager)[{dev.index(), stream}];
+  if (!e.ws.defined() || (size_t)e.ws.numel() < bytes || (capturing && e.capture != id)) {
+    // eager: any shape's need on this device is at most 2 partial tiles of 128 x 256 a CTA
+    const int64_t most =
+        kCounterBytes +
+        (int64_t)at::cuda::getDeviceProperties(dev.index())->multiProcessorCount * 2 * 128 * 256 * 4;
+    e.ws = at::empty({capturing ? (int64_t)bytes : std::max<int64_t>(most, (int64_t)bytes)},
+                     bytes_of);
+    e.ws.narrow(0, 0, kCounterBytes).zero_();
+    e.capture = id;
+  }
+  return e.ws;
+}
+
+struct Int8Args {
+  Rows x, w;
+  Tensor ws;
+};
+
+Int8Args check_int8(const Tensor& out, const Tensor& codes, const Tensor& token_scales,
+                    const Tensor& weight, const Tensor& channel_scales, bool gated,
+                    const c10::optional<Tensor>& workspace, const char* op) {
+  check_cuda(out, op, gated ? "out" : "out or residual");
+  TORCH_CHECK(is_float_type(out) && out.dim() == 2, op,
+              ": the output must be [tokens, features] of float32, float16 or bfloat16");
+  Int8Args a{codes_of(codes, token_scales, out, op, "codes", "token_scales"),
+             codes_of(weight, channel_scales, out, op, "weight", "channel_scales"), Tensor()};
+  const int64_t n = gated ? a.w.rows / 2 : a.w.rows;
+  TORCH_CHECK(!gated || a.w.rows % 2 == 0, op, ": weight needs as many gate as up rows");
+  TORCH_CHECK(a.x.width == a.w.width && out.size(0) == a.x.rows && out.size(1) == n, op,
+              ": shapes do not match: output ", out.sizes(), ", codes ", codes.sizes(),
+              ", weight ", weight.sizes());
+  if (a.x.rows == 0) return a;
+  const size_t need =
+      pace_int8_linear_workspace_size(a.x.rows, n, a.x.width, gated, out.device().index());
+  if (workspace.has_value()) {
+    a.ws = *workspace;
+    TORCH_CHECK(a.ws.is_cuda() && a.ws.device() == out.device() && a.ws.is_contiguous() &&
+                    (size_t)a.ws.nbytes() >= need,
+                op, ": workspace must be a contiguous tensor of at least ", need, " bytes on ",
+                out.device());
+  } else if (need > 0) {
+    a.ws = int8_workspace(out.device(), stream_of(out), need);
+  }
+  return a;
+}
+
+void int8_linear_into(Tensor& out, const Tensor& codes, const Tensor& token_scales,
+                      const Tensor& weight, const Tensor& channel_scales,
+                      const c10::optional<Tensor>& bias, bool residual,
+                      const c10::optional<Tensor>& workspace,
+                      const c10::optional<Tensor>& fault_flags, const char* op) {
+  check_cuda(out, op, residual ? "residual" : "out");
+  const at::cuda::CUDAGuard guard(out.device());
+  const Int8Args a =
+      check_int8(out, codes, token_scales, weight, channel_scales, false, workspace, op);
+  const Rows o = rows_of(out, op, residual ? "residual" : "out");
+  const void* b = nullptr;
+  if (bias.has_value()) {
+    check_same_device(*bias, out, op);
+    TORCH_CHECK(bias->scalar_type() == out.scalar_type() && bias->is_contiguous() &&
+                    bias->numel() == a.w.rows,
+                op, ": bias must be a contiguous [", a.w.rows, "] tensor of the output's dtype");
+    b = bias->data_ptr();
+  }
+  int32_t* fault = counter_ptr(fault_flags, out.device(), op, "fault_flags");
+  check_status(pace_int8_linear(out.data_ptr(), codes.data_ptr<int8_t>(),
+                                token_scales.data_ptr<float>(), weight.data_ptr<int8_t>(),
+                                channel_scales.data_ptr<float>(), b,
+                                residual ? out.data_ptr() : nullptr, a.x.rows, a.w.rows, a.x.width,
+                                a.x.stride, a.w.stride, o.stride, o.stride, pace_dtype(out),
+                                ws_ptr(a.ws), ws_bytes(a.ws), fault, stream_of(out)),
+               op);
+}
+
+void int8_linear(Tensor& out, const Tensor& codes, const Tensor& token_scales,
+                 const Tensor& weight, const Tensor& channel_scales,
+                 const c10::optional<Tensor>& bias, const c10::optional<Tensor>& workspace,
+                 const c10::optional<Tensor>& fault_flags) {
+  int8_linear_into(out, codes, token_scales, weight, channel_scales, bias, false, workspace,
+                   fault_flags, "int8_linear");
+}
+
+void int8_linear_residual(Tensor& residual, const Tensor& codes, const Tensor& token_scales,
+                          const Tensor& weight, const Tensor& channel_scales,
+                          const c10::optional<Tensor>& bias,
+                          const c10::optional<Tensor>& workspace,
+                          const c10::optional<Tensor>& fault_flags) {
+  int8_linear_into(residual, codes, token_scales, weight, channel_scales, bias, true, workspace,
+                   fault_flags, "int8_linear_residual");
+}
+
+void int8_gate_up_silu(Tensor& out, const Tensor& codes, const Tensor& token_scales,
+                       const Tensor& weight, const Tensor& channel_scales,
+                       const c10::optional<Tensor>& workspace,
+                       const c10::optional<Tensor>& fault_flags) {
+  const char* op = "int8_gate_up_silu";
+  check_cuda(out, op, "out");
+  const at::cuda::CUDAGuard guard(out.device());
+  const Int8Args a =
+      check_int8(out, codes, token_scales, weight, channel_scales, true, workspace, op);
+  const Rows o = rows_of(out, op, "out");
+  int32_t* fault = counter_ptr(fault_flags, out.device(), op, "fault_flags");
+  check_status(pace_int8_gate_up_silu(out.data_ptr(), codes.data_ptr<int8_t>(),
+                                      token_scales.data_ptr<float>(), weight.data_ptr<int8_t>(),
+                                      channel_scales.data_ptr<float>(), a.x.rows, o.width,
+                                      a.x.width, a.x.stride, a.w.stride, o.stride,
+                                      pace_dtype(out), ws_ptr(a.ws), ws_bytes(a.ws), fault,
+                                      stream_of(out)),
+               op);
+}
+
 py::tuple ipc_get_handle(const Tensor& t) {
   TORCH_CHECK(t.is_cuda(), "ipc_get_handle: tensor must be on a CUDA device");
   const at::cuda::CUDAGuard guard(t.device());
@@ -1230,6 +1608,18 @@ PYBIND11_MODULE(_C, m) {
          "Apply GPT-NeoX or GPT-J style rotary embedding to query and key", py::arg("positions"),
          py::arg("query"), py::arg("key"), py::arg("head_size"), py::arg("cos_sin_cache"),
          py::arg("is_neox"));
+  pe.def("qk_norm_rotary_embedding", &qk_norm_rotary_embedding,
+         "RMSNorm of every query and key head, then the rotary embedding, in place and in one "
+         "pass.",
+         py::arg("positions"), py::arg("query"), py::arg("key"), py::arg("q_weight"),
+         py::arg("k_weight"), py::arg("epsilon"), py::arg("head_size"), py::arg("cos_sin_cache"),
+         py::arg("is_neox"));
+  pe.def("qk_norm_rotary_append", &qk_norm_rotary_append,
+         "The same with the keys' result and the values written to their slots of a paged cache.",
+         py::arg("positions"), py::arg("query"), py::arg("key"), py::arg("value"),
+         py::arg("q_weight"), py::arg("k_weight"), py::arg("epsilon"), py::arg("head_size"),
+         py::arg("cos_sin_cache"), py::arg("is_neox"), py::arg("paged_kv_cache"),
+         py::arg("slot_mapping"), py::arg("bad_tokens") = py::none());
   pe.def("qkv_proj_rotary_embedding", &qkv_proj_rotary_embedding,
          "qkv = hidden @ weight^T on the tensor cores with the rotary embedding applied to the "
          "q and k heads before rounding (fused qkv_proj + rotary_embedding).",
@@ -1332,6 +1722,41 @@ PYBIND11_MODULE(_C, m) {
            py::arg("exponents"), py::arg("sm_scale"), py::arg("logits_soft_cap"),
            py::arg("alibi_slopes"), py::arg("out"), py::arg("lse"), py::arg("fault_flags"));
 
+  auto i8 = m.def_submodule("int8_ops");
+  i8.def("quantise_rows", &quantise_rows,
+         "Rows as 8-bit integers with a scale each (the largest magnitude is 127).",
+         py::arg("codes"), py::arg("scales"), py::arg("input"));
+  i8.def("rms_norm_quantise", &rms_norm_quantise,
+         "rms_norm(input) * weight quantised; with residual, residual += input and its norm.",
+         py::arg("codes"), py::arg("scales"), py::arg("input"), py::arg("weight"),
+         py::arg("epsilon"), py::arg("residual") = py::none());
+  i8.def("silu_and_mul_quantise", &silu_and_mul_quantise,
+         "silu(input[:, :d]) * input[:, d:] quantised.", py::arg("codes"), py::arg("scales"),
+         py::arg("input"));
+  i8.def("linear", &int8_linear,
+         "out = (codes @ weight^T) * token_scales * channel_scales (+ bias) on the tensor cores, "
+         "the sums exact in 32 bits.",
+         py::arg("out"), py::arg("codes"), py::arg("token_scales"), py::arg("weight"),
+         py::arg("channel_scales"), py::arg("bias") = py::none(),
+         py::arg("workspace") = py::none(), py::arg("fault_flags") = py::none());
+  i8.def("linear_residual", &int8_linear_residual, "residual += the same product.",
+         py::arg("residual"), py::arg("codes"), py::arg("token_scales"), py::arg("weight"),
+         py::arg("channel_scales"), py::arg("bias") = py::none(),
+         py::arg("workspace") = py::none(), py::arg("fault_flags") = py::none());
+  i8.def("gate_up_silu", &int8_gate_up_silu,
+         "out = silu(gate) * up, [gate | up] the same product with a weight [2 I, k].",
+         py::arg("out"), py::arg("codes"), py::arg("token_scales"), py::arg("weight"),
+         py::arg("channel_scales"), py::arg("workspace") = py::none(),
+         py::arg("fault_flags") = py::none());
+  i8.def("workspace_size",
+         [](int64_t num_tokens, int64_t out_features, int64_t k, bool gated, int64_t device) {
+           return pace_int8_linear_workspace_size(num_tokens, out_features, k, gated ? 1 : 0,
+                                                  (int)device);
+         },
+         "Bytes of workspace (its first 4096 zeroed) a product of this shape needs.",
+         py::arg("num_tokens"), py::arg("out_features"), py::arg("k"), py::arg("gated") = false,
+         py::arg("device") = 0);
+
   auto kv = m.def_submodule("kv_transfer_ops");
   kv.def("copy_blocks_p2p", &copy_blocks_p2p,
          "Copy KV blocks src_block_ids of src_caches onto dst_block_ids of dst_caches "
@@ -1375,6 +1800,19 @@ PYBIND11_MODULE(_C, m) {
          py::arg("value"), py::arg("out_indptr"), py::arg("codes"), py::arg("exponents"),
          py::arg("kv_indices"), py::arg("kv_indptr"), py::arg("kv_last_page_len"),
          py::arg("bad_tokens") = py::none());
+  kv.def("build_step_tables", &build_step_tables,
+         "Block tables, index arrays and slots of a step from its requests' lengths; new pages "
+         "come from a stack of free ones.",
+         py::arg("block_tables"), py::arg("seq_lens"), py::arg("new_lens"), py::arg("page_size"),
+         py::arg("free_pages"), py::arg("free_count"), py::arg("append_indptr"),
+         py::arg("kv_indptr"), py::arg("kv_indices"), py::arg("kv_last_page_len"),
+         py::arg("batch_indices"), py::arg("positions"), py::arg("slot_mapping"),
+         py::arg("status"), py::arg("arrivals"));
+  kv.def("release_pages", &release_pages,
+         "The pages past the requests' kept tokens go back onto the stack of free ones.",
+         py::arg("block_tables"), py::arg("held_lens"), py::arg("kept_lens"),
+         py::arg("page_size"), py::arg("free_pages"), py::arg("free_count"), py::arg("status"),
+         py::arg("arrivals"));
   kv.def("ipc_get_handle", &ipc_get_handle, py::arg("tensor"));
   kv.def("ipc_open_handle", &ipc_open_handle, py::arg("handle"), py::arg("device"));
   kv.def("ipc_close_handle", &ipc_close_handle, py::arg("base"));
