@@ -7,18 +7,16 @@
 // The sum is int32, so it is exact and the same in every order of its terms (K is
 // at most 131071, where 128 * 128 * K still fits); the rest is fp32, rounded once.
 //
-// One kernel (int8_gemm_kernel): TMA fills a ring of 128-byte K blocks (128-byte
-// swizzle), one thread issues tcgen05.mma.kind::i8 into one of two TMEM
-// accumulators, and eight warps drain the other through the scales.  Two ways
-// round:
-//  * tokens in the accumulator's rows (its lanes), channels in its columns: 256
-//    tokens on a CTA pair (cta_group::2) or 128 on one CTA, by 256 channels;
-//  * few tokens: channels in the rows, tokens in 16 to 64 columns, so that a
-//    decode batch's tile is not padding but the weight, and what is drained is
-//    small.  There the weight's bytes bound it.
-// Tiles that do not fill the SMs evenly are cut over K (stream-K): workers leave
-// int32 partial sums in the workspace, and the last to arrive at a tile adds them
-// up.  No CTA waits for another, and the result does not depend on who is last.
+// Two kernels on the tensor cores, both TMA (128-byte K blocks, 128-byte swizzle)
+// into a ring, one thread issuing tcgen05.mma.kind::i8, and eight warps that drain
+// the accumulator in TMEM through the scales:
+//  * int8_gemm_kernel, more than 64 tokens: tokens in the accumulator's rows, 256
+//    on a CTA pair (cta_group::2) or 128 on one CTA, by up to 256 channels;
+//  * int8_slice_kernel, up to 64 tokens, where the weight's bytes bound it: 32
+//    channels a tile, so that there are tiles for all SMs without cutting one over
+//    CTAs.  The 128 rows of the matrix instruction hold the channels' K in four
+//    slices, its columns the tokens' K in the same slices: the four blocks where
+//    the slices agree are partial sums, the others are not read.
 //
 // What TMA cannot take (K, a row stride or an address that is no multiple of 16
 // bytes) runs on the CUDA cores (int8_dot_kernel).
@@ -35,12 +33,15 @@ constexpr int EPI_WARPS = 8;
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
 constexpr int MAX_STAGES = 10;
 constexpr int kRingBytes = 196608;  // at most
+constexpr int kSmem = kRingBytes + 1024 + 256;
 constexpr int kEpiBarrier = 1;
+constexpr int CH = 16;  // columns drained at a time
 constexpr uint64_t kWaitLimitNs = 1000000000ull;  // 1 s per wait
 constexpr int32_t kFaultTimeout = 1 << 30;
 constexpr int64_t kMaxK = 131071;
 // The workspace: arrival counters of the tiles that are cut, then the partial sums.
 constexpr int64_t kCounterBytes = 4096;
+constexpr int kSlot = BM * 256;  // int32 of a partial tile
 
 struct Ctl {
   uint64_t full[MAX_STAGES];
@@ -61,30 +62,9 @@ struct GemmJob {
   const float *token_scales, *channel_scales;
   int64_t out_stride, add_stride;
   int tokens, channels;  // channels: output columns (half the weight's rows with SiLU)
-  int k_blocks, m_tiles, n_tiles;
-  int vec;  // out (and add) take 16-byte accesses
-};
-
-// TOK_ROWS: tokens in the accumulator's rows.  SILU: each tile has a gate and an
-// up part: the two halves of its columns (TOK_ROWS), or two accumulators.
-template <int BN_, bool PAIR_, bool TOK_ROWS_, bool SILU_>
-struct Shape {
-  static constexpr int BN = BN_;
-  static constexpr bool PAIR = PAIR_, TOK_ROWS = TOK_ROWS_, SILU = SILU_;
-  static constexpr int NACC = SILU && !TOK_ROWS ? 2 : 1;
-  static constexpr int kA = NACC * BM * BK;            // bytes per CTA and stage
-  static constexpr int kB = (PAIR ? BN / 2 : BN) * BK;
-  static constexpr int kStage = kA + kB;
-  static constexpr int kStages = kRingBytes / kStage < MAX_STAGES ? kRingBytes / kStage : MAX_STAGES;
-  static constexpr int kSmem = kStages * kStage + 1024 + 256;
-  static constexpr int kRows = PAIR ? 2 * BM : BM;     // of a tile
-  static constexpr int kCols = NACC * BN;              // accumulator columns
-  static constexpr int kTmem = 2 * kCols < 32 ? 32 : 2 * kCols;
-  static constexpr int kOutCols = SILU && TOK_ROWS ? BN / 2 : BN;  // output columns of a tile
-  static constexpr int kHalf = kOutCols / 2;           // of one of the two warps of a lane quarter
-  static constexpr int CH = kHalf < 16 ? kHalf : 16;   // columns drained at a time
-  static constexpr int kSlot = kCols * BM;             // int32 of a partial tile
-  static_assert(kTmem <= 512 && (kTmem & (kTmem - 1)) == 0 && CH % 8 == 0, "");
+  int k_blocks;
+  int vec;         // out (and add) take 16-byte accesses
+  int scales_vec;  // the channels' scales do
 };
 
 // Instruction descriptor of tcgen05.mma.kind::i8: int32 accumulator (bits 4-5 =
@@ -113,18 +93,22 @@ __device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a, uint64_t b, uint
         : "memory");
 }
 
-// N (8 or 16) consecutive columns of this thread's TMEM lane; valid after
-// tc::tmem_wait_ld.
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
-  tc::tmem_ld16(taddr, r);
-}
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[8]) {
+// 8 consecutive columns of this thread's TMEM lane; valid after tc::tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7])
       : "r"(taddr)
       : "memory");
+}
+
+// Pulls a box of a tensor map into L2.
+__device__ __forceinline__ void prefetch_box(const CUtensorMap* map, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y)
+               : "memory");
 }
 
 // Split of the K blocks of the tiles [t_stop, ...) over the first `workers` workers.
@@ -137,29 +121,43 @@ struct Split {
   }
 };
 
-// A worker's segments in order: whole tiles worker, worker + step, ... below
-// t_stop, then its range of the units of the tiles from t_stop on.
+// A worker's segments in order: its range of the units of the tiles from t_stop
+// on, then whole tiles worker, worker + step, ... below t_stop.  What is cut comes
+// first, so that its joining hides behind the whole tiles' products.
 struct Walk {
   int64_t t_next, t_stop, step;
   int64_t u, u_end;
   int k_blocks;
   __device__ __forceinline__ bool next(int64_t& t, int& kb0, int& kb1) {
-    if (t_next < t_stop) {
-      t = t_next;
-      t_next += step;
-      kb0 = 0;
-      kb1 = k_blocks;
+    if (u < u_end) {
+      const int64_t rt = u / k_blocks;
+      t = t_stop + rt;
+      kb0 = (int)(u - rt * k_blocks);
+      kb1 = (int)min((int64_t)k_blocks, kb0 + (u_end - u));
+      u += kb1 - kb0;
       return true;
     }
-    if (u >= u_end) return false;
-    const int64_t rt = u / k_blocks;
-    t = t_stop + rt;
-    kb0 = (int)(u - rt * k_blocks);
-    kb1 = (int)min((int64_t)k_blocks, kb0 + (u_end - u));
-    u += kb1 - kb0;
+    if (t_next >= t_stop) return false;
+    t = t_next;
+    t_next += step;
+    kb0 = 0;
+    kb1 = k_blocks;
     return true;
   }
 };
+
+// Tile t's place: groups of kGroup rows of tiles, and within a group the rows
+// fastest, so that the tiles in work at one time are about as many tokens high as
+// channels wide and read little besides one another's operands.
+constexpr int kGroup = 8;
+__device__ __forceinline__ void place_of(int64_t t, int m_tiles, int n_tiles, int& mt, int& nt) {
+  const int64_t group = (int64_t)kGroup * n_tiles;
+  const int first = (int)(t / group) * kGroup;
+  const int rows = min(kGroup, m_tiles - first);
+  const int r = (int)(t - (int64_t)first * n_tiles);
+  nt = r / rows;
+  mt = first + r - nt * rows;
+}
 
 __device__ __forceinline__ void raise_fault(Ctl* ctl, int32_t* fault) {
   *reinterpret_cast<volatile int*>(&ctl->abort) = 1;
@@ -192,7 +190,6 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 
 // Partial sums: [4 columns][lane][4], so that a warp's instruction moves 512
 // contiguous bytes; through L2 only, since another SM reads them.
-template <int CH>
 __device__ __forceinline__ void store_partial(int32_t* slot, int col, int row,
                                               const uint32_t (&r)[CH]) {
 #pragma unroll
@@ -200,7 +197,6 @@ __device__ __forceinline__ void store_partial(int32_t* slot, int col, int row,
     __stcg(reinterpret_cast<uint4*>(slot + ((int64_t)(col / 4 + q) * BM + row) * 4),
            make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]));
 }
-template <int CH>
 __device__ __forceinline__ void add_partial(const int32_t* slot, int col, int row,
                                             uint32_t (&r)[CH]) {
 #pragma unroll
@@ -214,8 +210,26 @@ __device__ __forceinline__ void add_partial(const int32_t* slot, int col, int ro
   }
 }
 
+// Scales of CH consecutive channels (those past the last are never used).
+__device__ __forceinline__ void load_scales(const GemmJob& j, int n, float (&s)[CH]) {
+  const int rows = n < j.channels ? j.channels : 2 * j.channels;
+  if (j.scales_vec && n + CH <= rows) {
+#pragma unroll
+    for (int i = 0; i < CH / 4; ++i) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(j.channel_scales + n) + i);
+      s[4 * i] = v.x;
+      s[4 * i + 1] = v.y;
+      s[4 * i + 2] = v.z;
+      s[4 * i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < CH; ++e) s[e] = __ldg(j.channel_scales + min(n + e, rows - 1));
+  }
+}
+
 // CH consecutive channels n .. of one token: add, round, store.
-template <typename T, int CH>
+template <typename T>
 __device__ __forceinline__ void put_channels(const GemmJob& j, int64_t t, int n, float* y) {
   constexpr int V = Traits<T>::kVec;
   T* o = static_cast<T*>(j.out) + t * j.out_stride + n;
@@ -248,29 +262,48 @@ __device__ __forceinline__ void put_channels(const GemmJob& j, int64_t t, int n,
   }
 }
 
-template <typename T, class S>
+// How the rows kernel is cut: bn channels (gate and up together with SiLU) a tile,
+// `stages` ring stages, the first split_workers workers sharing the tiles left over.
+struct Tiling {
+  int bn, stages, m_tiles, n_tiles, split_workers;
+};
+
+// A ring position: the stage, and the parity of the phase that its barriers wait for.
+struct Turn {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+template <typename T, bool PAIR, bool SILU>
 __global__ void __launch_bounds__(THREADS, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
-                     const __grid_constant__ CUtensorMap tm_b, const GemmJob j, int split_workers,
+                     const __grid_constant__ CUtensorMap tm_b, const GemmJob j, const Tiling p,
                      int32_t* counters, int32_t* slots, int32_t* fault) {
-  constexpr bool PAIR = S::PAIR, TOK_ROWS = S::TOK_ROWS, SILU = S::SILU;
-  constexpr int BN = S::BN, NST = S::kStages, SB = S::kStage, CH = S::CH;
+  constexpr int kRows = PAIR ? 2 * BM : BM, kA = BM * BK, kTmem = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  Ctl* ctl = reinterpret_cast<Ctl*>(tiles + NST * SB);
+  Ctl* ctl = reinterpret_cast<Ctl*>(tiles + kRingBytes);
+  const int nst = p.stages, bn = p.bn, out_cols = SILU ? bn / 2 : bn;
+  const int sb = kA + (PAIR ? bn / 2 : bn) * BK;  // bytes of a stage in this CTA
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
   const uint32_t rank = PAIR ? tc::cluster_rank() : 0u;
   const int worker = PAIR ? cta >> 1 : cta;
   const int workers = PAIR ? (int)gridDim.x >> 1 : (int)gridDim.x;
-  const int64_t n_all = (int64_t)j.m_tiles * j.n_tiles;
+  const int64_t n_all = (int64_t)p.m_tiles * p.n_tiles;
   const int64_t t_stop = n_all / workers * workers;
   Split sp;
   sp.units = (n_all - t_stop) * j.k_blocks;
-  sp.workers = split_workers;
+  sp.workers = p.split_workers;
   sp.k_blocks = j.k_blocks;
-  const bool splits = worker < split_workers;
+  const bool splits = worker < p.split_workers;
   const Walk walk0{worker,
                    t_stop,
                    (int64_t)workers,
@@ -280,7 +313,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NST; ++s) {
+    for (int s = 0; s < nst; ++s) {
       tc::mbar_init(&ctl->full[s], 1);
       tc::mbar_init(&ctl->empty[s], 1);
     }
@@ -298,9 +331,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   if (warp == 0) {
     if constexpr (PAIR)
-      tc::tmem_alloc_pair(&ctl->tmem, S::kTmem);
+      tc::tmem_alloc_pair(&ctl->tmem, kTmem);
     else
-      tc::tmem_alloc(&ctl->tmem, S::kTmem);
+      tc::tmem_alloc(&ctl->tmem, kTmem);
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -315,56 +348,55 @@ __global__ void __launch_bounds__(THREADS, 1)
       int64_t i = 0;
       bool ok = true;
       Walk walk = walk0;
+      Turn turn;
       int64_t t;
       int kb0, kb1;
       const uint32_t full0 = PAIR ? tc::map_to_rank(&ctl->full[0], 0) : 0u;
       while (ok && walk.next(t, kb0, kb1)) {
-        const int mt = (int)(t / j.n_tiles), nt = (int)(t % j.n_tiles);
-        const int a0 = mt * S::kRows + (int)rank * BM;
-        // B rows of this CTA: with SiLU in columns, gate rows and the up rows `channels` further
-        // (PAIR: the leader the gate's, its partner the up's)
-        const int b0 = SILU && TOK_ROWS ? nt * S::kOutCols + (int)rank * j.channels
-                                        : nt * BN + (int)rank * (BN / 2);
+        int mt, nt;
+        place_of(t, p.m_tiles, p.n_tiles, mt, nt);
+        const int a0 = mt * kRows + (int)rank * BM;
+        // B rows of this CTA: with SiLU gate rows and the up rows `channels` further (PAIR: the
+        // leader the gate's, its partner the up's)
+        const int b0 = SILU ? nt * out_cols + (int)rank * j.channels : nt * bn + (int)rank * (bn / 2);
         for (int kb = kb0; kb < kb1; ++kb, ++i) {
-          const int s = (int)(i % NST);
-          const uint32_t use = (uint32_t)(i / NST);
-          if (use > 0 &&
-              !tc::mbar_wait(&ctl->empty[s], (use - 1) & 1u, kWaitLimitNs, &ctl->abort)) {
+          const int s = turn.s;
+          if (i >= nst &&
+              !tc::mbar_wait(&ctl->empty[s], turn.phase ^ 1u, kWaitLimitNs, &ctl->abort)) {
             ok = false;
             break;
           }
-          uint8_t* a = tiles + s * SB;
-          uint8_t* b = a + S::kA;
+          uint8_t* a = tiles + s * sb;
+          uint8_t* b = a + kA;
           if constexpr (PAIR) {
             const uint32_t bar = full0 + (uint32_t)(s * sizeof(uint64_t));
-            if (rank == 0) tc::mbar_arrive_expect_tx(&ctl->full[s], 2 * SB);
+            if (rank == 0) tc::mbar_arrive_expect_tx(&ctl->full[s], 2 * sb);
             tc::tma_load_2d_pair(a, &tm_a, kb * BK, a0, bar);
             tc::tma_load_2d_pair(b, &tm_b, kb * BK, b0, bar);
           } else {
-            tc::mbar_arrive_expect_tx(&ctl->full[s], SB);
+            tc::mbar_arrive_expect_tx(&ctl->full[s], sb);
             tc::tma_load_2d(a, &tm_a, kb * BK, a0, &ctl->full[s]);
-            if constexpr (S::NACC == 2)
-              tc::tma_load_2d(a + BM * BK, &tm_a, kb * BK, j.channels + a0, &ctl->full[s]);
             tc::tma_load_2d(b, &tm_b, kb * BK, b0, &ctl->full[s]);
-            if constexpr (SILU && TOK_ROWS)
-              tc::tma_load_2d(b + S::kB / 2, &tm_b, kb * BK, j.channels + b0, &ctl->full[s]);
+            if (SILU)
+              tc::tma_load_2d(b + bn / 2 * BK, &tm_b, kb * BK, j.channels + b0, &ctl->full[s]);
           }
+          turn.next(nst);
         }
       }
       if (!ok) raise_fault(ctl, fault);
       // every copy has landed before the shared memory is given up
       if (!PAIR || rank == 0)
-        for (int64_t q = i > NST ? i - NST : 0; q < i; ++q)
-          tc::mbar_wait(&ctl->full[q % NST], (uint32_t)(q / NST) & 1u, kWaitLimitNs, nullptr);
+        for (int64_t q = i > nst ? i - nst : 0; q < i; ++q)
+          tc::mbar_wait(&ctl->full[q % nst], (uint32_t)(q / nst) & 1u, kWaitLimitNs, nullptr);
     }
   } else if (warp == EPI_WARPS + 1) {
     // ---- MMA issuer ---------------------------------------------------------
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = idesc_i8(S::kRows, BN);
-      int64_t i = 0;
+      const uint32_t idesc = idesc_i8(kRows, bn);
       int n = 0;
       bool ok = true;
       Walk walk = walk0;
+      Turn turn;
       int64_t t;
       int kb0, kb1;
       for (; ok && walk.next(t, kb0, kb1); ++n) {
@@ -376,28 +408,25 @@ __global__ void __launch_bounds__(THREADS, 1)
           break;
         }
         tc::tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(b * S::kCols);
-        for (int kb = kb0; kb < kb1; ++kb, ++i) {
-          const int s = (int)(i % NST);
-          if (!tc::mbar_wait(&ctl->full[s], (uint32_t)(i / NST) & 1u, kWaitLimitNs, &ctl->abort)) {
+        const uint32_t d = tmem + (uint32_t)(b * 256);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          const int s = turn.s;
+          if (!tc::mbar_wait(&ctl->full[s], turn.phase, kWaitLimitNs, &ctl->abort)) {
             ok = false;
             break;
           }
           tc::tc_fence_after();
-          const uint32_t a_addr = tc::smem_u32(tiles + s * SB);
+          const uint32_t a_addr = tc::smem_u32(tiles + s * sb);
           const uint64_t ad = tc::umma_desc_sw128(a_addr);
-          const uint64_t bd = tc::umma_desc_sw128(a_addr + S::kA);
+          const uint64_t bd = tc::umma_desc_sw128(a_addr + kA);
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k) {
-            const uint32_t acc = kb > kb0 || k > 0 ? 1u : 0u;
-            umma_i8<PAIR>(d, ad + 2 * k, bd + 2 * k, idesc, acc);
-            if constexpr (S::NACC == 2)
-              umma_i8<PAIR>(d + BN, ad + 2 * k + (BM * BK >> 4), bd + 2 * k, idesc, acc);
-          }
+          for (int k = 0; k < BK / 32; ++k)
+            umma_i8<PAIR>(d, ad + 2 * k, bd + 2 * k, idesc, kb > kb0 || k > 0 ? 1u : 0u);
           if constexpr (PAIR)
             tc::umma_commit_pair_both(&ctl->empty[s]);
           else
             tc::umma_commit(&ctl->empty[s]);
+          turn.next(nst);
         }
         if (ok) {
           if constexpr (PAIR)
@@ -416,28 +445,23 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     // ---- epilogue: warp w drains lanes 32 (w % 4) .. +31, half w / 4 of the columns --------
-    const int row = (warp % 4) * 32 + lane, c_begin = (warp / 4) * S::kHalf;
+    const int row = (warp % 4) * 32 + lane;
+    const int c_begin = (warp / 4) * (out_cols / 2), c_end = c_begin + out_cols / 2;
     const uint32_t tmem_empty0 = PAIR ? tc::map_to_rank(&ctl->tmem_empty[0], 0) : 0u;
+    const int up = bn / 2;  // SiLU: the up columns' distance
     int n = 0;
     Walk walk = walk0;
     int64_t t;
     int kb0, kb1;
     for (; walk.next(t, kb0, kb1); ++n) {
       const int b = n & 1;
-      const int mt = (int)(t / j.n_tiles), nt = (int)(t % j.n_tiles);
-      const int m = mt * S::kRows + (int)rank * BM + row;  // this thread's token or channel
-      const int c0 = nt * S::kOutCols;                     // the tile's first column
-      const int rows_all = TOK_ROWS ? j.tokens : j.channels;
-      const int cols_all = TOK_ROWS ? j.channels : j.tokens;
-      const bool valid = m < rows_all;
+      int mt, nt;
+      place_of(t, p.m_tiles, p.n_tiles, mt, nt);
+      const int m = mt * kRows + (int)rank * BM + row;  // this thread's token
+      const int c0 = nt * out_cols;                     // the tile's first channel
+      const bool valid = m < j.tokens;
       const bool whole = kb0 == 0 && kb1 == j.k_blocks;
-      float s_row = 0.f, s_row2 = 0.f;
-      float bias_row = 0.f;
-      if (valid) {
-        s_row = TOK_ROWS ? j.token_scales[m] : j.channel_scales[m];
-        if (S::NACC == 2) s_row2 = j.channel_scales[j.channels + m];
-        if (!TOK_ROWS && j.bias) bias_row = Traits<T>::to_f(static_cast<const T*>(j.bias)[m]);
-      }
+      const float s_row = valid ? j.token_scales[m] : 0.f;
       bool ready = tc::mbar_wait(&ctl->tmem_full[b], (uint32_t)(n >> 1) & 1u, kWaitLimitNs,
                                  &ctl->abort);
       ready = epi_all(ready);
@@ -446,9 +470,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         break;
       }
       tc::tc_fence_after();
-      const uint32_t acc = tmem + (uint32_t)(b * S::kCols) + ((uint32_t)(warp % 4 * 32) << 16);
-      // the second accumulator (SiLU): the up columns
-      constexpr int kUp = SILU ? (TOK_ROWS ? BN / 2 : BN) : 0;
+      const uint32_t acc = tmem + (uint32_t)(b * 256) + ((uint32_t)(warp % 4 * 32) << 16);
       int w0 = 0, w1 = 0;  // the tile's workers
       bool finish = true;
       if (!whole) {
@@ -456,16 +478,18 @@ __global__ void __launch_bounds__(THREADS, 1)
         w0 = sp.owner(u0);
         w1 = sp.owner(u0 + j.k_blocks - 1);
         // slot 0: the part that begins the tile, 1: one that goes on with it
-        int32_t* slot = slots + ((int64_t)cta * 2 + (kb0 == 0 ? 0 : 1)) * S::kSlot;
+        int32_t* slot = slots + ((int64_t)cta * 2 + (kb0 == 0 ? 0 : 1)) * kSlot;
 #pragma unroll 1
-        for (int c = c_begin; c < c_begin + S::kHalf && c0 + c < cols_all; c += CH) {
+        for (int c = c_begin; c < c_end && c0 + c < j.channels; c += CH) {
           __syncwarp();
-#pragma unroll
-          for (int up = 0; up <= kUp; up += kUp ? kUp : 1) {
-            uint32_t r[CH];
-            tmem_load(acc + (uint32_t)(c + up), r);
-            tc::tmem_wait_ld(r);
-            if (valid) store_partial(slot, c + up, row, r);
+          uint32_t r[CH], r2[CH];
+          tc::tmem_ld16(acc + (uint32_t)c, r);
+          if (SILU) tc::tmem_ld16(acc + (uint32_t)(c + up), r2);
+          tc::tmem_wait_ld(r);
+          if (SILU) tc::tmem_wait_ld(r2);
+          if (valid) {
+            store_partial(slot, c, row, r);
+            if (SILU) store_partial(slot, c + up, row, r2);
           }
         }
         // the last of the tile's workers finishes it.  A pair's CTAs have rows of their own
@@ -486,48 +510,39 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (finish) {
 #pragma unroll 1
-        for (int c = c_begin; c < c_begin + S::kHalf && c0 + c < cols_all; c += CH) {
+        for (int c = c_begin; c < c_end && c0 + c < j.channels; c += CH) {
           __syncwarp();
           uint32_t r[CH], r2[CH];
-          tmem_load(acc + (uint32_t)c, r);
-          if (SILU) tmem_load(acc + (uint32_t)(c + kUp), r2);
+          tc::tmem_ld16(acc + (uint32_t)c, r);
+          if (SILU) tc::tmem_ld16(acc + (uint32_t)(c + up), r2);
+          const int ch = c0 + c;
+          float sc[CH], sc2[CH];
+          load_scales(j, ch, sc);
+          if (SILU) load_scales(j, j.channels + ch, sc2);
           tc::tmem_wait_ld(r);
           if (SILU) tc::tmem_wait_ld(r2);
-          if (!valid) continue;
-          if (!whole) {
-            for (int w = w0; w <= w1; ++w) {
-              if (w == worker) continue;
-              const int32_t* slot =
-                  slots + ((int64_t)(PAIR ? 2 * w + (int)rank : w) * 2 + (w == w0 ? 0 : 1)) * S::kSlot;
-              add_partial(slot, c, row, r);
-              if (SILU) add_partial(slot, c + kUp, row, r2);
+          if (valid) {
+            if (!whole) {
+              for (int w = w0; w <= w1; ++w) {
+                if (w == worker) continue;
+                const int32_t* slot =
+                    slots + ((int64_t)(PAIR ? 2 * w + (int)rank : w) * 2 + (w == w0 ? 0 : 1)) * kSlot;
+                add_partial(slot, c, row, r);
+                if (SILU) add_partial(slot, c + up, row, r2);
+              }
             }
-          }
-          if constexpr (TOK_ROWS) {
-            const int ch = c0 + c;
             float y[CH];
 #pragma unroll
             for (int e = 0; e < CH; ++e) {
-              const int col = min(ch + e, j.channels - 1);
-              y[e] = (float)(int)r[e] * s_row * __ldg(j.channel_scales + col);
-              if (!SILU && j.bias) y[e] += Traits<T>::to_f(static_cast<const T*>(j.bias)[col]);
-              if (SILU)
-                y[e] = silu_mul<T>(
-                    y[e], (float)(int)r2[e] * s_row * __ldg(j.channel_scales + j.channels + col));
+              y[e] = (float)(int)r[e] * s_row * sc[e];
+              if (SILU) y[e] = silu_mul<T>(y[e], (float)(int)r2[e] * s_row * sc2[e]);
             }
-            put_channels<T, CH>(j, m, ch, y);
-          } else {
+            if (!SILU && j.bias) {
+              const T* bias = static_cast<const T*>(j.bias);
 #pragma unroll
-            for (int e = 0; e < CH; ++e) {
-              const int tok = c0 + c + e;
-              if (tok >= j.tokens) break;
-              const float st = __ldg(j.token_scales + tok);
-              float y = (float)(int)r[e] * st * s_row + bias_row;
-              if (SILU) y = silu_mul<T>(y, (float)(int)r2[e] * st * s_row2);
-              if (j.add)
-                y += Traits<T>::to_f(static_cast<const T*>(j.add)[tok * j.add_stride + m]);
-              static_cast<T*>(j.out)[tok * j.out_stride + m] = Traits<T>::from_f(y);
+              for (int e = 0; e < CH; ++e) y[e] += Traits<T>::to_f(bias[min(ch + e, j.channels - 1)]);
             }
+            put_channels<T>(j, m, ch, y);
           }
         }
       }
@@ -546,10 +561,212 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   if constexpr (PAIR) {
     tc::cluster_sync();
-    if (warp == 0) tc::tmem_dealloc_pair(tmem, S::kTmem);
+    if (warp == 0) tc::tmem_dealloc_pair(tmem, kTmem);
   } else {
-    if (warp == 0) tc::tmem_dealloc(tmem, S::kTmem);
+    if (warp == 0) tc::tmem_dealloc(tmem, kTmem);
   }
+}
+
+// ------------------------------------------------------------- few tokens --
+// 32 channels a tile.  Quarter q of the accumulator's rows holds them over slice
+// q of K; with SiLU quarters 0 and 1 the gate's two slices, 2 and 3 the up's.  The
+// columns hold the tokens, `tc` (a multiple of 8) for each slice.  So row quarter q
+// and column group (q mod slices) belong to one slice; the other blocks of the
+// accumulator are products of different slices and stay unread.  That costs matrix
+// rate, of which there is enough (64 tokens: 32 bytes of weight a clock and SM,
+// where memory delivers 23), and saves a reduction over CTAs: the slices are summed
+// through shared memory.  The ring is small enough for two CTAs an SM, so that the
+// next kernel's CTAs start, and pull their first weights into L2, beside this one's.
+// Each takes at most half of TMEM; the kernels that take all of it have over 160 KB of
+// shared memory, so none of their CTAs can wait beside one of these for its columns.
+constexpr int kSliceCh = 32, kSliceTok = 16;  // of a tile; of a pass through shared memory
+constexpr int kSliceRing = 98304;
+constexpr int kSliceStages = 6;
+constexpr int kSliceSum = 4 * kSliceCh * kSliceTok * 4;
+constexpr int kSliceSmem = kSliceRing + kSliceSum + 1024 + 256;
+
+struct SliceTiling {
+  int tc, stages, bufs, tmem_cols, tiles, slice_blocks;
+};
+
+template <typename T, bool SILU>
+__global__ void __launch_bounds__(THREADS, 2)
+    int8_slice_kernel(const __grid_constant__ CUtensorMap tm_w,
+                      const __grid_constant__ CUtensorMap tm_x, const GemmJob j,
+                      const SliceTiling p, int32_t* fault) {
+  constexpr int SL = SILU ? 2 : 4, kA = BM * BK, kBox = kSliceCh * BK;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* tiles = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  int32_t* sums = reinterpret_cast<int32_t*>(tiles + kSliceRing);  // [quarter][token][channel]
+  Ctl* ctl = reinterpret_cast<Ctl*>(tiles + kSliceRing + kSliceSum);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sb = kA + SL * p.tc * BK, cols = SL * p.tc;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      tc::mbar_init(&ctl->full[s], 1);
+      tc::mbar_init(&ctl->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      tc::mbar_init(&ctl->tmem_full[b], 1);
+      tc::mbar_init(&ctl->tmem_empty[b], EPI_WARPS);
+    }
+    tc::mbar_init(&ctl->drain, 1);
+    ctl->abort = 0;
+    tc::fence_barrier_init();
+  }
+  // The weight's boxes of quarter q: channels of tile t (the up's with SiLU from quarter 2 on)
+  auto w_row = [&](int t, int q) { return t * kSliceCh + (SILU && q >= SL ? j.channels : 0); };
+  auto w_col = [&](int kb, int q) { return ((q % SL) * p.slice_blocks + kb) * BK; };
+  if (warp == EPI_WARPS && lane == 0) {
+    tc::tma_prefetch_desc(&tm_w);
+    tc::tma_prefetch_desc(&tm_x);
+    // L2 is the point of coherence: what an earlier kernel still writes to the weight is read from
+    // there after the wait
+    for (int kb = 0; kb < min(p.slice_blocks, 2 * p.stages); ++kb)
+      for (int q = 0; q < 4; ++q)
+        prefetch_box(&tm_w, w_col(kb, q), w_row((int)blockIdx.x, q));
+  }
+  if (warp == 0) tc::tmem_alloc(&ctl->tmem, (uint32_t)p.tmem_cols);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+  pdl_wait();
+
+  if (warp == EPI_WARPS) {
+    // ---- TMA producer -----------------------------------------------------
+    if (lane == 0) {
+      int64_t i = 0;
+      bool ok = true;
+      Turn turn;
+      for (int t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+        for (int kb = 0; kb < p.slice_blocks; ++kb, ++i) {
+          const int s = turn.s;
+          if (i >= p.stages &&
+              !tc::mbar_wait(&ctl->empty[s], turn.phase ^ 1u, kWaitLimitNs, &ctl->abort)) {
+            ok = false;
+            break;
+          }
+          uint8_t* a = tiles + s * sb;
+          tc::mbar_arrive_expect_tx(&ctl->full[s], (uint32_t)sb);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            tc::tma_load_2d(a + q * kBox, &tm_w, w_col(kb, q), w_row(t, q), &ctl->full[s]);
+#pragma unroll
+          for (int q = 0; q < SL; ++q)
+            tc::tma_load_2d(a + kA + q * p.tc * BK, &tm_x, w_col(kb, q), 0, &ctl->full[s]);
+          turn.next(p.stages);
+        }
+      }
+      if (!ok) raise_fault(ctl, fault);
+      for (int64_t q = i > p.stages ? i - p.stages : 0; q < i; ++q)
+        tc::mbar_wait(&ctl->full[q % p.stages], (uint32_t)(q / p.stages) & 1u, kWaitLimitNs, nullptr);
+    }
+  } else if (warp == EPI_WARPS + 1) {
+    // ---- MMA issuer ---------------------------------------------------------
+    if (lane == 0) {
+      const uint32_t idesc = idesc_i8(BM, cols);
+      int n = 0;
+      bool ok = true;
+      Turn turn;
+      for (int t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++n) {
+        const int b = p.bufs == 2 ? n & 1 : 0;
+        const int use = p.bufs == 2 ? n >> 1 : n;
+        if (use > 0 && !tc::mbar_wait(&ctl->tmem_empty[b], (uint32_t)(use - 1) & 1u, kWaitLimitNs,
+                                      &ctl->abort)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(b * cols);
+        for (int kb = 0; kb < p.slice_blocks; ++kb) {
+          const int s = turn.s;
+          if (!tc::mbar_wait(&ctl->full[s], turn.phase, kWaitLimitNs, &ctl->abort)) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+          const uint32_t a_addr = tc::smem_u32(tiles + s * sb);
+          const uint64_t ad = tc::umma_desc_sw128(a_addr);
+          const uint64_t bd = tc::umma_desc_sw128(a_addr + kA);
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            umma_i8<false>(d, ad + 2 * k, bd + 2 * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
+          tc::umma_commit(&ctl->empty[s]);
+          turn.next(p.stages);
+        }
+        if (ok) tc::umma_commit(&ctl->tmem_full[b]);
+      }
+      if (!ok) raise_fault(ctl, fault);
+      tc::umma_commit(&ctl->drain);
+      tc::mbar_wait(&ctl->drain, 0, kWaitLimitNs, nullptr);
+    }
+  } else {
+    // ---- epilogue: warp w drains row quarter w % 4, tokens 8 (w / 4) .. +7 of each pass; then
+    // each warp sums the slices of two tokens, a channel a lane
+    const int q = warp % 4, tok8 = (warp / 4) * 8;
+    int n = 0;
+    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++n) {
+      const int b = p.bufs == 2 ? n & 1 : 0;
+      const int use = p.bufs == 2 ? n >> 1 : n;
+      const int ch = t * kSliceCh + lane;
+      const bool valid = ch < j.channels;
+      const float sc = valid ? j.channel_scales[ch] : 0.f;
+      const float sc2 = SILU && valid ? j.channel_scales[j.channels + ch] : 0.f;
+      const float bias =
+          !SILU && j.bias && valid ? Traits<T>::to_f(static_cast<const T*>(j.bias)[ch]) : 0.f;
+      bool ready =
+          tc::mbar_wait(&ctl->tmem_full[b], (uint32_t)use & 1u, kWaitLimitNs, &ctl->abort);
+      ready = epi_all(ready);
+      if (!ready) {
+        raise_fault(ctl, fault);
+        break;
+      }
+      tc::tc_fence_after();
+      const uint32_t acc = tmem + (uint32_t)(b * cols + (q % SL) * p.tc) + ((uint32_t)(q * 32) << 16);
+#pragma unroll 1
+      for (int tok0 = 0; tok0 < j.tokens; tok0 += kSliceTok) {
+        if (tok0 + tok8 < p.tc) {
+          uint32_t r[8];
+          tmem_ld8(acc + (uint32_t)(tok0 + tok8), r);
+          tc::tmem_wait_ld(r);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sums[(q * kSliceTok + tok8 + e) * kSliceCh + lane] = (int)r[e];
+        }
+        if (tok0 + kSliceTok >= j.tokens) {  // drained: the next tile's products may come
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&ctl->tmem_empty[b]);
+        }
+        epi_sync();
+#pragma unroll
+        for (int e = 0; e < kSliceTok / EPI_WARPS; ++e) {
+          const int i = warp + e * EPI_WARPS, tok = tok0 + i;
+          if (tok < j.tokens && valid) {
+            int v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = sums[(k * kSliceTok + i) * kSliceCh + lane];
+            const float st = __ldg(j.token_scales + tok);
+            float y;
+            if (SILU)
+              y = silu_mul<T>((float)(v[0] + v[1]) * st * sc, (float)(v[2] + v[3]) * st * sc2);
+            else
+              y = (float)(v[0] + v[1] + v[2] + v[3]) * st * sc + bias;
+            if (j.add) y += Traits<T>::to_f(static_cast<const T*>(j.add)[tok * j.add_stride + ch]);
+            static_cast<T*>(j.out)[tok * j.out_stride + ch] = Traits<T>::from_f(y);
+          }
+        }
+        epi_sync();
+      }
+    }
+  }
+
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tc::tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
 }
 
 // ------------------------------------------------------------ CUDA cores --
@@ -634,52 +851,39 @@ struct Call {
   const char* name;
 };
 
-// How the tokens lie in the tiles.  Up to 64 they are columns (16, 32 or 64 of
-// them); above that rows, of a CTA pair where more than 128.
-enum Way { kCols16, kCols32, kCols64, kRows128, kRows256 };
-inline Way way_of(int64_t tokens) {
-  if (tokens <= 16) return kCols16;
-  if (tokens <= 32) return kCols32;
-  if (tokens <= 64) return kCols64;
-  return tokens <= 128 ? kRows128 : kRows256;
-}
-
+constexpr int64_t kSliceTokens = 64;  // up to here the slice kernel
 // A worker's least share of a tile that is cut, in K blocks.
 constexpr int kLeastBlocks = 4;
 
 struct Plan {
-  int m_tiles, n_tiles, k_blocks, workers, split_workers;
+  Tiling t;
+  bool pair;
+  int workers;
   size_t slot_bytes;  // of all workers' partial sums
 };
 
-template <class S>
-inline Plan plan_of(int64_t tokens, int64_t channels, int64_t k, int sms) {
-  Plan p;
-  const int64_t rows = S::TOK_ROWS ? tokens : channels, cols = S::TOK_ROWS ? channels : tokens;
-  p.m_tiles = (int)ceil_div(rows, S::kRows);
-  p.n_tiles = (int)ceil_div(cols, S::kOutCols);
-  p.k_blocks = (int)ceil_div(k, BK);
-  const int64_t all = (int64_t)p.m_tiles * p.n_tiles;
-  const int most = std::max(1, S::PAIR ? sms / 2 : sms);
-  // all workers take whole tiles; those left over are cut over as many workers as have
-  // kLeastBlocks each
-  const int64_t left = all % most;
-  const int64_t units = left * p.k_blocks;
-  int64_t cut = std::min<int64_t>(most, std::max(left, units / kLeastBlocks));
-  if (cut == left && left > 0) cut = left;
-  p.split_workers = (int)cut;
+// The tiles left over after whole rounds, cut over as many workers as have
+// kLeastBlocks each.
+inline void cut_rest(Plan& p, int k_blocks, int most) {
+  const int64_t all = (int64_t)p.t.m_tiles * p.t.n_tiles, left = all % most;
+  const int64_t cut = std::min<int64_t>(most, std::max(left, left * k_blocks / kLeastBlocks));
+  p.t.split_workers = (int)cut;
   p.workers = all < most ? (int)std::max<int64_t>(1, cut) : most;
-  // whole tiles are dealt to `workers`, so with fewer than `most` none is whole
-  p.slot_bytes = left == 0 || cut == left
-                     ? 0
-                     : (size_t)p.split_workers * (S::PAIR ? 2 : 1) * 2 * S::kSlot * sizeof(int32_t);
-  return p;
+  p.slot_bytes = cut == left ? 0
+                             : (size_t)cut * (p.pair ? 2 : 1) * 2 * kSlot * sizeof(int32_t);
 }
 
-template <class S>
-size_t workspace_of(int64_t tokens, int64_t channels, int64_t k, int sms) {
-  const Plan p = plan_of<S>(tokens, channels, k, sms);
-  return p.slot_bytes ? (size_t)kCounterBytes + p.slot_bytes : 0;
+inline Plan plan_of(int64_t tokens, int64_t channels, int64_t k, bool silu, int sms) {
+  Plan p = {};
+  p.pair = tokens > BM;
+  p.t.bn = 256;
+  const int out_cols = silu ? p.t.bn / 2 : p.t.bn;
+  p.t.m_tiles = (int)ceil_div(tokens, p.pair ? 2 * BM : BM);
+  p.t.n_tiles = (int)ceil_div(channels, out_cols);
+  const int stage = BM * BK + (p.pair ? p.t.bn / 2 : p.t.bn) * BK;
+  p.t.stages = std::min(MAX_STAGES, kRingBytes / stage);
+  cut_rest(p, (int)ceil_div(k, BK), std::max(1, p.pair ? sms / 2 : sms));
+  return p;
 }
 
 int make_map(CUtensorMap* map, const int8_t* base, int64_t rows, int64_t k, int64_t stride, int box,
@@ -699,49 +903,63 @@ int make_map(CUtensorMap* map, const int8_t* base, int64_t rows, int64_t k, int6
   return PACE_OK;
 }
 
-template <typename T, class S>
-int launch_gemm(const Call& c, GemmJob j) {
-  const Plan p = plan_of<S>(c.tokens, c.channels, c.k, sm_count(c.device));
+inline int64_t weight_rows(const Call& c) { return c.silu ? 2 * c.channels : c.channels; }
+
+template <typename T, bool SILU>
+int launch_slices(const Call& c, const GemmJob& j) {
+  constexpr int SL = SILU ? 2 : 4;
+  SliceTiling p;
+  p.tc = (int)ceil_div(c.tokens, 8) * 8;
+  p.stages = std::min(kSliceStages, kSliceRing / (BM * BK + SL * p.tc * BK));
+  const int cols = SL * p.tc;
+  p.bufs = 2 * cols <= 256 ? 2 : 1;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < p.bufs * cols) p.tmem_cols *= 2;
+  p.tiles = (int)ceil_div(c.channels, kSliceCh);
+  p.slice_blocks = (int)ceil_div(j.k_blocks, SL);
+  CUtensorMap w, x;
+  int rc = make_map(&w, c.weight, weight_rows(c), c.k, c.weight_stride, kSliceCh, c.name);
+  if (rc == PACE_OK) rc = make_map(&x, c.codes, c.tokens, c.k, c.codes_stride, p.tc, c.name);
+  if (rc != PACE_OK) return rc;
+  auto kernel = int8_slice_kernel<T, SILU>;
+  cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kSliceSmem);
+  if (err != cudaSuccess) return cuda_fail(err, c.name);
+  const int grid = std::min(p.tiles, 2 * sm_count(c.device));
+  err = launch(kernel, dim3((unsigned)grid), dim3(THREADS), kSliceSmem, c.stream, w, x, j, p, c.fault);
+  return err == cudaSuccess ? PACE_OK : cuda_fail(err, c.name);
+}
+
+template <typename T, bool PAIR, bool SILU>
+int launch_gemm(const Call& c, const GemmJob& j, const Plan& p) {
   if (p.slot_bytes && (!c.workspace || c.workspace_bytes < kCounterBytes + p.slot_bytes ||
                        !aligned16(c.workspace)))
     return fail(PACE_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes (16-byte aligned) needed",
                 c.name, (size_t)kCounterBytes + p.slot_bytes);
-  j.m_tiles = p.m_tiles;
-  j.n_tiles = p.n_tiles;
-  j.k_blocks = p.k_blocks;
-  const int64_t w_rows = c.silu ? 2 * c.channels : c.channels;
-  CUtensorMap tok, ch;
-  constexpr int kTokBox = S::TOK_ROWS ? BM : S::BN;
-  constexpr int kChBox = S::TOK_ROWS ? (S::PAIR || S::SILU ? S::BN / 2 : S::BN) : BM;
-  int rc = make_map(&tok, c.codes, c.tokens, c.k, c.codes_stride, kTokBox, c.name);
-  if (rc == PACE_OK) rc = make_map(&ch, c.weight, w_rows, c.k, c.weight_stride, kChBox, c.name);
+  CUtensorMap a, b;
+  int rc = make_map(&a, c.codes, c.tokens, c.k, c.codes_stride, BM, c.name);
+  if (rc == PACE_OK)
+    rc = make_map(&b, c.weight, weight_rows(c), c.k, c.weight_stride,
+                  PAIR || SILU ? p.t.bn / 2 : p.t.bn, c.name);
   if (rc != PACE_OK) return rc;
-  auto kernel = int8_gemm_kernel<T, S>;
-  cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, S::kSmem);
+  auto kernel = int8_gemm_kernel<T, PAIR, SILU>;
+  cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kSmem);
   if (err != cudaSuccess) return cuda_fail(err, c.name);
   int32_t* counters = static_cast<int32_t*>(c.workspace);
   int32_t* slots = counters ? counters + kCounterBytes / 4 : nullptr;
-  const CUtensorMap& a = S::TOK_ROWS ? tok : ch;
-  const CUtensorMap& b = S::TOK_ROWS ? ch : tok;
-  if constexpr (S::PAIR)
-    err = launch_pairs(kernel, dim3((unsigned)(2 * p.workers)), dim3(THREADS), S::kSmem, c.stream,
-                       a, b, j, p.split_workers, counters, slots, c.fault);
+  if constexpr (PAIR)
+    err = launch_pairs(kernel, dim3((unsigned)(2 * p.workers)), dim3(THREADS), kSmem, c.stream, a,
+                       b, j, p.t, counters, slots, c.fault);
   else
-    err = launch(kernel, dim3((unsigned)p.workers), dim3(THREADS), S::kSmem, c.stream, a, b, j,
-                 p.split_workers, counters, slots, c.fault);
+    err = launch(kernel, dim3((unsigned)p.workers), dim3(THREADS), kSmem, c.stream, a, b, j, p.t,
+                 counters, slots, c.fault);
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, c.name);
 }
 
-// Calls f.template operator()<Shape>() for the tokens' way.
-template <bool SILU, typename F>
-auto with_shape(int64_t tokens, F f) {
-  switch (way_of(tokens)) {
-    case kCols16: return f(Shape<16, false, false, SILU>{});
-    case kCols32: return f(Shape<32, false, false, SILU>{});
-    case kCols64: return f(Shape<64, false, false, SILU>{});
-    case kRows128: return f(Shape<256, false, true, SILU>{});
-    default: return f(Shape<256, true, true, SILU>{});
-  }
+template <typename T, bool SILU>
+int launch_tensor(const Call& c, const GemmJob& j) {
+  if (c.tokens <= kSliceTokens) return launch_slices<T, SILU>(c, j);
+  const Plan p = plan_of(c.tokens, c.channels, c.k, SILU, sm_count(c.device));
+  return p.pair ? launch_gemm<T, true, SILU>(c, j, p) : launch_gemm<T, false, SILU>(c, j, p);
 }
 
 // Whether TMA takes both operands.
@@ -755,10 +973,9 @@ int run_typed(const Call& c, GemmJob j) {
   constexpr int V = Traits<T>::kVec;
   j.vec = aligned16(j.out) && j.out_stride % V == 0 &&
           (!j.add || (aligned16(j.add) && j.add_stride % V == 0));
-  if (for_tma(c)) {
-    auto go = [&](auto s) { return launch_gemm<T, decltype(s)>(c, j); };
-    return c.silu ? with_shape<true>(c.tokens, go) : with_shape<false>(c.tokens, go);
-  }
+  j.scales_vec = aligned16(j.channel_scales) && (!c.silu || c.channels % 4 == 0);
+  j.k_blocks = (int)ceil_div(c.k, BK);
+  if (for_tma(c)) return c.silu ? launch_tensor<T, true>(c, j) : launch_tensor<T, false>(c, j);
   const dim3 grid((unsigned)ceil_div(c.channels, kDotCh), (unsigned)ceil_div(c.tokens, kDotTok));
   if (ceil_div(c.tokens, kDotTok) > 65535)
     return fail(PACE_ERR_TOO_LARGE, "%s: over 2097120 tokens of rows that are not 16-byte aligned",
@@ -799,9 +1016,9 @@ extern "C" size_t pace_int8_linear_workspace_size(int64_t num_tokens, int64_t ou
   if (num_tokens <= 0 || num_tokens > INT32_MAX || out_features <= 0 ||
       out_features > (1 << 30) || k <= 0 || k > kMaxK)
     return 0;
-  const int sms = sm_count(device);
-  auto go = [&](auto s) { return workspace_of<decltype(s)>(num_tokens, out_features, k, sms); };
-  return gated ? with_shape<true>(num_tokens, go) : with_shape<false>(num_tokens, go);
+  if (num_tokens <= kSliceTokens) return 0;
+  const Plan p = plan_of(num_tokens, out_features, k, gated != 0, sm_count(device));
+  return p.slot_bytes ? (size_t)kCounterBytes + p.slot_bytes : 0;
 }
 
 extern "C" int pace_int8_linear(void* out, const int8_t* codes, const float* token_scales,

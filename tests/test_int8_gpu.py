@@ -287,7 +287,7 @@ def test_no_tokens():
     int8_ops.gate_up_silu(torch.empty(0, 16, device=DEV), x, s, w, sw)
 
 
-@pytest.mark.parametrize("t", [1, 64, 256])
+@pytest.mark.parametrize("t", [1, 64, 100, 256])
 def test_two_streams_and_graphs(t):
     """Cut tiles on two streams at once, and in two graphs replayed at once: a workspace each."""
     g = torch.Generator().manual_seed(t)
@@ -325,7 +325,7 @@ def test_two_streams_and_graphs(t):
 
 def test_callers_workspace():
     g = torch.Generator().manual_seed(3)
-    t, n, k = 5, 4096, 4096
+    t, n, k = 100, 2000, 4096  # more tokens than the kernel without a workspace takes
     x, sx, w, sw = make(g, t, n, k, torch.bfloat16)
     need = int8_ops.workspace_size(t, n, k)
     assert need > 4096
