@@ -569,28 +569,22 @@ int pace_silu_and_mul_quantise(int8_t* codes, float* scales, const void* input,
  *     llama.py:101-106, 176-178, 240-254).
  *   pace_int8_gate_up_silu: out[t, i] = (T)(silu(y[t, i]) * y[t, I + i]), as
  *     pace_gate_up_silu.
- * Out and residual are of `dtype`.  Workspace: 16-byte aligned, of
- * pace_int8_linear_workspace_size bytes (gated: 1 for gate_up_silu; 0 bytes:
- * NULL will do), its first 4096 bytes zero before the first call; calls leave
- * them zero, and calls that may overlap need one each.  On the tensor cores
- * where k, the row strides and the addresses of codes and weight are multiples
- * of 16 bytes, on the CUDA cores (slowly, without a workspace) otherwise.  Every
- * wait in the kernel is bounded by a second; one that runs out sets bit 30 of
- * *fault_flags, leaves the output undefined, and the workspace to be zeroed. */
-size_t pace_int8_linear_workspace_size(int64_t num_tokens, int64_t out_features, int64_t k,
-                                       int gated, int device);
+ * Out and residual are of `dtype`.  On the tensor cores where k, the row strides
+ * and the addresses of codes and weight are multiples of 16 bytes, on the CUDA
+ * cores (slowly) otherwise.  Every wait in the kernels is bounded by a second; one
+ * that runs out sets bit 30 of *fault_flags (may be NULL) and leaves the output
+ * undefined. */
 int pace_int8_linear(void* out, const int8_t* codes, const float* token_scales,
                      const int8_t* weight, const float* channel_scales, const void* bias,
                      const void* residual, int64_t num_tokens, int64_t out_features, int64_t k,
                      int64_t codes_row_stride, int64_t weight_row_stride, int64_t out_row_stride,
-                     int64_t residual_row_stride, int dtype, void* workspace,
-                     size_t workspace_bytes, int32_t* fault_flags, cudaStream_t stream);
+                     int64_t residual_row_stride, int dtype, int32_t* fault_flags,
+                     cudaStream_t stream);
 int pace_int8_gate_up_silu(void* out, const int8_t* codes, const float* token_scales,
                            const int8_t* weight, const float* channel_scales, int64_t num_tokens,
                            int64_t intermediate_size, int64_t k, int64_t codes_row_stride,
                            int64_t weight_row_stride, int64_t out_row_stride, int dtype,
-                           void* workspace, size_t workspace_bytes, int32_t* fault_flags,
-                           cudaStream_t stream);
+                           int32_t* fault_flags, cudaStream_t stream);
 
 /* ---- head norms with rotation ---------------------------------------------
  * pace_qk_norm_rotary_embedding: every head x of query and key (head_size

@@ -184,16 +184,14 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "pace_silu_and_mul_quantise": (
         c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int, _P]),
-    "pace_int8_linear_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
     "pace_int8_linear": (
         c_int,
         [_P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
-         c_int, _P, c_size_t, _P, _P],
+         c_int, _P, _P],
     ),
     "pace_int8_gate_up_silu": (
         c_int,
-        [_P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, _P,
-         c_size_t, _P, _P],
+        [_P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, _P, _P],
     ),
     "pace_qk_norm_rotary_embedding": (
         c_int,

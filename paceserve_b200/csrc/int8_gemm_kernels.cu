@@ -21,6 +21,7 @@
 // What TMA cannot take (K, a row stride or an address that is no multiple of 16
 // bytes) runs on the CUDA cores (int8_dot_kernel).
 #include <algorithm>
+#include <type_traits>
 
 #include "tcgen05.cuh"
 
@@ -39,9 +40,6 @@ constexpr int CH = 16;  // columns drained at a time
 constexpr uint64_t kWaitLimitNs = 1000000000ull;  // 1 s per wait
 constexpr int32_t kFaultTimeout = 1 << 30;
 constexpr int64_t kMaxK = 131071;
-// The workspace: arrival counters of the tiles that are cut, then the partial sums.
-constexpr int64_t kCounterBytes = 4096;
-constexpr int kSlot = BM * 256;  // int32 of a partial tile
 
 struct Ctl {
   uint64_t full[MAX_STAGES];
@@ -51,7 +49,6 @@ struct Ctl {
   uint64_t drain;
   uint32_t tmem;
   int abort;
-  int last;
 };
 static_assert(sizeof(Ctl) <= 256, "");
 
@@ -63,6 +60,7 @@ struct GemmJob {
   int64_t out_stride, add_stride;
   int tokens, channels;  // channels: output columns (half the weight's rows with SiLU)
   int k_blocks;
+  int deep;        // whole K blocks: the tensor maps have them as a third axis
   int vec;         // out (and add) take 16-byte accesses
   int scales_vec;  // the channels' scales do
 };
@@ -103,48 +101,38 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
       : "memory");
 }
 
+// The box of rows y .. of the K blocks z .. of a three-axis map (bytes of a block,
+// rows, blocks), in shared memory block by block; see make_map.
+__device__ __forceinline__ void tma_load_deep(void* dst, const CUtensorMap* map, int32_t y,
+                                              int32_t z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tc::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(y), "r"(z), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_deep_pair(void* dst, const CUtensorMap* map, int32_t y,
+                                                   int32_t z, uint32_t bar_cluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(tc::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(y), "r"(z), "r"(bar_cluster)
+      : "memory");
+}
+
 // Pulls a box of a tensor map into L2.
+__device__ __forceinline__ void prefetch_deep(const CUtensorMap* map, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(0), "r"(y), "r"(z)
+               : "memory");
+}
 __device__ __forceinline__ void prefetch_box(const CUtensorMap* map, int32_t x, int32_t y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
                "r"(x), "r"(y)
                : "memory");
 }
-
-// Split of the K blocks of the tiles [t_stop, ...) over the first `workers` workers.
-struct Split {
-  int64_t units;
-  int workers, k_blocks;
-  __device__ __forceinline__ int64_t start(int w) const { return (int64_t)w * units / workers; }
-  __device__ __forceinline__ int owner(int64_t u) const {
-    return (int)(((u + 1) * workers - 1) / units);
-  }
-};
-
-// A worker's segments in order: its range of the units of the tiles from t_stop
-// on, then whole tiles worker, worker + step, ... below t_stop.  What is cut comes
-// first, so that its joining hides behind the whole tiles' products.
-struct Walk {
-  int64_t t_next, t_stop, step;
-  int64_t u, u_end;
-  int k_blocks;
-  __device__ __forceinline__ bool next(int64_t& t, int& kb0, int& kb1) {
-    if (u < u_end) {
-      const int64_t rt = u / k_blocks;
-      t = t_stop + rt;
-      kb0 = (int)(u - rt * k_blocks);
-      kb1 = (int)min((int64_t)k_blocks, kb0 + (u_end - u));
-      u += kb1 - kb0;
-      return true;
-    }
-    if (t_next >= t_stop) return false;
-    t = t_next;
-    t_next += step;
-    kb0 = 0;
-    kb1 = k_blocks;
-    return true;
-  }
-};
 
 // Tile t's place: groups of kGroup rows of tiles, and within a group the rows
 // fastest, so that the tiles in work at one time are about as many tokens high as
@@ -186,28 +174,6 @@ template <typename T>
 __device__ __forceinline__ float silu_mul(float g, float u) {
   if constexpr (sizeof(T) == 2) return __fdividef(g, 1.f + __expf(-g)) * u;
   return g / (1.f + expf(-g)) * u;
-}
-
-// Partial sums: [4 columns][lane][4], so that a warp's instruction moves 512
-// contiguous bytes; through L2 only, since another SM reads them.
-__device__ __forceinline__ void store_partial(int32_t* slot, int col, int row,
-                                              const uint32_t (&r)[CH]) {
-#pragma unroll
-  for (int q = 0; q < CH / 4; ++q)
-    __stcg(reinterpret_cast<uint4*>(slot + ((int64_t)(col / 4 + q) * BM + row) * 4),
-           make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]));
-}
-__device__ __forceinline__ void add_partial(const int32_t* slot, int col, int row,
-                                            uint32_t (&r)[CH]) {
-#pragma unroll
-  for (int q = 0; q < CH / 4; ++q) {
-    const uint4 v =
-        __ldcg(reinterpret_cast<const uint4*>(slot + ((int64_t)(col / 4 + q) * BM + row) * 4));
-    r[4 * q] += v.x;
-    r[4 * q + 1] += v.y;
-    r[4 * q + 2] += v.z;
-    r[4 * q + 3] += v.w;
-  }
 }
 
 // Scales of CH consecutive channels (those past the last are never used).
@@ -262,11 +228,57 @@ __device__ __forceinline__ void put_channels(const GemmJob& j, int64_t t, int n,
   }
 }
 
-// How the rows kernel is cut: bn channels (gate and up together with SiLU) a tile,
-// `stages` ring stages, the first split_workers workers sharing the tiles left over.
+// Four consecutive channels n .. of one token, as put_channels.
+template <typename T>
+__device__ __forceinline__ void put_four(const GemmJob& j, int64_t t, int n, bool all, float* y) {
+  T* o = static_cast<T*>(j.out) + t * j.out_stride + n;
+  const T* add = j.add ? static_cast<const T*>(j.add) + t * j.add_stride + n : nullptr;
+  if (j.vec && all) {
+    using Four = std::conditional_t<sizeof(T) == 2, uint2, uint4>;
+    union {
+      Four v;
+      T x[4];
+    } f;
+    if (add) {
+      f.v = *reinterpret_cast<const Four*>(add);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += Traits<T>::to_f(f.x[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f.x[e] = Traits<T>::from_f(y[e]);
+    *reinterpret_cast<Four*>(o) = f.v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < j.channels)
+        o[e] = Traits<T>::from_f(add ? y[e] + Traits<T>::to_f(add[e]) : y[e]);
+  }
+}
+
+// Tiles of the rows kernel: bn channels (gate and up together with SiLU), `sub` K
+// blocks a ring stage.
 struct Tiling {
-  int bn, stages, m_tiles, n_tiles, split_workers;
+  int bn, sub, stages, m_tiles, n_tiles;
 };
+
+// One lane of the warp, the same in every call of the same warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
+// tc::mbar_wait with the clock read only when a wait is long.
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, Ctl* ctl) {
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (tc::mbar_try_wait(bar, parity)) return true;
+  return tc::mbar_wait(bar, parity, kWaitLimitNs, &ctl->abort);
+}
 
 // A ring position: the stage, and the parity of the phase that its barriers wait for.
 struct Turn {
@@ -280,36 +292,24 @@ struct Turn {
   }
 };
 
-template <typename T, bool PAIR, bool SILU>
+// 256 tokens a CTA pair: the leader's 128 in its accumulator, its partner's in its
+// own; each stages its tokens and half of the tile's channels.
+template <typename T, bool SILU>
 __global__ void __launch_bounds__(THREADS, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
                      const __grid_constant__ CUtensorMap tm_b, const GemmJob j, const Tiling p,
-                     int32_t* counters, int32_t* slots, int32_t* fault) {
-  constexpr int kRows = PAIR ? 2 * BM : BM, kA = BM * BK, kTmem = 512;
+                     int32_t* fault) {
+  constexpr int kA = BM * BK, kTmem = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   Ctl* ctl = reinterpret_cast<Ctl*>(tiles + kRingBytes);
-  const int nst = p.stages, bn = p.bn, out_cols = SILU ? bn / 2 : bn;
-  const int sb = kA + (PAIR ? bn / 2 : bn) * BK;  // bytes of a stage in this CTA
+  const int nst = p.stages, bn = p.bn, sub = p.sub, out_cols = SILU ? bn / 2 : bn;
+  const int kB = bn / 2 * BK, sb = kA + kB;  // bytes of a K block in this CTA
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cta = blockIdx.x;
-  const uint32_t rank = PAIR ? tc::cluster_rank() : 0u;
-  const int worker = PAIR ? cta >> 1 : cta;
-  const int workers = PAIR ? (int)gridDim.x >> 1 : (int)gridDim.x;
-  const int64_t n_all = (int64_t)p.m_tiles * p.n_tiles;
-  const int64_t t_stop = n_all / workers * workers;
-  Split sp;
-  sp.units = (n_all - t_stop) * j.k_blocks;
-  sp.workers = p.split_workers;
-  sp.k_blocks = j.k_blocks;
-  const bool splits = worker < p.split_workers;
-  const Walk walk0{worker,
-                   t_stop,
-                   (int64_t)workers,
-                   splits ? sp.start(worker) : 0,
-                   splits ? sp.start(worker + 1) : 0,
-                   j.k_blocks};
+  const uint32_t rank = tc::cluster_rank();
+  const int workers = (int)gridDim.x >> 1;
+  const int64_t t_first = blockIdx.x >> 1, t_end = (int64_t)p.m_tiles * p.n_tiles;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       tc::mbar_init(&ctl->tmem_full[b], 1);
-      tc::mbar_init(&ctl->tmem_empty[b], PAIR ? 2 * EPI_WARPS : EPI_WARPS);
+      tc::mbar_init(&ctl->tmem_empty[b], 2 * EPI_WARPS);
     }
     tc::mbar_init(&ctl->drain, 1);
     ctl->abort = 0;
@@ -329,77 +329,68 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc::tma_prefetch_desc(&tm_a);
     tc::tma_prefetch_desc(&tm_b);
   }
-  if (warp == 0) {
-    if constexpr (PAIR)
-      tc::tmem_alloc_pair(&ctl->tmem, kTmem);
-    else
-      tc::tmem_alloc(&ctl->tmem, kTmem);
-  }
+  if (warp == 0) tc::tmem_alloc_pair(&ctl->tmem, kTmem);
   tc::tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) tc::cluster_sync();
+  tc::cluster_sync();
   tc::tc_fence_after();
   const uint32_t tmem = ctl->tmem;
   pdl_wait();
 
   if (warp == EPI_WARPS) {
-    // ---- TMA producer -----------------------------------------------------
-    if (lane == 0) {
-      int64_t i = 0;
-      bool ok = true;
-      Walk walk = walk0;
-      Turn turn;
-      int64_t t;
-      int kb0, kb1;
-      const uint32_t full0 = PAIR ? tc::map_to_rank(&ctl->full[0], 0) : 0u;
-      while (ok && walk.next(t, kb0, kb1)) {
-        int mt, nt;
-        place_of(t, p.m_tiles, p.n_tiles, mt, nt);
-        const int a0 = mt * kRows + (int)rank * BM;
-        // B rows of this CTA: with SiLU gate rows and the up rows `channels` further (PAIR: the
-        // leader the gate's, its partner the up's)
-        const int b0 = SILU ? nt * out_cols + (int)rank * j.channels : nt * bn + (int)rank * (bn / 2);
-        for (int kb = kb0; kb < kb1; ++kb, ++i) {
-          const int s = turn.s;
-          if (i >= nst &&
-              !tc::mbar_wait(&ctl->empty[s], turn.phase ^ 1u, kWaitLimitNs, &ctl->abort)) {
-            ok = false;
-            break;
-          }
-          uint8_t* a = tiles + s * sb;
-          uint8_t* b = a + kA;
-          if constexpr (PAIR) {
-            const uint32_t bar = full0 + (uint32_t)(s * sizeof(uint64_t));
-            if (rank == 0) tc::mbar_arrive_expect_tx(&ctl->full[s], 2 * sb);
-            tc::tma_load_2d_pair(a, &tm_a, kb * BK, a0, bar);
-            tc::tma_load_2d_pair(b, &tm_b, kb * BK, b0, bar);
-          } else {
-            tc::mbar_arrive_expect_tx(&ctl->full[s], sb);
-            tc::tma_load_2d(a, &tm_a, kb * BK, a0, &ctl->full[s]);
-            tc::tma_load_2d(b, &tm_b, kb * BK, b0, &ctl->full[s]);
-            if (SILU)
-              tc::tma_load_2d(b + bn / 2 * BK, &tm_b, kb * BK, j.channels + b0, &ctl->full[s]);
-          }
-          turn.next(nst);
+    // ---- TMA producer: the whole warp walks, one lane issues ------------------
+    const bool issues = elect_one();
+    int64_t i = 0;
+    bool ok = true;
+    Turn turn;
+    // both CTAs' copies complete on the leader's barrier, which expects the bytes of both
+    const uint32_t full0 = tc::map_to_rank(&ctl->full[0], 0);
+    for (int64_t t = t_first; ok && t < t_end; t += workers) {
+      int mt, nt;
+      place_of(t, p.m_tiles, p.n_tiles, mt, nt);
+      const int a0 = (2 * mt + (int)rank) * BM;
+      // with SiLU the leader has the gate's rows, its partner the up's
+      const int b0 = SILU ? nt * out_cols + (int)rank * j.channels : nt * bn + (int)rank * (bn / 2);
+      for (int kb = 0; kb < j.k_blocks; kb += sub, ++i) {
+        const int s = turn.s;
+        if (i >= nst && !ring_wait(&ctl->empty[s], turn.phase ^ 1u, ctl)) {
+          ok = false;
+          break;
         }
+        if (issues) {
+          uint8_t* a = tiles + s * sub * sb;
+          uint8_t* b = a + sub * kA;
+          const uint32_t bar = full0 + (uint32_t)(s * sizeof(uint64_t));
+          if (rank == 0) tc::mbar_arrive_expect_tx(&ctl->full[s], 2 * sub * sb);
+          if (j.deep) {
+            tma_load_deep_pair(a, &tm_a, a0, kb, bar);
+            tma_load_deep_pair(b, &tm_b, b0, kb, bar);
+          } else {
+            for (int u = 0; u < sub; ++u) {
+              tc::tma_load_2d_pair(a + u * kA, &tm_a, (kb + u) * BK, a0, bar);
+              tc::tma_load_2d_pair(b + u * kB, &tm_b, (kb + u) * BK, b0, bar);
+            }
+          }
+        }
+        __syncwarp();
+        turn.next(nst);
       }
-      if (!ok) raise_fault(ctl, fault);
-      // every copy has landed before the shared memory is given up
-      if (!PAIR || rank == 0)
-        for (int64_t q = i > nst ? i - nst : 0; q < i; ++q)
-          tc::mbar_wait(&ctl->full[q % nst], (uint32_t)(q / nst) & 1u, kWaitLimitNs, nullptr);
     }
+    if (!ok && lane == 0) raise_fault(ctl, fault);
+    // every copy has landed before the shared memory is given up; the partner leaves after the
+    // leader, at the closing cluster barrier
+    if (rank == 0)
+      for (int64_t q = i > nst ? i - nst : 0; q < i; ++q)
+        tc::mbar_wait(&ctl->full[q % nst], (uint32_t)(q / nst) & 1u, kWaitLimitNs, nullptr);
   } else if (warp == EPI_WARPS + 1) {
-    // ---- MMA issuer ---------------------------------------------------------
-    if (lane == 0 && rank == 0) {
-      const uint32_t idesc = idesc_i8(kRows, bn);
+    // ---- MMA issuer, in the leader ------------------------------------------
+    if (rank == 0) {
+      const bool issues = elect_one();
+      const uint32_t idesc = idesc_i8(2 * BM, bn);
       int n = 0;
       bool ok = true;
-      Walk walk = walk0;
       Turn turn;
-      int64_t t;
-      int kb0, kb1;
-      for (; ok && walk.next(t, kb0, kb1); ++n) {
+      for (int64_t t = t_first; ok && t < t_end; t += workers, ++n) {
         const int b = n & 1;
         const uint32_t use_b = (uint32_t)(n >> 1);
         if (use_b > 0 &&
@@ -409,58 +400,51 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         tc::tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(b * 256);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = 0; kb < j.k_blocks; kb += sub) {
           const int s = turn.s;
-          if (!tc::mbar_wait(&ctl->full[s], turn.phase, kWaitLimitNs, &ctl->abort)) {
+          if (!ring_wait(&ctl->full[s], turn.phase, ctl)) {
             ok = false;
             break;
           }
           tc::tc_fence_after();
-          const uint32_t a_addr = tc::smem_u32(tiles + s * sb);
-          const uint64_t ad = tc::umma_desc_sw128(a_addr);
-          const uint64_t bd = tc::umma_desc_sw128(a_addr + kA);
+          if (issues) {
+            const uint32_t a_addr = tc::smem_u32(tiles + s * sub * sb);
+            uint64_t ad = tc::umma_desc_sw128(a_addr);
+            uint64_t bd = tc::umma_desc_sw128(a_addr + sub * kA);
+            for (int u = 0; u < sub; ++u) {  // blocks past K are zero
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            umma_i8<PAIR>(d, ad + 2 * k, bd + 2 * k, idesc, kb > kb0 || k > 0 ? 1u : 0u);
-          if constexpr (PAIR)
+              for (int k = 0; k < BK / 32; ++k)
+                umma_i8<true>(d, ad + 2 * k, bd + 2 * k, idesc, kb > 0 || u > 0 || k > 0 ? 1u : 0u);
+              ad += kA >> 4;
+              bd += (uint64_t)kB >> 4;
+            }
             tc::umma_commit_pair_both(&ctl->empty[s]);
-          else
-            tc::umma_commit(&ctl->empty[s]);
+          }
+          __syncwarp();
           turn.next(nst);
         }
-        if (ok) {
-          if constexpr (PAIR)
-            tc::umma_commit_pair_both(&ctl->tmem_full[b]);
-          else
-            tc::umma_commit(&ctl->tmem_full[b]);
-        }
+        if (ok && issues) tc::umma_commit_pair_both(&ctl->tmem_full[b]);
+        __syncwarp();
       }
-      if (!ok) raise_fault(ctl, fault);
+      if (!ok && lane == 0) raise_fault(ctl, fault);
       // every MMA has completed before TMEM is freed
-      if constexpr (PAIR)
-        tc::umma_commit_pair(&ctl->drain);
-      else
-        tc::umma_commit(&ctl->drain);
+      if (issues) tc::umma_commit_pair(&ctl->drain);
       tc::mbar_wait(&ctl->drain, 0, kWaitLimitNs, nullptr);
     }
   } else {
     // ---- epilogue: warp w drains lanes 32 (w % 4) .. +31, half w / 4 of the columns --------
     const int row = (warp % 4) * 32 + lane;
     const int c_begin = (warp / 4) * (out_cols / 2), c_end = c_begin + out_cols / 2;
-    const uint32_t tmem_empty0 = PAIR ? tc::map_to_rank(&ctl->tmem_empty[0], 0) : 0u;
+    const uint32_t tmem_empty0 = tc::map_to_rank(&ctl->tmem_empty[0], 0);
     const int up = bn / 2;  // SiLU: the up columns' distance
     int n = 0;
-    Walk walk = walk0;
-    int64_t t;
-    int kb0, kb1;
-    for (; walk.next(t, kb0, kb1); ++n) {
+    for (int64_t t = t_first; t < t_end; t += workers, ++n) {
       const int b = n & 1;
       int mt, nt;
       place_of(t, p.m_tiles, p.n_tiles, mt, nt);
-      const int m = mt * kRows + (int)rank * BM + row;  // this thread's token
-      const int c0 = nt * out_cols;                     // the tile's first channel
+      const int m = (2 * mt + (int)rank) * BM + row;  // this thread's token
+      const int c0 = nt * out_cols;                   // the tile's first channel
       const bool valid = m < j.tokens;
-      const bool whole = kb0 == 0 && kb1 == j.k_blocks;
       const float s_row = valid ? j.token_scales[m] : 0.f;
       bool ready = tc::mbar_wait(&ctl->tmem_full[b], (uint32_t)(n >> 1) & 1u, kWaitLimitNs,
                                  &ctl->abort);
@@ -471,100 +455,45 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       tc::tc_fence_after();
       const uint32_t acc = tmem + (uint32_t)(b * 256) + ((uint32_t)(warp % 4 * 32) << 16);
-      int w0 = 0, w1 = 0;  // the tile's workers
-      bool finish = true;
-      if (!whole) {
-        const int64_t u0 = (t - t_stop) * j.k_blocks;
-        w0 = sp.owner(u0);
-        w1 = sp.owner(u0 + j.k_blocks - 1);
-        // slot 0: the part that begins the tile, 1: one that goes on with it
-        int32_t* slot = slots + ((int64_t)cta * 2 + (kb0 == 0 ? 0 : 1)) * kSlot;
 #pragma unroll 1
-        for (int c = c_begin; c < c_end && c0 + c < j.channels; c += CH) {
-          __syncwarp();
-          uint32_t r[CH], r2[CH];
-          tc::tmem_ld16(acc + (uint32_t)c, r);
-          if (SILU) tc::tmem_ld16(acc + (uint32_t)(c + up), r2);
-          tc::tmem_wait_ld(r);
-          if (SILU) tc::tmem_wait_ld(r2);
-          if (valid) {
-            store_partial(slot, c, row, r);
-            if (SILU) store_partial(slot, c + up, row, r2);
-          }
-        }
-        // the last of the tile's workers finishes it.  A pair's CTAs have rows of their own
-        epi_sync();
-        if (threadIdx.x == 0) {
-          int32_t* counter = counters + (t - t_stop) * (PAIR ? 2 : 1) + rank;
-          uint32_t before;
-          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
-                       : "=r"(before)
-                       : "l"(counter)
-                       : "memory");
-          const bool last = before == (uint32_t)(w1 - w0);
-          if (last) *counter = 0;
-          ctl->last = last;
-        }
-        epi_sync();
-        finish = *reinterpret_cast<volatile int*>(&ctl->last) != 0;
-      }
-      if (finish) {
-#pragma unroll 1
-        for (int c = c_begin; c < c_end && c0 + c < j.channels; c += CH) {
-          __syncwarp();
-          uint32_t r[CH], r2[CH];
-          tc::tmem_ld16(acc + (uint32_t)c, r);
-          if (SILU) tc::tmem_ld16(acc + (uint32_t)(c + up), r2);
-          const int ch = c0 + c;
-          float sc[CH], sc2[CH];
-          load_scales(j, ch, sc);
-          if (SILU) load_scales(j, j.channels + ch, sc2);
-          tc::tmem_wait_ld(r);
-          if (SILU) tc::tmem_wait_ld(r2);
-          if (valid) {
-            if (!whole) {
-              for (int w = w0; w <= w1; ++w) {
-                if (w == worker) continue;
-                const int32_t* slot =
-                    slots + ((int64_t)(PAIR ? 2 * w + (int)rank : w) * 2 + (w == w0 ? 0 : 1)) * kSlot;
-                add_partial(slot, c, row, r);
-                if (SILU) add_partial(slot, c + up, row, r2);
-              }
-            }
-            float y[CH];
+      for (int c = c_begin; c < c_end && c0 + c < j.channels; c += CH) {
+        __syncwarp();
+        uint32_t r[CH], r2[CH];
+        tc::tmem_ld16(acc + (uint32_t)c, r);
+        if (SILU) tc::tmem_ld16(acc + (uint32_t)(c + up), r2);
+        const int ch = c0 + c;
+        float sc[CH], sc2[CH];
+        load_scales(j, ch, sc);
+        if (SILU) load_scales(j, j.channels + ch, sc2);
+        tc::tmem_wait_ld(r);
+        if (SILU) tc::tmem_wait_ld(r2);
+        if (valid) {
+          float y[CH];
 #pragma unroll
-            for (int e = 0; e < CH; ++e) {
-              y[e] = (float)(int)r[e] * s_row * sc[e];
-              if (SILU) y[e] = silu_mul<T>(y[e], (float)(int)r2[e] * s_row * sc2[e]);
-            }
-            if (!SILU && j.bias) {
-              const T* bias = static_cast<const T*>(j.bias);
-#pragma unroll
-              for (int e = 0; e < CH; ++e) y[e] += Traits<T>::to_f(bias[min(ch + e, j.channels - 1)]);
-            }
-            put_channels<T>(j, m, ch, y);
+          for (int e = 0; e < CH; ++e) {
+            y[e] = (float)(int)r[e] * s_row * sc[e];
+            if (SILU) y[e] = silu_mul<T>(y[e], (float)(int)r2[e] * s_row * sc2[e]);
           }
+          if (!SILU && j.bias) {
+            const T* bias = static_cast<const T*>(j.bias);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) y[e] += Traits<T>::to_f(bias[min(ch + e, j.channels - 1)]);
+          }
+          put_channels<T>(j, m, ch, y);
         }
       }
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if constexpr (PAIR)
-          tc::mbar_arrive_cluster(tmem_empty0 + (uint32_t)(b * sizeof(uint64_t)));
-        else
-          tc::mbar_arrive(&ctl->tmem_empty[b]);
-      }
+      if (lane == 0) tc::mbar_arrive_cluster(tmem_empty0 + (uint32_t)(b * sizeof(uint64_t)));
     }
   }
 
   tc::tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) {
-    tc::cluster_sync();
-    if (warp == 0) tc::tmem_dealloc_pair(tmem, kTmem);
-  } else {
-    if (warp == 0) tc::tmem_dealloc(tmem, kTmem);
-  }
+  // neither CTA leaves (nor frees TMEM) while its partner may still signal its barriers or read its
+  // shared memory
+  tc::cluster_sync();
+  if (warp == 0) tc::tmem_dealloc_pair(tmem, kTmem);
 }
 
 // ------------------------------------------------------------- few tokens --
@@ -581,12 +510,12 @@ __global__ void __launch_bounds__(THREADS, 1)
 // shared memory, so none of their CTAs can wait beside one of these for its columns.
 constexpr int kSliceCh = 32, kSliceTok = 16;  // of a tile; of a pass through shared memory
 constexpr int kSliceRing = 98304;
-constexpr int kSliceStages = 6;
+constexpr int kSliceAhead = 12;  // blocks that are pulled into L2 ahead of their copy
 constexpr int kSliceSum = 4 * kSliceCh * kSliceTok * 4;
-constexpr int kSliceSmem = kSliceRing + kSliceSum + 1024 + 256;
+constexpr int kSliceRest = kSliceSum + 1024 + 256;
 
 struct SliceTiling {
-  int tc, stages, bufs, tmem_cols, tiles, slice_blocks;
+  int tc, stages, ring, bufs, tmem_cols, tiles, slice_blocks;
 };
 
 template <typename T, bool SILU>
@@ -598,12 +527,11 @@ __global__ void __launch_bounds__(THREADS, 2)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  int32_t* sums = reinterpret_cast<int32_t*>(tiles + kSliceRing);  // [quarter][token][channel]
-  Ctl* ctl = reinterpret_cast<Ctl*>(tiles + kSliceRing + kSliceSum);
+  int32_t* sums = reinterpret_cast<int32_t*>(tiles + p.ring);  // [quarter][token][channel]
+  Ctl* ctl = reinterpret_cast<Ctl*>(tiles + p.ring + kSliceSum);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sb = kA + SL * p.tc * BK, cols = SL * p.tc;
 
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       tc::mbar_init(&ctl->full[s], 1);
@@ -619,55 +547,71 @@ __global__ void __launch_bounds__(THREADS, 2)
   }
   // The weight's boxes of quarter q: channels of tile t (the up's with SiLU from quarter 2 on)
   auto w_row = [&](int t, int q) { return t * kSliceCh + (SILU && q >= SL ? j.channels : 0); };
-  auto w_col = [&](int kb, int q) { return ((q % SL) * p.slice_blocks + kb) * BK; };
+  auto w_col = [&](int kb, int q) { return (kb * SL + q % SL) * BK; };
   if (warp == EPI_WARPS && lane == 0) {
     tc::tma_prefetch_desc(&tm_w);
     tc::tma_prefetch_desc(&tm_x);
     // L2 is the point of coherence: what an earlier kernel still writes to the weight is read from
     // there after the wait
-    for (int kb = 0; kb < min(p.slice_blocks, 2 * p.stages); ++kb)
-      for (int q = 0; q < 4; ++q)
-        prefetch_box(&tm_w, w_col(kb, q), w_row((int)blockIdx.x, q));
+    for (int kb = 0; kb < min(p.slice_blocks, kSliceAhead); ++kb)
+      for (int q = 0; q < 4; q += j.deep ? SL : 1) {
+        if (j.deep)
+          prefetch_deep(&tm_w, w_row((int)blockIdx.x, q), kb * SL);
+        else
+          prefetch_box(&tm_w, w_col(kb, q), w_row((int)blockIdx.x, q));
+      }
   }
   if (warp == 0) tc::tmem_alloc(&ctl->tmem, (uint32_t)p.tmem_cols);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = ctl->tmem;
+  pdl_launch_dependents();
   pdl_wait();
 
   if (warp == EPI_WARPS) {
-    // ---- TMA producer -----------------------------------------------------
-    if (lane == 0) {
+    // ---- TMA producer: the whole warp walks, one lane issues ------------------
+    {
+      const bool issues = elect_one();
       int64_t i = 0;
       bool ok = true;
       Turn turn;
       for (int t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
         for (int kb = 0; kb < p.slice_blocks; ++kb, ++i) {
           const int s = turn.s;
-          if (i >= p.stages &&
-              !tc::mbar_wait(&ctl->empty[s], turn.phase ^ 1u, kWaitLimitNs, &ctl->abort)) {
+          if (i >= p.stages && !ring_wait(&ctl->empty[s], turn.phase ^ 1u, ctl)) {
             ok = false;
             break;
           }
-          uint8_t* a = tiles + s * sb;
-          tc::mbar_arrive_expect_tx(&ctl->full[s], (uint32_t)sb);
+          if (issues) {
+            uint8_t* a = tiles + s * sb;
+            tc::mbar_arrive_expect_tx(&ctl->full[s], (uint32_t)sb);
+            if (j.deep) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            tc::tma_load_2d(a + q * kBox, &tm_w, w_col(kb, q), w_row(t, q), &ctl->full[s]);
+              for (int q = 0; q < 4; q += SL)
+                tma_load_deep(a + q * kBox, &tm_w, w_row(t, q), kb * SL, &ctl->full[s]);
+              tma_load_deep(a + kA, &tm_x, 0, kb * SL, &ctl->full[s]);
+            } else {
 #pragma unroll
-          for (int q = 0; q < SL; ++q)
-            tc::tma_load_2d(a + kA + q * p.tc * BK, &tm_x, w_col(kb, q), 0, &ctl->full[s]);
+              for (int q = 0; q < 4; ++q)
+                tc::tma_load_2d(a + q * kBox, &tm_w, w_col(kb, q), w_row(t, q), &ctl->full[s]);
+#pragma unroll
+              for (int q = 0; q < SL; ++q)
+                tc::tma_load_2d(a + kA + q * p.tc * BK, &tm_x, w_col(kb, q), 0, &ctl->full[s]);
+            }
+          }
+          __syncwarp();
           turn.next(p.stages);
         }
       }
-      if (!ok) raise_fault(ctl, fault);
+      if (!ok && lane == 0) raise_fault(ctl, fault);
       for (int64_t q = i > p.stages ? i - p.stages : 0; q < i; ++q)
         tc::mbar_wait(&ctl->full[q % p.stages], (uint32_t)(q / p.stages) & 1u, kWaitLimitNs, nullptr);
     }
   } else if (warp == EPI_WARPS + 1) {
     // ---- MMA issuer ---------------------------------------------------------
-    if (lane == 0) {
+    {
+      const bool issues = elect_one();
       const uint32_t idesc = idesc_i8(BM, cols);
       int n = 0;
       bool ok = true;
@@ -684,24 +628,28 @@ __global__ void __launch_bounds__(THREADS, 2)
         const uint32_t d = tmem + (uint32_t)(b * cols);
         for (int kb = 0; kb < p.slice_blocks; ++kb) {
           const int s = turn.s;
-          if (!tc::mbar_wait(&ctl->full[s], turn.phase, kWaitLimitNs, &ctl->abort)) {
+          if (!ring_wait(&ctl->full[s], turn.phase, ctl)) {
             ok = false;
             break;
           }
           tc::tc_fence_after();
-          const uint32_t a_addr = tc::smem_u32(tiles + s * sb);
-          const uint64_t ad = tc::umma_desc_sw128(a_addr);
-          const uint64_t bd = tc::umma_desc_sw128(a_addr + kA);
+          if (issues) {
+            const uint32_t a_addr = tc::smem_u32(tiles + s * sb);
+            const uint64_t ad = tc::umma_desc_sw128(a_addr);
+            const uint64_t bd = tc::umma_desc_sw128(a_addr + kA);
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            umma_i8<false>(d, ad + 2 * k, bd + 2 * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
-          tc::umma_commit(&ctl->empty[s]);
+            for (int k = 0; k < BK / 32; ++k)
+              umma_i8<false>(d, ad + 2 * k, bd + 2 * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
+            tc::umma_commit(&ctl->empty[s]);
+          }
+          __syncwarp();
           turn.next(p.stages);
         }
-        if (ok) tc::umma_commit(&ctl->tmem_full[b]);
+        if (ok && issues) tc::umma_commit(&ctl->tmem_full[b]);
+        __syncwarp();
       }
-      if (!ok) raise_fault(ctl, fault);
-      tc::umma_commit(&ctl->drain);
+      if (!ok && lane == 0) raise_fault(ctl, fault);
+      if (issues) tc::umma_commit(&ctl->drain);
       tc::mbar_wait(&ctl->drain, 0, kWaitLimitNs, nullptr);
     }
   } else {
@@ -718,6 +666,10 @@ __global__ void __launch_bounds__(THREADS, 2)
       const float sc2 = SILU && valid ? j.channel_scales[j.channels + ch] : 0.f;
       const float bias =
           !SILU && j.bias && valid ? Traits<T>::to_f(static_cast<const T*>(j.bias)[ch]) : 0.f;
+      float st[kSliceTok / EPI_WARPS];  // the next pass's token scales
+#pragma unroll
+      for (int e = 0; e < kSliceTok / EPI_WARPS; ++e)
+        st[e] = __ldg(j.token_scales + min(warp + e * EPI_WARPS, j.tokens - 1));
       bool ready =
           tc::mbar_wait(&ctl->tmem_full[b], (uint32_t)use & 1u, kWaitLimitNs, &ctl->abort);
       ready = epi_all(ready);
@@ -749,15 +701,15 @@ __global__ void __launch_bounds__(THREADS, 2)
             int v[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = sums[(k * kSliceTok + i) * kSliceCh + lane];
-            const float st = __ldg(j.token_scales + tok);
             float y;
             if (SILU)
-              y = silu_mul<T>((float)(v[0] + v[1]) * st * sc, (float)(v[2] + v[3]) * st * sc2);
+              y = silu_mul<T>((float)(v[0] + v[1]) * st[e] * sc, (float)(v[2] + v[3]) * st[e] * sc2);
             else
-              y = (float)(v[0] + v[1] + v[2] + v[3]) * st * sc + bias;
+              y = (float)(v[0] + v[1] + v[2] + v[3]) * st[e] * sc + bias;
             if (j.add) y += Traits<T>::to_f(static_cast<const T*>(j.add)[tok * j.add_stride + ch]);
             static_cast<T*>(j.out)[tok * j.out_stride + ch] = Traits<T>::from_f(y);
           }
+          st[e] = __ldg(j.token_scales + min(tok + kSliceTok, j.tokens - 1));
         }
         epi_sync();
       }
@@ -766,6 +718,212 @@ __global__ void __launch_bounds__(THREADS, 2)
 
   tc::tc_fence_before();
   __syncthreads();
+  if (warp == 0) tc::tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
+}
+
+// ------------------------------------------------------- a middling number --
+// 128 channels (64 gates and their 64 ups with SiLU) in the accumulator's rows and
+// up to 128 tokens in its columns, K cut over the CTAs of a cluster: each works out
+// a partial tile, puts it into its shared memory, and then sums its share of the
+// tokens over the cluster's shared memories.  So the tile is large enough not to
+// read the operands from L2 many times over, there are CTAs for all SMs, and the
+// joining costs two cluster barriers.  Which CTA sums what is fixed, and sums of
+// integers are exact.
+constexpr int kMidRing = 98304;
+constexpr int kMidAhead = 8;  // K blocks that are pulled into L2 before the wait
+constexpr int kMidSmem = kMidRing + 1024 + 256;
+constexpr int kMidTok = 128;  // of a tile, at most
+
+struct MidTiling {
+  int bt, stages, tmem_cols, tok_tiles, cut;  // tokens a tile; CTAs of a cluster
+};
+
+// 16 bytes of the shared memory of the cluster's CTA `rank`, at this CTA's address p.
+__device__ __forceinline__ int4 ld_cluster(const int32_t* p, uint32_t rank) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(tc::map_to_rank(p, rank))
+               : "memory");
+  return v;
+}
+
+template <typename T, bool SILU>
+__global__ void __launch_bounds__(THREADS, 2)
+    int8_mid_kernel(const __grid_constant__ CUtensorMap tm_w,
+                    const __grid_constant__ CUtensorMap tm_x, const GemmJob j, const MidTiling p,
+                    int32_t* fault) {
+  constexpr int kA = BM * BK, kOut = SILU ? BM / 2 : BM;  // channels of a tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* tiles = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  int32_t* part = reinterpret_cast<int32_t*>(tiles);  // [token][row], over the ring
+  Ctl* ctl = reinterpret_cast<Ctl*>(tiles + kMidRing);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sb = kA + p.bt * BK;  // bytes of a stage
+  const int rank = (int)tc::cluster_rank();
+  const int tile = (int)blockIdx.x / p.cut;
+  const int n0 = tile / p.tok_tiles * kOut, t0 = tile % p.tok_tiles * p.bt;
+  const int kb0 = (int)((int64_t)rank * j.k_blocks / p.cut);
+  const int kb1 = (int)((int64_t)(rank + 1) * j.k_blocks / p.cut);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      tc::mbar_init(&ctl->full[s], 1);
+      tc::mbar_init(&ctl->empty[s], 1);
+    }
+    tc::mbar_init(&ctl->tmem_full[0], 1);
+    ctl->abort = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == EPI_WARPS && lane == 0) {
+    tc::tma_prefetch_desc(&tm_w);
+    tc::tma_prefetch_desc(&tm_x);
+    // L2 is the point of coherence: what an earlier kernel still writes to the weight is read from
+    // there after the wait
+    for (int kb = kb0; kb < min(kb1, kb0 + kMidAhead); ++kb) {
+      prefetch_box(&tm_w, kb * BK, n0);
+      if (SILU) prefetch_box(&tm_w, kb * BK, j.channels + n0);
+    }
+  }
+  if (warp == 0) tc::tmem_alloc(&ctl->tmem, (uint32_t)p.tmem_cols);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  if (warp == EPI_WARPS) {
+    // ---- TMA producer: the whole warp walks, one lane issues ------------------
+    {
+      const bool issues = elect_one();
+      bool ok = true;
+      Turn turn;
+      int i = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++i) {
+        const int s = turn.s;
+        if (i >= p.stages && !ring_wait(&ctl->empty[s], turn.phase ^ 1u, ctl)) {
+          ok = false;
+          break;
+        }
+        if (issues) {
+          uint8_t* a = tiles + s * sb;
+          tc::mbar_arrive_expect_tx(&ctl->full[s], (uint32_t)sb);
+          tc::tma_load_2d(a, &tm_w, kb * BK, n0, &ctl->full[s]);
+          if (SILU) tc::tma_load_2d(a + kA / 2, &tm_w, kb * BK, j.channels + n0, &ctl->full[s]);
+          tc::tma_load_2d(a + kA, &tm_x, kb * BK, t0, &ctl->full[s]);
+        }
+        __syncwarp();
+        turn.next(p.stages);
+      }
+      if (!ok && lane == 0) raise_fault(ctl, fault);
+      for (int q = i > p.stages ? i - p.stages : 0; q < i; ++q)
+        tc::mbar_wait(&ctl->full[q % p.stages], (uint32_t)(q / p.stages) & 1u, kWaitLimitNs, nullptr);
+    }
+  } else if (warp == EPI_WARPS + 1) {
+    // ---- MMA issuer ---------------------------------------------------------
+    {
+      const bool issues = elect_one();
+      const uint32_t idesc = idesc_i8(BM, p.bt);
+      bool ok = true;
+      Turn turn;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int s = turn.s;
+        if (!ring_wait(&ctl->full[s], turn.phase, ctl)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        if (issues) {
+          const uint32_t a_addr = tc::smem_u32(tiles + s * sb);
+          const uint64_t ad = tc::umma_desc_sw128(a_addr);
+          const uint64_t bd = tc::umma_desc_sw128(a_addr + kA);
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            umma_i8<false>(tmem, ad + 2 * k, bd + 2 * k, idesc, kb > kb0 || k > 0 ? 1u : 0u);
+          tc::umma_commit(&ctl->empty[s]);
+        }
+        __syncwarp();
+        turn.next(p.stages);
+      }
+      if (!ok && lane == 0) raise_fault(ctl, fault);
+      // the last commit follows all products, whether or not all were issued
+      if (issues) tc::umma_commit(&ctl->tmem_full[0]);
+      tc::mbar_wait(&ctl->tmem_full[0], 0, kWaitLimitNs, nullptr);
+    }
+  } else {
+    // ---- the partial tile goes to shared memory: warp w row quarter w % 4, half w / 4 of the tokens
+    const int row = (warp % 4) * 32 + lane, c0 = (warp / 4) * (p.bt / 2);
+    const bool ready = tc::mbar_wait(&ctl->tmem_full[0], 0, kWaitLimitNs, &ctl->abort);
+    // all eight take one way: the ring is written over only when every product has read it
+    if (epi_all(ready)) {
+      tc::tc_fence_after();
+      const uint32_t acc = tmem + ((uint32_t)(warp % 4 * 32) << 16);
+#pragma unroll 1
+      for (int c = c0; c < c0 + p.bt / 2 && t0 + c < j.tokens; c += 8) {
+        uint32_t r[8];
+        tmem_ld8(acc + (uint32_t)c, r);
+        tc::tmem_wait_ld(r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[(c + e) * BM + row] = (int)r[e];
+      }
+    } else {
+      raise_fault(ctl, fault);
+    }
+  }
+  tc::tc_fence_before();
+  __syncwarp();
+  tc::cluster_sync();
+
+  // ---- a warp a token (two with SiLU), four channels a lane, summed over the cluster -----------
+  {
+    constexpr int kLanes = kOut / 4, kEach = 32 / kLanes;  // of a token; tokens of a warp
+    const int ch = n0 + (lane % kLanes) * 4;
+    const bool four = ch + 4 <= j.channels;
+    float sc[4], sc2[4], bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = min(ch + e, j.channels - 1);
+      sc[e] = __ldg(j.channel_scales + n);
+      sc2[e] = SILU ? __ldg(j.channel_scales + j.channels + n) : 0.f;
+      bias[e] = !SILU && j.bias ? Traits<T>::to_f(static_cast<const T*>(j.bias)[n]) : 0.f;
+    }
+    const int end = min(p.bt, j.tokens - t0);
+    for (int c = rank + (warp * kEach + lane / kLanes) * p.cut; c < end;
+         c += (THREADS / 32) * kEach * p.cut) {
+      int4 v = make_int4(0, 0, 0, 0), u = v;
+      const int32_t* at = part + c * BM + (lane % kLanes) * 4;
+#pragma unroll 4
+      for (int k = 0; k < p.cut; ++k) {
+        const int4 x = ld_cluster(at, (uint32_t)k);
+        v.x += x.x;
+        v.y += x.y;
+        v.z += x.z;
+        v.w += x.w;
+        if (SILU) {
+          const int4 z = ld_cluster(at + BM / 2, (uint32_t)k);
+          u.x += z.x;
+          u.y += z.y;
+          u.z += z.z;
+          u.w += z.w;
+        }
+      }
+      const int64_t t = t0 + c;
+      const float st = __ldg(j.token_scales + t);
+      const int g[4] = {v.x, v.y, v.z, v.w}, h[4] = {u.x, u.y, u.z, u.w};
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[e] = (float)g[e] * st * sc[e] + bias[e];
+        if (SILU) y[e] = silu_mul<T>(y[e], (float)h[e] * st * sc2[e]);
+      }
+      put_four<T>(j, t, ch, four, y);
+    }
+  }
+  // no CTA leaves while another reads its shared memory
+  __syncwarp();
+  tc::cluster_sync();
   if (warp == 0) tc::tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
 }
 
@@ -843,59 +1001,60 @@ struct Call {
   const int8_t *codes, *weight;
   int64_t codes_stride, weight_stride, tokens, k, channels;
   bool silu;
-  void* workspace;
-  size_t workspace_bytes;
   int32_t* fault;
   int dtype, device;
   cudaStream_t stream;
   const char* name;
 };
 
-constexpr int64_t kSliceTokens = 64;  // up to here the slice kernel
-// A worker's least share of a tile that is cut, in K blocks.
-constexpr int kLeastBlocks = 4;
+constexpr int64_t kSliceTokens = 32;  // up to here the slice kernel
+constexpr int64_t kMidTokens = 128;   // up to here the cluster kernel, above by rows_plan
 
-struct Plan {
+// Tiles for the rows kernel: 128, 192 or 256 channels, whichever takes least by what a round of tiles
+// over the pairs costs (B200, ns a K block, and us for a call's start and end):
+//   128: 195, 6.8;  192: 275, 8.0;  256: 295, 9.1
+// (512 tokens, K 4096: 6144 channels 19.2, 17.5, 19.3 us; 4096 channels 13.4, 16.7, 18.5.)
+struct RowsPlan {
   Tiling t;
-  bool pair;
-  int workers;
-  size_t slot_bytes;  // of all workers' partial sums
+  int pairs;
 };
-
-// The tiles left over after whole rounds, cut over as many workers as have
-// kLeastBlocks each.
-inline void cut_rest(Plan& p, int k_blocks, int most) {
-  const int64_t all = (int64_t)p.t.m_tiles * p.t.n_tiles, left = all % most;
-  const int64_t cut = std::min<int64_t>(most, std::max(left, left * k_blocks / kLeastBlocks));
-  p.t.split_workers = (int)cut;
-  p.workers = all < most ? (int)std::max<int64_t>(1, cut) : most;
-  p.slot_bytes = cut == left ? 0
-                             : (size_t)cut * (p.pair ? 2 : 1) * 2 * kSlot * sizeof(int32_t);
+inline RowsPlan rows_plan(int64_t tokens, int64_t channels, int k_blocks, bool silu, int sms) {
+  static constexpr struct {
+    int bn;
+    double block, fixed;
+  } kinds[] = {{128, 0.195, 6.8}, {192, 0.275, 8.0}, {256, 0.295, 9.1}};
+  RowsPlan best = {};
+  double least = 0;
+  const int pairs = std::max(1, sms / 2);
+  for (const auto& kind : kinds) {
+    const int64_t m = ceil_div(tokens, 2 * BM), n = ceil_div(channels, silu ? kind.bn / 2 : kind.bn);
+    const double cost = kind.fixed + (double)ceil_div(m * n, pairs) * k_blocks * kind.block;
+    if (best.pairs != 0 && cost >= least) continue;
+    least = cost;
+    best.t.bn = kind.bn;
+    best.t.m_tiles = (int)m;
+    best.t.n_tiles = (int)n;
+    best.pairs = (int)std::min<int64_t>(m * n, pairs);
+  }
+  // two K blocks a stage halve what a stage costs beside its bytes (128 channels: 270 -> 195 ns);
+  // at 256 the products take longer than that anyway, and more stages are better
+  best.t.sub = best.t.bn == 256 ? 1 : 2;
+  best.t.stages = std::min(MAX_STAGES, kRingBytes / (best.t.sub * (BM + best.t.bn / 2) * BK));
+  return best;
 }
 
-inline Plan plan_of(int64_t tokens, int64_t channels, int64_t k, bool silu, int sms) {
-  Plan p = {};
-  p.pair = tokens > BM;
-  p.t.bn = 256;
-  const int out_cols = silu ? p.t.bn / 2 : p.t.bn;
-  p.t.m_tiles = (int)ceil_div(tokens, p.pair ? 2 * BM : BM);
-  p.t.n_tiles = (int)ceil_div(channels, out_cols);
-  const int stage = BM * BK + (p.pair ? p.t.bn / 2 : p.t.bn) * BK;
-  p.t.stages = std::min(MAX_STAGES, kRingBytes / stage);
-  cut_rest(p, (int)ceil_div(k, BK), std::max(1, p.pair ? sms / 2 : sms));
-  return p;
-}
-
+// Boxes of `box` rows of a K block, or (deep, where K is whole blocks) of `blocks`
+// K blocks: the third axis steps by a block within the row.
 int make_map(CUtensorMap* map, const int8_t* base, int64_t rows, int64_t k, int64_t stride, int box,
-             const char* name) {
+             bool deep, int blocks, const char* name) {
   tc::EncodeTiledFn enc = tc::encode_tiled();
   if (!enc) return fail(PACE_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", name);
-  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)stride};
-  const cuuint32_t boxes[2] = {(cuuint32_t)BK, (cuuint32_t)box};
-  const cuuint32_t steps[2] = {1, 1};
-  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims,
-                         strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const cuuint64_t dims[3] = {(cuuint64_t)(deep ? BK : k), (cuuint64_t)rows, (cuuint64_t)(k / BK)};
+  const cuuint64_t strides[2] = {(cuuint64_t)stride, (cuuint64_t)BK};
+  const cuuint32_t boxes[3] = {(cuuint32_t)BK, (cuuint32_t)box, (cuuint32_t)blocks};
+  const cuuint32_t steps[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, deep ? 3 : 2, const_cast<int8_t*>(base),
+                         dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
@@ -910,56 +1069,87 @@ int launch_slices(const Call& c, const GemmJob& j) {
   constexpr int SL = SILU ? 2 : 4;
   SliceTiling p;
   p.tc = (int)ceil_div(c.tokens, 8) * 8;
-  p.stages = std::min(kSliceStages, kSliceRing / (BM * BK + SL * p.tc * BK));
+  p.tiles = (int)ceil_div(c.channels, kSliceCh);
+  const int stage = BM * BK + SL * p.tc * BK;
+  p.slice_blocks = (int)ceil_div(j.k_blocks, SL);
+  // With a tile for each SM at most, and more blocks than two turns of the ring, one CTA an SM takes
+  // the whole shared memory (a token, K 14336, 4096 channels: 12.3 us against 14.4); a short K has
+  // no use for it (K 4096: 5.6 against 5.5)
+  p.stages = kSliceRing / stage;
+  if (p.tiles <= sm_count(c.device) && p.slice_blocks > 2 * p.stages) p.stages = kRingBytes / stage;
+  p.stages = std::min(MAX_STAGES, p.stages);
+  p.ring = p.stages * stage;
   const int cols = SL * p.tc;
   p.bufs = 2 * cols <= 256 ? 2 : 1;
   p.tmem_cols = 32;
   while (p.tmem_cols < p.bufs * cols) p.tmem_cols *= 2;
-  p.tiles = (int)ceil_div(c.channels, kSliceCh);
-  p.slice_blocks = (int)ceil_div(j.k_blocks, SL);
   CUtensorMap w, x;
-  int rc = make_map(&w, c.weight, weight_rows(c), c.k, c.weight_stride, kSliceCh, c.name);
-  if (rc == PACE_OK) rc = make_map(&x, c.codes, c.tokens, c.k, c.codes_stride, p.tc, c.name);
+  int rc = make_map(&w, c.weight, weight_rows(c), c.k, c.weight_stride, kSliceCh, j.deep, SL, c.name);
+  if (rc == PACE_OK)
+    rc = make_map(&x, c.codes, c.tokens, c.k, c.codes_stride, p.tc, j.deep, SL, c.name);
   if (rc != PACE_OK) return rc;
   auto kernel = int8_slice_kernel<T, SILU>;
-  cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kSliceSmem);
+  cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kRingBytes + kSliceRest);
   if (err != cudaSuccess) return cuda_fail(err, c.name);
   const int grid = std::min(p.tiles, 2 * sm_count(c.device));
-  err = launch(kernel, dim3((unsigned)grid), dim3(THREADS), kSliceSmem, c.stream, w, x, j, p, c.fault);
+  err = launch(kernel, dim3((unsigned)grid), dim3(THREADS), p.ring + kSliceRest, c.stream, w, x, j, p, c.fault);
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, c.name);
 }
 
-template <typename T, bool PAIR, bool SILU>
-int launch_gemm(const Call& c, const GemmJob& j, const Plan& p) {
-  if (p.slot_bytes && (!c.workspace || c.workspace_bytes < kCounterBytes + p.slot_bytes ||
-                       !aligned16(c.workspace)))
-    return fail(PACE_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes (16-byte aligned) needed",
-                c.name, (size_t)kCounterBytes + p.slot_bytes);
-  CUtensorMap a, b;
-  int rc = make_map(&a, c.codes, c.tokens, c.k, c.codes_stride, BM, c.name);
+template <typename T, bool SILU>
+int launch_mid(const Call& c, const GemmJob& j) {
+  MidTiling p;
+  p.tok_tiles = (int)ceil_div(c.tokens, kMidTok);
+  p.bt = (int)ceil_div(ceil_div(c.tokens, p.tok_tiles), 16) * 16;
+  p.stages = std::min(MAX_STAGES, kMidRing / (BM * BK + p.bt * BK));
+  p.tmem_cols = 32;
+  while (p.tmem_cols < p.bt) p.tmem_cols *= 2;
+  const int tiles = (int)ceil_div(c.channels, SILU ? BM / 2 : BM) * p.tok_tiles;
+  // CTAs for two an SM, with 8 K blocks each at least (4096 x 4096, 64 tokens: 8 blocks 8.7 us, 4
+  // blocks 9.6), in clusters of a power of two, which find room on the SMs (48 tiles of 128
+  // channels, 64 tokens: clusters of 4 10.1 us, of 6 17.1)
+  p.cut = 1;
+  while (p.cut < 8 && tiles * p.cut * 2 <= 2 * sm_count(c.device) && j.k_blocks / (p.cut * 2) >= 8)
+    p.cut *= 2;
+  CUtensorMap w, x;
+  int rc = make_map(&w, c.weight, weight_rows(c), c.k, c.weight_stride, SILU ? BM / 2 : BM, false, 1,
+                    c.name);
   if (rc == PACE_OK)
-    rc = make_map(&b, c.weight, weight_rows(c), c.k, c.weight_stride,
-                  PAIR || SILU ? p.t.bn / 2 : p.t.bn, c.name);
+    rc = make_map(&x, c.codes, c.tokens, c.k, c.codes_stride, p.bt, false, 1, c.name);
   if (rc != PACE_OK) return rc;
-  auto kernel = int8_gemm_kernel<T, PAIR, SILU>;
+  auto kernel = int8_mid_kernel<T, SILU>;
+  cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kMidSmem);
+  if (err != cudaSuccess) return cuda_fail(err, c.name);
+  err = launch_clusters(kernel, p.cut, dim3((unsigned)(tiles * p.cut)), dim3(THREADS), kMidSmem,
+                        c.stream, w, x, j, p, c.fault);
+  return err == cudaSuccess ? PACE_OK : cuda_fail(err, c.name);
+}
+
+template <typename T, bool SILU>
+int launch_rows(const Call& c, const GemmJob& j, const RowsPlan& p) {
+  CUtensorMap a, b;
+  int rc = make_map(&a, c.codes, c.tokens, c.k, c.codes_stride, BM, j.deep, p.t.sub, c.name);
+  if (rc == PACE_OK)
+    rc = make_map(&b, c.weight, weight_rows(c), c.k, c.weight_stride, p.t.bn / 2, j.deep, p.t.sub,
+                  c.name);
+  if (rc != PACE_OK) return rc;
+  auto kernel = int8_gemm_kernel<T, SILU>;
   cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kSmem);
   if (err != cudaSuccess) return cuda_fail(err, c.name);
-  int32_t* counters = static_cast<int32_t*>(c.workspace);
-  int32_t* slots = counters ? counters + kCounterBytes / 4 : nullptr;
-  if constexpr (PAIR)
-    err = launch_pairs(kernel, dim3((unsigned)(2 * p.workers)), dim3(THREADS), kSmem, c.stream, a,
-                       b, j, p.t, counters, slots, c.fault);
-  else
-    err = launch(kernel, dim3((unsigned)p.workers), dim3(THREADS), kSmem, c.stream, a, b, j, p.t,
-                 counters, slots, c.fault);
+  err = launch_pairs(kernel, dim3((unsigned)(2 * p.pairs)), dim3(THREADS), kSmem, c.stream, a, b, j,
+                     p.t, c.fault);
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, c.name);
 }
 
 template <typename T, bool SILU>
 int launch_tensor(const Call& c, const GemmJob& j) {
   if (c.tokens <= kSliceTokens) return launch_slices<T, SILU>(c, j);
-  const Plan p = plan_of(c.tokens, c.channels, c.k, SILU, sm_count(c.device));
-  return p.pair ? launch_gemm<T, true, SILU>(c, j, p) : launch_gemm<T, false, SILU>(c, j, p);
+  // more tokens go to the cluster kernel too where whole tiles would leave half of the SMs idle
+  // (256 tokens, K 14336, 4096 channels: 22 us against 28)
+  const int sms = sm_count(c.device);
+  const RowsPlan p = rows_plan(c.tokens, c.channels, j.k_blocks, SILU, sms);
+  return c.tokens <= kMidTokens || p.pairs <= sms / 4 ? launch_mid<T, SILU>(c, j)
+                                                      : launch_rows<T, SILU>(c, j, p);
 }
 
 // Whether TMA takes both operands.
@@ -975,6 +1165,7 @@ int run_typed(const Call& c, GemmJob j) {
           (!j.add || (aligned16(j.add) && j.add_stride % V == 0));
   j.scales_vec = aligned16(j.channel_scales) && (!c.silu || c.channels % 4 == 0);
   j.k_blocks = (int)ceil_div(c.k, BK);
+  j.deep = c.k % BK == 0;
   if (for_tma(c)) return c.silu ? launch_tensor<T, true>(c, j) : launch_tensor<T, false>(c, j);
   const dim3 grid((unsigned)ceil_div(c.channels, kDotCh), (unsigned)ceil_div(c.tokens, kDotTok));
   if (ceil_div(c.tokens, kDotTok) > 65535)
@@ -1010,24 +1201,12 @@ int run_int8(Call c, GemmJob j) {
 }  // namespace
 }  // namespace pace
 
-extern "C" size_t pace_int8_linear_workspace_size(int64_t num_tokens, int64_t out_features,
-                                                  int64_t k, int gated, int device) {
-  using namespace pace;
-  if (num_tokens <= 0 || num_tokens > INT32_MAX || out_features <= 0 ||
-      out_features > (1 << 30) || k <= 0 || k > kMaxK)
-    return 0;
-  if (num_tokens <= kSliceTokens) return 0;
-  const Plan p = plan_of(num_tokens, out_features, k, gated != 0, sm_count(device));
-  return p.slot_bytes ? (size_t)kCounterBytes + p.slot_bytes : 0;
-}
-
 extern "C" int pace_int8_linear(void* out, const int8_t* codes, const float* token_scales,
                                 const int8_t* weight, const float* channel_scales,
                                 const void* bias, const void* residual, int64_t num_tokens,
                                 int64_t out_features, int64_t k, int64_t codes_row_stride,
                                 int64_t weight_row_stride, int64_t out_row_stride,
-                                int64_t residual_row_stride, int dtype, void* workspace,
-                                size_t workspace_bytes, int32_t* fault_flags,
+                                int64_t residual_row_stride, int dtype, int32_t* fault_flags,
                                 cudaStream_t stream) {
   pace::GemmJob j = {};
   j.out = out;
@@ -1038,8 +1217,7 @@ extern "C" int pace_int8_linear(void* out, const int8_t* codes, const float* tok
   j.out_stride = out_row_stride;
   j.add_stride = residual_row_stride;
   return pace::run_int8({codes, weight, codes_row_stride, weight_row_stride, num_tokens, k,
-                         out_features, false, workspace, workspace_bytes, fault_flags, dtype, 0,
-                         stream, "int8_linear"},
+                         out_features, false, fault_flags, dtype, 0, stream, "int8_linear"},
                         j);
 }
 
@@ -1047,8 +1225,7 @@ extern "C" int pace_int8_gate_up_silu(void* out, const int8_t* codes, const floa
                                       const int8_t* weight, const float* channel_scales,
                                       int64_t num_tokens, int64_t intermediate_size, int64_t k,
                                       int64_t codes_row_stride, int64_t weight_row_stride,
-                                      int64_t out_row_stride, int dtype, void* workspace,
-                                      size_t workspace_bytes, int32_t* fault_flags,
+                                      int64_t out_row_stride, int dtype, int32_t* fault_flags,
                                       cudaStream_t stream) {
   pace::GemmJob j = {};
   j.out = out;
@@ -1056,7 +1233,6 @@ extern "C" int pace_int8_gate_up_silu(void* out, const int8_t* codes, const floa
   j.channel_scales = channel_scales;
   j.out_stride = out_row_stride;
   return pace::run_int8({codes, weight, codes_row_stride, weight_row_stride, num_tokens, k,
-                         intermediate_size, true, workspace, workspace_bytes, fault_flags, dtype, 0,
-                         stream, "int8_gate_up_silu"},
+                         intermediate_size, true, fault_flags, dtype, 0, stream, "int8_gate_up_silu"},
                         j);
 }

@@ -1416,82 +1416,35 @@ void silu_and_mul_quantise(Tensor& codes, Tensor& scales, const Tensor& input) {
                op);
 }
 
-// The partial sums' workspace where the caller passes none.  Outside of a
-// capture: one for each (device, stream), large enough for any shape, so that
-// it is never exchanged under a kernel that uses it.  Inside: one for each
-// capture and stream, zeroed by the graph itself at its first use, so that no
-// two graphs share one; it lives in the graph's memory.
-Tensor int8_workspace(const at::Device& dev, cudaStream_t stream, size_t bytes) {
-  constexpr int64_t kCounterBytes = 4096;  // as the C ABI asks: zero before the first call
-  struct Entry {
-    unsigned long long capture = 0;
-    Tensor ws;
-  };
-  static std::mutex mu;
-  static std::map<std::pair<int, cudaStream_t>, Entry> eager, captured;
-  const auto bytes_of = at::TensorOptions().dtype(at::kByte).device(dev);
-  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-  unsigned long long id = 0;
-  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id));
-  std::lock_guard<std::mutex> lock(mu);
-  const bool capturing = status == cudaStreamCaptureStatusActive;
-  Entry& e = (capturing ? captured : eager)[{dev.index(), stream}];
-  if (!e.ws.defined() || (size_t)e.ws.numel() < bytes || (capturing && e.capture != id)) {
-    // eager: any shape's need on this device is at most 2 partial tiles of 128 x 256 a CTA
-    const int64_t most =
-        kCounterBytes +
-        (int64_t)at::cuda::getDeviceProperties(dev.index())->multiProcessorCount * 2 * 128 * 256 * 4;
-    e.ws = at::empty({capturing ? (int64_t)bytes : std::max<int64_t>(most, (int64_t)bytes)},
-                     bytes_of);
-    e.ws.narrow(0, 0, kCounterBytes).zero_();
-    e.capture = id;
-  }
-  return e.ws;
-}
-
 struct Int8Args {
-  Rows x, w;
-  Tensor ws;
+  Rows x, w, out;
+  int32_t* fault;
 };
 
-Int8Args check_int8(const Tensor& out, const Tensor& codes, const Tensor& token_scales,
-                    const Tensor& weight, const Tensor& channel_scales, bool gated,
-                    const c10::optional<Tensor>& workspace, const char* op) {
-  check_cuda(out, op, gated ? "out" : "out or residual");
-  TORCH_CHECK(is_float_type(out) && out.dim() == 2, op,
-              ": the output must be [tokens, features] of float32, float16 or bfloat16");
-  Int8Args a{codes_of(codes, token_scales, out, op, "codes", "token_scales"),
-             codes_of(weight, channel_scales, out, op, "weight", "channel_scales"), Tensor()};
-  const int64_t n = gated ? a.w.rows / 2 : a.w.rows;
+Int8Args check_int8(const Tensor& out, const char* out_name, const Tensor& codes,
+                    const Tensor& token_scales, const Tensor& weight, const Tensor& channel_scales,
+                    bool gated, const c10::optional<Tensor>& fault_flags, const char* op) {
+  check_cuda(out, op, out_name);
+  TORCH_CHECK(is_float_type(out) && out.dim() == 2, op, ": ", out_name,
+              " must be [tokens, features] of float32, float16 or bfloat16");
+  const Int8Args a{codes_of(codes, token_scales, out, op, "codes", "token_scales"),
+                   codes_of(weight, channel_scales, out, op, "weight", "channel_scales"),
+                   rows_of(out, op, out_name),
+                   counter_ptr(fault_flags, out.device(), op, "fault_flags")};
   TORCH_CHECK(!gated || a.w.rows % 2 == 0, op, ": weight needs as many gate as up rows");
-  TORCH_CHECK(a.x.width == a.w.width && out.size(0) == a.x.rows && out.size(1) == n, op,
-              ": shapes do not match: output ", out.sizes(), ", codes ", codes.sizes(),
+  TORCH_CHECK(a.x.width == a.w.width && a.out.rows == a.x.rows &&
+                  a.out.width == (gated ? a.w.rows / 2 : a.w.rows),
+              op, ": shapes do not match: ", out_name, " ", out.sizes(), ", codes ", codes.sizes(),
               ", weight ", weight.sizes());
-  if (a.x.rows == 0) return a;
-  const size_t need =
-      pace_int8_linear_workspace_size(a.x.rows, n, a.x.width, gated, out.device().index());
-  if (workspace.has_value()) {
-    a.ws = *workspace;
-    TORCH_CHECK(a.ws.is_cuda() && a.ws.device() == out.device() && a.ws.is_contiguous() &&
-                    (size_t)a.ws.nbytes() >= need,
-                op, ": workspace must be a contiguous tensor of at least ", need, " bytes on ",
-                out.device());
-  } else if (need > 0) {
-    a.ws = int8_workspace(out.device(), stream_of(out), need);
-  }
   return a;
 }
 
 void int8_linear_into(Tensor& out, const Tensor& codes, const Tensor& token_scales,
                       const Tensor& weight, const Tensor& channel_scales,
                       const c10::optional<Tensor>& bias, bool residual,
-                      const c10::optional<Tensor>& workspace,
                       const c10::optional<Tensor>& fault_flags, const char* op) {
-  check_cuda(out, op, residual ? "residual" : "out");
-  const at::cuda::CUDAGuard guard(out.device());
-  const Int8Args a =
-      check_int8(out, codes, token_scales, weight, channel_scales, false, workspace, op);
-  const Rows o = rows_of(out, op, residual ? "residual" : "out");
+  const Int8Args a = check_int8(out, residual ? "residual" : "out", codes, token_scales, weight,
+                                channel_scales, false, fault_flags, op);
   const void* b = nullptr;
   if (bias.has_value()) {
     check_same_device(*bias, out, op);
@@ -1500,50 +1453,43 @@ void int8_linear_into(Tensor& out, const Tensor& codes, const Tensor& token_scal
                 op, ": bias must be a contiguous [", a.w.rows, "] tensor of the output's dtype");
     b = bias->data_ptr();
   }
-  int32_t* fault = counter_ptr(fault_flags, out.device(), op, "fault_flags");
+  const at::cuda::CUDAGuard guard(out.device());
   check_status(pace_int8_linear(out.data_ptr(), codes.data_ptr<int8_t>(),
                                 token_scales.data_ptr<float>(), weight.data_ptr<int8_t>(),
                                 channel_scales.data_ptr<float>(), b,
                                 residual ? out.data_ptr() : nullptr, a.x.rows, a.w.rows, a.x.width,
-                                a.x.stride, a.w.stride, o.stride, o.stride, pace_dtype(out),
-                                ws_ptr(a.ws), ws_bytes(a.ws), fault, stream_of(out)),
+                                a.x.stride, a.w.stride, a.out.stride, a.out.stride,
+                                pace_dtype(out), a.fault, stream_of(out)),
                op);
 }
 
 void int8_linear(Tensor& out, const Tensor& codes, const Tensor& token_scales,
                  const Tensor& weight, const Tensor& channel_scales,
-                 const c10::optional<Tensor>& bias, const c10::optional<Tensor>& workspace,
-                 const c10::optional<Tensor>& fault_flags) {
-  int8_linear_into(out, codes, token_scales, weight, channel_scales, bias, false, workspace,
-                   fault_flags, "int8_linear");
+                 const c10::optional<Tensor>& bias, const c10::optional<Tensor>& fault_flags) {
+  int8_linear_into(out, codes, token_scales, weight, channel_scales, bias, false, fault_flags,
+                   "int8_linear");
 }
 
 void int8_linear_residual(Tensor& residual, const Tensor& codes, const Tensor& token_scales,
                           const Tensor& weight, const Tensor& channel_scales,
                           const c10::optional<Tensor>& bias,
-                          const c10::optional<Tensor>& workspace,
                           const c10::optional<Tensor>& fault_flags) {
-  int8_linear_into(residual, codes, token_scales, weight, channel_scales, bias, true, workspace,
-                   fault_flags, "int8_linear_residual");
+  int8_linear_into(residual, codes, token_scales, weight, channel_scales, bias, true, fault_flags,
+                   "int8_linear_residual");
 }
 
 void int8_gate_up_silu(Tensor& out, const Tensor& codes, const Tensor& token_scales,
                        const Tensor& weight, const Tensor& channel_scales,
-                       const c10::optional<Tensor>& workspace,
                        const c10::optional<Tensor>& fault_flags) {
   const char* op = "int8_gate_up_silu";
-  check_cuda(out, op, "out");
-  const at::cuda::CUDAGuard guard(out.device());
   const Int8Args a =
-      check_int8(out, codes, token_scales, weight, channel_scales, true, workspace, op);
-  const Rows o = rows_of(out, op, "out");
-  int32_t* fault = counter_ptr(fault_flags, out.device(), op, "fault_flags");
+      check_int8(out, "out", codes, token_scales, weight, channel_scales, true, fault_flags, op);
+  const at::cuda::CUDAGuard guard(out.device());
   check_status(pace_int8_gate_up_silu(out.data_ptr(), codes.data_ptr<int8_t>(),
                                       token_scales.data_ptr<float>(), weight.data_ptr<int8_t>(),
-                                      channel_scales.data_ptr<float>(), a.x.rows, o.width,
-                                      a.x.width, a.x.stride, a.w.stride, o.stride,
-                                      pace_dtype(out), ws_ptr(a.ws), ws_bytes(a.ws), fault,
-                                      stream_of(out)),
+                                      channel_scales.data_ptr<float>(), a.x.rows, a.out.width,
+                                      a.x.width, a.x.stride, a.w.stride, a.out.stride,
+                                      pace_dtype(out), a.fault, stream_of(out)),
                op);
 }
 
@@ -1738,24 +1684,15 @@ PYBIND11_MODULE(_C, m) {
          "the sums exact in 32 bits.",
          py::arg("out"), py::arg("codes"), py::arg("token_scales"), py::arg("weight"),
          py::arg("channel_scales"), py::arg("bias") = py::none(),
-         py::arg("workspace") = py::none(), py::arg("fault_flags") = py::none());
+         py::arg("fault_flags") = py::none());
   i8.def("linear_residual", &int8_linear_residual, "residual += the same product.",
          py::arg("residual"), py::arg("codes"), py::arg("token_scales"), py::arg("weight"),
          py::arg("channel_scales"), py::arg("bias") = py::none(),
-         py::arg("workspace") = py::none(), py::arg("fault_flags") = py::none());
+         py::arg("fault_flags") = py::none());
   i8.def("gate_up_silu", &int8_gate_up_silu,
          "out = silu(gate) * up, [gate | up] the same product with a weight [2 I, k].",
          py::arg("out"), py::arg("codes"), py::arg("token_scales"), py::arg("weight"),
-         py::arg("channel_scales"), py::arg("workspace") = py::none(),
-         py::arg("fault_flags") = py::none());
-  i8.def("workspace_size",
-         [](int64_t num_tokens, int64_t out_features, int64_t k, bool gated, int64_t device) {
-           return pace_int8_linear_workspace_size(num_tokens, out_features, k, gated ? 1 : 0,
-                                                  (int)device);
-         },
-         "Bytes of workspace (its first 4096 zeroed) a product of this shape needs.",
-         py::arg("num_tokens"), py::arg("out_features"), py::arg("k"), py::arg("gated") = false,
-         py::arg("device") = 0);
+         py::arg("channel_scales"), py::arg("fault_flags") = py::none());
 
   auto kv = m.def_submodule("kv_transfer_ops");
   kv.def("copy_blocks_p2p", &copy_blocks_p2p,

@@ -42,7 +42,7 @@ def test_int8_argument_errors():
     lib = cabi.load()
     bf = cabi.PACE_BF16
     linear = lambda t, n, k, xs, ws, os, p=None: lib.pace_int8_linear(  # noqa: E731
-        p, p, p, p, p, None, None, t, n, k, xs, ws, os, 0, bf, None, 0, None, None)
+        p, p, p, p, p, None, None, t, n, k, xs, ws, os, 0, bf, None, None)
     _expect(linear(-1, 8, 16, 16, 16, 8), BAD, "bad shape")
     _expect(linear(4, 0, 16, 16, 16, 8), BAD, "bad shape")
     _expect(linear(4, 8, 16, 15, 16, 8), BAD, "row stride")
@@ -57,19 +57,6 @@ def test_int8_argument_errors():
     _expect(lib.pace_silu_and_mul_quantise(None, None, None, 2, 8, 15, 8, bf, None), BAD, "row stride")
     _expect(lib.pace_quantise_rows(64, 64, 64, 2, 8, 8, 8, cabi.PACE_I32, None),
             cabi.PACE_ERR_UNSUPPORTED_DTYPE, "dtype")
-
-
-def test_workspace_sizes():
-    """None where no tile is cut over K; never more than two partial tiles of 128 x 256 a CTA."""
-    size = cabi.load().pace_int8_linear_workspace_size
-    most = 4096 + 148 * 2 * 128 * 256 * 4
-    assert size(0, 4096, 4096, 0, 0) == 0
-    assert size(1, 128 * 148, 4096, 0, 0) == 0  # a tile a CTA
-    for t in (1, 16, 17, 33, 64, 65, 128, 129, 500, 5000):
-        for n in (1, 300, 4096, 6144, 28672):
-            for k in (16, 512, 4096, 14336):
-                for gated in (0, 1):
-                    assert size(t, n, k, gated, 0) <= most
 
 
 def test_head_argument_errors():
