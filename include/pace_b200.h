@@ -569,9 +569,8 @@ int pace_silu_and_mul_quantise(int8_t* codes, float* scales, const void* input,
  *     llama.py:101-106, 176-178, 240-254).
  *   pace_int8_gate_up_silu: out[t, i] = (T)(silu(y[t, i]) * y[t, I + i]), as
  *     pace_gate_up_silu.
- * Out and residual are of `dtype`.  On the tensor cores where k, the row strides
- * and the addresses of codes and weight are multiples of 16 bytes, on the CUDA
- * cores (slowly) otherwise.  Every wait in the kernels is bounded by a second; one
+ * Out and residual are of `dtype`.  Any k, strides and addresses; fast where k, the
+ * row strides and the addresses of codes and weight are multiples of 16 bytes.  Every wait in the kernels is bounded by a second; one
  * that runs out sets bit 30 of *fault_flags (may be NULL) and leaves the output
  * undefined. */
 int pace_int8_linear(void* out, const int8_t* codes, const float* token_scales,
@@ -600,6 +599,8 @@ int pace_int8_gate_up_silu(void* out, const int8_t* codes, const float* token_sc
  *   outside it, and a slot of a token whose position is outside the table, is
  *   counted into *bad_tokens (may be NULL) and left out.  No two tokens may have
  *   the same slot.
+ * Every wait is bounded by a second; one that runs out sets bit 30 of *fault_flags
+ * (may be NULL) and leaves the outputs undefined.
  * No reference kernel; RMSNorm per head, rotary_embedding and the append in one. */
 int pace_qk_norm_rotary_embedding(const int64_t* positions, void* query, void* key,
                                   const void* q_weight, const void* k_weight, float epsilon,
@@ -607,7 +608,8 @@ int pace_qk_norm_rotary_embedding(const int64_t* positions, void* query, void* k
                                   int head_size, int64_t query_row_stride,
                                   int64_t key_row_stride, const void* cos_sin_cache,
                                   int cache_dtype, int rot_dim, int64_t max_position,
-                                  int is_neox, int dtype, cudaStream_t stream);
+                                  int is_neox, int dtype, int32_t* fault_flags,
+                                  cudaStream_t stream);
 int pace_qk_norm_rotary_append(const int64_t* positions, void* query, const void* key,
                                const void* value, const void* q_weight, const void* k_weight,
                                float epsilon, int64_t num_tokens, int num_heads, int num_kv_heads,
@@ -616,7 +618,7 @@ int pace_qk_norm_rotary_append(const int64_t* positions, void* query, const void
                                int cache_dtype, int rot_dim, int64_t max_position, int is_neox,
                                void* paged_cache, int64_t num_pages, int page_size,
                                const int64_t* slot_mapping, int32_t* bad_tokens, int dtype,
-                               cudaStream_t stream);
+                               int32_t* fault_flags, cudaStream_t stream);
 
 /* ---- paged attention ------------------------------------------------------
  * Attention of each request's newest tokens over its paged sequence.  For query

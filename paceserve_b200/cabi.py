@@ -196,12 +196,12 @@ SIGNATURES: dict[str, tuple] = {
     "pace_qk_norm_rotary_embedding": (
         c_int,
         [_P, _P, _P, _P, _P, c_float, c_int64, c_int, c_int, c_int, c_int64, c_int64, _P, c_int,
-         c_int, c_int64, c_int, c_int, _P],
+         c_int, c_int64, c_int, c_int, _P, _P],
     ),
     "pace_qk_norm_rotary_append": (
         c_int,
         [_P, _P, _P, _P, _P, _P, c_float, c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int64,
-         _P, c_int, c_int, c_int64, c_int, _P, c_int64, c_int, _P, _P, c_int, _P],
+         _P, c_int, c_int, c_int64, c_int, _P, c_int64, c_int, _P, _P, c_int, _P, _P],
     ),
     "pace_enable_peer_access": (c_int, [c_int, c_int]),
     "pace_can_access_peer": (c_int, [c_int, c_int, POINTER(c_int)]),

@@ -19,7 +19,7 @@
 //    the slices agree are partial sums, the others are not read.
 //
 // What TMA cannot take (K, a row stride or an address that is no multiple of 16
-// bytes) runs on the CUDA cores (int8_dot_kernel).
+// bytes) runs through registers and small matrix instructions (int8_dot_kernel).
 #include <algorithm>
 #include <type_traits>
 
@@ -927,72 +927,105 @@ __global__ void __launch_bounds__(THREADS, 2)
   if (warp == 0) tc::tmem_dealloc(tmem, (uint32_t)p.tmem_cols);
 }
 
-// ------------------------------------------------------------ CUDA cores --
-// Any K, stride and alignment: 32 tokens x 64 channels a CTA, 64 bytes of K at a
-// time through shared memory, four products an instruction.
-constexpr int kDotK = 64, kDotTok = 32, kDotCh = 64;
+// ------------------------------------------------------------ any rows --
+// Any K, stride and alignment: 32 tokens x 32 channels a CTA, 256 bytes of K at a
+// time through shared memory, a 16 x 8 x 32 matrix instruction's tile a warp.  A
+// row is read in the aligned words that hold its bytes, shifted together (77
+// tokens, K 1111, 1003 channels: byte by byte 54 us).  The next step's words are
+// under way while this one's products are formed; the latency of those few steps
+// bounds it.
+constexpr int kDotK = 256, kDotTok = 32, kDotCh = 32, kDotPitch = kDotK + 16;
+constexpr int kDotThreads = 256;
+
+// 16 bytes at `at` of a row of k bytes, zero past its end.
+__device__ __forceinline__ uint4 row_bytes(const int8_t* row, int at, int k) {
+  uint32_t v[4] = {};
+  if (at < k) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(row + at), end = reinterpret_cast<uintptr_t>(row + k);
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(p & ~static_cast<uintptr_t>(3));
+    const int shift = (int)(p & 3) * 8;
+    uint32_t w[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i)  // no word without a byte of the row
+      w[i] = reinterpret_cast<uintptr_t>(words + i) < end ? __ldg(words + i) : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = __funnelshift_r(w[i], w[i + 1], shift);
+      const int left = k - at - 4 * i;  // bytes of this word in the row
+      if (left < 4) v[i] = left <= 0 ? 0u : v[i] & ((1u << (8 * left)) - 1u);
+    }
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
 
 template <typename T, bool SILU>
-__global__ void __launch_bounds__(256)
-    int8_dot_kernel(const int8_t* __restrict__ codes, int64_t codes_stride,
-                    const int8_t* __restrict__ weight, int64_t weight_stride, int k,
-                    const GemmJob j) {
-  constexpr int NW = SILU ? 2 : 1;
-  __shared__ __align__(16) int8_t xs[kDotTok][kDotK + 4];
-  __shared__ __align__(16) int8_t ws[NW][kDotCh][kDotK + 4];
+__global__ void __launch_bounds__(kDotThreads)
+    int8_dot_kernel(const int8_t* codes, int64_t codes_stride, const int8_t* weight,
+                    int64_t weight_stride, int k, const GemmJob j) {
+  constexpr int NW = SILU ? 2 : 1, kRows = kDotTok + NW * kDotCh;
+  constexpr int kEach = kRows * (kDotK / 16) / kDotThreads;
+  static_assert(kEach * kDotThreads == kRows * (kDotK / 16), "");
+  __shared__ __align__(16) int8_t rows[kRows][kDotPitch];  // tokens, then channels
   const int64_t t0 = (int64_t)blockIdx.y * kDotTok;
   const int n0 = (int)blockIdx.x * kDotCh;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;  // 4 channels, 2 tokens each
+  const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
+  const int wt = warp / 4 * 16, wc = warp % 4 * 8;  // the warp's tokens and channels
   pdl_launch_dependents();
   pdl_wait();
-  int acc[NW][2][4] = {};
-  for (int k0 = 0; k0 < k; k0 += kDotK) {
-    for (int i = threadIdx.x; i < kDotTok * kDotK; i += 256) {
-      const int r = i / kDotK, c = i % kDotK;
-      xs[r][c] = t0 + r < j.tokens && k0 + c < k ? codes[(t0 + r) * codes_stride + k0 + c] : (int8_t)0;
-    }
+  uint4 next[kEach];
+  auto fetch = [&](int k0) {
 #pragma unroll
-    for (int h = 0; h < NW; ++h)
-      for (int i = threadIdx.x; i < kDotCh * kDotK; i += 256) {
-        const int r = i / kDotK, c = i % kDotK;
-        ws[h][r][c] = n0 + r < j.channels && k0 + c < k
-                          ? weight[((int64_t)h * j.channels + n0 + r) * weight_stride + k0 + c]
-                          : (int8_t)0;
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kDotThreads, r = i / (kDotK / 16), at = i % (kDotK / 16) * 16;
+      next[e] = make_uint4(0, 0, 0, 0);
+      if (r < kDotTok) {
+        if (t0 + r < j.tokens) next[e] = row_bytes(codes + (t0 + r) * codes_stride, k0 + at, k);
+      } else {
+        const int h = (r - kDotTok) / kDotCh, n = n0 + (r - kDotTok) % kDotCh;
+        if (n < j.channels)
+          next[e] = row_bytes(weight + ((int64_t)h * j.channels + n) * weight_stride, k0 + at, k);
       }
+    }
+  };
+  int acc[NW][4] = {};
+  fetch(0);
+  for (int k0 = 0; k0 < k; k0 += kDotK) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kDotThreads, r = i / (kDotK / 16), at = i % (kDotK / 16) * 16;
+      *reinterpret_cast<uint4*>(&rows[r][at]) = next[e];
+    }
     __syncthreads();
-#pragma unroll 4
-    for (int c = 0; c < kDotK; c += 4) {
-      int x[2];
+    if (k0 + kDotK < k) fetch(k0 + kDotK);
 #pragma unroll
-      for (int a = 0; a < 2; ++a) x[a] = *reinterpret_cast<const int*>(&xs[ty * 2 + a][c]);
+    for (int s = 0; s < kDotK; s += 32) {
+      auto word = [&](int r, int at) { return *reinterpret_cast<const uint32_t*>(&rows[r][at + 4 * c]); };
+      const uint32_t a0 = word(wt + g, s), a1 = word(wt + g + 8, s), a2 = word(wt + g, s + 16),
+                     a3 = word(wt + g + 8, s + 16);
 #pragma unroll
-      for (int h = 0; h < NW; ++h)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int w = *reinterpret_cast<const int*>(&ws[h][tx + 16 * b][c]);
-#pragma unroll
-          for (int a = 0; a < 2; ++a) acc[h][a][b] = __dp4a(x[a], w, acc[h][a][b]);
-        }
+      for (int h = 0; h < NW; ++h) {
+        const int r = kDotTok + h * kDotCh + wc + g;
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
+            : "+r"(acc[h][0]), "+r"(acc[h][1]), "+r"(acc[h][2]), "+r"(acc[h][3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(word(r, s)), "r"(word(r, s + 16)));
+      }
     }
     __syncthreads();
   }
 #pragma unroll
-  for (int a = 0; a < 2; ++a) {
-    const int64_t t = t0 + ty * 2 + a;
-    if (t >= j.tokens) continue;
+  for (int e = 0; e < 4; ++e) {
+    const int64_t t = t0 + wt + g + e / 2 * 8;
+    const int n = n0 + wc + 2 * c + e % 2;
+    if (t >= j.tokens || n >= j.channels) continue;
     const float st = j.token_scales[t];
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int n = n0 + tx + 16 * b;
-      if (n >= j.channels) continue;
-      float y = (float)acc[0][a][b] * st * j.channel_scales[n];
-      if (SILU)
-        y = silu_mul<T>(y, (float)acc[NW - 1][a][b] * st * j.channel_scales[j.channels + n]);
-      else if (j.bias)
-        y += Traits<T>::to_f(static_cast<const T*>(j.bias)[n]);
-      if (j.add) y += Traits<T>::to_f(static_cast<const T*>(j.add)[t * j.add_stride + n]);
-      static_cast<T*>(j.out)[t * j.out_stride + n] = Traits<T>::from_f(y);
-    }
+    float y = (float)acc[0][e] * st * j.channel_scales[n];
+    if (SILU)
+      y = silu_mul<T>(y, (float)acc[NW - 1][e] * st * j.channel_scales[j.channels + n]);
+    else if (j.bias)
+      y += Traits<T>::to_f(static_cast<const T*>(j.bias)[n]);
+    if (j.add) y += Traits<T>::to_f(static_cast<const T*>(j.add)[t * j.add_stride + n]);
+    static_cast<T*>(j.out)[t * j.out_stride + n] = Traits<T>::from_f(y);
   }
 }
 
@@ -1172,9 +1205,9 @@ int run_typed(const Call& c, GemmJob j) {
     return fail(PACE_ERR_TOO_LARGE, "%s: over 2097120 tokens of rows that are not 16-byte aligned",
                 c.name);
   const cudaError_t err =
-      c.silu ? launch(int8_dot_kernel<T, true>, grid, dim3(256), 0, c.stream, c.codes,
+      c.silu ? launch(int8_dot_kernel<T, true>, grid, dim3(kDotThreads), 0, c.stream, c.codes,
                       c.codes_stride, c.weight, c.weight_stride, (int)c.k, j)
-             : launch(int8_dot_kernel<T, false>, grid, dim3(256), 0, c.stream, c.codes,
+             : launch(int8_dot_kernel<T, false>, grid, dim3(kDotThreads), 0, c.stream, c.codes,
                       c.codes_stride, c.weight, c.weight_stride, (int)c.k, j);
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, c.name);
 }

@@ -12,7 +12,7 @@
 // The quotient is rounded as IEEE division gives it, without a division for
 // each element: y * (1 / scale) is off by less than 2^-15 at 127, so only where
 // it falls within 1e-4 of a half step can the nearest integer be another, and
-// there (one element in 5000) the division is done.
+// there (four elements in 1250 times) the division is done.
 //
 // Memory bounds it: a row is read once with 16-byte vectors, held in registers
 // over the one or two reductions, and stored as 8-byte groups of codes.
@@ -80,13 +80,27 @@ struct RowScale {
                    : __uint_as_float(0x7fc00000u);
     inverse = __fdiv_rn(1.f, scale);
   }
-  // The code in the low byte.
-  __device__ __forceinline__ uint32_t code(float y) const {
+  // Four codes, the first in the low byte.
+  __device__ __forceinline__ uint32_t four(const float* y) const {
     constexpr float kInteger = 12582912.f;  // 1.5 * 2^23: adding it leaves an integer in the low bits
-    const float q = y * inverse;
-    float r = q + kInteger;
-    if (fabsf(q - (r - kInteger)) > 0.4999f) r = __fdiv_rn(y, scale) + kInteger;
-    return finite ? __float_as_uint(r) & 0xffu : 0u;
+    float r[4], most = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      r[e] = fmaf(y[e], inverse, kInteger);
+      most = fmaxf(most, fabsf(fmaf(y[e], inverse, -(r[e] - kInteger))));
+    }
+    if (most > 0.4999f) {  // near a half step the quotient itself decides
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = __fdiv_rn(y[e], scale) + kInteger;
+    }
+    if (!finite) return 0u;
+    const uint32_t lo = __byte_perm(__float_as_uint(r[0]), __float_as_uint(r[1]), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(r[2]), __float_as_uint(r[3]), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+  }
+  __device__ __forceinline__ int8_t one(float y) const {
+    const float v[4] = {y, 0.f, 0.f, 0.f};
+    return (int8_t)four(v);
   }
 };
 
@@ -170,9 +184,7 @@ __global__ void __launch_bounds__(kMaxThreads) quantise_vec_kernel(const QuantJo
     if (c < nvec) {
       uint32_t word[V / 4];
 #pragma unroll
-      for (int i = 0; i < V / 4; ++i)
-        word[i] = s.code(y[j][4 * i]) | s.code(y[j][4 * i + 1]) << 8 |
-                  s.code(y[j][4 * i + 2]) << 16 | s.code(y[j][4 * i + 3]) << 24;
+      for (int i = 0; i < V / 4; ++i) word[i] = s.four(y[j] + 4 * i);
       if constexpr (V == 8)
         *reinterpret_cast<uint2*>(codes + (int64_t)c * V) = make_uint2(word[0], word[1]);
       else
@@ -218,8 +230,14 @@ __global__ void __launch_bounds__(256) quantise_scalar_kernel(const QuantJob job
   const RowScale s(block_max(top, red_max));
   if (threadIdx.x == 0) job.scales[row] = s.scale;
   int8_t* codes = job.codes + row * job.codes_stride;
-  for (int i = threadIdx.x; i < job.width; i += blockDim.x) codes[i] = (int8_t)s.code(value(i));
+  for (int i = threadIdx.x; i < job.width; i += blockDim.x) codes[i] = s.one(value(i));
 }
+
+// Threads a row, at most: many rows do best with several vectors a thread (4096
+// wide, norm with residual, us, 128 / 256 / 512 threads: 512 rows 6.4, 5.7, 4.4;
+// 2048 rows 12.3, 12.2, 13.7; 8192 rows 39, 41, 49), few rows with the shortest
+// chain (1 row, alone, 1.9, 1.2, 1.3).
+inline int most_threads(int64_t rows) { return rows > 4096 ? 128 : rows > 1024 ? 256 : kMaxThreads; }
 
 template <typename T, int SRC>
 int launch_quantise(const QuantJob& job, int64_t rows, cudaStream_t stream, const char* name) {
@@ -234,7 +252,7 @@ int launch_quantise(const QuantJob& job, int64_t rows, cudaStream_t stream, cons
   cudaError_t err;
   if (vec) {
     int nv = 1;
-    while (nv < 4 && ceil_div(nvec, nv) > kMaxThreads) nv *= 2;
+    while (nv < 4 && ceil_div(nvec, nv) > most_threads(rows)) nv *= 2;
     const dim3 threads((unsigned)(ceil_div(ceil_div(nvec, nv), 32) * 32));
     err = nv == 1   ? launch(quantise_vec_kernel<T, SRC, 1>, grid, threads, 0, stream, job)
           : nv == 2 ? launch(quantise_vec_kernel<T, SRC, 2>, grid, threads, 0, stream, job)

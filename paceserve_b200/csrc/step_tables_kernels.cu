@@ -11,13 +11,14 @@
 // in shared memory; so one launch does without a grid-wide barrier.  The one
 // value that is read by all and changed, the stack's height, is written by the
 // CTA that finishes last.  It is a matter of latency: a few dependent loads.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace pace {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreads = 512;  // at most
 constexpr int64_t kMaxRequests = 8192;  // three prefix sums of them in shared memory
 
 struct TableJob {
@@ -36,30 +37,39 @@ __device__ __forceinline__ int64_t pages_of(const TableJob& j, int64_t tokens) {
   return j.page_shift >= 0 ? t >> j.page_shift : t / j.page_size;
 }
 
+// Sums stop at this, far above any array: they are compared with the arrays'
+// lengths, and adding without overflow stays associative.
+constexpr uint32_t kTooMany = 0x7fffffffu;
+__device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) { return min(a + b, kTooMany); }
+
 // Exclusive prefix sums of three values over the CTA; totals in `all`.
-__device__ __forceinline__ void scan3(int64_t (&v)[3], int64_t (&all)[3], int64_t (*part)[3]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t mine[3];
+__device__ __forceinline__ void scan3(uint32_t (&v)[3], uint32_t (&all)[3], uint32_t (*part)[3]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  auto inclusive = [&](uint32_t (&x)[3]) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const uint32_t o = __shfl_up_sync(0xffffffffu, x[k], d);
+        if (lane >= d) x[k] = add(x[k], o);
+      }
+  };
+  uint32_t before[3], mine[3], w[3];
+  inclusive(v);
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
-    mine[k] = v[k];
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t o = __shfl_up_sync(0xffffffffu, v[k], d);
-      if (lane >= d) v[k] += o;
-    }
     if (lane == 31) part[warp][k] = v[k];
+    before[k] = __shfl_up_sync(0xffffffffu, v[k], 1);
   }
   __syncthreads();
 #pragma unroll
+  for (int k = 0; k < 3; ++k) w[k] = lane < warps ? part[lane][k] : 0u;
+  inclusive(w);  // by every warp
+#pragma unroll
   for (int k = 0; k < 3; ++k) {
-    int64_t before = 0;
-    all[k] = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += part[w][k];
-      all[k] += part[w][k];
-    }
-    v[k] += before - mine[k];
+    all[k] = __shfl_sync(0xffffffffu, w[k], 31);
+    mine[k] = __shfl_sync(0xffffffffu, w[k], max(warp - 1, 0));
+    v[k] = add(lane ? before[k] : 0u, warp ? mine[k] : 0u);
   }
 }
 
@@ -76,45 +86,49 @@ __device__ __forceinline__ int owner_of(const int32_t* sum, int requests, int i)
   return lo;
 }
 
-// Writes the stack's new height once every CTA has read the old one.
-__device__ __forceinline__ void leave(const TableJob& j, int64_t height, int32_t problems) {
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  uint32_t before;
-  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
-               : "=r"(before)
-               : "l"(j.arrivals)
-               : "memory");
-  if (before != gridDim.x - 1) return;
-  *j.arrivals = 0;
-  if (problems)
-    atomicOr(j.status, problems);
-  else
-    *j.free_count = (int32_t)height;
-}
-
 // BUILD: a step's arrays; otherwise pages go back onto the stack.
 template <bool BUILD>
 __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j) {
   extern __shared__ int32_t sums[];  // [requests + 1] each: first, pages, new pages
-  __shared__ int64_t part[kWarps][3];
-  __shared__ int problem_bits;
-  const int R = j.requests;
+  __shared__ uint32_t part[32][3];
+  __shared__ int problem_bits, height_read;
+  const int R = j.requests, threads = blockDim.x;
   int32_t* ip = sums;              // BUILD: new tokens; release: pages kept
   int32_t* kp = sums + R + 1;      // BUILD: pages
   int32_t* np = sums + 2 * R + 2;  // BUILD: new pages; release: pages given back
-  if (threadIdx.x == 0) problem_bits = 0;
   pdl_launch_dependents();
-  __syncthreads();
   pdl_wait();
-  const int64_t height = *reinterpret_cast<volatile int32_t*>(j.free_count);
+  // The stack's height is read once a CTA; the CTA that reads it last (no store is under way yet
+  // that its arrival would have to wait for) writes the new one at its end.
+  bool last = false;
+  if (threadIdx.x == 0) {
+    problem_bits = 0;
+    height_read = *reinterpret_cast<volatile int32_t*>(j.free_count);
+    last = true;
+    if (gridDim.x > 1) {
+      uint32_t before;
+      asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                   : "=r"(before)
+                   : "l"(j.arrivals)
+                   : "memory");
+      last = before == gridDim.x - 1;
+      if (last) *j.arrivals = 0;
+    }
+  }
+  auto leave = [&](int64_t height, int32_t problems) {
+    if (!last) return;
+    if (problems)
+      atomicOr(j.status, problems);
+    else
+      *j.free_count = (int32_t)height;
+  };
   // requests of this thread: consecutive ones
-  const int per = (R + kThreads - 1) / kThreads;
+  const int per = (R + threads - 1) / threads;
   const int b0 = threadIdx.x * per;
-  int64_t v[3] = {0, 0, 0}, all[3];
+  uint32_t v[3] = {0, 0, 0}, all[3];
   int32_t problems = 0;
   // what request b adds to the three sums
-  auto shares = [&](int b, int64_t (&s)[3]) {
+  auto shares = [&](int b, uint32_t (&s)[3]) {
     const int64_t x = j.lens_a[b], y = j.lens_b[b];
     const int64_t most = BUILD ? x + y : x;
     if (x < 0 || y < 0 || (!BUILD && y > x)) {
@@ -122,31 +136,34 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j)
       s[0] = s[1] = s[2] = 0;
       return;
     }
+    // pages at most 2^32: as many as fit a sum
     const int64_t pages = pages_of(j, most), less = pages_of(j, BUILD ? x : y);
     if (pages > j.max_blocks) problems |= PACE_TABLES_SHORT_ROW;
-    s[0] = BUILD ? y : 0;
-    s[1] = BUILD ? pages : 0;
-    s[2] = pages - less;
+    s[0] = BUILD ? (uint32_t)y : 0u;
+    s[1] = BUILD ? (uint32_t)min(pages, (int64_t)kTooMany) : 0u;
+    s[2] = (uint32_t)min(pages - less, (int64_t)kTooMany);
   };
   for (int i = 0; i < per && b0 + i < R; ++i) {
-    int64_t s[3];
+    uint32_t s[3];
     shares(b0 + i, s);
 #pragma unroll
-    for (int k = 0; k < 3; ++k) v[k] += s[k];
+    for (int k = 0; k < 3; ++k) v[k] = add(v[k], s[k]);
   }
   scan3(v, all, part);
+  const int64_t height = height_read;
   if (BUILD) {
-    if (all[1] > j.num_indices) problems |= PACE_TABLES_SHORT_INDICES;
-    if (all[0] > j.num_tokens) problems |= PACE_TABLES_SHORT_TOKENS;
-    if (height < 0 || height > j.num_free_pages || all[2] > height) problems |= PACE_TABLES_NO_PAGES;
-  } else if (height < 0 || height + all[2] > j.num_free_pages) {
+    if (all[1] > j.num_indices || all[1] == kTooMany) problems |= PACE_TABLES_SHORT_INDICES;
+    if (all[0] > j.num_tokens || all[0] == kTooMany) problems |= PACE_TABLES_SHORT_TOKENS;
+    if (height < 0 || height > j.num_free_pages || all[2] > height || all[2] == kTooMany)
+      problems |= PACE_TABLES_NO_PAGES;
+  } else if (height < 0 || height + all[2] > j.num_free_pages || all[2] == kTooMany) {
     problems |= PACE_TABLES_NO_PAGES;
   }
   if (problems) atomicOr(&problem_bits, problems);
   __syncthreads();
   problems = problem_bits;
-  const int64_t step = (int64_t)gridDim.x * kThreads;
-  const int64_t me = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t step = (int64_t)gridDim.x * threads;
+  const int64_t me = (int64_t)blockIdx.x * threads + threadIdx.x;
   if (problems) {
     // nothing is taken or given; tables that no token gets through
     if (BUILD) {
@@ -159,18 +176,18 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j)
         j.positions[i] = j.slots[i] = -1;
       }
     }
-    leave(j, height, problems);
+    leave(height, problems);
     return;
   }
   for (int i = 0; i < per && b0 + i < R; ++i) {
-    int64_t s[3];
+    uint32_t s[3];
     const int b = b0 + i;
     shares(b, s);
     ip[b] = BUILD ? (int32_t)v[0] : (int32_t)pages_of(j, j.lens_b[b]);
     kp[b] = (int32_t)v[1];
     np[b] = (int32_t)v[2];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) v[k] += s[k];
+    for (int k = 0; k < 3; ++k) v[k] = add(v[k], s[k]);
   }
   if (threadIdx.x == 0) {
     ip[R] = (int32_t)all[0];
@@ -196,36 +213,53 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j)
       }
     }
     const int pages = (int)all[1], tokens = (int)all[0];
-    for (int64_t i = me; i < pages; i += step) {
-      const int b = owner_of(kp, R, (int)i), k = (int)i - kp[b];
-      bool fresh;
-      const int32_t page = page_at(b, k, &fresh);
-      j.kv_indices[i] = page;
-      if (fresh) j.block_tables[(int64_t)b * j.table_stride + k] = page;
-    }
-    for (int64_t i = me; i < j.num_tokens; i += step) {
-      if (i >= tokens) {  // padding
-        j.batch_indices[i] = -1;
-        j.positions[i] = j.slots[i] = -1;
-        continue;
+    // a warp takes 128 neighbouring entries: each lane looks its first one's request up and walks
+    // on from there
+    const int64_t chunk = 4 * 32, chunks_step = step / 32 * chunk;
+    const int64_t mine = me / 32 * chunk + (threadIdx.x & 31);
+    for (int64_t i0 = mine; i0 < pages; i0 += chunks_step) {
+      int b = owner_of(kp, R, (int)i0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t i = i0 + u * 32;
+        if (i >= pages) break;
+        while (kp[b + 1] <= (int)i) ++b;
+        const int k = (int)i - kp[b];
+        bool fresh;
+        const int32_t page = page_at(b, k, &fresh);
+        j.kv_indices[i] = page;
+        if (fresh) j.block_tables[(int64_t)b * j.table_stride + k] = page;
       }
-      const int b = owner_of(ip, R, (int)i);
-      const int64_t pos = (int64_t)j.lens_a[b] + ((int)i - ip[b]);
-      const int k = (int)(j.page_shift >= 0 ? pos >> j.page_shift : pos / j.page_size);
-      bool fresh;
-      const int64_t page = page_at(b, k, &fresh);
-      j.batch_indices[i] = b;
-      j.positions[i] = pos;
-      j.slots[i] = page * j.page_size + (pos - (int64_t)k * j.page_size);
     }
-    leave(j, height - all[2], 0);
+    for (int64_t i0 = mine; i0 < j.num_tokens; i0 += chunks_step) {
+      int b = i0 < tokens ? owner_of(ip, R, (int)i0) : 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t i = i0 + u * 32;
+        if (i >= j.num_tokens) break;
+        if (i >= tokens) {  // padding
+          j.batch_indices[i] = -1;
+          j.positions[i] = j.slots[i] = -1;
+          continue;
+        }
+        while (ip[b + 1] <= (int)i) ++b;
+        const int64_t pos = (int64_t)j.lens_a[b] + ((int)i - ip[b]);
+        const int k = (int)(j.page_shift >= 0 ? pos >> j.page_shift : pos / j.page_size);
+        bool fresh;
+        const int64_t page = page_at(b, k, &fresh);
+        j.batch_indices[i] = b;
+        j.positions[i] = pos;
+        j.slots[i] = page * j.page_size + (pos - (int64_t)k * j.page_size);
+      }
+    }
+    leave(height - all[2], 0);
   } else {
     const int given = (int)all[2];
     for (int64_t i = me; i < given; i += step) {
       const int b = owner_of(np, R, (int)i), k = ip[b] + ((int)i - np[b]);
       j.free_pages[height + given - 1 - i] = j.block_tables[(int64_t)b * j.table_stride + k];
     }
-    leave(j, height + given, 0);
+    leave(height + given, 0);
   }
 }
 
@@ -261,14 +295,15 @@ int run_tables(TableJob& j, int64_t requests, int64_t page_size, cudaStream_t st
     if (err != cudaSuccess) return cuda_fail(err, name);
   }
   // a few entries a thread, of the arrays' full length: how much of it a step needs is known on
-  // the device only
+  // the device only.  One CTA where they are few: it needs no arrival
   const int64_t entries = BUILD ? j.num_indices + j.num_tokens
                                 : (j.max_blocks < 1 ? 0 : requests * j.max_blocks);
-  int64_t ctas = ceil_div(entries, 4 * kThreads);
-  if (ctas < 1) ctas = 1;
-  if (ctas > sm_count(guard.device())) ctas = sm_count(guard.device());
-  err = launch(step_tables_kernel<BUILD>, dim3((unsigned)ctas), dim3(kThreads), (size_t)smem,
-               stream, j);
+  const int threads = requests <= 128 && entries <= 1024 ? 128 : kThreads;
+  const int64_t each = (BUILD ? 4 : 32) * threads;  // a release seldom gives all that rows can hold
+  const int64_t ctas =
+      std::min<int64_t>(sm_count(guard.device()), std::max<int64_t>(1, ceil_div(entries, each)));
+  err = launch(step_tables_kernel<BUILD>, dim3((unsigned)ctas), dim3((unsigned)threads),
+               (size_t)smem, stream, j);
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, name);
 }
 

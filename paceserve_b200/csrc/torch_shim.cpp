@@ -1288,10 +1288,12 @@ HeadArgs check_heads(const Tensor& positions, const Tensor& query, const Tensor&
 
 void qk_norm_rotary_embedding(Tensor& positions, Tensor& query, Tensor& key, Tensor& q_weight,
                               Tensor& k_weight, double epsilon, int64_t head_size,
-                              Tensor& cos_sin_cache, bool is_neox) {
+                              Tensor& cos_sin_cache, bool is_neox,
+                              const c10::optional<Tensor>& fault_flags) {
   const char* op = "qk_norm_rotary_embedding";
   const HeadArgs a =
       check_heads(positions, query, key, q_weight, k_weight, head_size, cos_sin_cache, op);
+  int32_t* fault = counter_ptr(fault_flags, query.device(), op, "fault_flags");
   const at::cuda::CUDAGuard guard(query.device());
   check_status(pace_qk_norm_rotary_embedding(
                    positions.data_ptr<int64_t>(), query.data_ptr(), key.data_ptr(),
@@ -1299,7 +1301,7 @@ void qk_norm_rotary_embedding(Tensor& positions, Tensor& query, Tensor& key, Ten
                    a.num_kv_heads, (int)head_size, a.q.stride, a.k.stride,
                    cos_sin_cache.data_ptr(), pace_dtype(cos_sin_cache),
                    (int)cos_sin_cache.size(1), cos_sin_cache.size(0), is_neox ? 1 : 0,
-                   pace_dtype(query), stream_of(query)),
+                   pace_dtype(query), fault, stream_of(query)),
                op);
 }
 
@@ -1307,7 +1309,8 @@ void qk_norm_rotary_append(Tensor& positions, Tensor& query, const Tensor& key,
                            const Tensor& value, Tensor& q_weight, Tensor& k_weight, double epsilon,
                            int64_t head_size, Tensor& cos_sin_cache, bool is_neox,
                            Tensor& paged_kv_cache, const Tensor& slot_mapping,
-                           const c10::optional<Tensor>& bad_tokens) {
+                           const c10::optional<Tensor>& bad_tokens,
+                           const c10::optional<Tensor>& fault_flags) {
   const char* op = "qk_norm_rotary_append";
   const HeadArgs a =
       check_heads(positions, query, key, q_weight, k_weight, head_size, cos_sin_cache, op);
@@ -1326,6 +1329,7 @@ void qk_norm_rotary_append(Tensor& positions, Tensor& query, const Tensor& key,
                   slot_mapping.numel() >= a.q.rows,
               op, ": slot_mapping must be a contiguous int64 tensor with an entry for each token");
   int32_t* bad = counter_ptr(bad_tokens, query.device(), op, "bad_tokens");
+  int32_t* fault = counter_ptr(fault_flags, query.device(), op, "fault_flags");
   const at::cuda::CUDAGuard guard(query.device());
   check_status(pace_qk_norm_rotary_append(
                    positions.data_ptr<int64_t>(), query.data_ptr(), key.data_ptr(),
@@ -1334,7 +1338,7 @@ void qk_norm_rotary_append(Tensor& positions, Tensor& query, const Tensor& key,
                    v.stride, cos_sin_cache.data_ptr(), pace_dtype(cos_sin_cache),
                    (int)cos_sin_cache.size(1), cos_sin_cache.size(0), is_neox ? 1 : 0,
                    paged_kv_cache.data_ptr(), pc.pages, (int)pc.page_size,
-                   slot_mapping.data_ptr<int64_t>(), bad, pace_dtype(query), stream_of(query)),
+                   slot_mapping.data_ptr<int64_t>(), bad, pace_dtype(query), fault, stream_of(query)),
                op);
 }
 
@@ -1559,13 +1563,14 @@ PYBIND11_MODULE(_C, m) {
          "pass.",
          py::arg("positions"), py::arg("query"), py::arg("key"), py::arg("q_weight"),
          py::arg("k_weight"), py::arg("epsilon"), py::arg("head_size"), py::arg("cos_sin_cache"),
-         py::arg("is_neox"));
+         py::arg("is_neox"), py::arg("fault_flags") = py::none());
   pe.def("qk_norm_rotary_append", &qk_norm_rotary_append,
          "The same with the keys' result and the values written to their slots of a paged cache.",
          py::arg("positions"), py::arg("query"), py::arg("key"), py::arg("value"),
          py::arg("q_weight"), py::arg("k_weight"), py::arg("epsilon"), py::arg("head_size"),
          py::arg("cos_sin_cache"), py::arg("is_neox"), py::arg("paged_kv_cache"),
-         py::arg("slot_mapping"), py::arg("bad_tokens") = py::none());
+         py::arg("slot_mapping"), py::arg("bad_tokens") = py::none(),
+         py::arg("fault_flags") = py::none());
   pe.def("qkv_proj_rotary_embedding", &qkv_proj_rotary_embedding,
          "qkv = hidden @ weight^T on the tensor cores with the rotary embedding applied to the "
          "q and k heads before rounding (fused qkv_proj + rotary_embedding).",

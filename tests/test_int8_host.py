@@ -14,7 +14,8 @@ def test_signatures():
     assert _params(int8_ops.rms_norm_quantise) == ["codes", "scales", "input", "weight", "epsilon", "residual"]
     assert _params(int8_ops.linear)[:6] == ["out", "codes", "token_scales", "weight", "channel_scales", "bias"]
     assert _params(int8_ops.gate_up_silu)[:5] == ["out", "codes", "token_scales", "weight", "channel_scales"]
-    assert _params(pos_encoding_ops.qk_norm_rotary_append)[-3:] == ["paged_kv_cache", "slot_mapping", "bad_tokens"]
+    assert _params(pos_encoding_ops.qk_norm_rotary_append)[-4:] == ["paged_kv_cache", "slot_mapping",
+                                                                  "bad_tokens", "fault_flags"]
     assert _params(kv_transfer_ops.build_step_tables)[:4] == ["block_tables", "seq_lens", "new_lens", "page_size"]
 
 
@@ -63,7 +64,7 @@ def test_head_argument_errors():
     lib = cabi.load()
     call = lambda t, h, hk, d, qs, ks, rot, pos: lib.pace_qk_norm_rotary_embedding(  # noqa: E731
         None, None, None, None, None, 1e-5, t, h, hk, d, qs, ks, None, cabi.PACE_F32, rot, pos, 1,
-        cabi.PACE_BF16, None)
+        cabi.PACE_BF16, None, None)
     _expect(call(-1, 8, 2, 64, 512, 128, 64, 16), BAD, "bad shape")
     _expect(call(2, 8, 2, 64, 511, 128, 64, 16), BAD, "row stride")
     _expect(call(2, 8, 2, 64, 512, 128, 63, 16), BAD, "rot_dim")
@@ -73,7 +74,7 @@ def test_head_argument_errors():
     assert call(0, 8, 2, 64, 512, 128, 64, 16) == 0
     append = lambda pages, page: lib.pace_qk_norm_rotary_append(  # noqa: E731
         None, None, None, None, None, None, 1e-5, 2, 8, 2, 64, 512, 128, 128, None, cabi.PACE_F32, 64, 16,
-        1, None, pages, page, None, None, cabi.PACE_BF16, None)
+        1, None, pages, page, None, None, cabi.PACE_BF16, None, None)
     _expect(append(-1, 16), BAD, "bad cache shape")
     _expect(append(4, 0), BAD, "bad cache shape")
     _expect(append(4, 16), BAD, "null pointer")

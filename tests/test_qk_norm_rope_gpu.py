@@ -160,6 +160,37 @@ def test_many_tokens_match_few():
     assert torch.equal(one, many)
 
 
+@pytest.mark.parametrize("t,heads,kv_heads,d,rot,page", [
+    (3301, 64, 8, 128, 128, 16), (5601, 50, 3, 96, 48, 5), (6203, 9, 4, 256, 256, 1), (9000, 0, 70, 64, 32, 8),
+    (1301, 5, 3, 64, 32, 3)])
+@pytest.mark.parametrize("dtype,cache_dtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float16),
+                                               (torch.float32, torch.float32)])
+@pytest.mark.parametrize("neox", [True, False])
+def test_many_tokens(t, heads, kv_heads, d, rot, page, dtype, cache_dtype, neox):
+    """The kernel for many tokens, in place and with the append, against the one for few."""
+    qkv, (qw, kw), cs, pos = make(t, heads, kv_heads, d, rot, dtype, cache_dtype=cache_dtype, pad=16)
+    pages = -(-t // page) + 2
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(1))[:t]
+    pos[::97], pos[5] = -1, 512
+    slots[::97] = -1
+    slots[11], slots[12], slots[t - 1] = -1, pages * page, -7  # 5, 12 and the last count
+    qw, kw, cs, pos, slots = (x.to(DEV) for x in (qw, kw, cs, pos, slots))
+    bad = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = []
+    for few in (False, True):
+        dev, both = qkv.to(DEV), qkv.to(DEV)
+        cache = torch.full((pages, 2, page, kv_heads, d), 9.0, device=DEV).to(dtype)
+        for a, b in ((i, min(t, i + 500)) for i in range(0, t, 500)) if few else ((0, t),):
+            q, k, _ = split(dev[a:b], heads, kv_heads, d)
+            pe.qk_norm_rotary_embedding(pos[a:b], q, k, qw, kw, EPS, d, cs, neox)
+            q, k, v = split(both[a:b], heads, kv_heads, d)
+            pe.qk_norm_rotary_append(pos[a:b], q, k, v, qw, kw, EPS, d, cs, neox, cache, slots[a:b], bad)
+        assert bad.item() == (6 if few else 3)
+        got.append((dev, both, cache))
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
 def test_row_of_zeros_and_nan():
     qkv, (qw, kw), cs, pos = make(3, 2, 1, 64, 64, torch.bfloat16)
     qkv[0] = 0
