@@ -98,33 +98,28 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j)
   int32_t* np = sums + 2 * R + 2;  // BUILD: new pages; release: pages given back
   pdl_launch_dependents();
   pdl_wait();
-  // The stack's height is read once a CTA; the CTA that reads it last (no store is under way yet
-  // that its arrival would have to wait for) writes the new one at its end.
-  bool last = false;
+  // The stack's height is read once a CTA.  The CTA that has read it last writes the new one: an
+  // arrival is issued with the height in a register, so when the last one has counted, every CTA
+  // has its own.
+  uint32_t before = 0;
   if (threadIdx.x == 0) {
     problem_bits = 0;
-    height_read = *reinterpret_cast<volatile int32_t*>(j.free_count);
-    last = true;
-    if (gridDim.x > 1) {
-      uint32_t before;
-      asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+    const int32_t h = *reinterpret_cast<volatile int32_t*>(j.free_count);
+    height_read = h;
+    if (gridDim.x > 1)
+      asm volatile("{\n\t.reg .u32 h;\n\tmov.u32 h, %2;\n\tatom.add.relaxed.gpu.global.u32 %0, [%1], 1;\n\t}"
                    : "=r"(before)
-                   : "l"(j.arrivals)
+                   : "l"(j.arrivals), "r"(h)
                    : "memory");
-      last = before == gridDim.x - 1;
-      if (last) *j.arrivals = 0;
-    }
   }
   auto leave = [&](int64_t height, int32_t problems) {
-    if (!last) return;
+    if (threadIdx.x != 0 || before != gridDim.x - 1) return;
+    if (gridDim.x > 1) *j.arrivals = 0;
     if (problems)
       atomicOr(j.status, problems);
     else
       *j.free_count = (int32_t)height;
   };
-  // requests of this thread: consecutive ones
-  const int per = (R + threads - 1) / threads;
-  const int b0 = threadIdx.x * per;
   uint32_t v[3] = {0, 0, 0}, all[3];
   int32_t problems = 0;
   // what request b adds to the three sums
@@ -143,11 +138,27 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j)
     s[1] = BUILD ? (uint32_t)min(pages, (int64_t)kTooMany) : 0u;
     s[2] = (uint32_t)min(pages - less, (int64_t)kTooMany);
   };
-  for (int i = 0; i < per && b0 + i < R; ++i) {
-    uint32_t s[3];
-    shares(b0 + i, s);
-#pragma unroll
-    for (int k = 0; k < 3; ++k) v[k] = add(v[k], s[k]);
+  for (int b = threadIdx.x; b < R; b += threads) {
+    shares(b, v);
+    // release keeps what its rows begin with in ip
+    ip[b] = BUILD ? v[0] : (int32_t)pages_of(j, j.lens_b[b]);
+    kp[b] = v[1];
+    np[b] = v[2];
+  }
+  // a thread's requests: the one it has, or neighbours, an odd number of them, so that a warp's
+  // threads use different banks
+  const int per = (R + threads - 1) / threads | 1;
+  const int b0 = min(R, (int)threadIdx.x * per), b1 = min(R, b0 + per);
+  if (per > 1) {
+    __syncthreads();
+    v[0] = v[1] = v[2] = 0;
+    for (int b = b0; b < b1; ++b) {
+      if (BUILD) {
+        v[0] = add(v[0], ip[b]);
+        v[1] = add(v[1], kp[b]);
+      }
+      v[2] = add(v[2], np[b]);
+    }
   }
   scan3(v, all, part);
   const int64_t height = height_read;
@@ -179,15 +190,17 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j)
     leave(height, problems);
     return;
   }
-  for (int i = 0; i < per && b0 + i < R; ++i) {
-    uint32_t s[3];
-    const int b = b0 + i;
-    shares(b, s);
-    ip[b] = BUILD ? (int32_t)v[0] : (int32_t)pages_of(j, j.lens_b[b]);
-    kp[b] = (int32_t)v[1];
-    np[b] = (int32_t)v[2];
-#pragma unroll
-    for (int k = 0; k < 3; ++k) v[k] = add(v[k], s[k]);
+  for (int b = b0; b < b1; ++b) {
+    auto place = [&](int32_t* sum, uint32_t& at) {
+      const uint32_t share = sum[b];
+      sum[b] = (int32_t)at;
+      at = add(at, share);
+    };
+    if (BUILD) {
+      place(ip, v[0]);
+      place(kp, v[1]);
+    }
+    place(np, v[2]);
   }
   if (threadIdx.x == 0) {
     ip[R] = (int32_t)all[0];
@@ -213,44 +226,47 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j)
       }
     }
     const int pages = (int)all[1], tokens = (int)all[0];
-    // a warp takes 128 neighbouring entries: each lane looks its first one's request up and walks
-    // on from there
-    const int64_t chunk = 4 * 32, chunks_step = step / 32 * chunk;
+    // a warp takes 256 neighbouring pages: each lane has all its loads under way before the first
+    // store, and looks a page's request up only where it is another than the last one's
+    constexpr int kEach = 8;
+    const int64_t chunk = kEach * 32, chunks_step = step / 32 * chunk;
     const int64_t mine = me / 32 * chunk + (threadIdx.x & 31);
     for (int64_t i0 = mine; i0 < pages; i0 += chunks_step) {
       int b = owner_of(kp, R, (int)i0);
+      int32_t page[kEach];
+      int32_t* entry[kEach];  // of the block table, for a new page
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kEach; ++u) {
         const int64_t i = i0 + u * 32;
-        if (i >= pages) break;
-        while (kp[b + 1] <= (int)i) ++b;
+        entry[u] = nullptr;
+        if (i >= pages) continue;
+        if (kp[b + 1] <= (int)i) b = owner_of(kp, R, (int)i);
         const int k = (int)i - kp[b];
         bool fresh;
-        const int32_t page = page_at(b, k, &fresh);
-        j.kv_indices[i] = page;
-        if (fresh) j.block_tables[(int64_t)b * j.table_stride + k] = page;
+        page[u] = page_at(b, k, &fresh);
+        if (fresh) entry[u] = j.block_tables + (int64_t)b * j.table_stride + k;
+      }
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) {
+        const int64_t i = i0 + u * 32;
+        if (i < pages) j.kv_indices[i] = page[u];
+        if (entry[u]) *entry[u] = page[u];
       }
     }
-    for (int64_t i0 = mine; i0 < j.num_tokens; i0 += chunks_step) {
-      int b = i0 < tokens ? owner_of(ip, R, (int)i0) : 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t i = i0 + u * 32;
-        if (i >= j.num_tokens) break;
-        if (i >= tokens) {  // padding
-          j.batch_indices[i] = -1;
-          j.positions[i] = j.slots[i] = -1;
-          continue;
-        }
-        while (ip[b + 1] <= (int)i) ++b;
-        const int64_t pos = (int64_t)j.lens_a[b] + ((int)i - ip[b]);
+    // tokens from the other end of the grid: its first CTAs have pages
+    for (int64_t i = step - 1 - me; i < j.num_tokens; i += step) {
+      int64_t pos = -1, slot = -1;
+      int b = -1;  // padding
+      if (i < tokens) {
+        b = owner_of(ip, R, (int)i);
+        pos = (int64_t)j.lens_a[b] + ((int)i - ip[b]);
         const int k = (int)(j.page_shift >= 0 ? pos >> j.page_shift : pos / j.page_size);
         bool fresh;
-        const int64_t page = page_at(b, k, &fresh);
-        j.batch_indices[i] = b;
-        j.positions[i] = pos;
-        j.slots[i] = page * j.page_size + (pos - (int64_t)k * j.page_size);
+        slot = (int64_t)page_at(b, k, &fresh) * j.page_size + (pos - (int64_t)k * j.page_size);
       }
+      j.batch_indices[i] = b;
+      j.positions[i] = pos;
+      j.slots[i] = slot;
     }
     leave(height - all[2], 0);
   } else {
@@ -299,7 +315,7 @@ int run_tables(TableJob& j, int64_t requests, int64_t page_size, cudaStream_t st
   const int64_t entries = BUILD ? j.num_indices + j.num_tokens
                                 : (j.max_blocks < 1 ? 0 : requests * j.max_blocks);
   const int threads = requests <= 128 && entries <= 1024 ? 128 : kThreads;
-  const int64_t each = (BUILD ? 4 : 32) * threads;  // a release seldom gives all that rows can hold
+  const int64_t each = (BUILD ? 8 : 32) * threads;  // a release seldom gives all that rows can hold
   const int64_t ctas =
       std::min<int64_t>(sm_count(guard.device()), std::max<int64_t>(1, ceil_div(entries, each)));
   err = launch(step_tables_kernel<BUILD>, dim3((unsigned)ctas), dim3((unsigned)threads),
