@@ -731,11 +731,11 @@ __global__ void __launch_bounds__(THREADS, 2)
 // integers are exact.
 constexpr int kMidRing = 98304;
 constexpr int kMidAhead = 8;  // K blocks that are pulled into L2 before the wait
-constexpr int kMidSmem = kMidRing + 1024 + 256;
+constexpr int kMidRest = 1024 + 256;
 constexpr int kMidTok = 128;  // of a tile, at most
 
 struct MidTiling {
-  int bt, stages, tmem_cols, tok_tiles, cut;  // tokens a tile; CTAs of a cluster
+  int bt, stages, ring, tmem_cols, tok_tiles, cut;  // tokens a tile; CTAs of a cluster
 };
 
 // 16 bytes of the shared memory of the cluster's CTA `rank`, at this CTA's address p.
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   uint8_t* tiles = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   int32_t* part = reinterpret_cast<int32_t*>(tiles);  // [token][row], over the ring
-  Ctl* ctl = reinterpret_cast<Ctl*>(tiles + kMidRing);
+  Ctl* ctl = reinterpret_cast<Ctl*>(tiles + p.ring);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sb = kA + p.bt * BK;  // bytes of a stage
   const int rank = (int)tc::cluster_rank();
@@ -1134,16 +1134,29 @@ int launch_mid(const Call& c, const GemmJob& j) {
   MidTiling p;
   p.tok_tiles = (int)ceil_div(c.tokens, kMidTok);
   p.bt = (int)ceil_div(ceil_div(c.tokens, p.tok_tiles), 16) * 16;
-  p.stages = std::min(MAX_STAGES, kMidRing / (BM * BK + p.bt * BK));
   p.tmem_cols = 32;
   while (p.tmem_cols < p.bt) p.tmem_cols *= 2;
   const int tiles = (int)ceil_div(c.channels, SILU ? BM / 2 : BM) * p.tok_tiles;
-  // CTAs for two an SM, with 8 K blocks each at least (4096 x 4096, 64 tokens: 8 blocks 8.7 us, 4
-  // blocks 9.6), in clusters of a power of two, which find room on the SMs (48 tiles of 128
+  // K is cut for two CTAs an SM, with 8 K blocks each at least (4096 x 4096, 64 tokens: 8 blocks 8.7
+  // us, 4 blocks 9.6), in clusters of a power of two, which find room on the SMs (48 tiles of 128
   // channels, 64 tokens: clusters of 4 10.1 us, of 6 17.1)
-  p.cut = 1;
-  while (p.cut < 8 && tiles * p.cut * 2 <= 2 * sm_count(c.device) && j.k_blocks / (p.cut * 2) >= 8)
-    p.cut *= 2;
+  const int sms = sm_count(c.device), stage = BM * BK + p.bt * BK;
+  auto cut_for = [&](int ctas) {
+    int cut = 1;
+    while (cut < 8 && tiles * cut * 2 <= ctas && j.k_blocks / (cut * 2) >= 8) cut *= 2;
+    return cut;
+  };
+  p.cut = cut_for(2 * sms);
+  p.ring = kMidRing;
+  // or for one CTA, with a ring twice as long, where that leaves few SMs without any and its part
+  // of K fills the ring (4096 channels, K 14336, 64 / 128 tokens: 15.8 / 17.8 us against 16.4 /
+  // 19.9; 6144 channels, K 4096, 96 CTAs: 13.4 against 12.7)
+  const int one = cut_for(sms);
+  if (tiles * one <= sms && 5 * tiles * one >= 4 * sms && j.k_blocks / one * stage > kRingBytes) {
+    p.cut = one;
+    p.ring = kRingBytes;
+  }
+  p.stages = std::min(MAX_STAGES, p.ring / stage);
   CUtensorMap w, x;
   int rc = make_map(&w, c.weight, weight_rows(c), c.k, c.weight_stride, SILU ? BM / 2 : BM, false, 1,
                     c.name);
@@ -1151,9 +1164,9 @@ int launch_mid(const Call& c, const GemmJob& j) {
     rc = make_map(&x, c.codes, c.tokens, c.k, c.codes_stride, p.bt, false, 1, c.name);
   if (rc != PACE_OK) return rc;
   auto kernel = int8_mid_kernel<T, SILU>;
-  cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kMidSmem);
+  cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kRingBytes + kMidRest);
   if (err != cudaSuccess) return cuda_fail(err, c.name);
-  err = launch_clusters(kernel, p.cut, dim3((unsigned)(tiles * p.cut)), dim3(THREADS), kMidSmem,
+  err = launch_clusters(kernel, p.cut, dim3((unsigned)(tiles * p.cut)), dim3(THREADS), p.ring + kMidRest,
                         c.stream, w, x, j, p, c.fault);
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, c.name);
 }
