@@ -40,6 +40,7 @@ constexpr int CH = 16;  // columns drained at a time
 constexpr uint64_t kWaitLimitNs = 1000000000ull;  // 1 s per wait
 constexpr int32_t kFaultTimeout = 1 << 30;
 constexpr int64_t kMaxK = 131071;
+constexpr int64_t kMaxRows = 1 << 29;  // tokens, and channels: twice as many fit an int
 
 struct Ctl {
   uint64_t full[MAX_STAGES];
@@ -966,8 +967,8 @@ __global__ void __launch_bounds__(kDotThreads)
   constexpr int kEach = kRows * (kDotK / 16) / kDotThreads;
   static_assert(kEach * kDotThreads == kRows * (kDotK / 16), "");
   __shared__ __align__(16) int8_t rows[kRows][kDotPitch];  // tokens, then channels
-  const int64_t t0 = (int64_t)blockIdx.y * kDotTok;
-  const int n0 = (int)blockIdx.x * kDotCh;
+  const int64_t t0 = (int64_t)blockIdx.x * kDotTok;
+  const int n0 = (int)blockIdx.y * kDotCh;
   const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
   const int wt = warp / 4 * 16, wc = warp % 4 * 8;  // the warp's tokens and channels
   pdl_launch_dependents();
@@ -1213,9 +1214,9 @@ int run_typed(const Call& c, GemmJob j) {
   j.k_blocks = (int)ceil_div(c.k, BK);
   j.deep = c.k % BK == 0;
   if (for_tma(c)) return c.silu ? launch_tensor<T, true>(c, j) : launch_tensor<T, false>(c, j);
-  const dim3 grid((unsigned)ceil_div(c.channels, kDotCh), (unsigned)ceil_div(c.tokens, kDotTok));
-  if (ceil_div(c.tokens, kDotTok) > 65535)
-    return fail(PACE_ERR_TOO_LARGE, "%s: over 2097120 tokens of rows that are not 16-byte aligned",
+  const dim3 grid((unsigned)ceil_div(c.tokens, kDotTok), (unsigned)ceil_div(c.channels, kDotCh));
+  if (grid.y > 65535)
+    return fail(PACE_ERR_TOO_LARGE, "%s: over 2097120 channels of rows that are not 16-byte aligned",
                 c.name);
   const cudaError_t err =
       c.silu ? launch(int8_dot_kernel<T, true>, grid, dim3(kDotThreads), 0, c.stream, c.codes,
@@ -1226,7 +1227,7 @@ int run_typed(const Call& c, GemmJob j) {
 }
 
 int run_int8(Call c, GemmJob j) {
-  if (c.tokens < 0 || c.tokens > INT32_MAX || c.channels <= 0 || c.channels > (1 << 30) || c.k <= 0)
+  if (c.tokens < 0 || c.tokens > kMaxRows || c.channels <= 0 || c.channels > kMaxRows || c.k <= 0)
     return fail(PACE_ERR_INVALID_ARGUMENT, "%s: bad shape", c.name);
   if (c.k > kMaxK)
     return fail(PACE_ERR_TOO_LARGE, "%s: k %lld: sums of more than %lld products may not fit 32 bits",

@@ -16,7 +16,7 @@
 //
 // Memory bounds it: a row is read once with 16-byte vectors, held in registers
 // over the one or two reductions, and stored as 8-byte groups of codes.
-#include "common.cuh"
+#include "f32x2.cuh"
 
 namespace pace {
 namespace {
@@ -51,44 +51,64 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return warp_sum(lane < warps ? red[lane] : 0.f);
 }
 
-// Largest over the CTA of the bit patterns of magnitudes: the order of the
-// floats, with infinity and NaN above all.
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
-  v = __reduce_max_sync(0xffffffffu, v);
+// Largest magnitude over the CTA, of the threads' own; NaN if any is.
+__device__ __forceinline__ float block_max(float v, uint32_t* red) {
+  // as bit patterns, whose order is that of magnitudes, with infinity and NaN above all
+  uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu);
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  if (lane == 0) red[threadIdx.x >> 5] = v;
+  if (lane == 0) red[threadIdx.x >> 5] = bits;
   __syncthreads();
-  return __reduce_max_sync(0xffffffffu, lane < warps ? red[lane] : 0u);
+  bits = __reduce_max_sync(0xffffffffu, lane < warps ? red[lane] : 0u);
+  return __uint_as_float(bits);
 }
 
-__device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
+// The larger magnitude, NaN if either is.
+__device__ __forceinline__ float larger(float top, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(y)));
+  return r;
+}
 
-// 16-bit inputs take the approximate exponential and quotient (a few units of
-// 2^-24, far below the code's half step), float32 the library's.
+// silu(g) * u of two elements.  16-bit inputs take the approximate exponential and
+// reciprocal (a few units of 2^-24, far below the code's half step), float32 the
+// library's.
 template <typename T>
-__device__ __forceinline__ float silu_mul(float g, float u) {
-  if constexpr (sizeof(T) == 2) return __fdividef(g, 1.f + __expf(-g)) * u;
-  return g / (1.f + expf(-g)) * u;
+__device__ __forceinline__ void silu_mul2(float* g, const float* u) {
+  if constexpr (sizeof(T) == 2) {
+    float a, b, c, d;
+    apart(mul2(two(g[0], g[1]), two(-1.44269504f, -1.44269504f)), a, b);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(c) : "f"(a));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(b));
+    apart(add2(two(c, d), two(1.f, 1.f)), a, b);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(c) : "f"(a));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(b));
+    apart(mul2(mul2(two(g[0], g[1]), two(c, d)), two(u[0], u[1])), g[0], g[1]);
+  } else {
+    g[0] = g[0] / (1.f + expf(-g[0])) * u[0];
+    g[1] = g[1] / (1.f + expf(-g[1])) * u[1];
+  }
 }
 
 struct RowScale {
   float scale, inverse;
   bool finite;
-  __device__ __forceinline__ explicit RowScale(uint32_t top) {
-    finite = top < 0x7f800000u;
-    scale = finite ? fmaxf(__fdiv_rn(__uint_as_float(top), 127.f), kLeastScale)
-                   : __uint_as_float(0x7fc00000u);
+  __device__ __forceinline__ explicit RowScale(float top) {
+    finite = top <= 3.402823466e38f;
+    scale = finite ? fmaxf(__fdiv_rn(top, 127.f), kLeastScale) : __uint_as_float(0x7fc00000u);
     inverse = __fdiv_rn(1.f, scale);
   }
   // Four codes, the first in the low byte.
   __device__ __forceinline__ uint32_t four(const float* y) const {
     constexpr float kInteger = 12582912.f;  // 1.5 * 2^23: adding it leaves an integer in the low bits
-    float r[4], most = 0.f;
+    const uint64_t inv = two(inverse, inverse), up = two(kInteger, kInteger), minus = two(-1.f, -1.f);
+    float r[4], off[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      r[e] = fmaf(y[e], inverse, kInteger);
-      most = fmaxf(most, fabsf(fmaf(y[e], inverse, -(r[e] - kInteger))));
+    for (int e = 0; e < 4; e += 2) {
+      const uint64_t v = two(y[e], y[e + 1]), s = fma2(v, inv, up);
+      apart(s, r[e], r[e + 1]);
+      apart(fma2(v, inv, fma2(s, minus, up)), off[e], off[e + 1]);  // from the integer
     }
+    const float most = fmaxf(fmaxf(fabsf(off[0]), fabsf(off[1])), fmaxf(fabsf(off[2]), fabsf(off[3])));
     if (most > 0.4999f) {  // near a half step the quotient itself decides
 #pragma unroll
       for (int e = 0; e < 4; ++e) r[e] = __fdiv_rn(y[e], scale) + kInteger;
@@ -135,8 +155,8 @@ __global__ void __launch_bounds__(kMaxThreads) quantise_vec_kernel(const QuantJo
     }
   }
   float y[NV][V];
-  float ss = 0.f;
-  uint32_t top = 0;
+  uint64_t ss = 0;
+  float top = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = threadIdx.x + j * blockDim.x;
@@ -146,21 +166,31 @@ __global__ void __launch_bounds__(kMaxThreads) quantise_vec_kernel(const QuantJo
         float z[V];
         Tr::unpack(b[j], z);
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          y[j][e] = SRC == kSilu ? silu_mul<T>(y[j][e], z[e]) : Tr::round(y[j][e] + z[e]);
+        for (int e = 0; e < V; e += 2) {
+          if constexpr (SRC == kSilu) {
+            silu_mul2<T>(y[j] + e, z + e);
+          } else {
+            y[j][e] = Tr::round(y[j][e] + z[e]);
+            y[j][e + 1] = Tr::round(y[j][e + 1] + z[e + 1]);
+          }
+        }
         if (SRC == kAddNorm) st_v4(rr + (int64_t)c * V, Tr::pack(y[j]));
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
+      for (int e = 0; e < V; e += 2) {
+        const uint64_t v = two(y[j][e], y[j][e + 1]);
         if (SRC == kNorm || SRC == kAddNorm)
-          ss += y[j][e] * y[j][e];
+          ss = fma2(v, v, ss);
         else
-          top = max(top, magnitude(y[j][e]));
+          top = larger(larger(top, y[j][e]), y[j][e + 1]);
       }
     }
   }
   if constexpr (SRC == kNorm || SRC == kAddNorm) {
-    const float inv = rsqrtf(block_sum(ss, red_sum) / (float)job.width + job.eps);
+    float lo, hi;
+    apart(ss, lo, hi);
+    const float inv = rsqrtf(block_sum(lo + hi, red_sum) / (float)job.width + job.eps);
+    const uint64_t inv2 = two(inv, inv);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = threadIdx.x + j * blockDim.x;
@@ -168,9 +198,10 @@ __global__ void __launch_bounds__(kMaxThreads) quantise_vec_kernel(const QuantJo
         float wf[V];
         Tr::unpack(w[j], wf);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          y[j][e] = y[j][e] * inv * wf[e];
-          top = max(top, magnitude(y[j][e]));
+        for (int e = 0; e < V; e += 2) {
+          apart(mul2(mul2(two(y[j][e], y[j][e + 1]), inv2), two(wf[e], wf[e + 1])), y[j][e],
+                y[j][e + 1]);
+          top = larger(larger(top, y[j][e]), y[j][e + 1]);
         }
       }
     }
@@ -182,6 +213,11 @@ __global__ void __launch_bounds__(kMaxThreads) quantise_vec_kernel(const QuantJo
   for (int j = 0; j < NV; ++j) {
     const int c = threadIdx.x + j * blockDim.x;
     if (c < nvec) {
+      if constexpr (SRC == kRows && sizeof(T) == 2) {
+        // the row was held as it came, half the registers: 14336 wide, 2000 rows 24.9 us with fp32
+        asm volatile("" : "+r"(a[j].x), "+r"(a[j].y), "+r"(a[j].z), "+r"(a[j].w));
+        Tr::unpack(a[j], y[j]);
+      }
       uint32_t word[V / 4];
 #pragma unroll
       for (int i = 0; i < V / 4; ++i) word[i] = s.four(y[j] + 4 * i);
@@ -220,13 +256,18 @@ __global__ void __launch_bounds__(256) quantise_scalar_kernel(const QuantJob job
     inv = rsqrtf(block_sum(ss, red_sum) / (float)job.width + job.eps);
   }
   auto value = [&](int i) -> float {
-    if constexpr (SRC == kSilu) return silu_mul<T>(Tr::to_f(xr[i]), Tr::to_f(xr[job.width + i]));
+    if constexpr (SRC == kSilu) {
+      float g[2] = {Tr::to_f(xr[i]), 0.f};
+      const float u[2] = {Tr::to_f(xr[job.width + i]), 0.f};
+      silu_mul2<T>(g, u);
+      return g[0];
+    }
     if constexpr (SRC == kNorm) return Tr::to_f(xr[i]) * inv * Tr::to_f(weight[i]);
     if constexpr (SRC == kAddNorm) return Tr::to_f(rr[i]) * inv * Tr::to_f(weight[i]);
     return Tr::to_f(xr[i]);
   };
-  uint32_t top = 0;
-  for (int i = threadIdx.x; i < job.width; i += blockDim.x) top = max(top, magnitude(value(i)));
+  float top = 0.f;
+  for (int i = threadIdx.x; i < job.width; i += blockDim.x) top = larger(top, value(i));
   const RowScale s(block_max(top, red_max));
   if (threadIdx.x == 0) job.scales[row] = s.scale;
   int8_t* codes = job.codes + row * job.codes_stride;
@@ -267,7 +308,7 @@ int launch_quantise(const QuantJob& job, int64_t rows, cudaStream_t stream, cons
 template <typename F>
 int checked(const QuantJob& job, int64_t rows, int64_t width, int64_t inputs, bool pointers,
             const char* name, F run) {
-  if (rows < 0 || rows > INT32_MAX || width <= 0 || width > INT32_MAX)
+  if (rows < 0 || rows > INT32_MAX || width <= 0 || width > (1 << 30))
     return fail(PACE_ERR_INVALID_ARGUMENT, "%s: bad shape [%lld, %lld]", name, (long long)rows,
                 (long long)width);
   if (job.x_stride < inputs * width || job.codes_stride < width)

@@ -21,6 +21,7 @@
 #include <cstdlib>
 #include <algorithm>
 
+#include "f32x2.cuh"
 #include "tcgen05.cuh"
 
 namespace pace {
@@ -101,26 +102,6 @@ __device__ __forceinline__ void shared_floats(const C* p, float* out) {
   } else {
     Traits<C>::unpack(*reinterpret_cast<const uint4*>(p), out);
   }
-}
-
-// Two fp32 numbers in one instruction.
-__device__ __forceinline__ uint64_t two(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void apart(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
 }
 
 // The sum of a lane's squares.
@@ -618,7 +599,7 @@ template <bool APPEND>
 int run_heads(const HeadJob& j, int64_t num_tokens, int cache_dtype, bool neox, int dtype,
               int32_t* fault, cudaStream_t stream, const char* name) {
   if (num_tokens < 0 || num_tokens > INT32_MAX || j.heads < 0 || j.kv_heads < 0 ||
-      j.head_size <= 0 || (int64_t)(j.heads + 2 * (int64_t)j.kv_heads) * j.head_size > INT32_MAX)
+      j.head_size <= 0 || (j.heads + 2 * (int64_t)j.kv_heads) * j.head_size > (1 << 30))
     return fail(PACE_ERR_INVALID_ARGUMENT, "%s: bad shape", name);
   if (j.rot_dim <= 0 || j.rot_dim % 2 != 0 || j.rot_dim > j.head_size)
     return fail(PACE_ERR_INVALID_ARGUMENT, "%s: rot_dim %d must be even and in (0, head_size=%d]",

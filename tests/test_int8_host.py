@@ -46,6 +46,8 @@ def test_int8_argument_errors():
         p, p, p, p, p, None, None, t, n, k, xs, ws, os, 0, bf, None, None)
     _expect(linear(-1, 8, 16, 16, 16, 8), BAD, "bad shape")
     _expect(linear(4, 0, 16, 16, 16, 8), BAD, "bad shape")
+    _expect(linear((1 << 29) + 1, 8, 16, 16, 16, 8), BAD, "bad shape")
+    _expect(linear(4, (1 << 29) + 1, 16, 16, 16, 1 << 30), BAD, "bad shape")
     _expect(linear(4, 8, 16, 15, 16, 8), BAD, "row stride")
     _expect(linear(4, 8, 16, 16, 16, 7), BAD, "row stride")
     _expect(linear(4, 8, 131072, 131072, 131072, 8), LARGE, "32 bits")
@@ -53,6 +55,7 @@ def test_int8_argument_errors():
     assert linear(0, 8, 16, 16, 16, 8) == 0
     quant = lambda t, w, xs, cs: lib.pace_quantise_rows(None, None, None, t, w, xs, cs, bf, None)  # noqa: E731
     _expect(quant(-1, 8, 8, 8), BAD, "bad shape")
+    _expect(quant(2, (1 << 30) + 1, 1 << 31, 1 << 31), BAD, "bad shape")
     _expect(quant(2, 8, 7, 8), BAD, "row stride")
     _expect(quant(2, 8, 8, 8), BAD, "null pointer")
     _expect(lib.pace_silu_and_mul_quantise(None, None, None, 2, 8, 15, 8, bf, None), BAD, "row stride")
@@ -66,6 +69,7 @@ def test_head_argument_errors():
         None, None, None, None, None, 1e-5, t, h, hk, d, qs, ks, None, cabi.PACE_F32, rot, pos, 1,
         cabi.PACE_BF16, None, None)
     _expect(call(-1, 8, 2, 64, 512, 128, 64, 16), BAD, "bad shape")
+    _expect(call(2, 1 << 25, 2, 64, 1 << 31, 128, 64, 16), BAD, "bad shape")
     _expect(call(2, 8, 2, 64, 511, 128, 64, 16), BAD, "row stride")
     _expect(call(2, 8, 2, 64, 512, 128, 63, 16), BAD, "rot_dim")
     _expect(call(2, 8, 2, 64, 512, 128, 66, 16), BAD, "rot_dim")
