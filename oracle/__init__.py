@@ -15,6 +15,8 @@ leg of ``bench.py`` use it, as the checker.
                      index-put back), as layout oracle and timed baseline.
 * ``append_ref``  -- FlashInfer's paged-KV append semantics as PaceServe calls
                      them (get_seq_lens, get_batch_indices_positions, append).
+* ``int8_ref``    -- the 8-bit projections in 64 bits.
+* ``heads_ref``   -- head norms with rotation in 64 bits, step tables by a walk.
 * ``compare_ref_cuda`` -- times the reference's own CUDA ops (and FlashInfer's
                      append path) beside this package's kernels on a B200.
 

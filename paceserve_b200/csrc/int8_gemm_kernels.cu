@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 // joining costs two cluster barriers.  Which CTA sums what is fixed, and sums of
 // integers are exact.
 constexpr int kMidRing = 98304;
-constexpr int kMidAhead = 8;  // K blocks that are pulled into L2 before the wait
+constexpr int kMidAhead = 16;  // K blocks that are pulled into L2 before the wait
 constexpr int kMidRest = 1024 + 256;
 constexpr int kMidTok = 128;  // of a tile, at most
 
