@@ -10,7 +10,7 @@
 // then takes its share of the outputs, finding an entry's request by bisection
 // in shared memory; so one launch does without a grid-wide barrier.  The one
 // value that is read by all and changed, the stack's height, is written by the
-// CTA that finishes last.  It is a matter of latency: a few dependent loads.
+// CTA that read it last.  It is a matter of latency: a few dependent loads.
 #include <algorithm>
 
 #include "common.cuh"
@@ -30,6 +30,7 @@ struct TableJob {
   int32_t *status, *arrivals;
   int64_t table_stride, max_blocks, num_free_pages, num_indices, num_tokens;
   int requests, page_size, page_shift;
+  int no_bits;  // 0, which the compiler does not know
 };
 
 __device__ __forceinline__ int64_t pages_of(const TableJob& j, int64_t tokens) {
@@ -98,19 +99,15 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j)
   int32_t* np = sums + 2 * R + 2;  // BUILD: new pages; release: pages given back
   pdl_launch_dependents();
   pdl_wait();
-  // The stack's height is read once a CTA.  The CTA that has read it last writes the new one: an
-  // arrival is issued with the height in a register, so when the last one has counted, every CTA
-  // has its own.
+  // The stack's height is read once a CTA.  The CTA that has read it last writes the new one: what an
+  // arrival adds is made from the height (of no bit of it), so it is issued when the height has
+  // come, and when the last one has counted, every CTA has its own.
   uint32_t before = 0;
   if (threadIdx.x == 0) {
     problem_bits = 0;
     const int32_t h = *reinterpret_cast<volatile int32_t*>(j.free_count);
     height_read = h;
-    if (gridDim.x > 1)
-      asm volatile("{\n\t.reg .u32 h;\n\tmov.u32 h, %2;\n\tatom.add.relaxed.gpu.global.u32 %0, [%1], 1;\n\t}"
-                   : "=r"(before)
-                   : "l"(j.arrivals), "r"(h)
-                   : "memory");
+    if (gridDim.x > 1) before = atomicAdd(j.arrivals, 1 + (h & j.no_bits));
   }
   auto leave = [&](int64_t height, int32_t problems) {
     if (threadIdx.x != 0 || before != gridDim.x - 1) return;
