@@ -15,7 +15,10 @@
 // there (four elements in 1250 times) the division is done.
 //
 // Memory bounds it: a row is read once with 16-byte vectors, held in registers
-// over the one or two reductions, and stored as 8-byte groups of codes.
+// over the one or two reductions, and stored as 8-byte groups of codes.  Between
+// its loads and its stores a CTA has nothing under way, so each also asks for the
+// row a CTA of the next wave will read, into L2 (8192 rows of SiLU-and-mul, 14336
+// codes: 104 us, 5.6 TB/s, against 110; 1999 rows 29 against 30.5).
 #include "f32x2.cuh"
 
 namespace pace {
@@ -34,6 +37,7 @@ struct QuantJob {
   float eps;
   int width;  // codes per row
   int64_t x_stride, residual_stride, codes_stride;
+  int ahead;  // rows, of the asking ahead
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -137,9 +141,13 @@ __global__ void __launch_bounds__(kMaxThreads) quantise_vec_kernel(const QuantJo
   const T* weight = static_cast<const T*>(job.weight);
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    const int64_t bytes = (int64_t)job.width * sizeof(T);
-    prefetch_l2(xr, SRC == kSilu ? 2 * bytes : bytes);
+    const int64_t bytes = (int64_t)job.width * sizeof(T), read = SRC == kSilu ? 2 * bytes : bytes;
+    prefetch_l2(xr, read);
     if (SRC == kAddNorm) prefetch_l2(rr, bytes);
+    if (row + job.ahead < gridDim.x) {
+      prefetch_l2(xr + job.ahead * job.x_stride, read);
+      if (SRC == kAddNorm) prefetch_l2(rr + job.ahead * job.residual_stride, bytes);
+    }
     if ((SRC == kNorm || SRC == kAddNorm) && row < 4) prefetch_l2(weight, bytes);
   }
   pdl_wait();
@@ -281,7 +289,7 @@ __global__ void __launch_bounds__(256) quantise_scalar_kernel(const QuantJob job
 inline int most_threads(int64_t rows) { return rows > 4096 ? 128 : rows > 1024 ? 256 : kMaxThreads; }
 
 template <typename T, int SRC>
-int launch_quantise(const QuantJob& job, int64_t rows, cudaStream_t stream, const char* name) {
+int launch_quantise(QuantJob job, int64_t rows, int device, cudaStream_t stream, const char* name) {
   constexpr int V = Traits<T>::kVec;
   const int64_t nvec = job.width / V;
   bool vec = job.width % V == 0 && job.x_stride % V == 0 && job.codes_stride % V == 0 &&
@@ -292,6 +300,7 @@ int launch_quantise(const QuantJob& job, int64_t rows, cudaStream_t stream, cons
   const dim3 grid((unsigned)rows);
   cudaError_t err;
   if (vec) {
+    job.ahead = sm_count(device);
     int nv = 1;
     while (nv < 4 && ceil_div(nvec, nv) > most_threads(rows)) nv *= 2;
     const dim3 threads((unsigned)(ceil_div(ceil_div(nvec, nv), 32) * 32));
@@ -331,7 +340,7 @@ extern "C" int pace_quantise_rows(int8_t* codes, float* scales, const void* inpu
   return checked(job, rows, width, 1, true, "quantise_rows", [&] {
     StreamDeviceGuard guard(stream);
     return PACE_DISPATCH_FLOAT(dtype, "quantise_rows", [&] {
-      return launch_quantise<scalar_t, kRows>(job, rows, stream, "quantise_rows");
+      return launch_quantise<scalar_t, kRows>(job, rows, guard.device(), stream, "quantise_rows");
     });
   });
 }
@@ -357,9 +366,9 @@ extern "C" int pace_rms_norm_quantise(int8_t* codes, float* scales, const void* 
   return checked(job, num_tokens, hidden_size, 1, weight != nullptr, "rms_norm_quantise", [&] {
     StreamDeviceGuard guard(stream);
     return PACE_DISPATCH_FLOAT(dtype, "rms_norm_quantise", [&] {
-      return residual ? launch_quantise<scalar_t, kAddNorm>(job, num_tokens, stream,
+      return residual ? launch_quantise<scalar_t, kAddNorm>(job, num_tokens, guard.device(), stream,
                                                             "rms_norm_quantise")
-                      : launch_quantise<scalar_t, kNorm>(job, num_tokens, stream,
+                      : launch_quantise<scalar_t, kNorm>(job, num_tokens, guard.device(), stream,
                                                          "rms_norm_quantise");
     });
   });
@@ -375,7 +384,8 @@ extern "C" int pace_silu_and_mul_quantise(int8_t* codes, float* scales, const vo
   return checked(job, num_tokens, d, 2, true, "silu_and_mul_quantise", [&] {
     StreamDeviceGuard guard(stream);
     return PACE_DISPATCH_FLOAT(dtype, "silu_and_mul_quantise", [&] {
-      return launch_quantise<scalar_t, kSilu>(job, num_tokens, stream, "silu_and_mul_quantise");
+      return launch_quantise<scalar_t, kSilu>(job, num_tokens, guard.device(), stream,
+                                              "silu_and_mul_quantise");
     });
   });
 }
