@@ -7,12 +7,14 @@
 // The sum is int32, so it is exact and the same in every order of its terms (K is
 // at most 131071, where 128 * 128 * K still fits); the rest is fp32, rounded once.
 //
-// Two kernels on the tensor cores, both TMA (128-byte K blocks, 128-byte swizzle)
+// Three kernels on the tensor cores, all TMA (128-byte K blocks, 128-byte swizzle)
 // into a ring, one thread issuing tcgen05.mma.kind::i8, and eight warps that drain
 // the accumulator in TMEM through the scales:
-//  * int8_gemm_kernel, more than 64 tokens: tokens in the accumulator's rows, 256
-//    on a CTA pair (cta_group::2) or 128 on one CTA, by up to 256 channels;
-//  * int8_slice_kernel, up to 64 tokens, where the weight's bytes bound it: 32
+//  * int8_gemm_kernel, many tokens, bound by the matrix rate: tokens in the
+//    accumulator's rows, 256 on a CTA pair (cta_group::2), by up to 256 channels;
+//  * int8_mid_kernel, 33 to 128 tokens, or more where whole tiles of the former
+//    would leave half of the SMs idle: K cut over the CTAs of a cluster;
+//  * int8_slice_kernel, up to 32 tokens, where the weight's bytes bound it: 32
 //    channels a tile, so that there are tiles for all SMs without cutting one over
 //    CTAs.  The 128 rows of the matrix instruction hold the channels' K in four
 //    slices, its columns the tokens' K in the same slices: the four blocks where
@@ -503,20 +505,20 @@ __global__ void __launch_bounds__(THREADS, 1)
 // columns hold the tokens, `tc` (a multiple of 8) for each slice.  So row quarter q
 // and column group (q mod slices) belong to one slice; the other blocks of the
 // accumulator are products of different slices and stay unread.  That costs matrix
-// rate, of which there is enough (64 tokens: 32 bytes of weight a clock and SM,
-// where memory delivers 23), and saves a reduction over CTAs: the slices are summed
-// through shared memory.  The ring is small enough for two CTAs an SM, so that the
+// rate, of which there is enough (32 tokens: an instruction a K block is 128 columns
+// wide, 64 bytes of weight a clock and SM, where memory delivers 23), and saves a
+// reduction over CTAs: the slices are summed through shared memory.  The ring is small enough for two CTAs an SM, so that the
 // next kernel's CTAs start, and pull their first weights into L2, beside this one's.
 // Each takes at most half of TMEM; the kernels that take all of it have over 160 KB of
 // shared memory, so none of their CTAs can wait beside one of these for its columns.
 constexpr int kSliceCh = 32, kSliceTok = 16;  // of a tile; of a pass through shared memory
 constexpr int kSliceRing = 98304;
-constexpr int kSliceAhead = 12;  // blocks that are pulled into L2 ahead of their copy
+constexpr int kSliceAhead = 12;  // blocks that are pulled into L2 before the wait
 constexpr int kSliceSum = 4 * kSliceCh * kSliceTok * 4;
 constexpr int kSliceRest = kSliceSum + 1024 + 256;
 
 struct SliceTiling {
-  int tc, stages, ring, bufs, tmem_cols, tiles, slice_blocks;
+  int tc, stages, ring, tmem_cols, tiles, slice_blocks;
 };
 
 template <typename T, bool SILU>
@@ -618,8 +620,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       bool ok = true;
       Turn turn;
       for (int t = blockIdx.x; ok && t < p.tiles; t += gridDim.x, ++n) {
-        const int b = p.bufs == 2 ? n & 1 : 0;
-        const int use = p.bufs == 2 ? n >> 1 : n;
+        const int b = n & 1, use = n >> 1;
         if (use > 0 && !tc::mbar_wait(&ctl->tmem_empty[b], (uint32_t)(use - 1) & 1u, kWaitLimitNs,
                                       &ctl->abort)) {
           ok = false;
@@ -659,8 +660,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     const int q = warp % 4, tok8 = (warp / 4) * 8;
     int n = 0;
     for (int t = blockIdx.x; t < p.tiles; t += gridDim.x, ++n) {
-      const int b = p.bufs == 2 ? n & 1 : 0;
-      const int use = p.bufs == 2 ? n >> 1 : n;
+      const int b = n & 1, use = n >> 1;
       const int ch = t * kSliceCh + lane;
       const bool valid = ch < j.channels;
       const float sc = valid ? j.channel_scales[ch] : 0.f;
@@ -670,7 +670,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       float st[kSliceTok / EPI_WARPS];  // the next pass's token scales
 #pragma unroll
       for (int e = 0; e < kSliceTok / EPI_WARPS; ++e)
-        st[e] = __ldg(j.token_scales + min(warp + e * EPI_WARPS, j.tokens - 1));
+        st[e] = j.token_scales[min(warp + e * EPI_WARPS, j.tokens - 1)];
       bool ready =
           tc::mbar_wait(&ctl->tmem_full[b], (uint32_t)use & 1u, kWaitLimitNs, &ctl->abort);
       ready = epi_all(ready);
@@ -710,7 +710,7 @@ __global__ void __launch_bounds__(THREADS, 2)
             if (j.add) y += Traits<T>::to_f(static_cast<const T*>(j.add)[tok * j.add_stride + ch]);
             static_cast<T*>(j.out)[tok * j.out_stride + ch] = Traits<T>::from_f(y);
           }
-          st[e] = __ldg(j.token_scales + min(tok + kSliceTok, j.tokens - 1));
+          st[e] = j.token_scales[min(tok + kSliceTok, j.tokens - 1)];
         }
         epi_sync();
       }
@@ -911,7 +911,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         }
       }
       const int64_t t = t0 + c;
-      const float st = __ldg(j.token_scales + t);
+      const float st = j.token_scales[t];
       const int g[4] = {v.x, v.y, v.z, v.w}, h[4] = {u.x, u.y, u.z, u.w};
       float y[4];
 #pragma unroll
@@ -948,7 +948,7 @@ __device__ __forceinline__ uint4 row_bytes(const int8_t* row, int at, int k) {
     uint32_t w[5];
 #pragma unroll
     for (int i = 0; i < 5; ++i)  // no word without a byte of the row
-      w[i] = reinterpret_cast<uintptr_t>(words + i) < end ? __ldg(words + i) : 0u;
+      w[i] = reinterpret_cast<uintptr_t>(words + i) < end ? words[i] : 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[i] = __funnelshift_r(w[i], w[i + 1], shift);
@@ -1113,10 +1113,8 @@ int launch_slices(const Call& c, const GemmJob& j) {
   if (p.tiles <= sm_count(c.device) && p.slice_blocks > 2 * p.stages) p.stages = kRingBytes / stage;
   p.stages = std::min(MAX_STAGES, p.stages);
   p.ring = p.stages * stage;
-  const int cols = SL * p.tc;
-  p.bufs = 2 * cols <= 256 ? 2 : 1;
-  p.tmem_cols = 32;
-  while (p.tmem_cols < p.bufs * cols) p.tmem_cols *= 2;
+  p.tmem_cols = 32;  // two accumulators
+  while (p.tmem_cols < 2 * SL * p.tc) p.tmem_cols *= 2;
   CUtensorMap w, x;
   int rc = make_map(&w, c.weight, weight_rows(c), c.k, c.weight_stride, kSliceCh, j.deep, SL, c.name);
   if (rc == PACE_OK)

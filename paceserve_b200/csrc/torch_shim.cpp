@@ -6,9 +6,10 @@
 // paceserve_b200._C, adds the new ops (fused_add_rms_norm, gelu_and_mul,
 // gelu_tanh_and_mul) in the same style, a kv_transfer_ops submodule for the
 // paged-KV block copy, append, quantised cache and step tables, an attention_ops
-// submodule for paged attention and an int8_ops submodule for 8-bit projections.  Tensors are validated here; every launch goes
-// through the C ABI on the current stream of the tensors' device, and a
-// non-zero status becomes a RuntimeError carrying pace_last_error().
+// submodule for paged attention and an int8_ops submodule for 8-bit projections.
+// Tensors are validated here; every launch goes through the C ABI on the current
+// stream of the tensors' device, and a non-zero status becomes a RuntimeError
+// carrying pace_last_error().
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
