@@ -259,10 +259,24 @@ __device__ __forceinline__ void put_four(const GemmJob& j, int64_t t, int n, boo
 }
 
 // Tiles of the rows kernel: bn channels (gate and up together with SiLU), `sub` K
-// blocks a ring stage.
+// blocks a ring stage.  From tile `whole` on they are done in two halves.
 struct Tiling {
   int bn, sub, stages, m_tiles, n_tiles;
+  int64_t whole;
 };
+
+// A pair's piece of work: a tile, or the half of one that starts `part` half widths in.
+struct Piece {
+  int mt, nt, half, part;
+};
+__device__ __forceinline__ Piece piece_of(int64_t i, const Tiling& p) {
+  Piece w;
+  const int64_t past = i - p.whole;
+  w.half = past >= 0;
+  w.part = w.half ? (int)past & 1 : 0;
+  place_of(w.half ? p.whole + (past >> 1) : i, p.m_tiles, p.n_tiles, w.mt, w.nt);
+  return w;
+}
 
 // One lane of the warp, the same in every call of the same warp.
 __device__ __forceinline__ bool elect_one() {
@@ -300,7 +314,8 @@ struct Turn {
 template <typename T, bool SILU>
 __global__ void __launch_bounds__(THREADS, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
-                     const __grid_constant__ CUtensorMap tm_b, const GemmJob j, const Tiling p,
+                     const __grid_constant__ CUtensorMap tm_b,
+                     const __grid_constant__ CUtensorMap tm_half, const GemmJob j, const Tiling p,
                      int32_t* fault) {
   constexpr int kA = BM * BK, kTmem = 512;
   extern __shared__ uint8_t smem_raw[];
@@ -308,11 +323,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   Ctl* ctl = reinterpret_cast<Ctl*>(tiles + kRingBytes);
   const int nst = p.stages, bn = p.bn, sub = p.sub, out_cols = SILU ? bn / 2 : bn;
-  const int kB = bn / 2 * BK, sb = kA + kB;  // bytes of a K block in this CTA
+  const int kB = bn / 2 * BK, sb = kA + kB;  // bytes of a whole tile's K block in this CTA
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_rank();
   const int workers = (int)gridDim.x >> 1;
-  const int64_t t_first = blockIdx.x >> 1, t_end = (int64_t)p.m_tiles * p.n_tiles;
+  const int64_t t_first = blockIdx.x >> 1;
+  const int64_t t_end = 2 * ((int64_t)p.m_tiles * p.n_tiles) - p.whole;
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -331,6 +347,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == EPI_WARPS && lane == 0) {
     tc::tma_prefetch_desc(&tm_a);
     tc::tma_prefetch_desc(&tm_b);
+    tc::tma_prefetch_desc(&tm_half);
   }
   if (warp == 0) tc::tmem_alloc_pair(&ctl->tmem, kTmem);
   tc::tc_fence_before();
@@ -349,11 +366,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     // both CTAs' copies complete on the leader's barrier, which expects the bytes of both
     const uint32_t full0 = tc::map_to_rank(&ctl->full[0], 0);
     for (int64_t t = t_first; ok && t < t_end; t += workers) {
-      int mt, nt;
-      place_of(t, p.m_tiles, p.n_tiles, mt, nt);
-      const int a0 = (2 * mt + (int)rank) * BM;
+      const Piece w = piece_of(t, p);
+      const CUtensorMap* tm_w = w.half ? &tm_half : &tm_b;
+      const int a0 = (2 * w.mt + (int)rank) * BM, kW = kB >> w.half;
       // with SiLU the leader has the gate's rows, its partner the up's
-      const int b0 = SILU ? nt * out_cols + (int)rank * j.channels : nt * bn + (int)rank * (bn / 2);
+      const int b0 = w.nt * out_cols + w.part * (out_cols / 2) +
+                     (int)rank * (SILU ? j.channels : bn / 2 >> w.half);
       for (int kb = 0; kb < j.k_blocks; kb += sub, ++i) {
         const int s = turn.s;
         if (i >= nst && !ring_wait(&ctl->empty[s], turn.phase ^ 1u, ctl)) {
@@ -364,14 +382,14 @@ __global__ void __launch_bounds__(THREADS, 1)
           uint8_t* a = tiles + s * sub * sb;
           uint8_t* b = a + sub * kA;
           const uint32_t bar = full0 + (uint32_t)(s * sizeof(uint64_t));
-          if (rank == 0) tc::mbar_arrive_expect_tx(&ctl->full[s], 2 * sub * sb);
+          if (rank == 0) tc::mbar_arrive_expect_tx(&ctl->full[s], 2 * sub * (kA + kW));
           if (j.deep) {
             tma_load_deep_pair(a, &tm_a, a0, kb, bar);
-            tma_load_deep_pair(b, &tm_b, b0, kb, bar);
+            tma_load_deep_pair(b, tm_w, b0, kb, bar);
           } else {
             for (int u = 0; u < sub; ++u) {
               tc::tma_load_2d_pair(a + u * kA, &tm_a, (kb + u) * BK, a0, bar);
-              tc::tma_load_2d_pair(b + u * kB, &tm_b, (kb + u) * BK, b0, bar);
+              tc::tma_load_2d_pair(b + u * kW, tm_w, (kb + u) * BK, b0, bar);
             }
           }
         }
@@ -389,11 +407,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ---- MMA issuer, in the leader ------------------------------------------
     if (rank == 0) {
       const bool issues = elect_one();
-      const uint32_t idesc = idesc_i8(2 * BM, bn);
       int n = 0;
       bool ok = true;
       Turn turn;
       for (int64_t t = t_first; ok && t < t_end; t += workers, ++n) {
+        const int half = t >= p.whole, kW = kB >> half;
+        const uint32_t idesc = idesc_i8(2 * BM, bn >> half);
         const int b = n & 1;
         const uint32_t use_b = (uint32_t)(n >> 1);
         if (use_b > 0 &&
@@ -419,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               for (int k = 0; k < BK / 32; ++k)
                 umma_i8<true>(d, ad + 2 * k, bd + 2 * k, idesc, kb > 0 || u > 0 || k > 0 ? 1u : 0u);
               ad += kA >> 4;
-              bd += (uint64_t)kB >> 4;
+              bd += (uint64_t)kW >> 4;
             }
             tc::umma_commit_pair_both(&ctl->empty[s]);
           }
@@ -437,16 +456,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else {
     // ---- epilogue: warp w drains lanes 32 (w % 4) .. +31, half w / 4 of the columns --------
     const int row = (warp % 4) * 32 + lane;
-    const int c_begin = (warp / 4) * (out_cols / 2), c_end = c_begin + out_cols / 2;
     const uint32_t tmem_empty0 = tc::map_to_rank(&ctl->tmem_empty[0], 0);
-    const int up = bn / 2;  // SiLU: the up columns' distance
     int n = 0;
     for (int64_t t = t_first; t < t_end; t += workers, ++n) {
       const int b = n & 1;
-      int mt, nt;
-      place_of(t, p.m_tiles, p.n_tiles, mt, nt);
-      const int m = (2 * mt + (int)rank) * BM + row;  // this thread's token
-      const int c0 = nt * out_cols;                   // the tile's first channel
+      const Piece w = piece_of(t, p);
+      const int m = (2 * w.mt + (int)rank) * BM + row;  // this thread's token
+      const int c0 = w.nt * out_cols + w.part * (out_cols / 2);  // the piece's first channel
+      const int cols = out_cols / 2 >> w.half;                   // of this warp
+      const int c_begin = (warp / 4) * cols, c_end = c_begin + cols;
+      const int up = bn / 2 >> w.half;  // SiLU: the up columns' distance
       const bool valid = m < j.tokens;
       const float s_row = valid ? j.token_scales[m] : 0.f;
       bool ready = tc::mbar_wait(&ctl->tmem_full[b], (uint32_t)(n >> 1) & 1u, kWaitLimitNs,
@@ -1048,6 +1067,9 @@ constexpr int64_t kMidTokens = 128;   // up to here the cluster kernel, above by
 // over the pairs costs (B200, ns a K block, and us for a call's start and end):
 //   128: 195, 6.8;  192: 275, 8.0;  256: 295, 9.1
 // (512 tokens, K 4096: 6144 channels 19.2, 17.5, 19.3 us; 4096 channels 13.4, 16.7, 18.5.)
+// A last round that would leave half of the pairs idle takes its tiles of 256 in halves, at 190 ns a
+// K block (512 tokens, K 4096: gate and up of 14336, 2 tiles of 224 left, 47.9 us against 50.1; 20000
+// channels, 10 of 158 left, 37.0 against 39.0).
 struct RowsPlan {
   Tiling t;
   int pairs;
@@ -1062,12 +1084,16 @@ inline RowsPlan rows_plan(int64_t tokens, int64_t channels, int k_blocks, bool s
   const int pairs = std::max(1, sms / 2);
   for (const auto& kind : kinds) {
     const int64_t m = ceil_div(tokens, 2 * BM), n = ceil_div(channels, silu ? kind.bn / 2 : kind.bn);
-    const double cost = kind.fixed + (double)ceil_div(m * n, pairs) * k_blocks * kind.block;
+    const int64_t last = m * n % pairs;  // tiles of the last round
+    const bool halves = kind.bn == 256 && m * n > pairs && 2 * last <= pairs;
+    const double cost = kind.fixed + k_blocks * ((double)(m * n / pairs) * kind.block +
+                                                 (last == 0 ? 0. : halves ? 0.19 : kind.block));
     if (best.pairs != 0 && cost >= least) continue;
     least = cost;
     best.t.bn = kind.bn;
     best.t.m_tiles = (int)m;
     best.t.n_tiles = (int)n;
+    best.t.whole = halves ? m * n - last : m * n;
     best.pairs = (int)std::min<int64_t>(m * n, pairs);
   }
   // two K blocks a stage halve what a stage costs beside its bytes (128 channels: 270 -> 195 ns);
@@ -1172,17 +1198,21 @@ int launch_mid(const Call& c, const GemmJob& j) {
 
 template <typename T, bool SILU>
 int launch_rows(const Call& c, const GemmJob& j, const RowsPlan& p) {
-  CUtensorMap a, b;
+  CUtensorMap a, b, half;
   int rc = make_map(&a, c.codes, c.tokens, c.k, c.codes_stride, BM, j.deep, p.t.sub, c.name);
   if (rc == PACE_OK)
     rc = make_map(&b, c.weight, weight_rows(c), c.k, c.weight_stride, p.t.bn / 2, j.deep, p.t.sub,
+                  c.name);
+  half = b;
+  if (rc == PACE_OK && p.t.whole < (int64_t)p.t.m_tiles * p.t.n_tiles)
+    rc = make_map(&half, c.weight, weight_rows(c), c.k, c.weight_stride, p.t.bn / 4, j.deep, p.t.sub,
                   c.name);
   if (rc != PACE_OK) return rc;
   auto kernel = int8_gemm_kernel<T, SILU>;
   cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kSmem);
   if (err != cudaSuccess) return cuda_fail(err, c.name);
-  err = launch_pairs(kernel, dim3((unsigned)(2 * p.pairs)), dim3(THREADS), kSmem, c.stream, a, b, j,
-                     p.t, c.fault);
+  err = launch_pairs(kernel, dim3((unsigned)(2 * p.pairs)), dim3(THREADS), kSmem, c.stream, a, b, half,
+                     j, p.t, c.fault);
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, c.name);
 }
 

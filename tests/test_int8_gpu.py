@@ -161,6 +161,8 @@ SHAPES = [
     (1, 6144, 4096), (1, 128, 128), (1, 1, 16), (3, 130, 48), (16, 4096, 14336), (17, 200, 256),
     (32, 6144, 4096), (33, 72, 8192), (64, 4096, 14336), (65, 4096, 4096), (128, 1000, 2048),
     (129, 300, 4096), (256, 4096, 4096), (300, 264, 14336), (777, 1003, 1040), (520, 4096, 1152), (200, 6144, 656), (1000, 1500, 304), (1000, 6144, 4096),
+    # the last round's few tiles in halves, whole K blocks and not
+    (300, 9700, 4096), (300, 9700, 4112), (601, 8900, 5008),
 ]
 
 
@@ -188,7 +190,8 @@ def test_linear(t, n, k, dtype):
 
 
 @pytest.mark.parametrize("t,i,k", [(1, 14336, 4096), (2, 64, 64), (20, 200, 4096), (50, 1024, 2048),
-                                   (128, 700, 1024), (130, 130, 256), (512, 14336, 4096), (601, 2056, 14336)])
+                                   (128, 700, 1024), (130, 130, 256), (512, 14336, 4096), (601, 2056, 14336),
+                                   (300, 4850, 4112)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gate_up_silu(t, i, k, dtype):
     g = torch.Generator().manual_seed(t + i + k)
