@@ -197,13 +197,13 @@ __device__ __forceinline__ void load_scales(const GemmJob& j, int n, float (&s)[
   }
 }
 
-// CH consecutive channels n .. of one token: add, round, store.
+// CH consecutive channels n .. of one token in 16-byte accesses: add, round, store.
 template <typename T>
 __device__ __forceinline__ void put_channels(const GemmJob& j, int64_t t, int n, float* y) {
   constexpr int V = Traits<T>::kVec;
   T* o = static_cast<T*>(j.out) + t * j.out_stride + n;
   const T* add = j.add ? static_cast<const T*>(j.add) + t * j.add_stride + n : nullptr;
-  if (j.vec && n + CH <= j.channels) {
+  if (n + CH <= j.channels) {
     if (add) {
 #pragma unroll
       for (int i = 0; i < CH / V; ++i) {
@@ -229,6 +229,37 @@ __device__ __forceinline__ void put_channels(const GemmJob& j, int64_t t, int n,
       if (n + e < j.channels)
         o[e] = Traits<T>::from_f(add ? y[e] + Traits<T>::to_f(add[e]) : y[e]);
   }
+}
+
+// The same of a warp's 32 tokens t0 .., a token a lane, in single elements: by way of shared memory,
+// so that 16 lanes take neighbouring channels of a token (512 tokens, K 4096, 4095 channels 17.1 us,
+// a lane its own token 31.2; 2048 tokens, 32001 channels 228 and 716).
+constexpr int kTurnPitch = CH + 1, kTurn = EPI_WARPS * 32 * kTurnPitch * (int)sizeof(float);
+template <typename T>
+__device__ __forceinline__ void put_turned(const GemmJob& j, int t0, int n, const float (&y)[CH],
+                                           float* turn) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int e = 0; e < CH; ++e) turn[lane * kTurnPitch + e] = y[e];
+  __syncwarp();
+  constexpr int kRows = 32 / CH;  // at a time
+  const int e = lane % CH, r0 = lane / CH;
+  const int rows = n + e < j.channels ? min(32, j.tokens - t0) : 0;
+  float v[32 / kRows];
+#pragma unroll
+  for (int i = 0; i < 32 / kRows; ++i) {
+    const int r = r0 + i * kRows;
+    v[i] = turn[r * kTurnPitch + e];
+    if (j.add && r < rows)
+      v[i] += Traits<T>::to_f(static_cast<const T*>(j.add)[(int64_t)(t0 + r) * j.add_stride + n + e]);
+  }
+#pragma unroll
+  for (int i = 0; i < 32 / kRows; ++i) {
+    const int r = r0 + i * kRows;
+    if (r < rows)
+      static_cast<T*>(j.out)[(int64_t)(t0 + r) * j.out_stride + n + e] = Traits<T>::from_f(v[i]);
+  }
+  __syncwarp();
 }
 
 // Four consecutive channels n .. of one token, as put_channels.
@@ -457,6 +488,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ---- epilogue: warp w drains lanes 32 (w % 4) .. +31, half w / 4 of the columns --------
     const int row = (warp % 4) * 32 + lane;
     const uint32_t tmem_empty0 = tc::map_to_rank(&ctl->tmem_empty[0], 0);
+    float* turn = reinterpret_cast<float*>(ctl + 1) + warp * 32 * kTurnPitch;  // unless j.vec
     int n = 0;
     for (int64_t t = t_first; t < t_end; t += workers, ++n) {
       const int b = n & 1;
@@ -489,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (SILU) load_scales(j, j.channels + ch, sc2);
         tc::tmem_wait_ld(r);
         if (SILU) tc::tmem_wait_ld(r2);
-        if (valid) {
+        if (valid || !j.vec) {
           float y[CH];
 #pragma unroll
           for (int e = 0; e < CH; ++e) {
@@ -501,7 +533,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int e = 0; e < CH; ++e) y[e] += Traits<T>::to_f(bias[min(ch + e, j.channels - 1)]);
           }
-          put_channels<T>(j, m, ch, y);
+          if (j.vec)
+            put_channels<T>(j, m, ch, y);
+          else
+            put_turned<T>(j, m - lane, ch, y, turn);
         }
       }
       tc::tc_fence_before();
@@ -1209,9 +1244,10 @@ int launch_rows(const Call& c, const GemmJob& j, const RowsPlan& p) {
                   c.name);
   if (rc != PACE_OK) return rc;
   auto kernel = int8_gemm_kernel<T, SILU>;
-  cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kSmem);
+  cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), c.device, kSmem + kTurn);
   if (err != cudaSuccess) return cuda_fail(err, c.name);
-  err = launch_pairs(kernel, dim3((unsigned)(2 * p.pairs)), dim3(THREADS), kSmem, c.stream, a, b, half,
+  err = launch_pairs(kernel, dim3((unsigned)(2 * p.pairs)), dim3(THREADS),
+                     j.vec ? kSmem : kSmem + kTurn, c.stream, a, b, half,
                      j, p.t, c.fault);
   return err == cudaSuccess ? PACE_OK : cuda_fail(err, c.name);
 }
