@@ -56,7 +56,7 @@ def check_codes(codes, scales, y, error):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,width,strided", [
     (1, 4096, False), (3, 64, True), (5, 1, False), (7, 1111, False), (2, 8192, True), (2, 16392, False),
-    (300, 256, False), (2, 20000, False), (4, 14336, False)])
+    (300, 256, False), (2, 20000, False), (4, 14336, False), (2, 32776, False), (160, 18432, True)])
 def test_quantise_rows(dtype, rows, width, strided):
     g = torch.Generator().manual_seed(width)
     x = inputs(g, rows, width, dtype, strided)
@@ -98,7 +98,8 @@ def test_quantise_extremes(dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,width,strided", [
-    (1, 4096, False), (3, 64, True), (5, 7, False), (2, 1111, False), (130, 8192, False), (2, 20000, False)])
+    (1, 4096, False), (3, 64, True), (5, 7, False), (2, 1111, False), (130, 8192, False), (2, 20000, False),
+    (2, 16384, False), (160, 18432, True)])
 @pytest.mark.parametrize("add", [False, True])
 def test_rms_norm_quantise(dtype, rows, width, strided, add):
     g = torch.Generator().manual_seed(width + add)
@@ -130,7 +131,8 @@ def test_rms_norm_quantise_row_of_zeros_and_nan():
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,width,strided", [
-    (1, 14336, False), (3, 64, True), (5, 7, False), (2, 1111, False), (65, 4096, False), (2, 20000, False)])
+    (1, 14336, False), (3, 64, True), (5, 7, False), (2, 1111, False), (65, 4096, False), (2, 20000, False),
+    (2, 32776, False), (160, 18432, True)])
 def test_silu_and_mul_quantise(dtype, rows, width, strided):
     g = torch.Generator().manual_seed(width)
     x = inputs(g, rows, 2 * width, dtype, strided)
