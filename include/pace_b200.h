@@ -569,8 +569,8 @@ int pace_silu_and_mul_quantise(int8_t* codes, float* scales, const void* input,
  *     llama.py:101-106, 176-178, 240-254).
  *   pace_int8_gate_up_silu: out[t, i] = (T)(silu(y[t, i]) * y[t, I + i]), as
  *     pace_gate_up_silu.
- * Out and residual are of `dtype`.  Any k, strides and addresses; fast where k, the
- * row strides and the addresses of codes and weight are multiples of 16 bytes.
+ * Out and residual are of `dtype`.  Any k, strides and addresses; fast where the row
+ * strides and the addresses of codes and weight are multiples of 16 bytes.
  * Every wait in the kernels is bounded by a second; one that runs out sets bit 30
  * of *fault_flags (may be NULL) and leaves the output undefined. */
 int pace_int8_linear(void* out, const int8_t* codes, const float* token_scales,

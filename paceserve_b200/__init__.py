@@ -66,9 +66,11 @@ def fold_rmsnorm_weight(linear_weight, norm_weight):
 def quantise_weight(weight):
     """A linear weight [n, k] on the GPU as 8-bit integers with a scale for each
     output channel, (codes, channel_scales), for ``int8_ops.linear``,
-    ``linear_residual`` and ``gate_up_silu``.  Prepared once per model load."""
-    codes = torch.empty(weight.shape, dtype=torch.int8, device=weight.device)
-    scales = torch.empty(weight.shape[0], dtype=torch.float32, device=weight.device)
+    ``linear_residual`` and ``gate_up_silu``.  Prepared once per model load.  The
+    codes' rows are a multiple of 16 bytes apart, whatever k is."""
+    n, k = weight.shape
+    codes = torch.empty(n, -(-k // 16) * 16, dtype=torch.int8, device=weight.device)[:, :k]
+    scales = torch.empty(n, dtype=torch.float32, device=weight.device)
     int8_ops.quantise_rows(codes, scales, weight)
     return codes, scales
 

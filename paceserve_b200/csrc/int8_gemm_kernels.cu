@@ -20,8 +20,8 @@
 //    slices, its columns the tokens' K in the same slices: the four blocks where
 //    the slices agree are partial sums, the others are not read.
 //
-// What TMA cannot take (K, a row stride or an address that is no multiple of 16
-// bytes) runs through registers and small matrix instructions (int8_dot_kernel).
+// What TMA cannot take (a row stride or an address that is no multiple of 16 bytes)
+// runs through registers and small matrix instructions (int8_dot_kernel).
 #include <algorithm>
 #include <type_traits>
 
@@ -1265,8 +1265,8 @@ int launch_tensor(const Call& c, const GemmJob& j) {
 
 // Whether TMA takes both operands.
 inline bool for_tma(const Call& c) {
-  return c.k % 16 == 0 && c.codes_stride % 16 == 0 && c.weight_stride % 16 == 0 &&
-         aligned16(c.codes) && aligned16(c.weight);
+  return c.codes_stride % 16 == 0 && c.weight_stride % 16 == 0 && aligned16(c.codes) &&
+         aligned16(c.weight);
 }
 
 template <typename T>
@@ -1304,6 +1304,7 @@ int run_int8(Call c, GemmJob j) {
     return fail(PACE_ERR_INVALID_ARGUMENT, "%s: null pointer", c.name);
   StreamDeviceGuard guard(c.stream);
   c.device = guard.device();
+  if (c.tokens == 1) c.codes_stride = ceil_div(c.k, 16) * 16;  // of one row it says nothing
   j.tokens = (int)c.tokens;
   j.channels = (int)c.channels;
   return PACE_DISPATCH_FLOAT(c.dtype, c.name, [&] { return run_typed<scalar_t>(c, j); });

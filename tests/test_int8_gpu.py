@@ -239,6 +239,30 @@ def test_rows_that_tma_does_not_take(t, n, k, pad, dtype):
     assert ((out.double() - want).abs() <= (half(dtype) + error) * want.abs() + least).all()
 
 
+@pytest.mark.parametrize("t", [1, 20, 100, 300])
+@pytest.mark.parametrize("k,pad", [(1111, 9), (4090, 6), (3, 13), (129, 15)])
+def test_ragged_k_in_aligned_rows(t, k, pad):
+    """What lies behind a row's k codes is not read into the sums."""
+    g = torch.Generator().manual_seed(t + k)
+    dtype = torch.float32
+    x, sx, w, sw = make(g, t, 268, k, dtype, pad)
+    y = ref.linear(x, sx, w, sw)
+    out = torch.empty(t, 268, dtype=dtype, device=DEV)
+    int8_ops.linear(out, x, sx, w, sw)
+    check_linear(out, y, y.abs(), dtype)
+    out = torch.empty(t, 134, dtype=dtype, device=DEV)
+    int8_ops.gate_up_silu(out, x, sx, w, sw)
+    gate = y[:, :134]
+    error = silu_error(gate) + 3 * F32 * (gate.abs() + 1) + 4 * F32
+    want = ref.gate_up_silu(x, sx, w, sw)
+    # below the smallest normal number half a step is smallest_normal * eps / 2.  Where e^-gate passes
+    # 2^128 in fp32 (gate below -88.7), the quotient is 0: what is lost is |gate| e^gate |up|, at most
+    # |gate| |up| 2^-127, with both below 2^13 under 2^-100
+    assert y.abs().max() < 2.0 ** 13
+    least = torch.finfo(dtype).smallest_normal * half(dtype) + 2.0 ** -100
+    assert ((out.double() - want).abs() <= (half(dtype) + error) * want.abs() + least).all()
+
+
 @pytest.mark.parametrize("t", [1, 40, 100, 300])
 def test_strides_of_everything(t):
     """Rows of codes, weight, output and residual inside wider ones; what lies beside stays."""
@@ -343,6 +367,15 @@ def test_quantised_weight_near_the_linear():
     bound = 0.501 * (sx.double()[:, None] * w.double().abs().sum(-1)
                      + (cx.double().abs().sum(-1) * sx.double())[:, None] * sw.double())
     assert ((out.double() - x.double() @ w.double().T).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("n,k", [(5, 500), (1, 77), (3, 64)])
+def test_quantised_weight_rows_are_aligned(n, k):
+    g = torch.Generator().manual_seed(k)
+    w = torch.randn(n, k, generator=g).to(DEV)
+    codes, scales = quantise_weight(w)
+    assert codes.shape == (n, k) and codes.stride(0) % 16 == 0 and codes.data_ptr() % 16 == 0
+    check_codes(codes, scales, w.double(), 0.0)
 
 
 def test_refusals():
