@@ -284,9 +284,12 @@ __global__ void __launch_bounds__(256) quantise_scalar_kernel(const QuantJob job
 
 // Threads a row, at most: many rows do best with several vectors a thread (4096
 // wide, norm with residual, us, 128 / 256 / 512 threads: 512 rows 6.4, 5.7, 4.4;
-// 2048 rows 12.3, 12.2, 13.7; 8192 rows 39, 41, 49), few rows with the shortest
-// chain (1 row, alone, 1.9, 1.2, 1.3).
-inline int most_threads(int64_t rows) { return rows > 4096 ? 128 : rows > 1024 ? 256 : kMaxThreads; }
+// 2048 rows 12.3, 12.2, 13.7; 8192 rows 39, 41, 49), few rows, a CTA an SM, with the
+// shortest chain (SiLU-and-mul of 14336 codes, 256 / 512 / 1024 threads: 64 rows
+// 4.8, 4.7, 3.3; 256 rows 5.7, 5.7, 6.4).
+inline int most_threads(int64_t rows, int sms) {
+  return rows > 4096 ? 128 : rows > 1024 ? 256 : rows > sms ? kMaxThreads : kWideThreads;
+}
 
 template <typename T, int SRC>
 int launch_quantise(QuantJob job, int64_t rows, int device, cudaStream_t stream, const char* name) {
@@ -300,17 +303,19 @@ int launch_quantise(QuantJob job, int64_t rows, int device, cudaStream_t stream,
   const dim3 grid((unsigned)rows);
   cudaError_t err;
   if (vec) {
-    job.ahead = sm_count(device);
+    const int sms = sm_count(device);
+    job.ahead = sms;
     int nv = 1;
-    while (nv < 4 && ceil_div(nvec, nv) > most_threads(rows)) nv *= 2;
+    while (nv < 4 && ceil_div(nvec, nv) > most_threads(rows, sms)) nv *= 2;
     const dim3 threads((unsigned)(ceil_div(ceil_div(nvec, nv), 32) * 32));
     // more than 512 threads leave a thread 64 registers (2048 rows of SiLU-and-mul, 18432 codes: 35.6 us;
     // element by element 165)
-    err = threads.x > kMaxThreads
-              ? launch(quantise_vec_kernel<T, SRC, 4, kWideThreads>, grid, threads, 0, stream, job)
-          : nv == 1 ? launch(quantise_vec_kernel<T, SRC, 1>, grid, threads, 0, stream, job)
-          : nv == 2 ? launch(quantise_vec_kernel<T, SRC, 2>, grid, threads, 0, stream, job)
-                    : launch(quantise_vec_kernel<T, SRC, 4>, grid, threads, 0, stream, job);
+    auto go = [&](auto few, auto wide) {
+      return launch(threads.x > kMaxThreads ? wide : few, grid, threads, 0, stream, job);
+    };
+    err = nv == 1   ? go(quantise_vec_kernel<T, SRC, 1>, quantise_vec_kernel<T, SRC, 1, kWideThreads>)
+          : nv == 2 ? go(quantise_vec_kernel<T, SRC, 2>, quantise_vec_kernel<T, SRC, 2, kWideThreads>)
+                    : go(quantise_vec_kernel<T, SRC, 4>, quantise_vec_kernel<T, SRC, 4, kWideThreads>);
   } else {
     err = launch(quantise_scalar_kernel<T, SRC>, grid, dim3(256), 0, stream, job);
   }
