@@ -306,6 +306,25 @@ def test_nan_scale_reaches_its_row_alone():
         assert out[2].isnan().all() and out.isnan().any(-1).sum() == 1
 
 
+@pytest.mark.parametrize("n", [32768, 32769])
+def test_offsets_past_32_bits(n):
+    """Over 2^31 outputs: the last rows are those of a call with them alone."""
+    t, k, last = 66000, 128, 200
+    x = torch.randint(-127, 128, (t, k), device=DEV, dtype=torch.int8)
+    w = torch.randint(-127, 128, (n, k), device=DEV, dtype=torch.int8)
+    sx, sw = torch.rand(t, device=DEV) / 127, torch.rand(n, device=DEV) / 127
+    out = torch.zeros(t, n, dtype=torch.bfloat16, device=DEV)
+    int8_ops.linear(out, x, sx, w, sw)
+    want = ref.linear(x[-last:], sx[-last:], w, sw)
+    check_linear(out[-last:], want, want.abs(), torch.bfloat16)
+    codes = torch.zeros(t, n, dtype=torch.int8, device=DEV)
+    scales = torch.zeros(t, device=DEV)
+    int8_ops.quantise_rows(codes, scales, out)
+    check_codes(codes[-last:], scales[-last:], out[-last:].double(), 0.0)
+    int8_ops.linear_residual(out, x, sx, w, sw)
+    assert out[0].isfinite().all() and not torch.equal(out[-1].double(), want[-1])
+
+
 def test_no_tokens():
     x = torch.empty(0, 64, dtype=torch.int8, device=DEV)
     s = torch.empty(0, device=DEV)

@@ -231,3 +231,23 @@ def test_class_refuses_and_tells():
         tables.begin_step(ints([0, 0], torch.int64), ints([0, 0]))
     with pytest.raises(RuntimeError, match="all sizes"):
         BlockTables(0, 4, 16, 3, 100, DEV)
+
+
+def test_many_steps_without_a_pause():
+    """Every CTA of every call has the height that the call before left."""
+    n, page = 700, 16
+    held, new = lens(n, 500, 60, 5)
+    t = BlockTables(n, 40, page, 40 * n, 501 * n)
+    seq, new = ints(held), ints(new)
+    t.begin_step(torch.zeros_like(seq), seq)
+    t.check()
+    height, stack = t.free_count.item(), t.free_pages.clone()
+    total = seq + new
+    for _ in range(300):
+        step = t.begin_step(seq, new)
+        t.release(total, seq)
+    t.check()
+    assert t.free_count.item() == height and torch.equal(t.free_pages, stack)
+    assert step.append_indptr[-1].item() == new.sum().item()
+    used = step.kv_indices[:step.kv_indptr[-1].item()].tolist()
+    assert len(set(used)) == len(used)  # no page twice
