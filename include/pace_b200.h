@@ -512,12 +512,18 @@ int pace_read_quantised_paged_kv_cache(void* key, void* value, int64_t rows, int
  * If something does not fit, a PACE_TABLES_* bit is set in *status, block_tables
  * and the stack stay as they are, the indptr arrays and kv_last_page_len become
  * 0 and all token entries -1, so that no later kernel writes to a page by them.
+ * While *status is not 0, every call that is given it does the same and leaves it:
+ * lengths that have moved on count pages that were never given.  The caller zeroes
+ * it (also before the first call) and goes on with the lengths that the last call
+ * that fitted left; releases made meanwhile gave nothing and are made again.
  * *arrivals: a word of the caller's, zero, left zero; calls that share it, the
- * tables or the stack must not overlap.  Page numbers are not looked at.
+ * status, the tables or the stack must not overlap.  Page numbers, and whether a
+ * held page was ever given, are not looked at.
  *
  * pace_release_pages: request b keeps the pages of its first kept_lens[b] of
  * held_lens[b] tokens and the others go back onto the stack, so that taking and
- * releasing the same pages leaves it as it was.  block_tables is only read. */
+ * releasing the same pages leaves it as it was.  block_tables is only read.
+ * *status stops it, and is set, as above. */
 #define PACE_TABLES_BAD_LENGTH 1    /* negative, or more kept than held          */
 #define PACE_TABLES_SHORT_ROW 2     /* a request needs more than max_blocks      */
 #define PACE_TABLES_SHORT_INDICES 4 /* more pages than num_kv_indices            */

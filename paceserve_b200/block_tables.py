@@ -75,7 +75,8 @@ class BlockTables:
         """Take pages for ``new_lens[b]`` tokens after the ``seq_lens[b]`` that
         request b has (int32 on the device, one entry for each row in use) and
         build the step's arrays.  A step that does not fit takes nothing, leaves
-        every token entry at -1 and shows in ``check``."""
+        every token entry at -1 and shows in ``check``; until then all later steps
+        and releases do the same, whatever their lengths."""
         s, n = self._step, seq_lens.numel()
         if n > self.block_tables.shape[0]:
             raise RuntimeError("BlockTables.begin_step: more lengths than rows")
@@ -95,7 +96,12 @@ class BlockTables:
 
     def check(self) -> None:
         """Raise if a step or a release since the last call did not fit.  Waits
-        for the current stream, which has to come after those calls."""
+        for the current stream, which has to come after those calls.
+
+        From that step or release on nothing was taken, given or written to.  Go on
+        with the lengths that the last step that fitted left (lengths that moved on
+        since count pages that their requests were not given), and make the
+        releases since then again."""
         bits = int(self._status)
         if bits:
             self._status.zero_()

@@ -8,9 +8,14 @@
 // follows from three prefix sums over the requests (new tokens, pages, new
 // pages).  Every CTA works them out for itself (they are a few KB, from L2) and
 // then takes its share of the outputs, finding an entry's request by bisection
-// in shared memory; so one launch does without a grid-wide barrier.  The one
-// value that is read by all and changed, the stack's height, is written by the
-// CTA that read it last.  It is a matter of latency: a few dependent loads.
+// in shared memory; so one launch does without a grid-wide barrier.  The two
+// values that are read by all and changed, the stack's height and the status, are
+// written by the CTA that read them last.  It is a matter of latency: a few
+// dependent loads.
+//
+// Lengths that moved on after a step that did not fit would count pages as held
+// that were never given: their entries of the block table are an earlier owner's.
+// So a call does nothing while the status is set.
 #include <algorithm>
 
 #include "common.cuh"
@@ -92,22 +97,24 @@ template <bool BUILD>
 __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j) {
   extern __shared__ int32_t sums[];  // [requests + 1] each: first, pages, new pages
   __shared__ uint32_t part[32][3];
-  __shared__ int problem_bits, height_read;
+  __shared__ int problem_bits, height_read, status_read;
   const int R = j.requests, threads = blockDim.x;
   int32_t* ip = sums;              // BUILD: new tokens; release: pages kept
   int32_t* kp = sums + R + 1;      // BUILD: pages
   int32_t* np = sums + 2 * R + 2;  // BUILD: new pages; release: pages given back
   pdl_launch_dependents();
   pdl_wait();
-  // The stack's height is read once a CTA.  The CTA that has read it last writes the new one: what an
-  // arrival adds is made from the height (of no bit of it), so it is issued when the height has
-  // come, and when the last one has counted, every CTA has its own.
+  // The stack's height and the status are read once a CTA.  The CTA that has read them last writes the
+  // new ones: what an arrival adds is made from both (of no bit of them), so it is issued when they
+  // have come, and when the last one has counted, every CTA has its own.
   uint32_t before = 0;
   if (threadIdx.x == 0) {
     problem_bits = 0;
     const int32_t h = *reinterpret_cast<volatile int32_t*>(j.free_count);
+    const int32_t set = *reinterpret_cast<volatile int32_t*>(j.status);
     height_read = h;
-    if (gridDim.x > 1) before = atomicAdd(j.arrivals, 1 + (h & j.no_bits));
+    status_read = set;
+    if (gridDim.x > 1) before = atomicAdd(j.arrivals, 1 + ((h | set) & j.no_bits));
   }
   auto leave = [&](int64_t height, int32_t problems) {
     if (threadIdx.x != 0 || before != gridDim.x - 1) return;
@@ -169,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const TableJob j)
   }
   if (problems) atomicOr(&problem_bits, problems);
   __syncthreads();
-  problems = problem_bits;
+  problems = status_read ? status_read : problem_bits;  // the first cause stays the only one
   const int64_t step = (int64_t)gridDim.x * threads;
   const int64_t me = (int64_t)blockIdx.x * threads + threadIdx.x;
   if (problems) {
