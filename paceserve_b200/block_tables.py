@@ -24,6 +24,8 @@ from . import _C
 
 kv_transfer_ops = _C.kv_transfer_ops
 
+MAX_REQUESTS = 8192  # of a step: their prefix sums are in one CTA's shared memory
+
 PROBLEMS = {1: "a length is negative, or more tokens are kept than held",
             2: "a request needs more pages than its row holds",
             4: "the step needs more pages than kv_indices holds",
@@ -46,8 +48,8 @@ class StepTables(NamedTuple):
 
 class BlockTables:
     """Row b of a step's lengths is row b of ``block_tables``: a request keeps its
-    row while it lives, and a row without a request has lengths of 0.  Calls
-    belong to one stream (or are ordered by the caller) and may be captured into
+    row while it lives, and a row without a request has lengths of 0.  There are
+    at most ``MAX_REQUESTS`` rows.  Calls belong to one stream (or are ordered by the caller) and may be captured into
     a CUDA graph, which then reads the lengths' tensors anew at each replay."""
 
     def __init__(self, max_requests: int, max_blocks: int, page_size: int, num_pages: int,
@@ -57,6 +59,8 @@ class BlockTables:
             raise RuntimeError("BlockTables: a CUDA device is needed")
         if min(max_requests, max_blocks, page_size, num_pages, max_tokens) < 1:
             raise RuntimeError("BlockTables: all sizes must be positive")
+        if max_requests > MAX_REQUESTS:
+            raise RuntimeError(f"BlockTables: at most {MAX_REQUESTS} requests, not {max_requests}")
         if max(max_requests * max_blocks, num_pages, max_tokens) >= 1 << 31:
             raise RuntimeError("BlockTables: sizes past 32 bits")
         ints = lambda *n, kind=torch.int32: torch.zeros(*n, dtype=kind, device=device)  # noqa: E731
