@@ -38,6 +38,14 @@ class Layer:
         angle = torch.arange(2048, dtype=torch.float64)[:, None] \
             * 10000.0 ** (-torch.arange(0, HEAD_DIM, 2, dtype=torch.float64) / HEAD_DIM)
         self.cos_sin = torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
+        # a bit is set in it if a kernel's bounded wait runs out, whose output is then undefined
+        self.fault = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def check(self) -> None:
+        """Raise if a call since the last one gave up; where the engine waits for the GPU anyway."""
+        if int(self.fault):
+            self.fault.zero_()
+            raise RuntimeError("a kernel's wait ran out: the steps' outputs are undefined")
 
 
 def _codes(rows: int, width: int, device):
@@ -57,27 +65,28 @@ def forward(layer: Layer, hidden: torch.Tensor, step, attention: PagedAttention,
     int8_ops.rms_norm_quantise(codes, scales, hidden, layer.input_norm, EPS)
     q_size, kv_size = HEADS * HEAD_DIM, KV_HEADS * HEAD_DIM
     qkv = empty(q_size + 2 * kv_size)
-    int8_ops.linear(qkv, codes, scales, *layer.qkv)
+    int8_ops.linear(qkv, codes, scales, *layer.qkv, fault_flags=layer.fault)
     note(in_codes=codes, in_scales=scales, qkv=qkv)
     query, key, value = qkv.split([q_size, kv_size, kv_size], 1)
     pos_encoding_ops.qk_norm_rotary_append(step.positions, query, key, value, layer.q_norm, layer.k_norm, EPS,
-                                           HEAD_DIM, layer.cos_sin, True, layer.cache, step.slot_mapping)
+                                           HEAD_DIM, layer.cos_sin, True, layer.cache, step.slot_mapping,
+                                           fault_flags=layer.fault)
     attended = attention.forward(query.view(t, HEADS, HEAD_DIM), layer.cache).view(t, q_size)
     note(query=query, attended=attended)
 
     codes, scales = _codes(t, q_size, dev)
     int8_ops.quantise_rows(codes, scales, attended)
-    int8_ops.linear_residual(hidden, codes, scales, *layer.out)
+    int8_ops.linear_residual(hidden, codes, scales, *layer.out, fault_flags=layer.fault)
     note(out_codes=codes, out_scales=scales, middle=hidden)
 
     codes, scales = _codes(t, HIDDEN, dev)
     int8_ops.rms_norm_quantise(codes, scales, hidden, layer.post_norm, EPS)
     act = empty(INTER)
-    int8_ops.gate_up_silu(act, codes, scales, *layer.gate_up)
+    int8_ops.gate_up_silu(act, codes, scales, *layer.gate_up, fault_flags=layer.fault)
     note(post_codes=codes, post_scales=scales, act=act)
     codes, scales = _codes(t, INTER, dev)
     int8_ops.quantise_rows(codes, scales, act)
-    int8_ops.linear_residual(hidden, codes, scales, *layer.down)
+    int8_ops.linear_residual(hidden, codes, scales, *layer.down, fault_flags=layer.fault)
     note(act_codes=codes, act_scales=scales, result=hidden)
     return hidden
 
@@ -117,6 +126,7 @@ def main(device: str = "cuda:0", pages: int = 64, seed: int = 0):
     lens[0] = 0
     run([33, 1])                # another takes its row
     tables.check()
+    layer.check()
     attention.check()
     return layer, tables, done
 

@@ -49,8 +49,9 @@ class StepTables(NamedTuple):
 class BlockTables:
     """Row b of a step's lengths is row b of ``block_tables``: a request keeps its
     row while it lives, and a row without a request has lengths of 0.  There are
-    at most ``MAX_REQUESTS`` rows.  Calls belong to one stream (or are ordered by the caller) and may be captured into
-    a CUDA graph, which then reads the lengths' tensors anew at each replay."""
+    at most ``MAX_REQUESTS`` rows.  Calls belong to one stream (or are ordered by
+    the caller) and may be captured into a CUDA graph, which then reads the
+    lengths' tensors anew at each replay."""
 
     def __init__(self, max_requests: int, max_blocks: int, page_size: int, num_pages: int,
                  max_tokens: int, device: torch.device | str | int = "cuda"):
