@@ -171,8 +171,10 @@ __device__ __forceinline__ bool epi_all(bool pred) {
   return r != 0;
 }
 
-// 16-bit outputs take the approximate exponential and quotient, a few units of
-// 2^-24 that their own rounding hides; float32 the library's.
+// 16-bit outputs take the approximate exponential and quotient, float32 the
+// library's.  The approximate exponential's argument is rounded, which leaves an error
+// that goes with |g|: at most (4 |g| + 16) 2^-24 of the value.  Where 1 + e^-g passes
+// 2^126 (e^-g 2^128 in float32) the quotient is 0; what is lost is below |g| |u| 2^-126.
 template <typename T>
 __device__ __forceinline__ float silu_mul(float g, float u) {
   if constexpr (sizeof(T) == 2) return __fdividef(g, 1.f + __expf(-g)) * u;

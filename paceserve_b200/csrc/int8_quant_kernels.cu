@@ -74,8 +74,9 @@ __device__ __forceinline__ float larger(float top, float y) {
 }
 
 // silu(g) * u of two elements.  16-bit inputs take the approximate exponential and
-// reciprocal (a few units of 2^-24, far below the code's half step), float32 the
-// library's.
+// reciprocal, float32 the library's.  The approximate exponential's argument is
+// rounded, which leaves an error that goes with |g|: at most (4 |g| + 16) 2^-24 of the
+// value, at |g| = 100 a 150th of the code's half step.
 template <typename T>
 __device__ __forceinline__ void silu_mul2(float* g, const float* u) {
   if constexpr (sizeof(T) == 2) {

@@ -18,7 +18,6 @@
 // rotation's two halves (NeoX) or 2 x 8 neighbours (GPT-J), so that rotation is
 // in the thread and the norm is log2(G) shuffles.  Tokens and heads are dealt to
 // CTAs as one flat range, so few heads or narrow ones fill a CTA as well.
-#include <cstdlib>
 #include <algorithm>
 
 #include "f32x2.cuh"
